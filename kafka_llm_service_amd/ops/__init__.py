@@ -8,6 +8,7 @@ Kernel inventory:
   sample (greedy / temperature / top-k / top-p) csrc/sampling.hip
   moe_* / grouped GEMM                          csrc/moe.hip
   custom all-reduce                             csrc/allreduce.hip
+  4-bit cache: attention, eviction (kv4.py)     csrc/kv4.hip, csrc/kv4_attn.hip
 """
 from __future__ import annotations
 
@@ -24,6 +25,7 @@ PAGE = ref.PAGE
 kv_cache_shapes = ref.kv_cache_shapes
 kv_page_bytes = ref.kv_page_bytes
 is_fp8_cache = ref.is_fp8_cache
+is_mx4_cache = ref.is_mx4_cache
 
 
 def _gpu(t: torch.Tensor) -> bool:
@@ -146,8 +148,11 @@ def silu_mul(x: torch.Tensor, out: torch.Tensor | None = None, act: str = "silu"
 
 
 def rope_kv_write(qkv, positions, cos_sin, q_out, k_cache, v_cache, slot_mapping, Hq: int, Hkv: int) -> None:
-    """RoPE on q/k + paged KV write; ``qkv`` is bf16 [T, W] or a split-K slab [S, T, W]."""
-    if _gpu(qkv):
+    """RoPE on q/k + paged KV write; ``qkv`` is bf16 [T, W] or a split-K slab [S, T, W]. Slots below zero are left out. (The cache in 4
+    bits takes keys as the one in bf16 would hold them; not a number counts as zero there, an infinity as the largest.)"""
+    if _gpu(qkv) and is_mx4_cache(k_cache):
+        ext().kv4_rope_write(qkv, positions, cos_sin, q_out, k_cache, v_cache, slot_mapping, int(Hq), int(Hkv))
+    elif _gpu(qkv):
         ext().rope_kv_write(qkv, positions, cos_sin, q_out, k_cache, v_cache, slot_mapping, int(Hq), int(Hkv))
     else:
         ref.rope_kv_write(qkv.sum(0) if is_slab(qkv) else qkv, positions, cos_sin, q_out, k_cache, v_cache,

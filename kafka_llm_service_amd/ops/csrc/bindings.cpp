@@ -1357,10 +1357,12 @@ static void ep_combine(at::Tensor back, at::Tensor slot_map, at::Tensor topk_w, 
 }
 
 void kafka_bind_hybrid(pybind11::module_& m);  // hybrid_bindings.cpp
+void kafka_bind_kv4(pybind11::module_& m);     // kv4_bindings.cpp
 
 PYBIND11_MODULE(_kafka_ops, m) {
   m.doc() = "kafka_llm_service_amd CDNA4 (gfx950) HIP kernels";
   kafka_bind_hybrid(m);
+  kafka_bind_kv4(m);
   m.def("rmsnorm", &rmsnorm);
   m.def("fused_add_rmsnorm", &fused_add_rmsnorm);
   m.def("rows_norm", &rows_norm);

@@ -1,0 +1,339 @@
+// The 4-bit cache's writer, its reader and the eviction from it (pages: kv4.h).
+#include "kv4.h"
+
+namespace kafka {
+namespace kv4 {
+
+// ---- writer -----------------------------------------------------------------------------------------------------------
+// Of 32 numbers (eight in each of four neighbouring lanes) the least e with |x| <= 6 * 2^e, as a byte e + 127. With the bits of a
+// bf16 as an integer, 6 * 2^e is (e + 129) << 7 | 0x40, so the carry of + 0x3f says whether the mantissa is beyond 3/2.
+__device__ __forceinline__ uint32_t scale_byte(bf16x8 x) {
+  const u32x4 b = __builtin_bit_cast(u32x4, x);
+  uint32_t m = 0;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) m = max(m, max(b[j] & 0x7fffu, (b[j] >> 16) & 0x7fffu));
+  m = max(m, (uint32_t)__shfl_xor((int)m, 1, 64));
+  m = max(m, (uint32_t)__shfl_xor((int)m, 2, 64));
+  return (uint32_t)min(max((int)((m + 0x3f) >> 7) - 129, EXP_MIN), EXP_MAX) + 127u;
+}
+
+// not a number counts as zero, an infinity as the largest that the scale holds: what is read back is always a number, so that no
+// masked place can spoil a product
+__device__ __forceinline__ bf16x8 numbers(bf16x8 x) {
+#pragma unroll
+  for (int j = 0; j < 8; ++j) x[j] = x[j] == x[j] ? x[j] : (bf16)0.f;
+  return x;
+}
+
+// Rotation in fp32 without fused products (each product rounded by itself, as elementary operations give it: next to a border of
+// two codes the last bit decides), rounded to bf16 as the cache in bf16 holds it, then to 4 bits. A thread takes eight
+// pairs of a query or key head, or eight elements of a value head; four neighbours share a scale.
+template <int D>
+__global__ __launch_bounds__(256) void rope_write_kernel(const bf16* __restrict__ qkv, const float* __restrict__ qp, int S, int64_t ps,
+                                                         int64_t qkv_stride, const int64_t* __restrict__ positions,
+                                                         const float* __restrict__ cos_sin, bf16* __restrict__ q_out, int64_t q_stride,
+                                                         uint8_t* __restrict__ kc, uint8_t* __restrict__ vc,
+                                                         const int64_t* __restrict__ slots, int64_t n_slots, int64_t total, int Hq, int Hkv) {
+  constexpr int HALF = D / 2, RU = HALF / 8, VU = D / 8;
+  const int n_rope = (Hq + Hkv) * RU, n_row = n_rope + Hkv * VU;   // (multiples of four, as is total)
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i >= total) return;
+  const int t = (int)(i / n_row), u = (int)(i - (int64_t)t * n_row);
+  int64_t slot = slots ? slots[t] : -1;
+  if (slot >= n_slots) slot = -1;
+  const int64_t row = (int64_t)t * qkv_stride;
+  const int64_t page = slot >> 4;
+  const int o = (int)(slot & 15);
+  if (u < n_rope) {
+    const int head = u / RU, c = (u % RU) * 8;
+    float x1[8], x2[8];
+    load_in8(x1, qkv, qp, S, ps, row + head * D + c);
+    load_in8(x2, qkv, qp, S, ps, row + head * D + HALF + c);
+    const float* cs = cos_sin + positions[t] * D + c;
+    bf16x8 y1, y2;
+    {
+#pragma clang fp contract(off)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float co = cs[j], si = cs[HALF + j];
+        const float ac = x1[j] * co, bs = x2[j] * si, bc = x2[j] * co, as = x1[j] * si;
+        y1[j] = (bf16)(ac - bs);
+        y2[j] = (bf16)(bc + as);
+      }
+    }
+    if (head < Hq) {
+      bf16* dst = q_out + t * q_stride + head * D + c;
+      store_bf16x8(dst, y1);
+      store_bf16x8(dst + HALF, y2);
+      return;
+    }
+    y1 = numbers(y1);
+    y2 = numbers(y2);
+    const uint32_t b1 = scale_byte(y1), b2 = scale_byte(y2);
+    if (slot < 0) return;
+    uint8_t* k = kc + (page * Hkv + head - Hq) * (int64_t)Page<D>::BYTES;
+    *reinterpret_cast<uint32_t*>(k + o * (D / 2) + c / 2) = narrow8(y1, scale_of(b1));
+    *reinterpret_cast<uint32_t*>(k + o * (D / 2) + (HALF + c) / 2) = narrow8(y2, scale_of(b2));
+    if ((c & 31) == 0) {
+      k[Page<D>::DATA + o * (D / 32) + c / 32] = (uint8_t)b1;
+      k[Page<D>::DATA + o * (D / 32) + (HALF + c) / 32] = (uint8_t)b2;
+    }
+  } else {
+    const int head = (u - n_rope) / VU, p = (u - n_rope) % VU;
+    float x[8];
+    load_in8(x, qkv, qp, S, ps, row + (Hq + Hkv + head) * D + p * 8);
+    bf16x8 y;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) y[j] = (bf16)x[j];
+    y = numbers(y);
+    const uint32_t b = scale_byte(y);
+    if (slot < 0) return;
+    uint8_t* v = vc + (page * Hkv + head) * (int64_t)Page<D>::BYTES;
+    *reinterpret_cast<uint32_t*>(v + ((o >> 2) * VU + p) * 16 + (o & 3) * 4) = narrow8(y, scale_of(b));
+    if ((p & 3) == 0) v[Page<D>::DATA + (p >> 2) * 16 + o] = (uint8_t)b;
+  }
+}
+
+// ---- reader -----------------------------------------------------------------------------------------------------------
+// Keys and values of slots as bf16 rows, exactly: two bits of mantissa and a power of two. Negative slots give zeros, slots behind
+// the cache no numbers. A thread takes eight elements of a key and of its value.
+template <int D>
+__global__ __launch_bounds__(256) void read_kernel(const uint8_t* __restrict__ kc, const uint8_t* __restrict__ vc,
+                                                   const int64_t* __restrict__ slots, int64_t n_slots, int64_t total, int Hkv,
+                                                   bf16* __restrict__ k, bf16* __restrict__ v) {
+  constexpr int U = D / 8;
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i >= total) return;
+  const int p = (int)(i % U);
+  const int64_t th = i / U, t = th / Hkv;
+  const int h = (int)(th - t * Hkv);
+  const int64_t slot = slots[t];
+  bf16x8 a, b;
+  if (slot < 0 || slot >= n_slots) {
+    const bf16 none = slot < 0 ? (bf16)0.f : (bf16)__builtin_nanf("");
+#pragma unroll
+    for (int j = 0; j < 8; ++j) a[j] = b[j] = none;
+  } else {
+    const int o = (int)(slot & 15);
+    const int64_t at = ((slot >> 4) * Hkv + h) * (int64_t)Page<D>::BYTES;
+    const uint32_t kw = *reinterpret_cast<const uint32_t*>(kc + at + o * (D / 2) + p * 4);
+    const uint32_t vw = *reinterpret_cast<const uint32_t*>(vc + at + ((o >> 2) * U + p) * 16 + (o & 3) * 4);
+    a = widen8(kw, scale_of(kc[at + Page<D>::DATA + o * (D / 32) + (p >> 2)]));
+    b = widen8(vw, scale_of(vc[at + Page<D>::DATA + (p >> 2) * 16 + o]));
+  }
+  store_bf16x8(k + i * 8, a);
+  store_bf16x8(v + i * 8, b);
+}
+
+// ---- eviction ---------------------------------------------------------------------------------------------------------
+// Order of masses as of unsigned integers: the two zeros alike, not a number below everything.
+__device__ __forceinline__ uint32_t rank_of(float x) {
+  const uint32_t b = __float_as_uint(x), a = b & 0x7fffffffu;   // (by its bits: comparisons take the smallest numbers for zeros)
+  if (a > 0x7f800000u) return 0u;
+  return a == 0u ? 0x80000000u : (b & 0x80000000u) ? ~b : b | 0x80000000u;
+}
+
+constexpr int KEEP_NT = 1024;
+
+// Kept keys of one (sequence, head), ascending: the first ones, the most recent ones, and of those between them the ``room`` largest, ties to
+// the lowest index. Radix select: four counts of a byte each narrow the threshold down, then one ordered pass writes.
+__global__ __launch_bounds__(KEEP_NT) void evict_keep_kernel(const float* __restrict__ mass, int64_t ms, int64_t mh, int N,
+                                                             const int* __restrict__ lens, int budget, int first, int recent,
+                                                             int* __restrict__ kept, int Hkv) {
+  __shared__ int hist[256];
+  __shared__ int s_digit, s_above;
+  __shared__ int wsum[2][KEEP_NT / 64];
+  const int h = blockIdx.x, r = blockIdx.y, tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
+  const float* m = mass + r * ms + h * mh;
+  int* out = kept + ((int64_t)r * Hkv + h) * budget;
+  const int n = min(max(lens[r], 0), N);
+  if (n <= budget) {
+    for (int i = tid; i < budget; i += KEEP_NT) out[i] = i < n ? i : -1;
+    return;
+  }
+  const int a = first, b = n - recent, room = budget - first - recent;   // (b - a = n - budget + room > room)
+  uint32_t lead = 0, known = 0;
+  int need = room;                                                       // of those with the leading digits of the threshold
+  for (int shift = 24; shift >= 0 && need > 0; shift -= 8) {
+    if (tid < 256) hist[tid] = 0;
+    __syncthreads();
+    for (int i = a + tid; i < b; i += KEEP_NT) {
+      const uint32_t k = rank_of(m[i]);
+      if ((k & known) == lead) atomicAdd(&hist[(k >> shift) & 255], 1);
+    }
+    __syncthreads();
+    if (w == 0) {                                                        // four digits a lane, from the largest down
+      const int d0 = 255 - 4 * lane;
+      const int c0 = hist[d0], c1 = hist[d0 - 1], c2 = hist[d0 - 2], c3 = hist[d0 - 3];
+      int inc = c0 + c1 + c2 + c3;
+      for (int o = 1; o < 64; o <<= 1) {
+        const int y = __shfl_up(inc, o, 64);
+        if (lane >= o) inc += y;
+      }
+      int before = inc - (c0 + c1 + c2 + c3);
+      if (before < need && inc >= need) {
+        int d = d0;
+        if (before + c0 < need) {
+          before += c0;
+          d = d0 - 1;
+          if (before + c1 < need) {
+            before += c1;
+            d = d0 - 2;
+            if (before + c2 < need) {
+              before += c2;
+              d = d0 - 3;
+            }
+          }
+        }
+        s_digit = d;
+        s_above = before;
+      }
+    }
+    __syncthreads();
+    lead |= (uint32_t)s_digit << shift;
+    known |= 255u << shift;
+    need -= s_above;
+    __syncthreads();
+  }
+  // ``lead`` is the threshold: everything above it stays, and the first ``need`` of its equals (room 0: nothing between the two ends)
+  int ties = 0, done = 0;                                                // before this chunk
+  for (int i0 = 0; i0 < n; i0 += KEEP_NT) {
+    const int i = i0 + tid;
+    const bool fixed = i < a || (i >= b && i < n), mid = i >= a && i < b && room > 0;
+    const uint32_t k = mid ? rank_of(m[i]) : 0u;
+    const bool above = mid && k > lead, tie = mid && k == lead;
+    const uint64_t tb = __ballot(tie);
+    if (lane == 0) wsum[0][w] = __popcll(tb);
+    __syncthreads();
+    int tr = ties, tall = 0;
+    for (int x = 0; x < KEEP_NT / 64; ++x) {
+      if (x < w) tr += wsum[0][x];
+      tall += wsum[0][x];
+    }
+    tr += __popcll(tb & ((1ull << lane) - 1));
+    const bool keep = fixed || above || (tie && tr < need);
+    const uint64_t kb = __ballot(keep);
+    if (lane == 0) wsum[1][w] = __popcll(kb);
+    __syncthreads();
+    int at = done, kall = 0;
+    for (int x = 0; x < KEEP_NT / 64; ++x) {
+      if (x < w) at += wsum[1][x];
+      kall += wsum[1][x];
+    }
+    at += __popcll(kb & ((1ull << lane) - 1));
+    if (keep && at < budget) out[at] = i;
+    ties += tall;
+    done += kall;
+  }
+}
+
+// Kept keys, values and masses into new pages, a wave per new page and head. K goes by 16-byte pieces, V by the words of its keys.
+// Keys outside of their table or cache leave their place in the new page as it was.
+template <int D>
+__global__ __launch_bounds__(256) void evict_copy_kernel(uint8_t* __restrict__ kc, uint8_t* __restrict__ vc, int64_t n_pages,
+                                                         const int* __restrict__ tables, int tw, int64_t ts, const int* __restrict__ kept,
+                                                         int budget, const int* __restrict__ new_tables, int nw, int64_t ns, int Hkv,
+                                                         const float* __restrict__ mass, int64_t ms, int64_t mh, int N,
+                                                         float* __restrict__ new_mass) {
+  constexpr int U = D / 8, KP = D / 32;     // words of a key; 16-byte pieces of it
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  const int h = blockIdx.y, r = blockIdx.z, pg = blockIdx.x * 4 + w;
+  const int i0 = pg * PAGE;
+  if (i0 >= budget) return;
+  const int* kp = kept + ((int64_t)r * Hkv + h) * budget + i0;
+  const int o = lane & 15;
+  int src = i0 + o < budget ? kp[o] : -1;   // lane o: the page's key o
+  if (new_mass && lane < 16 && i0 + o < budget)
+    new_mass[((int64_t)r * Hkv + h) * budget + i0 + o] = src >= 0 && src < N ? mass[r * ms + h * mh + src] : 0.f;
+  int64_t from = -1;                        // its page and head, in pages
+  if (src >= 0 && (src >> 4) < tw) {
+    const int p = tables[r * ts + (src >> 4)];
+    if (p >= 0 && p < n_pages) from = (int64_t)p * Hkv + h;
+  }
+  if (pg >= nw) return;
+  const int np = new_tables[r * ns + pg];
+  if (np < 0 || np >= n_pages) return;
+  const int so = src & 15;
+  uint8_t* kd = kc + ((int64_t)np * Hkv + h) * Page<D>::BYTES;
+  uint8_t* vd = vc + ((int64_t)np * Hkv + h) * Page<D>::BYTES;
+  auto of = [&](int64_t x, int l) {
+    return (int64_t)(uint32_t)__shfl((int)(uint32_t)x, l, 64) | (int64_t)__shfl((int)(x >> 32), l, 64) << 32;
+  };
+  // K: lane = (key, piece)
+  const int key = lane / KP, pc = lane % KP;
+  const int64_t kf = of(from, key & 15);
+  const int ko = __shfl(so, key & 15, 64);
+  if (key < 16 && kf >= 0)
+    *reinterpret_cast<u32x4*>(kd + key * (D / 2) + pc * 16) =
+        *reinterpret_cast<const u32x4*>(kc + kf * Page<D>::BYTES + ko * (D / 2) + pc * 16);
+  // V: lane = (four keys, eight elements)
+  const int c = lane / U, p = lane % U;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int k4 = (4 * c + i) & 15;
+    const int64_t vf = of(from, k4);
+    const int vo = __shfl(so, k4, 64);
+    if (c < 4 && vf >= 0)
+      *reinterpret_cast<uint32_t*>(vd + (c * U + p) * 16 + i * 4) =
+          *reinterpret_cast<const uint32_t*>(vc + vf * Page<D>::BYTES + ((vo >> 2) * U + p) * 16 + (vo & 3) * 4);
+  }
+  // scales: lane = (group, key)
+  const int g = lane >> 4;
+  if (g < D / 32 && from >= 0) {
+    kd[Page<D>::DATA + o * (D / 32) + g] = kc[from * Page<D>::BYTES + Page<D>::DATA + so * (D / 32) + g];
+    vd[Page<D>::DATA + g * 16 + o] = vc[from * Page<D>::BYTES + Page<D>::DATA + g * 16 + so];
+  }
+}
+
+}  // namespace kv4
+
+using namespace kv4;
+
+extern "C" hipError_t kafka_kv4_rope_write(const bf16* qkv, const float* qp, int S, int64_t ps, int64_t qkv_stride, const int64_t* positions,
+                                           const float* cos_sin, bf16* q_out, int64_t q_stride, uint8_t* kc, uint8_t* vc,
+                                           const int64_t* slots, int64_t n_slots, int T, int Hq, int Hkv, int D, hipStream_t st) {
+  if (T == 0) return hipSuccess;
+  const int64_t total = (int64_t)T * ((Hq + Hkv) * (D / 16) + Hkv * (D / 8));
+  if ((D != 64 && D != 128) || total > 0xffffff00ll) return hipErrorInvalidValue;
+  auto go = [&](auto kern) {
+    kern<<<(unsigned)((total + 255) / 256), 256, 0, st>>>(qkv, qp, S, ps, qkv_stride, positions, cos_sin, q_out, q_stride, kc, vc, slots,
+                                                          n_slots, total, Hq, Hkv);
+    return hipGetLastError();
+  };
+  return D == 64 ? go(rope_write_kernel<64>) : go(rope_write_kernel<128>);
+}
+
+extern "C" hipError_t kafka_kv4_read(const uint8_t* kc, const uint8_t* vc, const int64_t* slots, int64_t n_slots, int64_t T, int Hkv, int D,
+                                     bf16* k, bf16* v, hipStream_t st) {
+  if (T == 0) return hipSuccess;
+  const int64_t total = T * Hkv * (D / 8);
+  if ((D != 64 && D != 128) || total > 0xffffff00ll) return hipErrorInvalidValue;
+  auto go = [&](auto kern) {
+    kern<<<(unsigned)((total + 255) / 256), 256, 0, st>>>(kc, vc, slots, n_slots, total, Hkv, k, v);
+    return hipGetLastError();
+  };
+  return D == 64 ? go(read_kernel<64>) : go(read_kernel<128>);
+}
+
+extern "C" hipError_t kafka_kv4_evict_keep(const float* mass, int64_t ms, int64_t mh, int N, const int* lens, int R, int Hkv, int budget,
+                                           int first, int recent, int* kept, hipStream_t st) {
+  if (R == 0 || budget == 0) return hipSuccess;
+  if (first < 0 || recent < 0 || (int64_t)first + recent > budget || R > 65535) return hipErrorInvalidValue;
+  evict_keep_kernel<<<dim3(Hkv, R), KEEP_NT, 0, st>>>(mass, ms, mh, N, lens, budget, first, recent, kept, Hkv);
+  return hipGetLastError();
+}
+
+extern "C" hipError_t kafka_kv4_evict_copy(uint8_t* kc, uint8_t* vc, int64_t n_pages, const int* tables, int tw, int64_t ts,
+                                           const int* kept, int R, int Hkv, int budget, const int* new_tables, int nw, int64_t ns,
+                                           const float* mass, int64_t ms, int64_t mh, int N, float* new_mass, int D, hipStream_t st) {
+  if (R == 0 || budget == 0) return hipSuccess;
+  if ((D != 64 && D != 128) || R > 65535 || Hkv > 65535) return hipErrorInvalidValue;
+  auto go = [&](auto kern) {
+    kern<<<dim3((budget + 63) / 64, Hkv, R), 256, 0, st>>>(kc, vc, n_pages, tables, tw, ts, kept, budget, new_tables, nw, ns, Hkv, mass, ms,
+                                                           mh, N, new_mass);
+    return hipGetLastError();
+  };
+  return D == 64 ? go(evict_copy_kernel<64>) : go(evict_copy_kernel<128>);
+}
+
+}  // namespace kafka

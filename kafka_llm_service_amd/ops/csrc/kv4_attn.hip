@@ -1,0 +1,500 @@
+// Attention over the 4-bit cache, and the weight that its keys receive (pages: kv4.h; gfx950).
+//
+// A call's rows are segments of consecutive tokens of one sequence each; the row at position p sees the keys j <= p, with a window only
+// those with j > p - window or j < first. A work item is a tile of a segment's tokens and a range of the blocks of 64 keys that
+// any of them sees (the first ones, then those from the window's start on: a block in the range is a place in this list).
+//
+//   S^T[key][row] = K . Q^T    A: a lane's key and quarter of its elements, widened to bf16 (exactly), B: Q's fragments in registers
+//   O^T[d][row]  += V^T . P    A: a lane's eight d's, widened and turned by v_perm to pairs of keys, B: P as S^T's registers hold it
+// The softmax runs in one pass with a running maximum per row; its sums and maxima are fp32, P is rounded to bf16 for the product.
+#include "kv4.h"
+
+namespace kafka {
+namespace kv4 {
+
+constexpr int KB = 64;   // keys of a block
+
+struct Item {
+  int row, tokens;       // first row, rows
+  int pos;               // position of the first
+  int table;             // row of the block table
+  int lo, hi;            // blocks of its list
+  int slot;              // < 0: the rows are written, else partial results number ``slot``
+  int pad;
+};
+
+struct Args {
+  const bf16* q;
+  int64_t qs;
+  const uint8_t *kc, *vc;
+  int64_t n_pages;
+  const int* tables;
+  int64_t ts;
+  const Item* items;
+  int T, Hkv, G;
+  int window, first;     // (no window: 2^30)
+  float scale2;          // scale * log2(e)
+  bf16* out;
+  int64_t os;
+  float* lse;            // [T][Hq], may be null
+  float *part, *plse;    // [slots][Hkv][rows of a tile][D], [slots][Hkv][rows of a tile]
+};
+
+__device__ __forceinline__ float vmax(float a, float b) { return __builtin_elementwise_maximum(a, b); }
+__device__ __forceinline__ float over_quarters_max(float x) {   // of the lanes with the same l & 15
+  x = vmax(x, __shfl_xor(x, 16, 64));
+  return vmax(x, __shfl_xor(x, 32, 64));
+}
+__device__ __forceinline__ float over_quarters_sum(float x) {
+  x += __shfl_xor(x, 16, 64);
+  return x + __shfl_xor(x, 32, 64);
+}
+
+// The list of blocks that a tile of rows at positions [p0, p1] sees
+struct Blocks {
+  int head, tail, count;   // blocks below ``head``, then from ``tail`` on
+  __device__ __forceinline__ Blocks(int p0, int p1, int window, int first) {
+    tail = max(0, p0 - window + 1) / KB;
+    head = min((first + KB - 1) / KB, tail);
+    count = p1 < 0 ? 0 : head + p1 / KB + 1 - tail;
+  }
+  __device__ __forceinline__ int operator[](int v) const { return v < head ? v : v - head + tail; }
+};
+
+template <int D>
+struct KFrag {
+  uint32_t d[4][D / 32];   // a lane's words of four tiles of 16 keys
+  uint32_t s[4];
+};
+struct VFrag {
+  u32x4 d[4];              // a word for each of four keys, of four pages
+  uint32_t s[4];
+};
+
+// Page ids of block b; keys behind ``last`` take its page (they are masked). An id that is not of the cache counts as page 0 and
+// sets ``bad``: such rows come out as no numbers.
+__device__ __forceinline__ void block_pages(const int* bt, int b, int last, int64_t n_pages, int (&pg)[4], bool& bad) {
+#pragma unroll
+  for (int t = 0; t < 4; ++t) {
+    const int p = bt[min(b * 4 + t, last >> 4)];
+    const bool ok = p >= 0 && p < n_pages;
+    bad |= !ok;
+    pg[t] = ok ? p : 0;
+  }
+}
+
+template <int D>
+__device__ __forceinline__ void load_k(KFrag<D>& f, const uint8_t* kc, int Hkv, int h, const int (&pg)[4], int lane) {
+  const int key = lane & 15, c = lane >> 4;
+#pragma unroll
+  for (int t = 0; t < 4; ++t) {
+    const uint8_t* p = kc + ((int64_t)pg[t] * Hkv + h) * Page<D>::BYTES;
+    if constexpr (D == 128) {
+      const u32x4 x = *reinterpret_cast<const u32x4*>(p + key * 64 + c * 16);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) f.d[t][i] = x[i];
+    } else {
+      const u32x2 x = *reinterpret_cast<const u32x2*>(p + key * 32 + c * 8);
+      f.d[t][0] = x[0];
+      f.d[t][1] = x[1];
+    }
+    f.s[t] = p[Page<D>::DATA + key * (D / 32) + c * (D / 32) / 4];
+  }
+}
+
+template <int D>
+__device__ __forceinline__ void load_v(VFrag& f, const uint8_t* vc, int Hkv, int h, const int (&pg)[4], int lane) {
+  const int dl = lane & 15, c = lane >> 4;
+#pragma unroll
+  for (int t = 0; t < 4; ++t) {
+    const uint8_t* p = vc + ((int64_t)pg[t] * Hkv + h) * Page<D>::BYTES;
+    f.d[t] = *reinterpret_cast<const u32x4*>(p + (c * (D / 8) + dl * (D / 8) / 16) * 16);
+    f.s[t] = *reinterpret_cast<const uint32_t*>(p + Page<D>::DATA + (dl * (D / 16) / 32) * 16 + c * 4);
+  }
+}
+
+template <int D, int NQ>
+struct Rows {
+  bf16x8 q[NQ][D / 32];
+  int lim[NQ];              // a column's position; -1: no row
+  f32x4 o[NQ][D / 16];      // register i of tile n: d = (D / 16) (4 c + i) + n
+  float m[NQ], l[NQ];       // maximum so far (times scale, log2), this lane's part of the sum
+};
+
+// Q's fragments of 16 columns from column R0 of the tile on
+template <int D>
+__device__ __forceinline__ int load_q(bf16x8 (&q)[D / 32], const Args& a, int row, int tokens, int pos, int h, int R0, int lane) {
+  const int R = R0 + (lane & 15), tok = R / a.G, g = R - tok * a.G;
+  const bool there = tok < tokens;
+  const bf16* p = a.q + (int64_t)(row + (there ? tok : 0)) * a.qs + (int64_t)(h * a.G + g) * D + (lane >> 4) * (D / 4);
+#pragma unroll
+  for (int s = 0; s < D / 32; ++s) {
+    q[s] = load_bf16x8(p + 8 * s);
+    if (!there) q[s] = bf16x8{};
+  }
+  return there ? pos + tok : -1;
+}
+
+// Scores of 64 keys
+template <int D, int NQ>
+__device__ __forceinline__ void scores(const KFrag<D>& f, const bf16x8 (&q)[NQ][D / 32], f32x4 (&s)[4][NQ]) {
+#pragma unroll
+  for (int t = 0; t < 4; ++t) {
+    const float sc = scale_of(f.s[t]);
+#pragma unroll
+    for (int n = 0; n < NQ; ++n) s[t][n] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i) {
+      const bf16x8 k = widen8(f.d[t][i], sc);
+#pragma unroll
+      for (int n = 0; n < NQ; ++n) s[t][n] = mfma16(k, q[n][i], s[t][n]);
+    }
+  }
+}
+
+__device__ __forceinline__ bool sees(int key, int lim, int window, int first) { return key <= lim && (key > lim - window || key < first); }
+
+// One block of keys: scores, softmax, values
+template <int D, int NQ>
+__device__ __forceinline__ void block_step(const KFrag<D>& kf, const VFrag& vf, Rows<D, NQ>& r, int key0, int pmin, int pmax, int window,
+                                           int first, float scale2, int lane) {
+  const int c = lane >> 4;
+  f32x4 s[4][NQ];
+  scores<D, NQ>(kf, r.q, s);
+  const bool masked = key0 + KB - 1 > pmin || (key0 <= pmax - window && key0 + KB > first);
+  if (masked) {
+#pragma unroll
+    for (int n = 0; n < NQ; ++n)
+#pragma unroll
+      for (int t = 0; t < 4; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (!sees(key0 + 16 * t + 4 * c + i, r.lim[n], window, first)) s[t][n][i] = -INFINITY;
+  }
+  bf16x8 p[NQ][2];
+#pragma unroll
+  for (int n = 0; n < NQ; ++n) {
+    float mx = vmax(vmax(s[0][n][0], s[0][n][1]), vmax(s[0][n][2], s[0][n][3]));
+#pragma unroll
+    for (int t = 1; t < 4; ++t) mx = vmax(vmax(vmax(mx, s[t][n][0]), s[t][n][1]), vmax(s[t][n][2], s[t][n][3]));
+    mx = vmax(r.m[n], over_quarters_max(mx) * scale2);
+    const float use = mx == -INFINITY ? 0.f : mx;
+    if (!__all(mx == r.m[n])) {
+      const float f = fast_exp2(r.m[n] - use);
+      r.l[n] *= f;
+#pragma unroll
+      for (int d = 0; d < D / 16; ++d) r.o[n][d] *= f;
+    }
+    r.m[n] = mx;
+    float sum = 0.f;
+#pragma unroll
+    for (int t = 0; t < 4; ++t)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float e = fast_exp2(fmaf(s[t][n][i], scale2, -use));
+        sum += e;
+        p[n][t >> 1][4 * (t & 1) + i] = (bf16)e;
+      }
+    r.l[n] += sum;
+  }
+  constexpr int W = D / 32;                                     // pairs of d a lane
+  const int dl = lane & 15;
+#pragma unroll
+  for (int u = 0; u < 2; ++u) {
+    uint32_t x[W][8];
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        uint32_t w = vf.d[2 * u + t][i], e = (vf.s[2 * u + t] >> (8 * i)) & 255u;
+        if (D == 64) w >>= 16 * (dl & 1);
+        // (behind the last position the page may hold anything, also scales that are no numbers: their weight is zero, so must they be)
+        if (masked && key0 + 32 * u + 16 * t + 4 * c + i > pmax) w = 0u, e = 0u;
+        const float sc = scale_of(e);
+        x[0][4 * t + i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, sc, 0));
+        x[1][4 * t + i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, sc, 1));
+        if constexpr (D == 128) {
+          x[2][4 * t + i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, sc, 2));
+          x[3][4 * t + i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, sc, 3));
+        }
+      }
+#pragma unroll
+    for (int m = 0; m < W; ++m) {
+      u32x4 lo, hi;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        lo[j] = __builtin_amdgcn_perm(x[m][2 * j + 1], x[m][2 * j], 0x05040100u);
+        hi[j] = __builtin_amdgcn_perm(x[m][2 * j + 1], x[m][2 * j], 0x07060302u);
+      }
+#pragma unroll
+      for (int n = 0; n < NQ; ++n) {
+        r.o[n][2 * m] = mfma16(__builtin_bit_cast(bf16x8, lo), p[n][u], r.o[n][2 * m]);
+        r.o[n][2 * m + 1] = mfma16(__builtin_bit_cast(bf16x8, hi), p[n][u], r.o[n][2 * m + 1]);
+      }
+    }
+  }
+}
+
+// Four waves take a tile of 16 NQ rows, every fourth block each; their results meet in LDS.
+template <int D, int NQ>
+__global__ __launch_bounds__(256) void attn_kernel(Args a) {
+  constexpr int LD = D + 4;                                     // (16 lanes a quarter write 16 rows: other banks each)
+  __shared__ float sO[4][16][LD];
+  __shared__ float sM[4][16], sL[4][16];
+  const Item it = a.items[blockIdx.x / a.Hkv];
+  const int h = blockIdx.x % a.Hkv, lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int q = lane & 15, c = lane >> 4;
+  // (an item outside of the rows is dropped)
+  if (it.row < 0 || it.tokens <= 0 || it.row + it.tokens > a.T || it.tokens * a.G > 16 * NQ) return;
+  const int pmin = it.pos, pmax = it.pos + it.tokens - 1;
+  const Blocks list(pmin, pmax, a.window, a.first);
+  const int* bt = a.tables + it.table * a.ts;
+  const int hi = min(it.hi, list.count);
+  Rows<D, NQ> r;
+#pragma unroll
+  for (int n = 0; n < NQ; ++n) {
+    r.lim[n] = load_q<D>(r.q[n], a, it.row, it.tokens, it.pos, h, 16 * n, lane);
+    r.m[n] = -INFINITY;
+    r.l[n] = 0.f;
+#pragma unroll
+    for (int d = 0; d < D / 16; ++d) r.o[n][d] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+  bool bad = false;
+  int v = it.lo + w;
+  if (v < hi) {
+    int pg[4];
+    KFrag<D> kf;
+    VFrag vf;
+    block_pages(bt, list[v], pmax, a.n_pages, pg, bad);
+    load_k<D>(kf, a.kc, a.Hkv, h, pg, lane);
+    load_v<D>(vf, a.vc, a.Hkv, h, pg, lane);
+    for (; v < hi; v += 4) {
+      const int nv = v + 4 < hi ? v + 4 : v;
+      KFrag<D> kn;
+      VFrag vn;
+      block_pages(bt, list[nv], pmax, a.n_pages, pg, bad);
+      load_k<D>(kn, a.kc, a.Hkv, h, pg, lane);
+      load_v<D>(vn, a.vc, a.Hkv, h, pg, lane);
+      block_step<D, NQ>(kf, vf, r, list[v] * KB, pmin, pmax, a.window, a.first, a.scale2, lane);
+      kf = kn;
+      vf = vn;
+    }
+  }
+  const int Hq = a.Hkv * a.G;
+#pragma unroll
+  for (int n = 0; n < NQ; ++n) {
+    const float l = over_quarters_sum(r.l[n]);
+    if (n) __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int d = 0; d < D / 16; d += 4)
+        *reinterpret_cast<f32x4*>(&sO[w][q][(D / 16) * (4 * c + i) + d]) =
+            f32x4{r.o[n][d][i], r.o[n][d + 1][i], r.o[n][d + 2][i], r.o[n][d + 3][i]};
+    if (c == 0) {
+      sM[w][q] = r.m[n];
+      sL[w][q] = bad ? __builtin_nanf("") : l;
+    }
+    __syncthreads();
+    for (int x = threadIdx.x; x < 16 * (D / 8); x += 256) {
+      const int row = x / (D / 8), d0 = (x % (D / 8)) * 8, R = 16 * n + row, tok = R / a.G, g = R - tok * a.G;
+      if (tok >= it.tokens) continue;
+      const float M = vmax(vmax(sM[0][row], sM[1][row]), vmax(sM[2][row], sM[3][row]));
+      float L = 0.f;
+      float o[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float f = M == -INFINITY ? 1.f : fast_exp2(sM[i][row] - M);
+        L += f * sL[i][row];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) o[j] = fmaf(f, sO[i][row][d0 + j], o[j]);
+      }
+      const float inv = L == 0.f ? 0.f : 1.f / L, lse = L == 0.f ? -INFINITY : M + log2f(L);
+      if (it.slot < 0) {
+        bf16x8 y;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) y[j] = (bf16)(o[j] * inv);
+        store_bf16x8(a.out + (int64_t)(it.row + tok) * a.os + (int64_t)(h * a.G + g) * D + d0, y);
+        if (a.lse && d0 == 0) a.lse[(int64_t)(it.row + tok) * Hq + h * a.G + g] = lse;
+      } else {
+        const int64_t at = ((int64_t)it.slot * a.Hkv + h) * (16 * NQ) + R;
+        *reinterpret_cast<f32x4*>(a.part + at * D + d0) = f32x4{o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv};
+        *reinterpret_cast<f32x4*>(a.part + at * D + d0 + 4) = f32x4{o[4] * inv, o[5] * inv, o[6] * inv, o[7] * inv};
+        if (d0 == 0) a.plse[at] = lse;
+      }
+    }
+  }
+}
+
+// Partial results of split tiles. Merge items: first row, rows, first slot, slots.
+template <int D>
+__global__ __launch_bounds__(256) void merge_kernel(Args a, const int* __restrict__ merges, int tile_rows) {
+  const int* it = merges + 4 * (blockIdx.x / a.Hkv);
+  const int row0 = it[0], tokens = it[1], slot0 = it[2], n = it[3];
+  const int h = blockIdx.x % a.Hkv, R = blockIdx.y * (256 / (D / 4)) + threadIdx.x / (D / 4), d0 = (threadIdx.x % (D / 4)) * 4;
+  const int tok = R / a.G, g = R - tok * a.G;
+  if (tok >= tokens || row0 + tokens > a.T || R >= tile_rows) return;
+  const int64_t at = ((int64_t)slot0 * a.Hkv + h) * tile_rows + R, step = (int64_t)a.Hkv * tile_rows;
+  float M = -INFINITY;
+  for (int s = 0; s < n; ++s) M = vmax(M, a.plse[at + s * step]);
+  f32x4 o = {0.f, 0.f, 0.f, 0.f};
+  float L = 0.f;
+  for (int s = 0; s < n; ++s) {
+    const float f = M == -INFINITY ? 0.f : fast_exp2(a.plse[at + s * step] - M);
+    L += f;
+    o += *reinterpret_cast<const f32x4*>(a.part + (at + s * step) * D + d0) * f;
+  }
+  const float inv = L == 0.f ? 0.f : 1.f / L;
+  bf16x4 y;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) y[j] = (bf16)(o[j] * inv);
+  *reinterpret_cast<bf16x4*>(a.out + (int64_t)(row0 + tok) * a.os + (int64_t)(h * a.G + g) * D + d0) = y;
+  if (a.lse && d0 == 0) a.lse[(int64_t)(row0 + tok) * (a.Hkv * a.G) + h * a.G + g] = L == 0.f ? -INFINITY : M + log2f(L);
+}
+
+// ---- weights of the keys ------------------------------------------------------------------------------------------------
+// out[segment][head][key] = base + sum over the segment's rows and the head's queries of 2^(s - lse). Every key is one wave's or one
+// workgroup's, so that no sums meet in memory and a call's result does not depend on their order.
+// Items: first row, rows, position, table row, segment, first block, blocks, 0.
+struct MassArgs {
+  Args a;
+  const float* base;      // may be null, or out
+  float* out;
+  int N;
+};
+
+template <int D, bool SPLIT>
+__global__ __launch_bounds__(256) void mass_kernel(MassArgs ma) {
+  const Args& a = ma.a;
+  __shared__ float sum[4][KB];
+  const int* it = reinterpret_cast<const int*>(a.items) + 8 * (blockIdx.x / a.Hkv);
+  const int row = it[0], rows = it[1], pos = it[2], table = it[3], seg = it[4];
+  const int h = blockIdx.x % a.Hkv, lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int c = lane >> 4, q = lane & 15;
+  if (row < 0 || rows < 0 || row + rows > a.T) return;
+  const int b = SPLIT ? it[5] : it[5] + w, key0 = b * KB, last = pos + rows - 1;
+  if (!SPLIT && b >= it[6]) return;
+  float acc[4][4] = {};
+  const Blocks list(pos, last, a.window, a.first);
+  bool bad = false;
+  if (key0 <= last && (b < list.head || b >= list.tail)) {
+    int pg[4];
+    KFrag<D> kf;
+    block_pages(a.tables + table * a.ts, b, last, a.n_pages, pg, bad);
+    load_k<D>(kf, a.kc, a.Hkv, h, pg, lane);
+    const int Hq = a.Hkv * a.G, R1 = rows * a.G;
+    // rows that may see the block: from its first key's position on (tiles of 16 columns)
+    const int R0 = max(0, (key0 - pos) * a.G) & ~15;
+    for (int R = R0 + (SPLIT ? 16 * w : 0); R < R1; R += SPLIT ? 64 : 16) {
+      const int pmin = pos + R / a.G, pmax = min(pos + (R + 15) / a.G, last);
+      if (key0 + KB <= pmin - a.window + 1 && key0 >= a.first) break;             // (so do all rows after these)
+      bf16x8 qf[1][D / 32];
+      const int lim = load_q<D>(qf[0], a, row, rows, pos, h, R, lane);
+      const int tok = (R + q) / a.G, g = R + q - tok * a.G;
+      float ls = lim >= 0 ? a.lse[(int64_t)(row + tok) * Hq + h * a.G + g] : INFINITY;
+      if (ls == -INFINITY) ls = INFINITY;                                           // (a row that sees nothing gives nothing)
+      f32x4 s[4][1];
+      scores<D, 1>(kf, qf, s);
+      const bool masked = key0 + KB - 1 > pmin || (key0 <= pmax - a.window && key0 + KB > a.first);
+#pragma unroll
+      for (int t = 0; t < 4; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          float e = fast_exp2(fmaf(s[t][0][i], a.scale2, -ls));
+          if ((masked && !sees(key0 + 16 * t + 4 * c + i, lim, a.window, a.first)) || lim < 0) e = 0.f;
+          acc[t][i] += e;
+        }
+    }
+  }
+#pragma unroll
+  for (int t = 0; t < 4; ++t)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      float x = acc[t][i];
+#pragma unroll
+      for (int o = 1; o < 16; o <<= 1) x += __shfl_xor(x, o, 64);
+      acc[t][i] = bad ? __builtin_nanf("") : x;
+    }
+  float mine = 0.f;                      // lane = key of the block: from quarter (key / 4) % 4, register key % 4 of tile key / 16
+#pragma unroll
+  for (int t = 0; t < 4; ++t)
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (q == 0) sum[w][16 * t + 4 * c + i] = acc[t][i];
+  if (SPLIT) {
+    __syncthreads();
+    if (w) return;
+    mine = (sum[0][lane] + sum[1][lane]) + (sum[2][lane] + sum[3][lane]);
+  } else {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    mine = sum[w][lane];
+  }
+  const int key = key0 + lane;
+  if (key < ma.N) {
+    const int64_t at = ((int64_t)seg * a.Hkv + h) * ma.N + key;
+    ma.out[at] = (ma.base ? ma.base[at] : 0.f) + mine;
+  }
+}
+
+}  // namespace kv4
+
+using namespace kv4;
+
+static Args make_args(const bf16* q, int64_t qs, const uint8_t* kc, const uint8_t* vc, int64_t n_pages, const int* tables, int64_t ts,
+                      const int* items, int T, int Hkv, int G, int window, int first, float scale, bf16* out, int64_t os, float* lse,
+                      float* part, float* plse) {
+  return Args{q,   qs, kc,  vc,   n_pages, tables, ts, reinterpret_cast<const Item*>(items), T, Hkv, G, window > 0 ? window : 1 << 30,
+              first, scale * 1.4426950408889634f, out, os, lse, part, plse};
+}
+
+// tiles of 16 nq rows (nq 1, 2)
+extern "C" hipError_t kafka_kv4_attn(const bf16* q, int64_t qs, const uint8_t* kc, const uint8_t* vc, int64_t n_pages, const int* tables,
+                                     int64_t ts, const int* items, int n_items, int nq, const int* merges, int n_merges, int T, int Hkv,
+                                     int G, int D, int window, int first, float scale, bf16* out, int64_t os, float* lse, float* part,
+                                     float* plse, hipStream_t st) {
+  if (n_items == 0) return hipSuccess;
+  if ((D != 64 && D != 128) || (nq != 1 && nq != 2) || G < 1 || G > 16)
+    return hipErrorInvalidValue;
+  const Args a = make_args(q, qs, kc, vc, n_pages, tables, ts, items, T, Hkv, G, window, first, scale, out, os, lse, part, plse);
+  const int64_t wgs = (int64_t)Hkv * n_items, mwgs = (int64_t)Hkv * n_merges;
+  if (wgs >= 1 << 24 || mwgs >= 1 << 24) return hipErrorInvalidValue;
+  const dim3 grid((unsigned)wgs);
+  auto go = [&](auto kern) { kern<<<grid, 256, 0, st>>>(a); };
+  if (D == 128)
+    nq == 1 ? go(attn_kernel<128, 1>) : go(attn_kernel<128, 2>);
+  else
+    nq == 1 ? go(attn_kernel<64, 1>) : go(attn_kernel<64, 2>);
+  if (n_merges) {
+    const int rows = 16 * nq, per = 256 / (D / 4);
+    const dim3 mg((unsigned)mwgs, (rows + per - 1) / per);
+    if (D == 128)
+      merge_kernel<128><<<mg, 256, 0, st>>>(a, merges, rows);
+    else
+      merge_kernel<64><<<mg, 256, 0, st>>>(a, merges, rows);
+  }
+  return hipGetLastError();
+}
+
+// items of segments whose rows one wave takes for a block, then of those that four share
+extern "C" hipError_t kafka_kv4_mass(const bf16* q, int64_t qs, const float* lse, const uint8_t* kc, int64_t n_pages, const int* tables,
+                                     int64_t ts, const int* items, int n_whole, int n_split, int T, int Hkv, int G, int D, int window,
+                                     int first, float scale, const float* base, float* out, int N, hipStream_t st) {
+  if ((D != 64 && D != 128) || G < 1 || G > 16 || (int64_t)Hkv * n_whole >= 1 << 24 || (int64_t)Hkv * n_split >= 1 << 24)
+    return hipErrorInvalidValue;
+  for (int split = 0; split < 2; ++split) {
+    const int n = split ? n_split : n_whole;
+    if (!n) continue;
+    MassArgs m{make_args(q, qs, kc, nullptr, n_pages, tables, ts, items + (split ? 8 * (int64_t)n_whole : 0), T, Hkv, G, window, first,
+                         scale, nullptr, 0, const_cast<float*>(lse), nullptr, nullptr),
+               base, out, N};
+    const dim3 grid((unsigned)(Hkv * n));
+    if (D == 128)
+      split ? mass_kernel<128, true><<<grid, 256, 0, st>>>(m) : mass_kernel<128, false><<<grid, 256, 0, st>>>(m);
+    else
+      split ? mass_kernel<64, true><<<grid, 256, 0, st>>>(m) : mass_kernel<64, false><<<grid, 256, 0, st>>>(m);
+  }
+  return hipGetLastError();
+}
+
+}  // namespace kafka

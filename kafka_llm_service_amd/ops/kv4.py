@@ -1,0 +1,278 @@
+"""Operators of the 4-bit KV cache (``kv_cache_shapes(..., "mx4")``): elements e2m1, one power of two for every 32 elements of a key's or
+value's head vector, 4.25 bits each in all; a sixteenth of the bf16 cache's head dims of 64 and 128, pages of 16 keys (csrc/kv4.h).
+
+  ops.rope_kv_write   writes a step's rows (a cache of this kind given)            csrc/kv4.hip
+  read                keys and values of slots as numbers                          csrc/kv4.hip
+  attn_plan / attn    attention of single tokens and prompt portions over pages,   csrc/kv4_attn.hip
+                      causal, or a window and the first tokens
+  attn_mass           the weight that every cached key has received                csrc/kv4_attn.hip
+  evict_keep / evict  the keys that stay, by their weight; their move to new pages csrc/kv4.hip
+
+Rows of a call are described by segments (first row, rows, position of the first, row of the block table): consecutive tokens of
+one sequence, whose keys lie in the cache at their positions. GPU tensors run the HIP kernels on the caches' device and its current
+stream, CPU tensors the references of ``kv4_reference.py``. Workspaces are made per call, so calls on several streams and captured
+graphs do not meet; a plan holds only tables that the kernels read.
+"""
+from __future__ import annotations
+
+import numpy as np
+import torch
+
+from . import kv4_reference as ref
+from ._ext import ext
+
+PAGE = ref.PAGE
+BLOCK = 64                 # keys that a wave takes at a time
+MAX_POS = 1 << 26
+MAX_GROUP = 16             # query heads for a key/value head
+
+
+def _gpu(t: torch.Tensor) -> bool:
+    return t.is_cuda
+
+
+def _check_cache(k_cache, v_cache, who: str) -> None:
+    for c in (k_cache, v_cache):
+        if c.dtype != torch.uint8 or c.dim() != 4 or c.shape[2] != PAGE or c.shape[3] not in (34, 68) or c.shape != k_cache.shape:
+            raise ValueError(f"{who}: caches of kv_cache_shapes(..., \"mx4\") with head dim 64 or 128 expected")
+
+
+def read(k_cache: torch.Tensor, v_cache: torch.Tensor, slots: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """(K, V) [T, heads, D] bf16 of ``slots`` int64 [T] (page * 16 + key), exactly what the cache holds. Negative slots give zeros,
+    slots behind the cache no numbers."""
+    _check_cache(k_cache, v_cache, "kv4.read")
+    if slots.dim() != 1 or slots.dtype != torch.int64:
+        raise ValueError("kv4.read: slots int64 [T]")
+    if not _gpu(k_cache):
+        return ref.read(k_cache, v_cache, slots)
+    k = torch.empty(slots.shape[0], k_cache.shape[1], ref.head_dim(k_cache), dtype=torch.bfloat16, device=k_cache.device)
+    v = torch.empty_like(k)
+    ext().kv4_read(k_cache, v_cache, slots.contiguous(), k, v)
+    return k, v
+
+
+# ---- plans --------------------------------------------------------------------------------------------------------------
+FEW_ROWS = 16              # rows (tokens x query heads of a group) of a tile for single tokens
+TILE_ROWS = 32             # of a tile for portions
+TARGET_WGS = 1024          # workgroups that a launch of few tiles is split towards
+MIN_BLOCKS = 4             # blocks of a piece: one for each of a workgroup's waves
+MASS_WHOLE_ROWS = 32       # rows of a segment up to which a wave takes them all for its block of keys
+
+
+class AttnPlan:
+    """Work of ``attn`` and ``attn_mass`` for a step's segments (``attn_plan``); every layer of the step uses the same."""
+
+    def __init__(self):
+        self.segs: list[tuple[int, int, int, int]] = []
+        self.heads = self.kv_heads = self.dim = self.window = self.first = 0
+        self.rows = self.covered = self.keys = self.tables = 0
+        self.parts: list = []       # (rows of a tile, items, merges, slots of partial results)
+        self.mass_items = None
+        self.mass_whole = 0
+
+
+def _blocks(pos, tokens, window: int, first: int):
+    """(blocks below the window, blocks in all) that tiles of ``tokens`` rows from ``pos`` on see: csrc/kv4_attn.hip Blocks."""
+    tail = np.maximum(0, pos - window + 1) // BLOCK if window else np.zeros_like(pos)
+    head = np.minimum((first + BLOCK - 1) // BLOCK, tail)
+    return head, head + (pos + tokens - 1) // BLOCK + 1 - tail
+
+
+def _tiles(segs: np.ndarray, tokens: int):
+    """Tiles of at most ``tokens`` rows: int64 [n, 4] (first row, rows, position, table row)."""
+    n = (segs[:, 1] + tokens - 1) // tokens
+    s = np.repeat(np.arange(len(segs)), n)
+    i = (np.arange(len(s)) - np.repeat(np.cumsum(n) - n, n)) * tokens
+    return np.stack([segs[s, 0] + i, np.minimum(segs[s, 1] - i, tokens), segs[s, 2] + i, segs[s, 3]], 1)
+
+
+def _pieces(tiles: np.ndarray, window: int, first: int, kv_heads: int):
+    """(items int32 [n, 8], merges int32 [m, 4], slots): tiles of long ranges in pieces of about the same length, if the tiles by
+    themselves are too few workgroups; the longest first."""
+    _, count = _blocks(tiles[:, 2], tiles[:, 1], window, first)
+    size = max(MIN_BLOCKS, -(-int(count.sum()) * kv_heads // TARGET_WGS))
+    n = np.maximum(1, (count + size - 1) // size)
+    each = (count + n - 1) // n
+    n = np.maximum(1, (count + each - 1) // each)
+    t = np.repeat(np.arange(len(tiles)), n)
+    at = np.cumsum(n) - n
+    i = np.arange(len(t)) - at[t]
+    split = n > 1
+    base = np.cumsum(np.where(split, n, 0)) - np.where(split, n, 0)
+    lo = i * each[t]
+    items = np.stack([tiles[t, 0], tiles[t, 1], tiles[t, 2], tiles[t, 3], lo, np.minimum(lo + each[t], count[t]),
+                      np.where(split[t], base[t] + i, -1), np.zeros_like(t)], 1)
+    items = items[np.argsort(items[:, 4] - items[:, 5], kind="stable")]
+    merges = np.stack([tiles[split, 0], tiles[split, 1], base[split], n[split]], 1)
+    return items.astype(np.int32), merges.astype(np.int32), int(n[split].sum())
+
+
+def attn_plan(segs, heads: int, kv_heads: int, dim: int, window: int = 0, first: int = 0, device="cuda") -> AttnPlan:
+    """Plan for ``segs``, host integers (first row, rows, position of the first, row of the block table) each: the row at position p sees
+    the keys j <= p, with ``window`` > 0 only those with j > p - window or j < ``first``. Rows of different segments are different."""
+    if dim not in (64, 128) or kv_heads < 1 or heads % kv_heads or not 1 <= heads // kv_heads <= MAX_GROUP:
+        raise ValueError("kv4.attn_plan: head dim 64 or 128, 1 to 16 query heads for each key/value head")
+    if window < 0 or first < 0 or window >= 1 << 30 or first >= MAX_POS:
+        raise ValueError("kv4.attn_plan: window and first may not be negative (window 0: every earlier position)")
+    if first and not window:
+        raise ValueError("kv4.attn_plan: first tokens stay visible beside a window")
+    p = AttnPlan()
+    p.segs = [tuple(int(x) for x in s) for s in segs]
+    a = np.array(p.segs, dtype=np.int64).reshape(-1, 4)
+    if (a < 0).any() or (a[:, 0] + a[:, 1] >= MAX_POS).any() or (a[:, 2] + a[:, 1] >= MAX_POS).any() or (a[:, 3] >= 1 << 30).any():
+        raise ValueError("kv4.attn_plan: segments of (first row, rows, position, table row), none negative, positions below 2^26")
+    full = a[a[:, 1] > 0]
+    byrow = full[np.argsort(full[:, 0], kind="stable")]
+    if (byrow[1:, 0] < byrow[:-1, 0] + byrow[:-1, 1]).any():
+        raise ValueError("kv4.attn_plan: a row in two segments")
+    p.heads, p.kv_heads, p.dim, p.window, p.first = heads, kv_heads, dim, int(window), int(first)
+    if len(full):
+        p.rows, p.covered = int((full[:, 0] + full[:, 1]).max()), int(full[:, 1].sum())
+        p.keys, p.tables = int((full[:, 2] + full[:, 1]).max()), int(full[:, 3].max()) + 1
+    dev = torch.device(device)
+    if dev.type != "cuda":
+        return p
+    G = heads // kv_heads
+    few = full[:, 1] * G <= FEW_ROWS
+    tables, shapes = [], []
+    for rows, part in ((FEW_ROWS, full[few]), (TILE_ROWS, full[~few])):
+        if len(part):
+            items, merges, slots = _pieces(_tiles(part, rows // G), p.window, p.first, kv_heads)
+            tables += [items, merges]
+            shapes.append((rows, len(items), len(merges), slots))
+    nb = (p.keys + BLOCK - 1) // BLOCK
+    whole = a[:, 1] * G <= MASS_WHOLE_ROWS
+    mass = []
+    for pick, step in ((whole, 4), (~whole, 1)):
+        idx = np.nonzero(pick)[0]
+        b = np.arange(0, nb, step)
+        s = np.repeat(idx, len(b))
+        b = np.tile(b, len(idx))
+        mass.append(np.stack([a[s, 0], a[s, 1], a[s, 2], a[s, 3], s, b, np.full_like(s, nb), np.zeros_like(s)], 1).astype(np.int32))
+    p.mass_whole = len(mass[0])
+    tables += mass
+    flat = torch.from_numpy(np.concatenate([t.reshape(-1) for t in tables]) if tables else np.zeros(0, np.int32)).to(dev)
+    at = 0
+
+    def take(n, cols):
+        nonlocal at
+        t = flat[at:at + n * cols].view(n, cols)
+        at += n * cols
+        return t
+
+    for rows, n, m, slots in shapes:
+        p.parts.append((rows, take(n, 8), take(m, 4), slots))
+    p.mass_items = take(len(mass[0]) + len(mass[1]), 8)
+    return p
+
+
+def _check_call(q, k_cache, block_tables, plan: AttnPlan, who: str) -> None:
+    if q.dim() != 3 or q.dtype != torch.bfloat16 or q.shape[1] != plan.heads or q.shape[2] != plan.dim or \
+            k_cache.shape[1] != plan.kv_heads or ref.head_dim(k_cache) != plan.dim:
+        raise ValueError(f"{who}: q bf16 [T, heads, dim] and a cache of the plan's heads expected")
+    if q.shape[0] < plan.rows:
+        raise ValueError(f"{who}: the plan has {plan.rows} rows, q {q.shape[0]}")
+    if block_tables.dim() != 2 or block_tables.dtype != torch.int32 or block_tables.shape[0] < plan.tables or \
+            block_tables.shape[1] * PAGE < plan.keys:
+        raise ValueError(f"{who}: int32 block tables of {plan.tables} rows for {plan.keys} keys expected")
+    if _gpu(q) and plan.mass_items is None or _gpu(q) and plan.mass_items.device != q.device:
+        raise ValueError(f"{who}: the plan was made for another device")
+
+
+def attn(q, k_cache, v_cache, block_tables, plan: AttnPlan, scale: float, out=None, lse=None) -> torch.Tensor:
+    """softmax(scale q k^T) v of the plan's rows: q [T, heads, dim] bf16 -> out (a new tensor unless given), the same shape.
+    ``lse`` fp32 [T, heads] gets the base-2 logarithm of each row's sum of 2^(scores in base 2). Rows of no segment are left as they
+    were (zeros in a new ``out``). Rows whose block table names a page outside of the cache come out as no numbers."""
+    _check_cache(k_cache, v_cache, "kv4.attn")
+    _check_call(q, k_cache, block_tables, plan, "kv4.attn")
+    if out is None:
+        out = (torch.empty if plan.covered == q.shape[0] else torch.zeros)(q.shape, dtype=q.dtype, device=q.device)
+    elif out.shape != q.shape or out.dtype != q.dtype:
+        raise ValueError("kv4.attn: out like q expected")
+    if lse is not None and (lse.shape != q.shape[:2] or lse.dtype != torch.float32):
+        raise ValueError("kv4.attn: lse fp32 [T, heads] expected")
+    if not _gpu(q):
+        ref.attn(q, k_cache, v_cache, block_tables, plan.segs, plan.window, plan.first, float(scale), out, lse)
+        return out
+    for rows, items, merges, slots in plan.parts:
+        part = plse = None
+        if slots:
+            n = slots * plan.kv_heads * rows
+            part = torch.empty(n * plan.dim, dtype=torch.float32, device=q.device)
+            plse = torch.empty(n, dtype=torch.float32, device=q.device)
+        ext().kv4_attn(q, k_cache, v_cache, block_tables, items, rows // 16, merges, plan.window, plan.first, float(scale), out, lse, part,
+                       plse, slots)
+    return out
+
+
+def attn_mass(q, lse, k_cache, block_tables, plan: AttnPlan, scale: float, base=None, out=None) -> torch.Tensor:
+    """Weight of every key: out[s, h, j] = base[s, h, j] + the sum over segment s's rows and the query heads of h of
+    2^(score - lse), fp32 [segments, kv heads, keys], with ``lse`` from ``attn`` over the same rows. ``out`` may be ``base``: weights that
+    accumulate from step to step. Without either, a new tensor as wide as the plan's longest sequence. A key's sum is always formed in
+    the same order."""
+    _check_cache(k_cache, k_cache, "kv4.attn_mass")
+    _check_call(q, k_cache, block_tables, plan, "kv4.attn_mass")
+    if lse.shape != q.shape[:2] or lse.dtype != torch.float32:
+        raise ValueError("kv4.attn_mass: lse fp32 [T, heads] expected")
+    like = base if base is not None else out
+    shape = (len(plan.segs), plan.kv_heads, like.shape[2] if like is not None and like.dim() == 3 else plan.keys)
+    for t in (base, out):
+        if t is not None and (t.shape != shape or t.dtype != torch.float32 or not t.is_contiguous() or t.shape[2] < plan.keys):
+            raise ValueError(f"kv4.attn_mass: base and out contiguous fp32 [segments, kv heads, at least {plan.keys}], alike, expected")
+    if out is None:
+        out = torch.empty(shape, dtype=torch.float32, device=q.device)
+    if not _gpu(q):
+        if base is None:
+            out.zero_()
+        elif base is not out:
+            out.copy_(base)
+        ref.attn_mass(q, lse, k_cache, block_tables, plan.segs, plan.window, plan.first, float(scale), out)
+        return out
+    done = -(-plan.keys // BLOCK) * BLOCK
+    if shape[2] > done and base is not out:     # (behind the plan's last block nothing is added)
+        out[:, :, done:].copy_(base[:, :, done:]) if base is not None else out[:, :, done:].zero_()
+    ext().kv4_mass(q, lse, k_cache, block_tables, plan.mass_items, plan.mass_whole, plan.window, plan.first, float(scale), base, out, shape[0])
+    return out
+
+
+# ---- eviction -----------------------------------------------------------------------------------------------------------
+def evict_keep(mass: torch.Tensor, lens: torch.Tensor, budget: int, first: int = 0, recent: int = 0) -> torch.Tensor:
+    """The keys that stay, int32 [sequences, kv heads, budget], ascending, per head: of a sequence of ``lens`` keys the ``first`` ones,
+    the ``recent`` last ones, and of the rest those of the largest ``mass`` [sequences, kv heads, keys] fp32 (equal masses: the
+    lowest index; not a number: after all others). Sequences within the budget keep everything, -1 behind their last."""
+    if mass.dim() != 3 or mass.dtype != torch.float32 or lens.shape != (mass.shape[0],) or lens.dtype != torch.int32 or \
+            lens.device != mass.device:
+        raise ValueError("kv4.evict_keep: mass fp32 [sequences, kv heads, keys] and lens int32 [sequences] on its device expected")
+    if budget < 1 or first < 0 or recent < 0 or first + recent > budget or budget >= MAX_POS:
+        raise ValueError("kv4.evict_keep: first and recent keys within a budget of at least one")
+    if not _gpu(mass):
+        return ref.evict_keep(mass, lens, int(budget), int(first), int(recent))
+    if mass.stride(2) != 1 and mass.shape[2] > 1:
+        mass = mass.contiguous()
+    kept = torch.empty(mass.shape[0], mass.shape[1], int(budget), dtype=torch.int32, device=mass.device)
+    ext().kv4_evict_keep(mass, lens.contiguous(), int(budget), int(first), int(recent), kept)
+    return kept
+
+
+def evict(k_cache, v_cache, block_tables, kept, new_tables, mass=None):
+    """Copies the ``kept`` keys and values (``evict_keep``) of every sequence and head from the pages of ``block_tables`` to those of
+    ``new_tables``, int32 [sequences, pages] both, in order: key i of a head becomes kept[.., i]. The new pages are none of the old ones
+    (which other sequences may share, and which their owner may free afterwards); places behind a sequence's last key are left as they
+    were, as are keys whose index, or whose page, is outside. Returns the kept keys' ``mass`` [sequences, kv heads, budget]
+    (zero behind the last) if it is given, else None."""
+    _check_cache(k_cache, v_cache, "kv4.evict")
+    if kept.dim() != 3 or kept.dtype != torch.int32 or kept.shape[1] != k_cache.shape[1]:
+        raise ValueError("kv4.evict: kept int32 [sequences, kv heads, budget] expected")
+    for t in (block_tables, new_tables):
+        if t.dim() != 2 or t.dtype != torch.int32 or t.shape[0] != kept.shape[0]:
+            raise ValueError("kv4.evict: int32 tables [sequences, pages] expected")
+    if mass is not None and (mass.dim() != 3 or mass.shape[:2] != kept.shape[:2] or mass.dtype != torch.float32):
+        raise ValueError("kv4.evict: mass fp32 [sequences, kv heads, keys] expected")
+    new_mass = torch.empty(kept.shape, dtype=torch.float32, device=kept.device) if mass is not None else None
+    if not _gpu(k_cache):
+        ref.evict_copy(k_cache, v_cache, block_tables, kept, new_tables, mass, new_mass)
+        return new_mass
+    if mass is not None and mass.stride(2) != 1 and mass.shape[2] > 1:
+        mass = mass.contiguous()
+    ext().kv4_evict_copy(k_cache, v_cache, block_tables, kept.contiguous(), new_tables, mass, new_mass)
+    return new_mass

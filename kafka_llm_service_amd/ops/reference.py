@@ -8,12 +8,15 @@ or, for the fp8 cache (kv_dtype="fp8", ops/csrc/rope_kv.hip), uint8 pages
   K page: [num_blocks, Hkv, 16 * D + 32]: e4m3 units [D/32 j][2 h][16 keys][2 s][8 e] holding d = 32j + 16s + 8h + e,
           then int8 exponents: K of key o at 16D + o, V of key o at 16D + 16 + vt_pos(o) (value = e4m3 * 2^e)
   V page: [num_blocks, Hkv, D * 16]: e4m3 V^T [D][16], key o at vt_pos(o).
+or, for the 4-bit cache (kv_dtype="mx4", kv4_reference.py), uint8 pages [num_blocks, Hkv, 16, D/2 + D/32] for K and for V.
 """
 from __future__ import annotations
 
 import math
 
 import torch
+
+from . import kv4_reference as kv4
 
 PAGE = 16
 LOG2E = 1.4426950408889634
@@ -34,10 +37,16 @@ FP8_EXP_MIN, FP8_EXP_MAX = -100, 100
 
 
 def is_fp8_cache(k_cache: torch.Tensor) -> bool:
-    return k_cache.dtype == torch.uint8
+    return k_cache.dtype == torch.uint8 and k_cache.dim() == 3
+
+
+def is_mx4_cache(k_cache: torch.Tensor) -> bool:
+    return k_cache.dtype == torch.uint8 and k_cache.dim() == 4
 
 
 def cache_head_dim(k_cache: torch.Tensor, v_cache: torch.Tensor) -> int:
+    if is_mx4_cache(k_cache):
+        return kv4.head_dim(k_cache)
     return v_cache.shape[-1] // PAGE if is_fp8_cache(k_cache) else k_cache.shape[-1]
 
 
@@ -45,13 +54,19 @@ def kv_cache_shapes(num_blocks: int, hkv: int, D: int, kv_dtype: str = "bf16"):
     """(K shape, V shape, torch dtype) of one layer's paged cache."""
     if kv_dtype == "fp8":
         return (num_blocks, hkv, PAGE * D + 32), (num_blocks, hkv, D * PAGE), torch.uint8
+    if kv_dtype == "mx4":
+        if D not in (64, 128):
+            raise ValueError(f"kv_dtype mx4 takes head dims of 64 and 128, not {D}")
+        return (num_blocks, hkv, PAGE, D // 2 + D // 32), (num_blocks, hkv, PAGE, D // 2 + D // 32), torch.uint8
     if kv_dtype != "bf16":
-        raise ValueError(f"kv_dtype must be bf16 or fp8, not {kv_dtype!r}")
+        raise ValueError(f"kv_dtype must be bf16, fp8 or mx4, not {kv_dtype!r}")
     return (num_blocks, hkv, PAGE, D), (num_blocks, hkv, D, PAGE), torch.bfloat16
 
 
 def kv_page_bytes(hkv: int, D: int, kv_dtype: str = "bf16") -> int:
     """Bytes of K + V for one 16-token page of one layer."""
+    if kv_dtype == "mx4":
+        return hkv * 2 * PAGE * (D // 2 + D // 32)
     return hkv * (2 * PAGE * D + 32) if kv_dtype == "fp8" else hkv * 2 * PAGE * D * 2
 
 
@@ -140,6 +155,10 @@ def rope_kv_write(qkv, positions, cos_sin, q_out, k_cache, v_cache, slot_mapping
     q_out.copy_(rot[:, :Hq])
     if slot_mapping is None:
         return
+    if is_mx4_cache(k_cache):
+        kv4.store(rot32[:, Hq:].bfloat16(), k_cache, slot_mapping, False)
+        kv4.store(x[:, Hq + Hkv:], v_cache, slot_mapping, True)
+        return
     if is_fp8_cache(k_cache):
         kq, ke = fp8_quant(rot32[:, Hq:])
         vq, ve = fp8_quant(x[:, Hq + Hkv:])
@@ -167,6 +186,8 @@ def rope_kv_write(qkv, positions, cos_sin, q_out, k_cache, v_cache, slot_mapping
 
 def gather_kv(k_cache, v_cache, block_table, length: int):
     """Materialise [length, Hkv, D] K and V for one sequence from the paged caches (fp32)."""
+    if is_mx4_cache(k_cache):
+        return kv4.gather(k_cache, v_cache, block_table, length)
     nb = (length + PAGE - 1) // PAGE
     ids = block_table[:nb].long()
     if is_fp8_cache(k_cache):
