@@ -90,8 +90,8 @@ def parse(argv=None):
     ap.add_argument("--no-graphs", dest="graphs", action="store_false")
     ap.add_argument("--kv-run-pages", type=int, default=1,
                     help="KV pages handed out per growth step in consecutive runs (EngineConfig.kv_run_pages)")
-    ap.add_argument("--kv-dtype", default="bf16", choices=["bf16", "fp8"],
-                    help="paged KV cache precision (fp8 = e4m3 + per-token scales; an opt-in A/B, not the headline)")
+    ap.add_argument("--kv-dtype", default="bf16", choices=["bf16", "fp8", "mx4"],
+                    help="paged KV cache precision (fp8 = e4m3 + per-token scales, mx4 = 4 bits + a scale per 32; opt-in A/Bs, not the headline)")
     ap.add_argument("--seed", type=int, default=0)
     ap.add_argument("--json-out", default=None)
     ap.add_argument("--arch-compare", action="store_true",

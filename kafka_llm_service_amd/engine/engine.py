@@ -60,7 +60,9 @@ class EngineConfig:
     # step there), off at TP = 1 (the host already runs a step ahead: measured no faster, profiles/r02/graphs_ab_*)
     use_graphs: bool | None = None
     # paged KV cache: "bf16", or "fp8" = e4m3 with one power-of-two scale per (token, kv head) for K and for V
-    # (half the bytes per page: twice the pages, half the decode attention traffic; ops/csrc/rope_kv.hip)
+    # (half the bytes per page: twice the pages, half the decode attention traffic; ops/csrc/rope_kv.hip), or "mx4" = 4 bits with one
+    # power-of-two scale per 32 elements (3.8 times the pages; steps are not captured into graphs, prefixes are shared page by
+    # page but read by every row for itself; ops/kv4.py)
     kv_dtype: str = "bf16"
     # decode GEMMs: "stream" = weight-streaming MFMA kernel on wave-tiled weight copies (csrc/wstream_gemm.hip),
     # "blas" = hipBLASLt only; "auto" = stream on GPU (env KAFKA_DECODE_GEMM overrides)
@@ -204,7 +206,9 @@ class LLMEngine:
         if cfg.use_graphs is None:  # env KAFKA_GRAPHS=0/1 overrides the default (on for TP > 1 on GPUs)
             env = os.environ.get("KAFKA_GRAPHS")
             cfg.use_graphs = (env == "1") if env in ("0", "1") else (cfg.tp > 1 and self.device.type == "cuda")
-            cfg.use_graphs = cfg.use_graphs and self.device.type == "cuda"
+            cfg.use_graphs = cfg.use_graphs and self.device.type == "cuda" and cfg.kv_dtype != "mx4"
+        if cfg.use_graphs and self.runner.mx4:
+            raise ValueError("kv_dtype mx4: steps are planned by their lengths, not captured into graphs")
         if cfg.use_graphs:
             from kafka_llm_service_amd.engine.graphs import DecodeGraphs
 

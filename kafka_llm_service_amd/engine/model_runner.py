@@ -24,6 +24,7 @@ from kafka_llm_service_amd.engine.logits_proc import LogitsProcessor, ProcUpdate
 from kafka_llm_service_amd.engine.scheduler import ScheduledBatch
 from kafka_llm_service_amd.engine.sequence import Sequence
 from kafka_llm_service_amd.models.attention import AttnMeta
+from kafka_llm_service_amd.ops import kv4
 from kafka_llm_service_amd.models.llama import StepInput, TransformerLM
 
 PAGE = 16
@@ -585,9 +586,12 @@ class ModelRunner:
             self._init_common(max_num_seqs)
             return
         self.G = model.hq // model.hkv
+        # the cache in 4 bits has an attention of its own (ops.kv4: no cascade, no tile variants); CPU runs take the references' items
+        self.mx4 = self.device.type == "cuda" and bool(k_caches) and ops.is_mx4_cache(k_caches[0])
+        use_cascade = use_cascade and not self.mx4
         # tile-kernel variant (ops.tile_rows): 3 = LDS-DMA kernel (csrc/attn_tile.hip, 256 query rows an item on 8 waves
         # or on two workgroups of 4, bf16 pages); 0 = register-staged 8 waves x 256 rows (fp8 pages); 1 = 4 waves x 128 rows
-        fp8 = bool(k_caches) and ops.is_fp8_cache(k_caches[0])
+        fp8 = bool(k_caches) and k_caches[0].dtype == torch.uint8
         self.variant = int(os.environ.get("KAFKA_TILE_VARIANT", "0" if fp8 else "3"))
         if fp8 and self.variant == 3:
             raise ValueError("tile variant 3 reads bf16 KV pages only")
@@ -634,7 +638,7 @@ class ModelRunner:
 
     def _init_common(self, max_num_seqs: int) -> None:
         """The runner state every plan kind needs (a segment-planned model has no tile variants or cascade)."""
-        self.variant, self.pad_rows, self.use_cascade, self.graphs = 0, False, False, None
+        self.variant, self.pad_rows, self.use_cascade, self.graphs, self.mx4 = 0, False, False, None, False
         self.vocab = self.model.cfg.vocab_size
         self._pin = self.device.type == "cuda"
         self.last_stats = {}
@@ -799,6 +803,16 @@ class ModelRunner:
         h = HostStep(B=B, T=T, nbt=nbt, bt_w=bt_w, bt_need=min(need, bt_w), n_rows=len(logit_rows), patch=patch,
                      owners=owners)
         i32_parts = [bt.reshape(-1), q_limit]
+        if self.mx4:
+            segs = [(i, 1, int(n) - 1, i) for i, n in enumerate(seq_lens)]
+            r = B
+            for j, (_, a, b) in enumerate(pre):
+                segs.append((r, b - a, a, B + j))
+                r += b - a
+            h.i64 = np.concatenate([tokens, positions, slots, np.asarray(logit_rows, dtype=np.int64)])
+            h.i32 = np.concatenate(i32_parts + [kv4.step_tables(segs, self.model.hq, self.model.hkv, self.model.D)])
+            h.stats = {"B": B, "T": T, "segments": len(segs)}
+            return h, sample_seqs
         # new-turn prefill chunks whose block table starts with a cascade group's prefix pages (the ~18k shared
         # system prompt every new turn of a thread re-attends): their tokens join the group's prefix pass — one read
         # of the prefix pages per step for all rows — and their own tiles attend only the keys behind the prefix
@@ -1074,7 +1088,9 @@ class ModelRunner:
         meta.q_limit = d32[o:o + T]
         o += T
         Hq, D = self.model.hq, self.model.D
-        if B:
+        if self.mx4:
+            meta.plan = kv4.step_plan(h.i32[o:], d32[o:], Hq, self.model.hkv, D)
+        elif B:
             meta.decode_items = d32[o:o + h.n_dec_items * 8].view(-1, 8)
             o += h.n_dec_items * 8
             if h.n_prefix_items:

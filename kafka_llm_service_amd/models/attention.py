@@ -14,6 +14,8 @@ chunk tokens. Per layer:
     group's prefix rides in the group's prefix pass twice over: its prefix pieces and its own keys' pieces are items
     of the same launch (model_runner.build_host ``join_suffix``), leaving only the merge.
 
+On a cache in 4 bits (``plan``) all rows of the step go through ``ops.kv4.attn``.
+
 ``AttnMeta`` holds only device tensors that the model runner prepares once per step (shared by all layers), so
 the decode path is hipGraph-capturable (fixed shapes per batch bucket).
 """
@@ -58,6 +60,7 @@ class AttnMeta:
     alt_lse: torch.Tensor | None = None
     alt_off: int = 0
     prefix_joined: bool = False                # prefill rows take part in the cascade prefix pass (alt partials)
+    plan: object | None = None                 # ops.kv4.AttnPlan: all rows of a step on a cache in 4 bits
     scale: float = 1.0
     variant: int = 0                           # tile-kernel variant (ops.tile_rows): 0 = 8 waves / 256 rows
     extra: dict = field(default_factory=dict)
@@ -78,6 +81,9 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
                     out: torch.Tensor) -> None:
     """q [T, Hq, D] (post-RoPE) -> out [T, Hq, D] bf16."""
     B = meta.num_decode
+    if meta.plan is not None:
+        ops.kv4.attn(q, k_cache, v_cache, meta.block_tables, meta.plan, meta.scale, out=out)
+        return
     if B > 0 and meta.row_parts is not None:
         # prefix items and decode items (and the new turns' rows that they cover) in one launch
         n = meta.row_parts.numel()

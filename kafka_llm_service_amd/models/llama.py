@@ -311,7 +311,7 @@ class TransformerLM:
             lw0 = self.layers[0]
             ok = all(lw.router is None and lw.glu and lw.qkv_t is not None and lw.o_t is not None and
                      lw.down_t is not None for lw in self.layers)
-            self._fused_shapes = ok and self.D == 128 and not ops.is_fp8_cache(k_caches[0]) and \
+            self._fused_shapes = ok and self.D == 128 and k_caches[0].dtype == torch.bfloat16 and \
                 ops.stream_plan(1, self.cfg.hidden_size, lw0.down_t.shape[1] * 16) is not None
         if not self._fused_shapes:
             return False

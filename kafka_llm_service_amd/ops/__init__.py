@@ -18,6 +18,7 @@ from functools import lru_cache
 import numpy as np
 import torch
 
+from . import kv4
 from . import reference as ref
 from ._ext import ext
 

@@ -154,7 +154,7 @@ void evict_copy(Tensor kc, Tensor vc, Tensor tables, Tensor kept, Tensor new_tab
 
 const int* ints(const Tensor& t, const Tensor& home, int64_t cols, const char* name) {
   on(t, home, at::kInt, name);
-  TORCH_CHECK(t.dim() == 2 && t.size(1) == cols && t.is_contiguous() && aligned(t) && t.size(0) < 1 << 24, name, ": plan");
+  TORCH_CHECK(t.dim() == 2 && t.size(1) == cols && t.is_contiguous() && t.size(0) < 1 << 24, name, ": plan");
   return t.data_ptr<int>();
 }
 

@@ -107,9 +107,31 @@ def _pieces(tiles: np.ndarray, window: int, first: int, kv_heads: int):
     return items.astype(np.int32), merges.astype(np.int32), int(n[split].sum())
 
 
-def attn_plan(segs, heads: int, kv_heads: int, dim: int, window: int = 0, first: int = 0, device="cuda") -> AttnPlan:
-    """Plan for ``segs``, host integers (first row, rows, position of the first, row of the block table) each: the row at position p sees
-    the keys j <= p, with ``window`` > 0 only those with j > p - window or j < ``first``. Rows of different segments are different."""
+def _tables(full: np.ndarray, heads: int, kv_heads: int, window: int, first: int):
+    """(shapes, arrays) of ``attn``: for single tokens and for portions (rows of a tile, items, merges, slots), and their items and merges."""
+    G = heads // kv_heads
+    few = full[:, 1] * G <= FEW_ROWS
+    shapes, arrays = [], []
+    for rows, part in ((FEW_ROWS, full[few]), (TILE_ROWS, full[~few])):
+        if len(part):
+            items, merges, slots = _pieces(_tiles(part, rows // G), window, first, kv_heads)
+            shapes.append((rows, len(items), len(merges), slots))
+            arrays += [items, merges]
+    return shapes, arrays
+
+
+class _Take:
+    """Tables one behind the other in a flat int32 tensor."""
+
+    def __init__(self, flat: torch.Tensor):
+        self.flat, self.at = flat, 0
+
+    def __call__(self, n: int, cols: int) -> torch.Tensor:
+        self.at += n * cols
+        return self.flat[self.at - n * cols:self.at].view(n, cols)
+
+
+def _plan(segs, heads: int, kv_heads: int, dim: int, window: int, first: int) -> tuple[AttnPlan, np.ndarray]:
     if dim not in (64, 128) or kv_heads < 1 or heads % kv_heads or not 1 <= heads // kv_heads <= MAX_GROUP:
         raise ValueError("kv4.attn_plan: head dim 64 or 128, 1 to 16 query heads for each key/value head")
     if window < 0 or first < 0 or window >= 1 << 30 or first >= MAX_POS:
@@ -117,8 +139,8 @@ def attn_plan(segs, heads: int, kv_heads: int, dim: int, window: int = 0, first:
     if first and not window:
         raise ValueError("kv4.attn_plan: first tokens stay visible beside a window")
     p = AttnPlan()
-    p.segs = [tuple(int(x) for x in s) for s in segs]
-    a = np.array(p.segs, dtype=np.int64).reshape(-1, 4)
+    a = np.array([tuple(int(x) for x in s) for s in segs], dtype=np.int64).reshape(-1, 4)
+    p.segs = [tuple(s) for s in a.tolist()]
     if (a < 0).any() or (a[:, 0] + a[:, 1] >= MAX_POS).any() or (a[:, 2] + a[:, 1] >= MAX_POS).any() or (a[:, 3] >= 1 << 30).any():
         raise ValueError("kv4.attn_plan: segments of (first row, rows, position, table row), none negative, positions below 2^26")
     full = a[a[:, 1] > 0]
@@ -129,40 +151,53 @@ def attn_plan(segs, heads: int, kv_heads: int, dim: int, window: int = 0, first:
     if len(full):
         p.rows, p.covered = int((full[:, 0] + full[:, 1]).max()), int(full[:, 1].sum())
         p.keys, p.tables = int((full[:, 2] + full[:, 1]).max()), int(full[:, 3].max()) + 1
+    return p, a
+
+
+def attn_plan(segs, heads: int, kv_heads: int, dim: int, window: int = 0, first: int = 0, device="cuda") -> AttnPlan:
+    """Plan for ``segs``, host integers (first row, rows, position of the first, row of the block table) each: the row at position p sees
+    the keys j <= p, with ``window`` > 0 only those with j > p - window or j < ``first``. Rows of different segments are different."""
+    p, a = _plan(segs, heads, kv_heads, dim, window, first)
     dev = torch.device(device)
     if dev.type != "cuda":
         return p
-    G = heads // kv_heads
-    few = full[:, 1] * G <= FEW_ROWS
-    tables, shapes = [], []
-    for rows, part in ((FEW_ROWS, full[few]), (TILE_ROWS, full[~few])):
-        if len(part):
-            items, merges, slots = _pieces(_tiles(part, rows // G), p.window, p.first, kv_heads)
-            tables += [items, merges]
-            shapes.append((rows, len(items), len(merges), slots))
+    shapes, arrays = _tables(a[a[:, 1] > 0], heads, kv_heads, p.window, p.first)
     nb = (p.keys + BLOCK - 1) // BLOCK
-    whole = a[:, 1] * G <= MASS_WHOLE_ROWS
+    whole = a[:, 1] * (heads // kv_heads) <= MASS_WHOLE_ROWS
     mass = []
     for pick, step in ((whole, 4), (~whole, 1)):
-        idx = np.nonzero(pick)[0]
-        b = np.arange(0, nb, step)
-        s = np.repeat(idx, len(b))
-        b = np.tile(b, len(idx))
+        idx, b = np.nonzero(pick)[0], np.arange(0, nb, step)
+        s, b = np.repeat(idx, len(b)), np.tile(b, len(idx))
         mass.append(np.stack([a[s, 0], a[s, 1], a[s, 2], a[s, 3], s, b, np.full_like(s, nb), np.zeros_like(s)], 1).astype(np.int32))
-    p.mass_whole = len(mass[0])
-    tables += mass
-    flat = torch.from_numpy(np.concatenate([t.reshape(-1) for t in tables]) if tables else np.zeros(0, np.int32)).to(dev)
-    at = 0
+    take = _Take(torch.from_numpy(np.concatenate([t.reshape(-1) for t in arrays + mass])).to(dev))
+    p.parts = [(rows, take(n, 8), take(m, 4), slots) for rows, n, m, slots in shapes]
+    p.mass_whole, p.mass_items = len(mass[0]), take(len(mass[0]) + len(mass[1]), 8)
+    return p
 
-    def take(n, cols):
-        nonlocal at
-        t = flat[at:at + n * cols].view(n, cols)
-        at += n * cols
-        return t
 
-    for rows, n, m, slots in shapes:
-        p.parts.append((rows, take(n, 8), take(m, 4), slots))
-    p.mass_items = take(len(mass[0]) + len(mass[1]), 8)
+STEP_PARTS = 2             # kinds of tiles that a step may have
+
+
+def step_tables(segs, heads: int, kv_heads: int, dim: int) -> np.ndarray:
+    """The plan of an engine step as one int32 array, for its upload: what ``step_plan`` reads on the host, then the tables."""
+    p, a = _plan(segs, heads, kv_heads, dim, 0, 0)
+    shapes, arrays = _tables(a[a[:, 1] > 0], heads, kv_heads, 0, 0)
+    head = np.zeros(4 + 4 * STEP_PARTS, dtype=np.int32)
+    head[:4] = p.rows, p.covered, p.keys, p.tables
+    for i, s in enumerate(shapes):
+        head[4 + 4 * i:8 + 4 * i] = s
+    return np.concatenate([head] + [t.reshape(-1) for t in arrays])
+
+
+def step_plan(host: np.ndarray, device: torch.Tensor, heads: int, kv_heads: int, dim: int) -> AttnPlan:
+    """The ``attn`` plan in ``step_tables``' array and its copy on the device (no segments are kept: ``attn_mass`` has a plan of its own)."""
+    p = AttnPlan()
+    p.heads, p.kv_heads, p.dim = heads, kv_heads, dim
+    p.rows, p.covered, p.keys, p.tables = (int(x) for x in host[:4])
+    take = _Take(device[4 + 4 * STEP_PARTS:])
+    for rows, n, m, slots in host[4:4 + 4 * STEP_PARTS].reshape(-1, 4).tolist():
+        if rows:
+            p.parts.append((rows, take(n, 8), take(m, 4), slots))
     return p
 
 
@@ -175,7 +210,7 @@ def _check_call(q, k_cache, block_tables, plan: AttnPlan, who: str) -> None:
     if block_tables.dim() != 2 or block_tables.dtype != torch.int32 or block_tables.shape[0] < plan.tables or \
             block_tables.shape[1] * PAGE < plan.keys:
         raise ValueError(f"{who}: int32 block tables of {plan.tables} rows for {plan.keys} keys expected")
-    if _gpu(q) and plan.mass_items is None or _gpu(q) and plan.mass_items.device != q.device:
+    if _gpu(q) and plan.rows and (not plan.parts or plan.parts[0][1].device != q.device):
         raise ValueError(f"{who}: the plan was made for another device")
 
 
@@ -214,6 +249,8 @@ def attn_mass(q, lse, k_cache, block_tables, plan: AttnPlan, scale: float, base=
     _check_call(q, k_cache, block_tables, plan, "kv4.attn_mass")
     if lse.shape != q.shape[:2] or lse.dtype != torch.float32:
         raise ValueError("kv4.attn_mass: lse fp32 [T, heads] expected")
+    if _gpu(q) and (plan.mass_items is None or plan.mass_items.device != q.device):
+        raise ValueError("kv4.attn_mass: a plan of attn_plan for this device expected")
     like = base if base is not None else out
     shape = (len(plan.segs), plan.kv_heads, like.shape[2] if like is not None and like.dim() == 3 else plan.keys)
     for t in (base, out):

@@ -656,3 +656,70 @@ def test_refusals_on_the_gpu(cuda):
         ops.rope_kv_write(torch.zeros(2, 100, dtype=torch.bfloat16, device=cuda), torch.zeros(2, dtype=torch.long, device=cuda),
                           torch.zeros(9, 128, device=cuda), q, kc, vc, None, 8, 2)
     kv4.attn(q, kc, vc, bt, plan, 0.1)
+
+
+# ---- engine ---------------------------------------------------------------------------------------------------------------
+def _dense(model, tokens):
+    """Logits of the dense model in fp32 whose keys and values stand for what the cache holds of them."""
+    from kafka_llm_service_amd.models import oracle as orc
+
+    cfg, D, hq, hkv = model.cfg, model.D, model.hq, model.hkv
+    t = torch.tensor(tokens, device=model.device)
+    T = t.shape[0]
+    cs = model.cos_sin[:T].float()
+    h = model.embed[t].float()
+    see = torch.ones(T, T, dtype=torch.bool, device=h.device).tril()
+    four = lambda x: kref.values(*kref.quant(x))
+    for lw in model.layers:
+        qkv = orc._lin(orc._rms(h, lw.input_norm, cfg.rms_norm_eps), lw.qkv).view(T, hq + 2 * hkv, D)
+        q, k, v = orc._rope(qkv[:, :hq], cs), four(orc._rope(qkv[:, hq:hq + hkv], cs)), four(qkv[:, hq + hkv:])
+        o = torch.empty(T, hq, D, device=h.device)
+        for x in range(hq):
+            s = (q[:, x] @ k[:, x * hkv // hq].T.contiguous() * model.scale).masked_fill(~see, -math.inf)
+            o[:, x] = torch.softmax(s, -1) @ v[:, x * hkv // hq].contiguous()
+        h = h + orc._lin(o.view(T, -1), lw.o)
+        gu = orc._lin(orc._rms(h, lw.post_norm, cfg.rms_norm_eps), lw.gate_up)
+        f = gu.shape[-1] // 2
+        h = h + orc._lin(torch.nn.functional.silu(gu[:, :f]) * gu[:, f:], lw.down)
+    return orc._lin(orc._rms(h, model.final_norm, cfg.rms_norm_eps), model.lm_head)[:, :cfg.vocab_size]
+
+
+def _engine(model, device, gap):
+    """Every greedy token is the oracle's best within ``gap`` of its logits, as with the other caches; prefixes are shared."""
+    from kafka_llm_service_amd.engine.engine import EngineConfig, LLMEngine
+    from kafka_llm_service_amd.engine.sequence import SamplingParams
+
+    eng = LLMEngine(EngineConfig(model=model, device=device, num_kv_blocks=1024, max_model_len=4096, kv_dtype="mx4"))
+    assert ops.is_mx4_cache(eng.runner.k_caches[0])
+    g = torch.Generator().manual_seed(11)
+    pre = torch.randint(0, 5000, (130,), generator=g).tolist()
+    prompts = [pre + torch.randint(0, 5000, (n,), generator=g).tolist() for n in (3, 60, 150, 7)]
+    sp = SamplingParams(temperature=0.0, max_tokens=6, ignore_eos=True)
+    for _ in range(2):                                      # (the second time behind cached prefixes)
+        for p, o in zip(prompts, eng.generate(prompts, sp)):
+            assert len(o) == 6
+            lg = _dense(eng.model, p + o).cpu()
+            for i, tok in enumerate(o):
+                row = lg[len(p) - 1 + i]
+                assert (row.max() - row[tok]).item() < gap, f"token {i}: gap {(row.max() - row[tok]).item():.3f}"
+
+
+def test_engine_cpu():
+    _engine("tiny-llama", "cpu", 0.15)
+
+
+@pytest.mark.gpu
+def test_engine_on_the_gpu(cuda):
+    _engine("small-llama", str(cuda), 0.25)
+
+
+def test_step_plan_is_the_plan():
+    """An engine step's tables, as uploaded, are those of attn_plan."""
+    segs = [(0, 1, 500, 0), (1, 1, 33, 1), (2, 77, 9, 2), (79, 3, 4000, 3)]
+    flat = kv4.step_tables(segs, 8, 2, 128)
+    p = kv4.step_plan(flat, torch.from_numpy(flat), 8, 2, 128)
+    shapes, arrays = kv4._tables(kv4._plan(segs, 8, 2, 128, 0, 0)[1], 8, 2, 0, 0)
+    assert [(r, len(i), len(m), s) for r, i, m, s in p.parts] == shapes
+    for (_, items, merges, _), (a, b) in zip(p.parts, zip(arrays[::2], arrays[1::2])):
+        assert (items.numpy() == a).all() and (merges.numpy() == b).all()
+    assert (p.rows, p.covered, p.keys, p.tables) == (82, 82, 4003, 4)
