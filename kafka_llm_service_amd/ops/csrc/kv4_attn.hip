@@ -448,6 +448,20 @@ static Args make_args(const bf16* q, int64_t qs, const uint8_t* kc, const uint8_
               first, scale * 1.4426950408889634f, out, os, lse, part, plse};
 }
 
+extern "C" hipError_t kafka_kv4_merge(const int* merges, int n_merges, int tile_rows, int T, int Hkv, int G, int D, bf16* out, int64_t os,
+                                      float* lse, float* part, float* plse, hipStream_t st) {
+  const int per = 256 / (D / 4);
+  const int64_t wgs = (int64_t)Hkv * n_merges;
+  if ((D != 64 && D != 128) || wgs >= 1 << 24) return hipErrorInvalidValue;
+  const Args a = make_args(nullptr, 0, nullptr, nullptr, 0, nullptr, 0, nullptr, T, Hkv, G, 0, 0, 1.f, out, os, lse, part, plse);
+  const dim3 grid((unsigned)wgs, (tile_rows + per - 1) / per);
+  if (D == 128)
+    merge_kernel<128><<<grid, 256, 0, st>>>(a, merges, tile_rows);
+  else
+    merge_kernel<64><<<grid, 256, 0, st>>>(a, merges, tile_rows);
+  return hipGetLastError();
+}
+
 // tiles of 16 nq rows (nq 1, 2)
 extern "C" hipError_t kafka_kv4_attn(const bf16* q, int64_t qs, const uint8_t* kc, const uint8_t* vc, int64_t n_pages, const int* tables,
                                      int64_t ts, const int* items, int n_items, int nq, const int* merges, int n_merges, int T, int Hkv,
@@ -457,22 +471,15 @@ extern "C" hipError_t kafka_kv4_attn(const bf16* q, int64_t qs, const uint8_t* k
   if ((D != 64 && D != 128) || (nq != 1 && nq != 2) || G < 1 || G > 16)
     return hipErrorInvalidValue;
   const Args a = make_args(q, qs, kc, vc, n_pages, tables, ts, items, T, Hkv, G, window, first, scale, out, os, lse, part, plse);
-  const int64_t wgs = (int64_t)Hkv * n_items, mwgs = (int64_t)Hkv * n_merges;
-  if (wgs >= 1 << 24 || mwgs >= 1 << 24) return hipErrorInvalidValue;
+  const int64_t wgs = (int64_t)Hkv * n_items;
+  if (wgs >= 1 << 24) return hipErrorInvalidValue;
   const dim3 grid((unsigned)wgs);
   auto go = [&](auto kern) { kern<<<grid, 256, 0, st>>>(a); };
   if (D == 128)
     nq == 1 ? go(attn_kernel<128, 1>) : go(attn_kernel<128, 2>);
   else
     nq == 1 ? go(attn_kernel<64, 1>) : go(attn_kernel<64, 2>);
-  if (n_merges) {
-    const int rows = 16 * nq, per = 256 / (D / 4);
-    const dim3 mg((unsigned)mwgs, (rows + per - 1) / per);
-    if (D == 128)
-      merge_kernel<128><<<mg, 256, 0, st>>>(a, merges, rows);
-    else
-      merge_kernel<64><<<mg, 256, 0, st>>>(a, merges, rows);
-  }
+  if (n_merges) return kafka_kv4_merge(merges, n_merges, 16 * nq, T, Hkv, G, D, out, os, lse, part, plse, st);
   return hipGetLastError();
 }
 

@@ -19,6 +19,10 @@ hipError_t kafka_kv4_evict_copy(uint8_t* kc, uint8_t* vc, int64_t n_pages, const
 hipError_t kafka_kv4_attn(const void* q, int64_t qs, const uint8_t* kc, const uint8_t* vc, int64_t n_pages, const int* tables, int64_t ts,
                           const int* items, int n_items, int nq, const int* merges, int n_merges, int T, int Hkv, int G, int D, int window,
                           int first, float scale, void* out, int64_t os, float* lse, float* part, float* plse, hipStream_t st);
+hipError_t kafka_kv4_tiles(const void* q, int64_t qs, const uint8_t* kc, const uint8_t* vc, int64_t n_pages, const int* tables, int64_t ts,
+                           const int* items, int n_items, const int* wtiles, int n_wtiles, const int* merges, int n_merges, int T, int Hkv,
+                           int G, int D, int window, int first, float scale, void* out, int64_t os, float* lse, float* part, float* plse,
+                           char* ws, hipStream_t st);
 hipError_t kafka_kv4_mass(const void* q, int64_t qs, const float* lse, const uint8_t* kc, int64_t n_pages, const int* tables, int64_t ts,
                           const int* items, int n_whole, int n_split, int T, int Hkv, int G, int D, int window, int first, float scale,
                           const float* base, float* out, int N, hipStream_t st);
@@ -158,8 +162,9 @@ const int* ints(const Tensor& t, const Tensor& home, int64_t cols, const char* n
   return t.data_ptr<int>();
 }
 
-void attn(Tensor q, Tensor kc, Tensor vc, Tensor tables, Tensor items, int64_t nq, Tensor merges, int64_t window, int64_t first, double scale,
-          Tensor out, OptT lse, OptT part, OptT plse, int64_t slots) {
+// ``rows`` of a tile; ``wtiles``, ``ws``: what of the cache is widened first, and where to
+void attn(Tensor q, Tensor kc, Tensor vc, Tensor tables, int64_t rows, Tensor items, Tensor merges, int64_t window, int64_t first, double scale,
+          Tensor out, OptT lse, OptT part, OptT plse, int64_t slots, OptT wtiles, OptT ws) {
   const int D = caches(kc, vc);
   const c10::DeviceGuard guard(kc.device());
   const int64_t T = q.size(0), Hq = q.dim() == 3 ? q.size(1) : 0, H = kc.size(1);
@@ -167,7 +172,7 @@ void attn(Tensor q, Tensor kc, Tensor vc, Tensor tables, Tensor items, int64_t n
   rows3(out, kc, T, Hq, D, "out");
   TORCH_CHECK(Hq > 0 && Hq % H == 0 && Hq / H <= 16 && T < 1 << 26, "attn: 1 to 16 query heads for each key/value head");
   const int* tp = table(tables, kc, "block_tables");
-  const int *ip = ints(items, kc, 8, "items"), *mp = ints(merges, kc, 4, "merges");
+  const int *ip = ints(items, kc, wtiles.has_value() ? 12 : 8, "items"), *mp = ints(merges, kc, 4, "merges");
   float *lp = nullptr, *pp = nullptr, *pl = nullptr;
   if (lse.has_value()) {
     on(*lse, kc, at::kFloat, "lse");
@@ -178,14 +183,24 @@ void attn(Tensor q, Tensor kc, Tensor vc, Tensor tables, Tensor items, int64_t n
     TORCH_CHECK(part.has_value() && plse.has_value(), "attn: split tiles need their workspace");
     on(*part, kc, at::kFloat, "part");
     on(*plse, kc, at::kFloat, "plse");
-    TORCH_CHECK(part->is_contiguous() && plse->is_contiguous() && aligned(*part) && plse->numel() >= slots * H * 16 * nq &&
-                    part->numel() >= slots * H * 16 * nq * D, "attn: workspace");
+    TORCH_CHECK(part->is_contiguous() && plse->is_contiguous() && aligned(*part) && plse->numel() >= slots * H * rows &&
+                    part->numel() >= slots * H * rows * D, "attn: workspace");
     pp = part->data_ptr<float>();
     pl = plse->data_ptr<float>();
   }
-  KV4_HIP(kafka_kv4_attn(q.data_ptr(), q.stride(0), kc.data_ptr<uint8_t>(), vc.data_ptr<uint8_t>(), kc.size(0), tp, tables.stride(0), ip,
-                         (int)items.size(0), (int)nq, mp, (int)merges.size(0), (int)T, (int)H, (int)(Hq / H), D, (int)window, (int)first,
-                         (float)scale, out.data_ptr(), out.stride(0), lp, pp, pl, stream()));
+  if (!wtiles.has_value()) {
+    KV4_HIP(kafka_kv4_attn(q.data_ptr(), q.stride(0), kc.data_ptr<uint8_t>(), vc.data_ptr<uint8_t>(), kc.size(0), tp, tables.stride(0), ip,
+                           (int)items.size(0), (int)(rows / 16), mp, (int)merges.size(0), (int)T, (int)H, (int)(Hq / H), D, (int)window,
+                           (int)first, (float)scale, out.data_ptr(), out.stride(0), lp, pp, pl, stream()));
+    return;
+  }
+  const int* wp = ints(*wtiles, kc, 4, "wtiles");
+  on(*ws, kc, at::kByte, "ws");
+  TORCH_CHECK(rows == 256 && ws->is_contiguous() && aligned(*ws) && ws->numel() >= wtiles->size(0) * H * 256 * D, "attn: workspace");
+  KV4_HIP(kafka_kv4_tiles(q.data_ptr(), q.stride(0), kc.data_ptr<uint8_t>(), vc.data_ptr<uint8_t>(), kc.size(0), tp, tables.stride(0), ip,
+                          (int)items.size(0), wp, (int)wtiles->size(0), mp, (int)merges.size(0), (int)T, (int)H, (int)(Hq / H), D,
+                          (int)window, (int)first, (float)scale, out.data_ptr(), out.stride(0), lp, pp, pl,
+                          reinterpret_cast<char*>(ws->data_ptr()), stream()));
 }
 
 void mass(Tensor q, Tensor lse, Tensor kc, Tensor tables, Tensor items, int64_t n_whole, int64_t window, int64_t first, double scale, OptT base,

@@ -53,9 +53,13 @@ def read(k_cache: torch.Tensor, v_cache: torch.Tensor, slots: torch.Tensor) -> t
 
 # ---- plans --------------------------------------------------------------------------------------------------------------
 FEW_ROWS = 16              # rows (tokens x query heads of a group) of a tile for single tokens
-TILE_ROWS = 32             # of a tile for portions
+SOME_ROWS = 32             # of a tile for short portions
+MANY_ROWS = 256            # of a tile for portions whose keys are widened first
+MANY_MIN = 128             # rows of a segment from which on that is done
 TARGET_WGS = 1024          # workgroups that a launch of few tiles is split towards
+MANY_WGS = 256             # ... of wide ones (one to a CU)
 MIN_BLOCKS = 4             # blocks of a piece: one for each of a workgroup's waves
+MANY_BLOCKS = 8
 MASS_WHOLE_ROWS = 32       # rows of a segment up to which a wave takes them all for its block of keys
 
 
@@ -66,7 +70,8 @@ class AttnPlan:
         self.segs: list[tuple[int, int, int, int]] = []
         self.heads = self.kv_heads = self.dim = self.window = self.first = 0
         self.rows = self.covered = self.keys = self.tables = 0
-        self.parts: list = []       # (rows of a tile, items, merges, slots of partial results)
+        # kinds of tiles: (rows of one, items, merges, slots of partial results, tiles of keys to widen first)
+        self.parts: list[tuple[int, torch.Tensor, torch.Tensor, int, torch.Tensor]] = []
         self.mass_items = None
         self.mass_whole = 0
 
@@ -79,19 +84,19 @@ def _blocks(pos, tokens, window: int, first: int):
 
 
 def _tiles(segs: np.ndarray, tokens: int):
-    """Tiles of at most ``tokens`` rows: int64 [n, 4] (first row, rows, position, table row)."""
+    """Tiles of at most ``tokens`` rows: int64 [n, 5] (first row, rows, position, table row, segment)."""
     n = (segs[:, 1] + tokens - 1) // tokens
     s = np.repeat(np.arange(len(segs)), n)
     i = (np.arange(len(s)) - np.repeat(np.cumsum(n) - n, n)) * tokens
-    return np.stack([segs[s, 0] + i, np.minimum(segs[s, 1] - i, tokens), segs[s, 2] + i, segs[s, 3]], 1)
+    return np.stack([segs[s, 0] + i, np.minimum(segs[s, 1] - i, tokens), segs[s, 2] + i, segs[s, 3], s], 1)
 
 
-def _pieces(tiles: np.ndarray, window: int, first: int, kv_heads: int):
-    """(items int32 [n, 8], merges int32 [m, 4], slots): tiles of long ranges in pieces of about the same length, if the tiles by
-    themselves are too few workgroups; the longest first."""
+def _pieces(tiles: np.ndarray, window: int, first: int, kv_heads: int, many: bool = False):
+    """(tile, first block, last + 1, slot) int64 [n, 4], merges int64 [m, 4], slots: tiles of long ranges in pieces of about the same
+    length, if the tiles by themselves are too few workgroups; the longest first."""
     _, count = _blocks(tiles[:, 2], tiles[:, 1], window, first)
-    size = max(MIN_BLOCKS, -(-int(count.sum()) * kv_heads // TARGET_WGS))
-    n = np.maximum(1, (count + size - 1) // size)
+    size = max(MANY_BLOCKS if many else MIN_BLOCKS, -(-int(count.sum()) * kv_heads // (MANY_WGS if many else TARGET_WGS)))
+    n = np.maximum(1, (count + (size // 2 if many else size - 1)) // size)
     each = (count + n - 1) // n
     n = np.maximum(1, (count + each - 1) // each)
     t = np.repeat(np.arange(len(tiles)), n)
@@ -100,23 +105,39 @@ def _pieces(tiles: np.ndarray, window: int, first: int, kv_heads: int):
     split = n > 1
     base = np.cumsum(np.where(split, n, 0)) - np.where(split, n, 0)
     lo = i * each[t]
-    items = np.stack([tiles[t, 0], tiles[t, 1], tiles[t, 2], tiles[t, 3], lo, np.minimum(lo + each[t], count[t]),
-                      np.where(split[t], base[t] + i, -1), np.zeros_like(t)], 1)
-    items = items[np.argsort(items[:, 4] - items[:, 5], kind="stable")]
+    pieces = np.stack([t, lo, np.minimum(lo + each[t], count[t]), np.where(split[t], base[t] + i, -1)], 1)
     merges = np.stack([tiles[split, 0], tiles[split, 1], base[split], n[split]], 1)
-    return items.astype(np.int32), merges.astype(np.int32), int(n[split].sum())
+    return pieces[np.argsort(pieces[:, 1] - pieces[:, 2], kind="stable")], merges, int(n[split].sum())
 
 
 def _tables(full: np.ndarray, heads: int, kv_heads: int, window: int, first: int):
-    """(shapes, arrays) of ``attn``: for single tokens and for portions (rows of a tile, items, merges, slots), and their items and merges."""
+    """(shapes, arrays) of ``attn``: of each kind of tiles (rows of one, items, merges, slots, tiles of keys) and its items, merges, tiles of keys."""
     G = heads // kv_heads
-    few = full[:, 1] * G <= FEW_ROWS
+    rows = full[:, 1] * G
     shapes, arrays = [], []
-    for rows, part in ((FEW_ROWS, full[few]), (TILE_ROWS, full[~few])):
-        if len(part):
-            items, merges, slots = _pieces(_tiles(part, rows // G), window, first, kv_heads)
-            shapes.append((rows, len(items), len(merges), slots))
-            arrays += [items, merges]
+    for size, part in ((FEW_ROWS, full[rows <= FEW_ROWS]), (SOME_ROWS, full[(rows > FEW_ROWS) & (rows < MANY_MIN)]),
+                       (MANY_ROWS, full[rows >= MANY_MIN])):
+        if not len(part):
+            continue
+        many = size == MANY_ROWS
+        tiles = _tiles(part, size // G)
+        pieces, merges, slots = _pieces(tiles, window, first, kv_heads, many)
+        t = tiles[pieces[:, 0]]
+        if many:  # a segment's blocks lie one after the other in the workspace, those below the window first
+            head, count = _blocks(part[:, 2], part[:, 1], window, first)
+            tail = head + (part[:, 2] + part[:, 1] - 1) // BLOCK + 1 - count
+            base = np.cumsum(count) - count
+            s = np.repeat(np.arange(len(part)), count)
+            i = np.arange(len(s)) - base[s]
+            keys = np.stack([part[s, 3], np.where(i < head[s], i, i - head[s] + tail[s]), (part[:, 2] + part[:, 1] - 1)[s], np.zeros_like(s)], 1)
+            s = t[:, 4]
+            cols = [t[:, 0], t[:, 1], t[:, 2], base[s], head[s], tail[s]]
+        else:
+            keys, cols = np.zeros((0, 4)), [t[:, 0], t[:, 1], t[:, 2], t[:, 3]]
+        cols += [pieces[:, 1], pieces[:, 2], pieces[:, 3]]
+        items = np.stack(cols + [np.zeros_like(t[:, 0])] * ((12 if many else 8) - len(cols)), 1)
+        shapes.append((size, len(items), len(merges), slots, len(keys)))
+        arrays += [x.astype(np.int32) for x in (items, merges, keys)]
     return shapes, arrays
 
 
@@ -129,6 +150,10 @@ class _Take:
     def __call__(self, n: int, cols: int) -> torch.Tensor:
         self.at += n * cols
         return self.flat[self.at - n * cols:self.at].view(n, cols)
+
+
+def _part(take: _Take, rows: int, items: int, merges: int, slots: int, keys: int):
+    return rows, take(items, 12 if keys else 8), take(merges, 4), slots, take(keys, 4)
 
 
 def _plan(segs, heads: int, kv_heads: int, dim: int, window: int, first: int) -> tuple[AttnPlan, np.ndarray]:
@@ -170,22 +195,22 @@ def attn_plan(segs, heads: int, kv_heads: int, dim: int, window: int = 0, first:
         s, b = np.repeat(idx, len(b)), np.tile(b, len(idx))
         mass.append(np.stack([a[s, 0], a[s, 1], a[s, 2], a[s, 3], s, b, np.full_like(s, nb), np.zeros_like(s)], 1).astype(np.int32))
     take = _Take(torch.from_numpy(np.concatenate([t.reshape(-1) for t in arrays + mass])).to(dev))
-    p.parts = [(rows, take(n, 8), take(m, 4), slots) for rows, n, m, slots in shapes]
+    p.parts = [_part(take, *shape) for shape in shapes]
     p.mass_whole, p.mass_items = len(mass[0]), take(len(mass[0]) + len(mass[1]), 8)
     return p
 
 
-STEP_PARTS = 2             # kinds of tiles that a step may have
+STEP_PARTS = 3             # kinds of tiles that a step may have
 
 
 def step_tables(segs, heads: int, kv_heads: int, dim: int) -> np.ndarray:
     """The plan of an engine step as one int32 array, for its upload: what ``step_plan`` reads on the host, then the tables."""
     p, a = _plan(segs, heads, kv_heads, dim, 0, 0)
     shapes, arrays = _tables(a[a[:, 1] > 0], heads, kv_heads, 0, 0)
-    head = np.zeros(4 + 4 * STEP_PARTS, dtype=np.int32)
+    head = np.zeros(4 + 5 * STEP_PARTS, dtype=np.int32)
     head[:4] = p.rows, p.covered, p.keys, p.tables
     for i, s in enumerate(shapes):
-        head[4 + 4 * i:8 + 4 * i] = s
+        head[4 + 5 * i:9 + 5 * i] = s
     return np.concatenate([head] + [t.reshape(-1) for t in arrays])
 
 
@@ -194,10 +219,8 @@ def step_plan(host: np.ndarray, device: torch.Tensor, heads: int, kv_heads: int,
     p = AttnPlan()
     p.heads, p.kv_heads, p.dim = heads, kv_heads, dim
     p.rows, p.covered, p.keys, p.tables = (int(x) for x in host[:4])
-    take = _Take(device[4 + 4 * STEP_PARTS:])
-    for rows, n, m, slots in host[4:4 + 4 * STEP_PARTS].reshape(-1, 4).tolist():
-        if rows:
-            p.parts.append((rows, take(n, 8), take(m, 4), slots))
+    take = _Take(device[4 + 5 * STEP_PARTS:])
+    p.parts = [_part(take, *shape) for shape in host[4:4 + 5 * STEP_PARTS].reshape(-1, 5).tolist() if shape[0]]
     return p
 
 
@@ -229,14 +252,16 @@ def attn(q, k_cache, v_cache, block_tables, plan: AttnPlan, scale: float, out=No
     if not _gpu(q):
         ref.attn(q, k_cache, v_cache, block_tables, plan.segs, plan.window, plan.first, float(scale), out, lse)
         return out
-    for rows, items, merges, slots in plan.parts:
-        part = plse = None
+    for rows, items, merges, slots, keys in plan.parts:
+        part = plse = ws = None
         if slots:
             n = slots * plan.kv_heads * rows
             part = torch.empty(n * plan.dim, dtype=torch.float32, device=q.device)
             plse = torch.empty(n, dtype=torch.float32, device=q.device)
-        ext().kv4_attn(q, k_cache, v_cache, block_tables, items, rows // 16, merges, plan.window, plan.first, float(scale), out, lse, part,
-                       plse, slots)
+        if rows == MANY_ROWS:
+            ws = torch.empty(keys.shape[0] * plan.kv_heads * 4 * BLOCK * plan.dim, dtype=torch.uint8, device=q.device)
+        ext().kv4_attn(q, k_cache, v_cache, block_tables, rows, items, merges, plan.window, plan.first, float(scale), out, lse, part,
+                       plse, slots, keys if ws is not None else None, ws)
     return out
 
 

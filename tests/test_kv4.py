@@ -140,6 +140,11 @@ CASES = [
     (8, 8, 128, [(0, 70, 150, 0)], 1, 0),                                         # a window of the row itself
     (14, 2, 128, [(0, 130, 65, 0)], 64, 129),
     (8, 2, 64, [(0, 300, 500, 0), (300, 1, 2000, 1), (301, 2, 100, 2)], 5000, 4), # a window that hides nothing
+    (32, 2, 128, [(0, 130, 1, 0), (130, 9, 700, 1)], 0, 0),                       # 16 heads a group, keys widened first
+    (10, 2, 64, [(0, 333, 61, 0)], 200, 65),
+    (8, 2, 128, [(0, 64, 0, 0), (64, 40, 3000, 1), (110, 33, 130, 2)], 0, 0),     # ranges in pieces
+    (4, 4, 128, [(0, 600, 0, 0)], 64, 3),
+    (8, 2, 128, [(0, 40, 2000, 0), (40, 40, 2000, 1)], 300, 100),
 ]
 
 
@@ -436,12 +441,12 @@ def test_plan_covers_every_block_once():
         tok = 1 + r(16)
         tiles = kv4._tiles(segs, tok)
         assert sum(t[1] for t in tiles) == segs[:, 1].sum() and max(t[1] for t in tiles) <= tok
-        items, merges, slots = kv4._pieces(tiles, window, first, 2)
+        pieces, merges, slots = kv4._pieces(tiles, window, first, 2, bool(r(2)))
         seen = {}
-        for row, n, pos, tab, lo, hi, slot, _ in items.tolist():
+        for t, lo, hi, slot in pieces.tolist():
             assert lo < hi
-            seen.setdefault(row, []).append((lo, hi, slot))
-        for row, n, pos, tab in tiles.tolist():
+            seen.setdefault(int(tiles[t, 0]), []).append((lo, hi, slot))
+        for row, n, pos, tab, _ in tiles.tolist():
             parts = sorted(seen[row])
             need = {j // 64 for p in range(pos, pos + n) for j in range(p + 1) if not window or j > p - window or j < first}
             head, count = (int(x) for x in kv4._blocks(np.array(pos), np.array(n), window, first))
@@ -715,11 +720,32 @@ def test_engine_on_the_gpu(cuda):
 
 def test_step_plan_is_the_plan():
     """An engine step's tables, as uploaded, are those of attn_plan."""
-    segs = [(0, 1, 500, 0), (1, 1, 33, 1), (2, 77, 9, 2), (79, 3, 4000, 3)]
+    segs = [(0, 1, 500, 0), (1, 1, 33, 1), (2, 77, 9, 2), (79, 3, 4000, 3), (82, 10, 70, 4)]
     flat = kv4.step_tables(segs, 8, 2, 128)
     p = kv4.step_plan(flat, torch.from_numpy(flat), 8, 2, 128)
     shapes, arrays = kv4._tables(kv4._plan(segs, 8, 2, 128, 0, 0)[1], 8, 2, 0, 0)
-    assert [(r, len(i), len(m), s) for r, i, m, s in p.parts] == shapes
-    for (_, items, merges, _), (a, b) in zip(p.parts, zip(arrays[::2], arrays[1::2])):
-        assert (items.numpy() == a).all() and (merges.numpy() == b).all()
-    assert (p.rows, p.covered, p.keys, p.tables) == (82, 82, 4003, 4)
+    assert [(r, len(i), len(m), s, len(k)) for r, i, m, s, k in p.parts] == shapes and len(shapes) == 3
+    for (_, items, merges, _, keys), (a, b, c) in zip(p.parts, zip(*(arrays[i::3] for i in range(3)))):
+        assert (items.numpy() == a).all() and (merges.numpy() == b).all() and (keys.numpy() == c).all()
+    assert (p.rows, p.covered, p.keys, p.tables) == (92, 92, 4003, 5)
+
+
+def test_widened_keys_are_those_that_a_tile_sees():
+    """Every block of a wide tile's list is at its place among its segment's in the workspace."""
+    import numpy as np
+
+    g = torch.Generator().manual_seed(1)
+    r = lambda hi: int(torch.randint(0, hi, (1,), generator=g))
+    for _ in range(100):
+        segs = np.array([(1000 * i, 33 + r(400), r(6000), 10 + i) for i in range(1 + r(4))])
+        window, first = (0, 0) if r(3) == 0 else (1 + r(1500), r(300))
+        shapes, (items, merges, keys) = kv4._tables(segs, 8, 2, window, first)
+        assert [s[0] for s in shapes] == [256]
+        for row, n, pos, base, head, tail, lo, hi, _, *_ in items.tolist():
+            t, f = max(0, pos - window + 1) // 64 if window else 0, 0
+            f = min(-(-first // 64), t)
+            for v in range(lo, hi):
+                b = v if v < f else v - f + t
+                k = keys[base + (b if b < head else b - tail + head)].tolist()
+                seg = segs[row // 1000]
+                assert k[:3] == [seg[3], b, seg[1] + seg[2] - 1]
