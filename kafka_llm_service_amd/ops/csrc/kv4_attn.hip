@@ -9,6 +9,8 @@
 // The softmax runs in one pass with a running maximum per row; its sums and maxima are fp32, P is rounded to bf16 for the product.
 #include "kv4.h"
 
+#include <type_traits>
+
 namespace kafka {
 namespace kv4 {
 
@@ -235,12 +237,12 @@ __device__ __forceinline__ void block_step(const KFrag<D>& kf, const VFrag& vf, 
   }
 }
 
-// Four waves take a tile of 16 NQ rows, every fourth block each; their results meet in LDS.
-template <int D, int NQ>
-__global__ __launch_bounds__(256) void attn_kernel(Args a) {
+// NW waves take a tile of 16 NQ rows, every NW-th block each; their results meet in LDS.
+template <int D, int NQ, int NW>
+__global__ __launch_bounds__(64 * NW) void attn_kernel(Args a) {
   constexpr int LD = D + 4;                                     // (16 lanes a quarter write 16 rows: other banks each)
-  __shared__ float sO[4][16][LD];
-  __shared__ float sM[4][16], sL[4][16];
+  __shared__ float sO[NW][16][LD];
+  __shared__ float sM[NW][16], sL[NW][16];
   const Item it = a.items[blockIdx.x / a.Hkv];
   const int h = blockIdx.x % a.Hkv, lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int q = lane & 15, c = lane >> 4;
@@ -253,7 +255,7 @@ __global__ __launch_bounds__(256) void attn_kernel(Args a) {
   Rows<D, NQ> r;
 #pragma unroll
   for (int n = 0; n < NQ; ++n) {
-    r.lim[n] = load_q<D>(r.q[n], a, it.row, it.tokens, it.pos, h, 16 * n, lane);
+    r.lim[n] = -1;
     r.m[n] = -INFINITY;
     r.l[n] = 0.f;
 #pragma unroll
@@ -268,8 +270,10 @@ __global__ __launch_bounds__(256) void attn_kernel(Args a) {
     block_pages(bt, list[v], pmax, a.n_pages, pg, bad);
     load_k<D>(kf, a.kc, a.Hkv, h, pg, lane);
     load_v<D>(vf, a.vc, a.Hkv, h, pg, lane);
-    for (; v < hi; v += 4) {
-      const int nv = v + 4 < hi ? v + 4 : v;
+#pragma unroll
+    for (int n = 0; n < NQ; ++n) r.lim[n] = load_q<D>(r.q[n], a, it.row, it.tokens, it.pos, h, 16 * n, lane);
+    for (; v < hi; v += NW) {
+      const int nv = v + NW < hi ? v + NW : v;
       KFrag<D> kn;
       VFrag vn;
       block_pages(bt, list[nv], pmax, a.n_pages, pg, bad);
@@ -283,66 +287,89 @@ __global__ __launch_bounds__(256) void attn_kernel(Args a) {
   const int Hq = a.Hkv * a.G;
 #pragma unroll
   for (int n = 0; n < NQ; ++n) {
+    const int live = min(16, it.tokens * a.G - 16 * n);         // columns of the tile that are rows
+    if (live <= 0) break;
     const float l = over_quarters_sum(r.l[n]);
     if (n) __syncthreads();
+    if (q < live) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+      for (int i = 0; i < 4; ++i)
 #pragma unroll
-      for (int d = 0; d < D / 16; d += 4)
-        *reinterpret_cast<f32x4*>(&sO[w][q][(D / 16) * (4 * c + i) + d]) =
-            f32x4{r.o[n][d][i], r.o[n][d + 1][i], r.o[n][d + 2][i], r.o[n][d + 3][i]};
-    if (c == 0) {
-      sM[w][q] = r.m[n];
-      sL[w][q] = bad ? __builtin_nanf("") : l;
+        for (int d = 0; d < D / 16; d += 4)
+          *reinterpret_cast<f32x4*>(&sO[w][q][(D / 16) * (4 * c + i) + d]) =
+              f32x4{r.o[n][d][i], r.o[n][d + 1][i], r.o[n][d + 2][i], r.o[n][d + 3][i]};
+      if (c == 0) {
+        sM[w][q] = r.m[n];
+        sL[w][q] = bad ? __builtin_nanf("") : l;
+      }
     }
     __syncthreads();
-    for (int x = threadIdx.x; x < 16 * (D / 8); x += 256) {
-      const int row = x / (D / 8), d0 = (x % (D / 8)) * 8, R = 16 * n + row, tok = R / a.G, g = R - tok * a.G;
-      if (tok >= it.tokens) continue;
-      const float M = vmax(vmax(sM[0][row], sM[1][row]), vmax(sM[2][row], sM[3][row]));
+    for (int x = threadIdx.x; x < live * (D / 4); x += 64 * NW) {
+      const int row = x / (D / 4), d0 = (x % (D / 4)) * 4, R = 16 * n + row, tok = R / a.G, g = R - tok * a.G;
+      float M = sM[0][row];
+#pragma unroll
+      for (int i = 1; i < NW; ++i) M = vmax(M, sM[i][row]);
       float L = 0.f;
-      float o[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+      f32x4 o = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
+      for (int i = 0; i < NW; ++i) {
         const float f = M == -INFINITY ? 1.f : fast_exp2(sM[i][row] - M);
-        L += f * sL[i][row];
+        const f32x4 y = *reinterpret_cast<const f32x4*>(&sO[i][row][d0]);
+        L = fmaf(f, sL[i][row], L);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) o[j] = fmaf(f, sO[i][row][d0 + j], o[j]);
+        for (int j = 0; j < 4; ++j) o[j] = fmaf(f, y[j], o[j]);
       }
       const float inv = L == 0.f ? 0.f : 1.f / L, lse = L == 0.f ? -INFINITY : M + log2f(L);
-      if (it.slot < 0) {
-        bf16x8 y;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) y[j] = (bf16)(o[j] * inv);
-        store_bf16x8(a.out + (int64_t)(it.row + tok) * a.os + (int64_t)(h * a.G + g) * D + d0, y);
+      for (int j = 0; j < 4; ++j) o[j] *= inv;
+      if (it.slot < 0) {
+        *reinterpret_cast<bf16x4*>(a.out + (int64_t)(it.row + tok) * a.os + (int64_t)(h * a.G + g) * D + d0) =
+            bf16x4{(bf16)o[0], (bf16)o[1], (bf16)o[2], (bf16)o[3]};
         if (a.lse && d0 == 0) a.lse[(int64_t)(it.row + tok) * Hq + h * a.G + g] = lse;
       } else {
         const int64_t at = ((int64_t)it.slot * a.Hkv + h) * (16 * NQ) + R;
-        *reinterpret_cast<f32x4*>(a.part + at * D + d0) = f32x4{o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv};
-        *reinterpret_cast<f32x4*>(a.part + at * D + d0 + 4) = f32x4{o[4] * inv, o[5] * inv, o[6] * inv, o[7] * inv};
+        *reinterpret_cast<f32x4*>(a.part + at * D + d0) = o;
         if (d0 == 0) a.plse[at] = lse;
       }
     }
   }
 }
 
-// Partial results of split tiles. Merge items: first row, rows, first slot, slots.
+// Partial results of split tiles, eight on their way at a time. Merge items: first row, rows, first slot, slots.
 template <int D>
 __global__ __launch_bounds__(256) void merge_kernel(Args a, const int* __restrict__ merges, int tile_rows) {
+  constexpr int B = 8;
   const int* it = merges + 4 * (blockIdx.x / a.Hkv);
   const int row0 = it[0], tokens = it[1], slot0 = it[2], n = it[3];
   const int h = blockIdx.x % a.Hkv, R = blockIdx.y * (256 / (D / 4)) + threadIdx.x / (D / 4), d0 = (threadIdx.x % (D / 4)) * 4;
   const int tok = R / a.G, g = R - tok * a.G;
   if (tok >= tokens || row0 + tokens > a.T || R >= tile_rows) return;
   const int64_t at = ((int64_t)slot0 * a.Hkv + h) * tile_rows + R, step = (int64_t)a.Hkv * tile_rows;
-  float M = -INFINITY;
-  for (int s = 0; s < n; ++s) M = vmax(M, a.plse[at + s * step]);
+  float M = -INFINITY, L = 0.f;
   f32x4 o = {0.f, 0.f, 0.f, 0.f};
-  float L = 0.f;
-  for (int s = 0; s < n; ++s) {
-    const float f = M == -INFINITY ? 0.f : fast_exp2(a.plse[at + s * step] - M);
-    L += f;
-    o += *reinterpret_cast<const f32x4*>(a.part + (at + s * step) * D + d0) * f;
+  for (int s0 = 0; s0 < n; s0 += B) {
+    float l[B];
+    f32x4 p[B];
+#pragma unroll
+    for (int s = 0; s < B; ++s) {
+      const int64_t i = at + min(s0 + s, n - 1) * step;
+      l[s] = a.plse[i];
+      p[s] = *reinterpret_cast<const f32x4*>(a.part + i * D + d0);
+    }
+    float mx = M;
+#pragma unroll
+    for (int s = 0; s < B; ++s) mx = vmax(mx, l[s]);
+    const float use = mx == -INFINITY ? 0.f : mx, f0 = fast_exp2(M - use);
+    M = mx;
+    L *= f0;
+    o *= f0;
+#pragma unroll
+    for (int s = 0; s < B; ++s) {
+      const float f = s0 + s < n ? fast_exp2(l[s] - use) : 0.f;
+      L += f;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) o[j] = fmaf(p[s][j], f, o[j]);
+    }
   }
   const float inv = L == 0.f ? 0.f : 1.f / L;
   bf16x4 y;
@@ -355,7 +382,7 @@ __global__ __launch_bounds__(256) void merge_kernel(Args a, const int* __restric
 // ---- weights of the keys ------------------------------------------------------------------------------------------------
 // out[segment][head][key] = base + sum over the segment's rows and the head's queries of 2^(s - lse). Every key is one wave's or one
 // workgroup's, so that no sums meet in memory and a call's result does not depend on their order.
-// Items: first row, rows, position, table row, segment, first block, blocks, 0.
+// Items: first row, rows, position, table row, segment, first block, last block + 1, 0.
 struct MassArgs {
   Args a;
   const float* base;      // may be null, or out
@@ -363,78 +390,167 @@ struct MassArgs {
   int N;
 };
 
-template <int D, bool SPLIT>
-__global__ __launch_bounds__(256) void mass_kernel(MassArgs ma) {
+// sum over the 16 lanes of a quarter, in every one of them
+__device__ __forceinline__ float over_columns(float x) {
+  x += __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(x), 0x128, 0xf, 0xf, true));   // row_ror 8, 4, 2, 1
+  x += __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(x), 0x124, 0xf, 0xf, true));
+  x += __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(x), 0x122, 0xf, 0xf, true));
+  return x + __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(x), 0x121, 0xf, 0xf, true));
+}
+
+// lse of 16 columns from R0 on; +infinity where there is no row or the row sees nothing (its weights are zero)
+__device__ __forceinline__ float load_lse(const Args& a, int row, int tokens, int h, int R0, int lane) {
+  const int R = R0 + (lane & 15), tok = R / a.G, g = R - tok * a.G;
+  const float x = a.lse[(int64_t)(row + min(tok, tokens - 1)) * (a.Hkv * a.G) + h * a.G + g];
+  return tok >= tokens || x == -INFINITY ? INFINITY : x;
+}
+
+// acc[t][i] += weights of the block's keys 16 t + 4 c + i in 16 columns
+template <int NQ>
+__device__ __forceinline__ void add_weights(float (&acc)[4][4], const f32x4 (&s)[4][NQ], int n, float ls, bool masked, int key0, int lim,
+                                            const Args& a, int lane) {
+#pragma unroll
+  for (int t = 0; t < 4; ++t)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      float e = fast_exp2(fmaf(s[t][n][i], a.scale2, -ls));
+      if (masked && !sees(key0 + 16 * t + 4 * (lane >> 4) + i, lim, a.window, a.first)) e = 0.f;
+      acc[t][i] += e;
+    }
+}
+
+__device__ __forceinline__ void store_mass(const MassArgs& ma, int seg, int h, int key, float x) {
+  if (key >= ma.N) return;
+  const int64_t at = ((int64_t)seg * ma.a.Hkv + h) * ma.N + key;
+  ma.out[at] = (ma.base ? ma.base[at] : 0.f) + x;
+}
+
+// Segments of at most 16 NQ rows: four waves take every fourth block of an item's, its keys widened as they come.
+template <int D, int NQ>
+__global__ __launch_bounds__(256) void mass_few_kernel(MassArgs ma) {
   const Args& a = ma.a;
   __shared__ float sum[4][KB];
   const int* it = reinterpret_cast<const int*>(a.items) + 8 * (blockIdx.x / a.Hkv);
-  const int row = it[0], rows = it[1], pos = it[2], table = it[3], seg = it[4];
+  const int row = it[0], rows = it[1], pos = it[2], table = it[3], seg = it[4], end = it[6];
   const int h = blockIdx.x % a.Hkv, lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int c = lane >> 4, q = lane & 15;
-  if (row < 0 || rows < 0 || row + rows > a.T) return;
-  const int b = SPLIT ? it[5] : it[5] + w, key0 = b * KB, last = pos + rows - 1;
-  if (!SPLIT && b >= it[6]) return;
-  float acc[4][4] = {};
+  const int c = lane >> 4, last = pos + rows - 1;
+  if (row < 0 || rows < 0 || row + rows > a.T || rows * a.G > 16 * NQ) return;
+  const int* bt = a.tables + table * a.ts;
   const Blocks list(pos, last, a.window, a.first);
-  bool bad = false;
-  if (key0 <= last && (b < list.head || b >= list.tail)) {
-    int pg[4];
-    KFrag<D> kf;
-    block_pages(a.tables + table * a.ts, b, last, a.n_pages, pg, bad);
+  // blocks that no row sees give nothing: behind the last key, between the first ones and the window
+  auto seen = [&](int b) { return rows > 0 && b * KB <= last && (b < list.head || b >= list.tail); };
+  int b = it[5] + w;
+  if (b >= end) return;
+  bool bad = false, badn = false;
+  int pg[4];
+  KFrag<D> kf, kn;
+  if (seen(b)) {
+    block_pages(bt, b, last, a.n_pages, pg, bad);
     load_k<D>(kf, a.kc, a.Hkv, h, pg, lane);
-    const int Hq = a.Hkv * a.G, R1 = rows * a.G;
-    // rows that may see the block: from its first key's position on (tiles of 16 columns)
-    const int R0 = max(0, (key0 - pos) * a.G) & ~15;
-    for (int R = R0 + (SPLIT ? 16 * w : 0); R < R1; R += SPLIT ? 64 : 16) {
-      const int pmin = pos + R / a.G, pmax = min(pos + (R + 15) / a.G, last);
-      if (key0 + KB <= pmin - a.window + 1 && key0 >= a.first) break;             // (so do all rows after these)
-      bf16x8 qf[1][D / 32];
-      const int lim = load_q<D>(qf[0], a, row, rows, pos, h, R, lane);
-      const int tok = (R + q) / a.G, g = R + q - tok * a.G;
-      float ls = lim >= 0 ? a.lse[(int64_t)(row + tok) * Hq + h * a.G + g] : INFINITY;
-      if (ls == -INFINITY) ls = INFINITY;                                           // (a row that sees nothing gives nothing)
-      f32x4 s[4][1];
-      scores<D, 1>(kf, qf, s);
-      const bool masked = key0 + KB - 1 > pmin || (key0 <= pmax - a.window && key0 + KB > a.first);
+  }
+  bf16x8 qf[NQ][D / 32];
+  int lim[NQ];
+  float ls[NQ];
+#pragma unroll
+  for (int n = 0; n < NQ; ++n)
+    if (rows > 0) {
+      lim[n] = load_q<D>(qf[n], a, row, rows, pos, h, 16 * n, lane);
+      ls[n] = load_lse(a, row, rows, h, 16 * n, lane);
+    }
+  for (; b < end; b += 4) {
+    const int nb = b + 4;
+    if (nb < end && seen(nb)) {
+      badn = false;
+      block_pages(bt, nb, last, a.n_pages, pg, badn);
+      load_k<D>(kn, a.kc, a.Hkv, h, pg, lane);
+    }
+    float mine = 0.f;
+    const int key0 = b * KB;
+    if (seen(b)) {
+      float acc[4][4] = {};
+      f32x4 s[4][NQ];
+      scores<D, NQ>(kf, qf, s);
+      const bool masked = key0 + KB - 1 > pos || (key0 <= last - a.window && key0 + KB > a.first);
+#pragma unroll
+      for (int n = 0; n < NQ; ++n) add_weights<NQ>(acc, s, n, ls[n], masked, key0, lim[n], a, lane);
 #pragma unroll
       for (int t = 0; t < 4; ++t)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          float e = fast_exp2(fmaf(s[t][0][i], a.scale2, -ls));
-          if ((masked && !sees(key0 + 16 * t + 4 * c + i, lim, a.window, a.first)) || lim < 0) e = 0.f;
-          acc[t][i] += e;
+          const float x = over_columns(acc[t][i]);
+          if ((lane & 15) == 0) sum[w][16 * t + 4 * c + i] = bad ? __builtin_nanf("") : x;
         }
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+      mine = sum[w][lane];
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+    }
+    store_mass(ma, seg, h, key0 + lane, mine);
+    kf = kn;
+    bad = badn;
+  }
+}
+
+// Longer segments: NW waves share the rows that may see a block, whose keys stay widened in registers.
+template <int D, int NW>
+__global__ __launch_bounds__(64 * NW) void mass_many_kernel(MassArgs ma) {
+  const Args& a = ma.a;
+  __shared__ float sum[NW][KB];
+  const int* it = reinterpret_cast<const int*>(a.items) + 8 * (blockIdx.x / a.Hkv);
+  const int row = it[0], rows = it[1], pos = it[2], table = it[3], seg = it[4], b = it[5], key0 = b * KB;
+  const int h = blockIdx.x % a.Hkv, lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int c = lane >> 4, last = pos + rows - 1;
+  if (row < 0 || rows < 0 || row + rows > a.T) return;
+  const Blocks list(pos, last, a.window, a.first);
+  float acc[4][4] = {};
+  bool bad = false;
+  if (rows > 0 && key0 <= last && (b < list.head || b >= list.tail)) {
+    int pg[4];
+    KFrag<D> kf;
+    block_pages(a.tables + table * a.ts, b, last, a.n_pages, pg, bad);
+    load_k<D>(kf, a.kc, a.Hkv, h, pg, lane);
+    const int R1 = rows * a.G;
+    int R = (max(0, (key0 - pos) * a.G) & ~15) + 16 * w;                 // rows that may see the block: from its first key's position on
+    bf16x8 qf[D / 32];
+    int lim = load_q<D>(qf, a, row, rows, pos, h, R, lane);
+    float ls = load_lse(a, row, rows, h, R, lane);
+    bf16x8 k[4][D / 32];
+#pragma unroll
+    for (int t = 0; t < 4; ++t)
+#pragma unroll
+      for (int i = 0; i < D / 32; ++i) k[t][i] = widen8(kf.d[t][i], scale_of(kf.s[t]));
+    for (; R < R1; R += 16 * NW) {
+      const int pmin = pos + R / a.G, pmax = min(pos + (R + 15) / a.G, last);
+      if (key0 + KB <= pmin - a.window + 1 && key0 >= a.first) break;    // (so do all rows after these)
+      f32x4 s[4][1];
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+        s[t][0] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int i = 0; i < D / 32; ++i) s[t][0] = mfma16(k[t][i], qf[i], s[t][0]);
+      }
+      const int lim0 = lim;
+      const float ls0 = ls;
+      lim = load_q<D>(qf, a, row, rows, pos, h, R + 16 * NW, lane);      // (behind the last row: the first one again)
+      ls = load_lse(a, row, rows, h, R + 16 * NW, lane);
+      const bool masked = key0 + KB - 1 > pmin || (key0 <= pmax - a.window && key0 + KB > a.first);
+      add_weights<1>(acc, s, 0, ls0, masked, key0, lim0, a, lane);
     }
   }
 #pragma unroll
   for (int t = 0; t < 4; ++t)
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      float x = acc[t][i];
-#pragma unroll
-      for (int o = 1; o < 16; o <<= 1) x += __shfl_xor(x, o, 64);
-      acc[t][i] = bad ? __builtin_nanf("") : x;
+      const float x = over_columns(acc[t][i]);
+      if ((lane & 15) == 0) sum[w][16 * t + 4 * c + i] = bad ? __builtin_nanf("") : x;
     }
-  float mine = 0.f;                      // lane = key of the block: from quarter (key / 4) % 4, register key % 4 of tile key / 16
+  __syncthreads();
+  if (w) return;
+  float mine = 0.f;
 #pragma unroll
-  for (int t = 0; t < 4; ++t)
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (q == 0) sum[w][16 * t + 4 * c + i] = acc[t][i];
-  if (SPLIT) {
-    __syncthreads();
-    if (w) return;
-    mine = (sum[0][lane] + sum[1][lane]) + (sum[2][lane] + sum[3][lane]);
-  } else {
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-    mine = sum[w][lane];
-  }
-  const int key = key0 + lane;
-  if (key < ma.N) {
-    const int64_t at = ((int64_t)seg * a.Hkv + h) * ma.N + key;
-    ma.out[at] = (ma.base ? ma.base[at] : 0.f) + mine;
-  }
+  for (int i = 0; i < NW; ++i) mine += sum[i][lane];
+  store_mass(ma, seg, h, key0 + lane, mine);
 }
 
 }  // namespace kv4
@@ -462,44 +578,55 @@ extern "C" hipError_t kafka_kv4_merge(const int* merges, int n_merges, int tile_
   return hipGetLastError();
 }
 
-// tiles of 16 nq rows (nq 1, 2)
+// tiles of 16 nq rows, nw waves each
 extern "C" hipError_t kafka_kv4_attn(const bf16* q, int64_t qs, const uint8_t* kc, const uint8_t* vc, int64_t n_pages, const int* tables,
-                                     int64_t ts, const int* items, int n_items, int nq, const int* merges, int n_merges, int T, int Hkv,
-                                     int G, int D, int window, int first, float scale, bf16* out, int64_t os, float* lse, float* part,
-                                     float* plse, hipStream_t st) {
+                                     int64_t ts, const int* items, int n_items, int nq, int nw, const int* merges, int n_merges, int T,
+                                     int Hkv, int G, int D, int window, int first, float scale, bf16* out, int64_t os, float* lse,
+                                     float* part, float* plse, hipStream_t st) {
   if (n_items == 0) return hipSuccess;
-  if ((D != 64 && D != 128) || (nq != 1 && nq != 2) || G < 1 || G > 16)
-    return hipErrorInvalidValue;
-  const Args a = make_args(q, qs, kc, vc, n_pages, tables, ts, items, T, Hkv, G, window, first, scale, out, os, lse, part, plse);
   const int64_t wgs = (int64_t)Hkv * n_items;
-  if (wgs >= 1 << 24) return hipErrorInvalidValue;
-  const dim3 grid((unsigned)wgs);
-  auto go = [&](auto kern) { kern<<<grid, 256, 0, st>>>(a); };
-  if (D == 128)
-    nq == 1 ? go(attn_kernel<128, 1>) : go(attn_kernel<128, 2>);
-  else
-    nq == 1 ? go(attn_kernel<64, 1>) : go(attn_kernel<64, 2>);
+  if ((D != 64 && D != 128) || G < 1 || G > 16 || wgs >= 1 << 24) return hipErrorInvalidValue;
+  const Args a = make_args(q, qs, kc, vc, n_pages, tables, ts, items, T, Hkv, G, window, first, scale, out, os, lse, part, plse);
+  auto go = [&](auto kern) { kern<<<(unsigned)wgs, 64 * nw, 0, st>>>(a); };
+  auto dim = [&](auto d) {
+    constexpr int DD = decltype(d)::value;
+    if (nq == 1 && nw == 4) go(attn_kernel<DD, 1, 4>);
+    else if (nq == 1 && nw == 8) go(attn_kernel<DD, 1, 8>);
+    else if (nq == 2 && nw == 4) go(attn_kernel<DD, 2, 4>);
+    else return false;
+    return true;
+  };
+  if (!(D == 128 ? dim(std::integral_constant<int, 128>{}) : dim(std::integral_constant<int, 64>{}))) return hipErrorInvalidValue;
   if (n_merges) return kafka_kv4_merge(merges, n_merges, 16 * nq, T, Hkv, G, D, out, os, lse, part, plse, st);
   return hipGetLastError();
 }
 
-// items of segments whose rows one wave takes for a block, then of those that four share
+constexpr int MASS_NW = 8;
+
+// items of segments of at most 32 rows, then of those of more
 extern "C" hipError_t kafka_kv4_mass(const bf16* q, int64_t qs, const float* lse, const uint8_t* kc, int64_t n_pages, const int* tables,
-                                     int64_t ts, const int* items, int n_whole, int n_split, int T, int Hkv, int G, int D, int window,
+                                     int64_t ts, const int* items, int n_few, int n_many, int T, int Hkv, int G, int D, int window,
                                      int first, float scale, const float* base, float* out, int N, hipStream_t st) {
-  if ((D != 64 && D != 128) || G < 1 || G > 16 || (int64_t)Hkv * n_whole >= 1 << 24 || (int64_t)Hkv * n_split >= 1 << 24)
+  if ((D != 64 && D != 128) || G < 1 || G > 16 || (int64_t)Hkv * n_few >= 1 << 24 || (int64_t)Hkv * n_many >= 1 << 24)
     return hipErrorInvalidValue;
-  for (int split = 0; split < 2; ++split) {
-    const int n = split ? n_split : n_whole;
-    if (!n) continue;
-    MassArgs m{make_args(q, qs, kc, nullptr, n_pages, tables, ts, items + (split ? 8 * (int64_t)n_whole : 0), T, Hkv, G, window, first,
-                         scale, nullptr, 0, const_cast<float*>(lse), nullptr, nullptr),
-               base, out, N};
-    const dim3 grid((unsigned)(Hkv * n));
+  auto args = [&](const int* at) {
+    return MassArgs{make_args(q, qs, kc, nullptr, n_pages, tables, ts, at, T, Hkv, G, window, first, scale, nullptr, 0,
+                              const_cast<float*>(lse), nullptr, nullptr),
+                    base, out, N};
+  };
+  if (n_few) {
+    const MassArgs m = args(items);
     if (D == 128)
-      split ? mass_kernel<128, true><<<grid, 256, 0, st>>>(m) : mass_kernel<128, false><<<grid, 256, 0, st>>>(m);
+      mass_few_kernel<128, 2><<<Hkv * n_few, 256, 0, st>>>(m);
     else
-      split ? mass_kernel<64, true><<<grid, 256, 0, st>>>(m) : mass_kernel<64, false><<<grid, 256, 0, st>>>(m);
+      mass_few_kernel<64, 2><<<Hkv * n_few, 256, 0, st>>>(m);
+  }
+  if (n_many) {
+    const MassArgs m = args(items + 8 * (int64_t)n_few);
+    if (D == 128)
+      mass_many_kernel<128, MASS_NW><<<Hkv * n_many, 64 * MASS_NW, 0, st>>>(m);
+    else
+      mass_many_kernel<64, MASS_NW><<<Hkv * n_many, 64 * MASS_NW, 0, st>>>(m);
   }
   return hipGetLastError();
 }

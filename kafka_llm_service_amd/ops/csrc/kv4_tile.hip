@@ -113,7 +113,7 @@ struct TileArgs {
 // fragments after it; keys run a tile ahead of the values, and the slots that a step has read are filled again in its middle, behind one counted
 // wait and one barrier. The maximum is raised only where it has grown by more than 2^24 (sums of weights up to that are exact enough in fp32).
 template <int D, int NW, int NSLOT>
-__global__ __launch_bounds__(64 * NW) void tile_kernel(TileArgs a) {
+__global__ __launch_bounds__(64 * NW, D == 64 ? 3 : 1) void tile_kernel(TileArgs a) {
   constexpr int F = D / 16, NT = D / 32, KBYTES = Image<D>::KBYTES, PB = Image<D>::PAGE_BYTES;
   constexpr int PIECES = KBYTES / 1024, DPT = 2 * PIECES / NW;             // LDS copies of 1 KiB: of K or V of a tile, of a wave for both
   constexpr float THR = 24.f;
@@ -355,26 +355,24 @@ using namespace kv4;
 extern "C" hipError_t kafka_kv4_merge(const int* merges, int n_merges, int tile_rows, int T, int Hkv, int G, int D, bf16* out, int64_t os,
                                       float* lse, float* part, float* plse, hipStream_t st);
 
-constexpr int TILE_NW = 8;
-
-// items of 32 TILE_NW rows; wtiles: what of the cache the workspace holds, tile after tile
+// items of 256 rows (D 128) or 128 (D 64); wtiles: what of the cache the workspace holds, tile after tile
 extern "C" hipError_t kafka_kv4_tiles(const bf16* q, int64_t qs, const uint8_t* kc, const uint8_t* vc, int64_t n_pages, const int* tables,
-                                      int64_t ts, const int* items, int n_items, const int* wtiles, int n_wtiles, const int* merges,
-                                      int n_merges, int T, int Hkv, int G, int D, int window, int first, float scale, bf16* out, int64_t os,
+                                      int64_t ts, int rows, const int* items, int n_items, const int* wtiles, int n_wtiles,
+                                      const int* merges, int n_merges, int T, int Hkv, int G, int D, int window, int first, float scale, bf16* out, int64_t os,
                                       float* lse, float* part, float* plse, char* ws, hipStream_t st) {
   if (n_items == 0) return hipSuccess;
   const int64_t wgs = (int64_t)Hkv * n_items, wws = (int64_t)Hkv * n_wtiles;
-  if ((D != 64 && D != 128) || G < 1 || G > 16 || wgs >= 1 << 24 || wws >= 1 << 24) return hipErrorInvalidValue;
+  if ((D != 64 && D != 128) || rows != (D == 128 ? 256 : 128) || G < 1 || G > 16 || wgs >= 1 << 24 || wws >= 1 << 24) return hipErrorInvalidValue;
   const TileArgs a{q,  qs, ws, reinterpret_cast<const TileItem4*>(items), T, Hkv, G, window > 0 ? window : 1 << 30, first,
                    scale * 1.4426950408889634f, out, os, lse, part, plse};
   if (D == 128) {
     widen_kernel<128><<<(unsigned)wws, 256, 0, st>>>(kc, vc, n_pages, tables, ts, wtiles, Hkv, ws);
-    tile_kernel<128, TILE_NW, 3><<<(unsigned)wgs, 64 * TILE_NW, 0, st>>>(a);
+    tile_kernel<128, 8, 3><<<(unsigned)wgs, 512, 0, st>>>(a);
   } else {
     widen_kernel<64><<<(unsigned)wws, 256, 0, st>>>(kc, vc, n_pages, tables, ts, wtiles, Hkv, ws);
-    tile_kernel<64, TILE_NW, 3><<<(unsigned)wgs, 64 * TILE_NW, 0, st>>>(a);
+    tile_kernel<64, 4, 3><<<(unsigned)wgs, 256, 0, st>>>(a);
   }
-  if (n_merges) return kafka_kv4_merge(merges, n_merges, 32 * TILE_NW, T, Hkv, G, D, out, os, lse, part, plse, st);
+  if (n_merges) return kafka_kv4_merge(merges, n_merges, rows, T, Hkv, G, D, out, os, lse, part, plse, st);
   return hipGetLastError();
 }
 

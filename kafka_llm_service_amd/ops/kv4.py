@@ -40,27 +40,29 @@ def _check_cache(k_cache, v_cache, who: str) -> None:
 def read(k_cache: torch.Tensor, v_cache: torch.Tensor, slots: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     """(K, V) [T, heads, D] bf16 of ``slots`` int64 [T] (page * 16 + key), exactly what the cache holds. Negative slots give zeros,
     slots behind the cache no numbers."""
+    if _gpu(k_cache):
+        return ext().kv4_read(k_cache, v_cache, slots)
     _check_cache(k_cache, v_cache, "kv4.read")
     if slots.dim() != 1 or slots.dtype != torch.int64:
         raise ValueError("kv4.read: slots int64 [T]")
-    if not _gpu(k_cache):
-        return ref.read(k_cache, v_cache, slots)
-    k = torch.empty(slots.shape[0], k_cache.shape[1], ref.head_dim(k_cache), dtype=torch.bfloat16, device=k_cache.device)
-    v = torch.empty_like(k)
-    ext().kv4_read(k_cache, v_cache, slots.contiguous(), k, v)
-    return k, v
+    return ref.read(k_cache, v_cache, slots)
 
 
 # ---- plans --------------------------------------------------------------------------------------------------------------
 FEW_ROWS = 16              # rows (tokens x query heads of a group) of a tile for single tokens
 SOME_ROWS = 32             # of a tile for short portions
-MANY_ROWS = 256            # of a tile for portions whose keys are widened first
-MANY_MIN = 128             # rows of a segment from which on that is done
-TARGET_WGS = 1024          # workgroups that a launch of few tiles is split towards
-MANY_WGS = 256             # ... of wide ones (one to a CU)
-MIN_BLOCKS = 4             # blocks of a piece: one for each of a workgroup's waves
-MANY_BLOCKS = 8
-MASS_WHOLE_ROWS = 32       # rows of a segment up to which a wave takes them all for its block of keys
+MANY_ROWS = {128: 256, 64: 128}   # of a tile for portions whose keys are widened first, by head dim (csrc/kv4_tile.hip)
+MANY_WGS = {128: 256, 64: 768}    # workgroups of these that the CUs hold
+MANY_MIN = 128             # rows of a segment from which on its keys may be widened first,
+MANY_WORK = 1 << 29        # and work (pairs of rows and keys, times heads, times dim) of all such segments from which on they are
+MANY_BLOCKS = 8            # blocks of a piece of a wide tile
+CUS = 256
+SHORT_BLOCKS = 32          # blocks a CU up to which a launch is short: workgroups of eight waves, tiles whole
+SHORT_PIECE = 16           # blocks of a piece in it: two for each wave
+LONG_WGS = 1024            # workgroups of four waves that a longer launch is split towards
+LONG_PIECE = 4
+MASS_FEW = 32              # rows of a segment up to which a wave takes them all for its block of keys
+MASS_WGS = 1024
 
 
 class AttnPlan:
@@ -70,10 +72,7 @@ class AttnPlan:
         self.segs: list[tuple[int, int, int, int]] = []
         self.heads = self.kv_heads = self.dim = self.window = self.first = 0
         self.rows = self.covered = self.keys = self.tables = 0
-        # kinds of tiles: (rows of one, items, merges, slots of partial results, tiles of keys to widen first)
-        self.parts: list[tuple[int, torch.Tensor, torch.Tensor, int, torch.Tensor]] = []
-        self.mass_items = None
-        self.mass_whole = 0
+        self.native = None          # what the kernels' callers read (csrc/kv4_bindings.cpp Plan), on a GPU
 
 
 def _blocks(pos, tokens, window: int, first: int):
@@ -91,12 +90,9 @@ def _tiles(segs: np.ndarray, tokens: int):
     return np.stack([segs[s, 0] + i, np.minimum(segs[s, 1] - i, tokens), segs[s, 2] + i, segs[s, 3], s], 1)
 
 
-def _pieces(tiles: np.ndarray, window: int, first: int, kv_heads: int, many: bool = False):
-    """(tile, first block, last + 1, slot) int64 [n, 4], merges int64 [m, 4], slots: tiles of long ranges in pieces of about the same
-    length, if the tiles by themselves are too few workgroups; the longest first."""
-    _, count = _blocks(tiles[:, 2], tiles[:, 1], window, first)
-    size = max(MANY_BLOCKS if many else MIN_BLOCKS, -(-int(count.sum()) * kv_heads // (MANY_WGS if many else TARGET_WGS)))
-    n = np.maximum(1, (count + (size // 2 if many else size - 1)) // size)
+def _pieces(tiles: np.ndarray, count: np.ndarray, n: np.ndarray):
+    """(tile, first block, last + 1, slot) int64 [n, 4], merges int64 [m, 4], slots: tiles of ``count`` blocks in ``n`` pieces each (or fewer), the
+    longest first."""
     each = (count + n - 1) // n
     n = np.maximum(1, (count + each - 1) // each)
     t = np.repeat(np.arange(len(tiles)), n)
@@ -110,20 +106,42 @@ def _pieces(tiles: np.ndarray, window: int, first: int, kv_heads: int, many: boo
     return pieces[np.argsort(pieces[:, 1] - pieces[:, 2], kind="stable")], merges, int(n[split].sum())
 
 
-def _tables(full: np.ndarray, heads: int, kv_heads: int, window: int, first: int):
-    """(shapes, arrays) of ``attn``: of each kind of tiles (rows of one, items, merges, slots, tiles of keys) and its items, merges, tiles of keys."""
+def _narrow_split(count: np.ndarray, kv_heads: int, rows: int) -> tuple[int, np.ndarray]:
+    """(waves of a workgroup, pieces of every tile) for tiles of ``rows`` rows that see ``count`` blocks."""
+    total = int(count.sum()) * kv_heads
+    if rows == FEW_ROWS and total <= SHORT_BLOCKS * CUS:
+        return 8, np.maximum(1, count // max(SHORT_PIECE, -(-total // CUS)))
+    size = max(LONG_PIECE, -(-total // LONG_WGS))
+    return 4, np.maximum(1, (count + size - 1) // size)
+
+
+def _wide_split(count: np.ndarray, kv_heads: int, wgs: int) -> np.ndarray:
+    """Pieces of every wide tile: the nearest whole number to its share of the CUs' work."""
+    size = max(MANY_BLOCKS, -(-int(count.sum()) * kv_heads // wgs))
+    return np.maximum(1, (count + size // 2) // size)
+
+
+def _tables(full: np.ndarray, heads: int, kv_heads: int, dim: int, window: int, first: int):
+    """(shapes, arrays) of ``attn``: of each kind of tiles (rows of one, waves, slots, items, merges, tiles of keys) and its items, merges, tiles of
+    keys."""
     G = heads // kv_heads
     rows = full[:, 1] * G
+    seen = full[:, 2] + (full[:, 1] + 1) // 2                              # keys of the segment's middle row
+    if window:
+        seen = np.minimum(seen, window + first)
+    wide = rows >= MANY_MIN
+    if int((full[:, 1] * seen)[wide].sum()) * heads * dim < MANY_WORK:
+        wide[:] = False
     shapes, arrays = [], []
-    for size, part in ((FEW_ROWS, full[rows <= FEW_ROWS]), (SOME_ROWS, full[(rows > FEW_ROWS) & (rows < MANY_MIN)]),
-                       (MANY_ROWS, full[rows >= MANY_MIN])):
+    for size, part in ((FEW_ROWS, full[(rows <= FEW_ROWS) & ~wide]), (SOME_ROWS, full[(rows > FEW_ROWS) & ~wide]), (MANY_ROWS[dim], full[wide])):
         if not len(part):
             continue
-        many = size == MANY_ROWS
         tiles = _tiles(part, size // G)
-        pieces, merges, slots = _pieces(tiles, window, first, kv_heads, many)
-        t = tiles[pieces[:, 0]]
-        if many:  # a segment's blocks lie one after the other in the workspace, those below the window first
+        _, count = _blocks(tiles[:, 2], tiles[:, 1], window, first)
+        if size > SOME_ROWS:  # a segment's blocks lie one after the other in the workspace, those below the window first
+            waves = 0
+            pieces, merges, slots = _pieces(tiles, count, _wide_split(count, kv_heads, MANY_WGS[dim]))
+            t = tiles[pieces[:, 0]]
             head, count = _blocks(part[:, 2], part[:, 1], window, first)
             tail = head + (part[:, 2] + part[:, 1] - 1) // BLOCK + 1 - count
             base = np.cumsum(count) - count
@@ -133,10 +151,13 @@ def _tables(full: np.ndarray, heads: int, kv_heads: int, window: int, first: int
             s = t[:, 4]
             cols = [t[:, 0], t[:, 1], t[:, 2], base[s], head[s], tail[s]]
         else:
+            waves, n = _narrow_split(count, kv_heads, size)
+            pieces, merges, slots = _pieces(tiles, count, n)
+            t = tiles[pieces[:, 0]]
             keys, cols = np.zeros((0, 4)), [t[:, 0], t[:, 1], t[:, 2], t[:, 3]]
         cols += [pieces[:, 1], pieces[:, 2], pieces[:, 3]]
-        items = np.stack(cols + [np.zeros_like(t[:, 0])] * ((12 if many else 8) - len(cols)), 1)
-        shapes.append((size, len(items), len(merges), slots, len(keys)))
+        items = np.stack(cols + [np.zeros_like(t[:, 0])] * ((12 if len(keys) else 8) - len(cols)), 1)
+        shapes.append((size, waves, slots, len(items), len(merges), len(keys)))
         arrays += [x.astype(np.int32) for x in (items, merges, keys)]
     return shapes, arrays
 
@@ -152,8 +173,10 @@ class _Take:
         return self.flat[self.at - n * cols:self.at].view(n, cols)
 
 
-def _part(take: _Take, rows: int, items: int, merges: int, slots: int, keys: int):
-    return rows, take(items, 12 if keys else 8), take(merges, 4), slots, take(keys, 4)
+def _native(p: AttnPlan, take: _Take, shapes) -> None:
+    p.native = ext().Kv4Plan(p.heads, p.kv_heads, p.dim, p.window, p.first, p.rows, p.covered, p.keys, p.tables)
+    for rows, waves, slots, items, merges, keys in shapes:
+        p.native.add(rows, waves, slots, take(items, 12 if keys else 8), take(merges, 4), take(keys, 4))
 
 
 def _plan(segs, heads: int, kv_heads: int, dim: int, window: int, first: int) -> tuple[AttnPlan, np.ndarray]:
@@ -186,31 +209,31 @@ def attn_plan(segs, heads: int, kv_heads: int, dim: int, window: int = 0, first:
     dev = torch.device(device)
     if dev.type != "cuda":
         return p
-    shapes, arrays = _tables(a[a[:, 1] > 0], heads, kv_heads, p.window, p.first)
+    shapes, arrays = _tables(a[a[:, 1] > 0], heads, kv_heads, dim, p.window, p.first)
+    few = a[:, 1] * (heads // kv_heads) <= MASS_FEW
     nb = (p.keys + BLOCK - 1) // BLOCK
-    whole = a[:, 1] * (heads // kv_heads) <= MASS_WHOLE_ROWS
     mass = []
-    for pick, step in ((whole, 4), (~whole, 1)):
+    for pick, step in ((few, min(32, max(4, -(-nb * int(few.sum()) * kv_heads // MASS_WGS // 4) * 4))), (~few, 1)):
         idx, b = np.nonzero(pick)[0], np.arange(0, nb, step)
         s, b = np.repeat(idx, len(b)), np.tile(b, len(idx))
-        mass.append(np.stack([a[s, 0], a[s, 1], a[s, 2], a[s, 3], s, b, np.full_like(s, nb), np.zeros_like(s)], 1).astype(np.int32))
+        mass.append(np.stack([a[s, 0], a[s, 1], a[s, 2], a[s, 3], s, b, np.minimum(b + step, nb), np.zeros_like(s)], 1).astype(np.int32))
     take = _Take(torch.from_numpy(np.concatenate([t.reshape(-1) for t in arrays + mass])).to(dev))
-    p.parts = [_part(take, *shape) for shape in shapes]
-    p.mass_whole, p.mass_items = len(mass[0]), take(len(mass[0]) + len(mass[1]), 8)
+    _native(p, take, shapes)
+    p.native.weigh(take(len(mass[0]) + len(mass[1]), 8), len(mass[0]), len(a))
     return p
 
 
-STEP_PARTS = 3             # kinds of tiles that a step may have
+STEP_PARTS, STEP_SHAPE = 3, 6   # kinds of tiles that a step may have; numbers that describe one
 
 
 def step_tables(segs, heads: int, kv_heads: int, dim: int) -> np.ndarray:
     """The plan of an engine step as one int32 array, for its upload: what ``step_plan`` reads on the host, then the tables."""
     p, a = _plan(segs, heads, kv_heads, dim, 0, 0)
-    shapes, arrays = _tables(a[a[:, 1] > 0], heads, kv_heads, 0, 0)
-    head = np.zeros(4 + 5 * STEP_PARTS, dtype=np.int32)
+    shapes, arrays = _tables(a[a[:, 1] > 0], heads, kv_heads, dim, 0, 0)
+    head = np.zeros(4 + STEP_SHAPE * STEP_PARTS, dtype=np.int32)
     head[:4] = p.rows, p.covered, p.keys, p.tables
     for i, s in enumerate(shapes):
-        head[4 + 5 * i:9 + 5 * i] = s
+        head[4 + STEP_SHAPE * i:4 + STEP_SHAPE * (i + 1)] = s
     return np.concatenate([head] + [t.reshape(-1) for t in arrays])
 
 
@@ -219,8 +242,8 @@ def step_plan(host: np.ndarray, device: torch.Tensor, heads: int, kv_heads: int,
     p = AttnPlan()
     p.heads, p.kv_heads, p.dim = heads, kv_heads, dim
     p.rows, p.covered, p.keys, p.tables = (int(x) for x in host[:4])
-    take = _Take(device[4 + 5 * STEP_PARTS:])
-    p.parts = [_part(take, *shape) for shape in host[4:4 + 5 * STEP_PARTS].reshape(-1, 5).tolist() if shape[0]]
+    n = 4 + STEP_SHAPE * STEP_PARTS
+    _native(p, _Take(device[n:]), [shape for shape in host[4:n].reshape(-1, STEP_SHAPE).tolist() if shape[0]])
     return p
 
 
@@ -233,35 +256,25 @@ def _check_call(q, k_cache, block_tables, plan: AttnPlan, who: str) -> None:
     if block_tables.dim() != 2 or block_tables.dtype != torch.int32 or block_tables.shape[0] < plan.tables or \
             block_tables.shape[1] * PAGE < plan.keys:
         raise ValueError(f"{who}: int32 block tables of {plan.tables} rows for {plan.keys} keys expected")
-    if _gpu(q) and plan.rows and (not plan.parts or plan.parts[0][1].device != q.device):
-        raise ValueError(f"{who}: the plan was made for another device")
 
 
 def attn(q, k_cache, v_cache, block_tables, plan: AttnPlan, scale: float, out=None, lse=None) -> torch.Tensor:
     """softmax(scale q k^T) v of the plan's rows: q [T, heads, dim] bf16 -> out (a new tensor unless given), the same shape.
     ``lse`` fp32 [T, heads] gets the base-2 logarithm of each row's sum of 2^(scores in base 2). Rows of no segment are left as they
     were (zeros in a new ``out``). Rows whose block table names a page outside of the cache come out as no numbers."""
+    if _gpu(q):
+        if plan.native is None:
+            raise ValueError("kv4.attn: the plan was made for another device")
+        return ext().kv4_attn(q, k_cache, v_cache, block_tables, plan.native, scale, out, lse)
     _check_cache(k_cache, v_cache, "kv4.attn")
     _check_call(q, k_cache, block_tables, plan, "kv4.attn")
     if out is None:
-        out = (torch.empty if plan.covered == q.shape[0] else torch.zeros)(q.shape, dtype=q.dtype, device=q.device)
+        out = torch.zeros(q.shape, dtype=q.dtype)
     elif out.shape != q.shape or out.dtype != q.dtype:
         raise ValueError("kv4.attn: out like q expected")
     if lse is not None and (lse.shape != q.shape[:2] or lse.dtype != torch.float32):
         raise ValueError("kv4.attn: lse fp32 [T, heads] expected")
-    if not _gpu(q):
-        ref.attn(q, k_cache, v_cache, block_tables, plan.segs, plan.window, plan.first, float(scale), out, lse)
-        return out
-    for rows, items, merges, slots, keys in plan.parts:
-        part = plse = ws = None
-        if slots:
-            n = slots * plan.kv_heads * rows
-            part = torch.empty(n * plan.dim, dtype=torch.float32, device=q.device)
-            plse = torch.empty(n, dtype=torch.float32, device=q.device)
-        if rows == MANY_ROWS:
-            ws = torch.empty(keys.shape[0] * plan.kv_heads * 4 * BLOCK * plan.dim, dtype=torch.uint8, device=q.device)
-        ext().kv4_attn(q, k_cache, v_cache, block_tables, rows, items, merges, plan.window, plan.first, float(scale), out, lse, part,
-                       plse, slots, keys if ws is not None else None, ws)
+    ref.attn(q, k_cache, v_cache, block_tables, plan.segs, plan.window, plan.first, float(scale), out, lse)
     return out
 
 
@@ -270,30 +283,26 @@ def attn_mass(q, lse, k_cache, block_tables, plan: AttnPlan, scale: float, base=
     2^(score - lse), fp32 [segments, kv heads, keys], with ``lse`` from ``attn`` over the same rows. ``out`` may be ``base``: weights that
     accumulate from step to step. Without either, a new tensor as wide as the plan's longest sequence. A key's sum is always formed in
     the same order."""
+    if _gpu(q):
+        if plan.native is None:
+            raise ValueError("kv4.attn_mass: the plan was made for another device")
+        return ext().kv4_mass(q, lse, k_cache, block_tables, plan.native, scale, base, out)
     _check_cache(k_cache, k_cache, "kv4.attn_mass")
     _check_call(q, k_cache, block_tables, plan, "kv4.attn_mass")
     if lse.shape != q.shape[:2] or lse.dtype != torch.float32:
         raise ValueError("kv4.attn_mass: lse fp32 [T, heads] expected")
-    if _gpu(q) and (plan.mass_items is None or plan.mass_items.device != q.device):
-        raise ValueError("kv4.attn_mass: a plan of attn_plan for this device expected")
     like = base if base is not None else out
     shape = (len(plan.segs), plan.kv_heads, like.shape[2] if like is not None and like.dim() == 3 else plan.keys)
     for t in (base, out):
         if t is not None and (t.shape != shape or t.dtype != torch.float32 or not t.is_contiguous() or t.shape[2] < plan.keys):
             raise ValueError(f"kv4.attn_mass: base and out contiguous fp32 [segments, kv heads, at least {plan.keys}], alike, expected")
     if out is None:
-        out = torch.empty(shape, dtype=torch.float32, device=q.device)
-    if not _gpu(q):
-        if base is None:
-            out.zero_()
-        elif base is not out:
-            out.copy_(base)
-        ref.attn_mass(q, lse, k_cache, block_tables, plan.segs, plan.window, plan.first, float(scale), out)
-        return out
-    done = -(-plan.keys // BLOCK) * BLOCK
-    if shape[2] > done and base is not out:     # (behind the plan's last block nothing is added)
-        out[:, :, done:].copy_(base[:, :, done:]) if base is not None else out[:, :, done:].zero_()
-    ext().kv4_mass(q, lse, k_cache, block_tables, plan.mass_items, plan.mass_whole, plan.window, plan.first, float(scale), base, out, shape[0])
+        out = torch.empty(shape, dtype=torch.float32)
+    if base is None:
+        out.zero_()
+    elif base is not out:
+        out.copy_(base)
+    ref.attn_mass(q, lse, k_cache, block_tables, plan.segs, plan.window, plan.first, float(scale), out)
     return out
 
 
@@ -302,18 +311,14 @@ def evict_keep(mass: torch.Tensor, lens: torch.Tensor, budget: int, first: int =
     """The keys that stay, int32 [sequences, kv heads, budget], ascending, per head: of a sequence of ``lens`` keys the ``first`` ones,
     the ``recent`` last ones, and of the rest those of the largest ``mass`` [sequences, kv heads, keys] fp32 (equal masses: the
     lowest index; not a number: after all others). Sequences within the budget keep everything, -1 behind their last."""
+    if _gpu(mass):
+        return ext().kv4_evict_keep(mass, lens, budget, first, recent)
     if mass.dim() != 3 or mass.dtype != torch.float32 or lens.shape != (mass.shape[0],) or lens.dtype != torch.int32 or \
             lens.device != mass.device:
         raise ValueError("kv4.evict_keep: mass fp32 [sequences, kv heads, keys] and lens int32 [sequences] on its device expected")
     if budget < 1 or first < 0 or recent < 0 or first + recent > budget or budget >= MAX_POS:
         raise ValueError("kv4.evict_keep: first and recent keys within a budget of at least one")
-    if not _gpu(mass):
-        return ref.evict_keep(mass, lens, int(budget), int(first), int(recent))
-    if mass.stride(2) != 1 and mass.shape[2] > 1:
-        mass = mass.contiguous()
-    kept = torch.empty(mass.shape[0], mass.shape[1], int(budget), dtype=torch.int32, device=mass.device)
-    ext().kv4_evict_keep(mass, lens.contiguous(), int(budget), int(first), int(recent), kept)
-    return kept
+    return ref.evict_keep(mass, lens, int(budget), int(first), int(recent))
 
 
 def evict(k_cache, v_cache, block_tables, kept, new_tables, mass=None):
@@ -322,6 +327,8 @@ def evict(k_cache, v_cache, block_tables, kept, new_tables, mass=None):
     (which other sequences may share, and which their owner may free afterwards); places behind a sequence's last key are left as they
     were, as are keys whose index, or whose page, is outside. Returns the kept keys' ``mass`` [sequences, kv heads, budget]
     (zero behind the last) if it is given, else None."""
+    if _gpu(k_cache):
+        return ext().kv4_evict_copy(k_cache, v_cache, block_tables, kept, new_tables, mass)
     _check_cache(k_cache, v_cache, "kv4.evict")
     if kept.dim() != 3 or kept.dtype != torch.int32 or kept.shape[1] != k_cache.shape[1]:
         raise ValueError("kv4.evict: kept int32 [sequences, kv heads, budget] expected")
@@ -330,11 +337,6 @@ def evict(k_cache, v_cache, block_tables, kept, new_tables, mass=None):
             raise ValueError("kv4.evict: int32 tables [sequences, pages] expected")
     if mass is not None and (mass.dim() != 3 or mass.shape[:2] != kept.shape[:2] or mass.dtype != torch.float32):
         raise ValueError("kv4.evict: mass fp32 [sequences, kv heads, keys] expected")
-    new_mass = torch.empty(kept.shape, dtype=torch.float32, device=kept.device) if mass is not None else None
-    if not _gpu(k_cache):
-        ref.evict_copy(k_cache, v_cache, block_tables, kept, new_tables, mass, new_mass)
-        return new_mass
-    if mass is not None and mass.stride(2) != 1 and mass.shape[2] > 1:
-        mass = mass.contiguous()
-    ext().kv4_evict_copy(k_cache, v_cache, block_tables, kept.contiguous(), new_tables, mass, new_mass)
+    new_mass = torch.empty(kept.shape, dtype=torch.float32) if mass is not None else None
+    ref.evict_copy(k_cache, v_cache, block_tables, kept, new_tables, mass, new_mass)
     return new_mass

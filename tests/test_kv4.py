@@ -441,7 +441,9 @@ def test_plan_covers_every_block_once():
         tok = 1 + r(16)
         tiles = kv4._tiles(segs, tok)
         assert sum(t[1] for t in tiles) == segs[:, 1].sum() and max(t[1] for t in tiles) <= tok
-        pieces, merges, slots = kv4._pieces(tiles, window, first, 2, bool(r(2)))
+        _, count = kv4._blocks(tiles[:, 2], tiles[:, 1], window, first)
+        n = (kv4._narrow_split(count, 2, 16 + 16 * r(2))[1], kv4._wide_split(count, 2, 256), np.array([1 + r(9) for _ in tiles]))[r(3)]
+        pieces, merges, slots = kv4._pieces(tiles, count, n)
         seen = {}
         for t, lo, hi, slot in pieces.tolist():
             assert lo < hi
@@ -501,14 +503,22 @@ def test_writer_on_the_gpu(cuda, T, Hq, H, D, slab, special):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("wide", [False, True])
 @pytest.mark.parametrize("case", CASES, ids=_id)
-def test_attention_on_the_gpu(cuda, case):
+def test_attention_on_the_gpu(cuda, monkeypatch, case, wide):
+    """Every kind of tile, whatever the sizes from which on a plan takes it."""
+    if wide:
+        monkeypatch.setattr(kv4, "MANY_WORK", 0)
+        monkeypatch.setattr(kv4, "SHORT_BLOCKS", 0)
+    else:
+        monkeypatch.setattr(kv4, "MANY_WORK", 1 << 60)
     _check_attention(case, cuda)
 
 
 @pytest.mark.gpu
-def test_attention_again_is_the_same(cuda):
+def test_attention_again_is_the_same(cuda, monkeypatch):
     """Bit for bit, whatever ran in between; on another stream; as rows of a wider tensor."""
+    monkeypatch.setattr(kv4, "MANY_WORK", 0)
     segs = [(0, 1, 3000, 0), (1, 40, 500, 1), (41, 1, 70, 2)]
     kc, vc, tables = world(segs, 2, 128, 0, cuda)
     q = queries(42, 8, 128, 1, cuda)
@@ -653,11 +663,11 @@ def test_refusals_on_the_gpu(cuda):
         kv4.attn(q, kc, vc, bt, kv4.attn_plan([(0, 2, 30, 1)], 8, 2, 128, device="cpu"), 0.1)
     odd = torch.zeros(2 * 8 * 128 + 4, dtype=torch.bfloat16, device=cuda)[4:].view(2, 8, 128)
     for args in ((odd, kc, vc, bt), (q, kc, vc, bt.cpu()), (q, kc, vc.cpu(), bt)):
-        with pytest.raises(RuntimeError):
+        with pytest.raises(ValueError):
             kv4.attn(*args, plan, 0.1)
-    with pytest.raises(RuntimeError):
+    with pytest.raises(ValueError):
         kv4.read(kc, vc, torch.zeros(3, dtype=torch.int64))
-    with pytest.raises(RuntimeError):
+    with pytest.raises(ValueError):
         ops.rope_kv_write(torch.zeros(2, 100, dtype=torch.bfloat16, device=cuda), torch.zeros(2, dtype=torch.long, device=cuda),
                           torch.zeros(9, 128, device=cuda), q, kc, vc, None, 8, 2)
     kv4.attn(q, kc, vc, bt, plan, 0.1)
@@ -718,28 +728,33 @@ def test_engine_on_the_gpu(cuda):
     _engine("small-llama", str(cuda), 0.25)
 
 
-def test_step_plan_is_the_plan():
-    """An engine step's tables, as uploaded, are those of attn_plan."""
-    segs = [(0, 1, 500, 0), (1, 1, 33, 1), (2, 77, 9, 2), (79, 3, 4000, 3), (82, 10, 70, 4)]
-    flat = kv4.step_tables(segs, 8, 2, 128)
-    p = kv4.step_plan(flat, torch.from_numpy(flat), 8, 2, 128)
-    shapes, arrays = kv4._tables(kv4._plan(segs, 8, 2, 128, 0, 0)[1], 8, 2, 0, 0)
-    assert [(r, len(i), len(m), s, len(k)) for r, i, m, s, k in p.parts] == shapes and len(shapes) == 3
-    for (_, items, merges, _, keys), (a, b, c) in zip(p.parts, zip(*(arrays[i::3] for i in range(3)))):
-        assert (items.numpy() == a).all() and (merges.numpy() == b).all() and (keys.numpy() == c).all()
-    assert (p.rows, p.covered, p.keys, p.tables) == (92, 92, 4003, 5)
+@pytest.mark.gpu
+def test_step_plan_is_the_plan(cuda):
+    """An engine step's tables, as uploaded, give what attn_plan's give."""
+    segs = [(0, 1, 500, 0), (1, 1, 33, 1), (2, 177, 900, 2), (179, 3, 4000, 3), (182, 10, 70, 4)]
+    flat = kv4.step_tables(segs, 32, 2, 128)
+    p = kv4.step_plan(flat, torch.from_numpy(flat).to(cuda), 32, 2, 128)
+    assert (p.rows, p.covered, p.keys, p.tables) == (192, 192, 4003, 5)
+    assert [s[0] for s in kv4._tables(kv4._plan(segs, 32, 2, 128, 0, 0)[1], 32, 2, 128, 0, 0)[0]] == [16, 32, 256]
+    kc, vc, tables = world(segs, 2, 128, 0, cuda)
+    q = queries(192, 32, 128, 1, cuda)
+    want = kv4.attn(q, kc, vc, tables, kv4.attn_plan(segs, 32, 2, 128, device=cuda), 0.1)
+    assert torch.equal(kv4.attn(q, kc, vc, tables, p, 0.1), want)
+    with pytest.raises(ValueError):
+        kv4.attn_mass(q, torch.zeros(192, 32, device=cuda), kc, tables, p, 0.1)
 
 
-def test_widened_keys_are_those_that_a_tile_sees():
+def test_widened_keys_are_those_that_a_tile_sees(monkeypatch):
     """Every block of a wide tile's list is at its place among its segment's in the workspace."""
     import numpy as np
 
     g = torch.Generator().manual_seed(1)
     r = lambda hi: int(torch.randint(0, hi, (1,), generator=g))
+    monkeypatch.setattr(kv4, "MANY_WORK", 0)
     for _ in range(100):
         segs = np.array([(1000 * i, 33 + r(400), r(6000), 10 + i) for i in range(1 + r(4))])
         window, first = (0, 0) if r(3) == 0 else (1 + r(1500), r(300))
-        shapes, (items, merges, keys) = kv4._tables(segs, 8, 2, window, first)
+        shapes, (items, merges, keys) = kv4._tables(segs, 8, 2, 128, window, first)
         assert [s[0] for s in shapes] == [256]
         for row, n, pos, base, head, tail, lo, hi, _, *_ in items.tolist():
             t, f = max(0, pos - window + 1) // 64 if window else 0, 0
