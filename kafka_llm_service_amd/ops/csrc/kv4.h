@@ -44,6 +44,16 @@ __device__ __forceinline__ uint32_t narrow8(bf16x8 x, float sc) {
   return w;
 }
 
+typedef int i32x8 __attribute__((ext_vector_type(8)));
+
+// a [16 rows][128] in e2m1, a lane's 32 elements of k = 32 (l >> 4) on in its first four words, times 2^(sa - 127); b [128][16 columns] in e4m3, a
+// lane's elements of k = 16 (l >> 4) on and of 64 + 16 (l >> 4) on, the block of k = 32 (l >> 4) on times 2^(sb - 127) of that lane.
+// (The compiler does not know that the product needs every lane of its operands: results are pinned where control flow is uniform.)
+__device__ __forceinline__ f32x4 mfma4x8(const uint32_t* a, uint32_t sa, i32x8 b, uint32_t sb, f32x4 c) {
+  const i32x8 x = {(int)a[0], (int)a[1], (int)a[2], (int)a[3], 0, 0, 0, 0};
+  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(x, b, c, 4, 0, 0, (int)sa, 0, (int)sb);
+}
+
 __device__ __forceinline__ f32x4 mfma16(bf16x8 a, bf16x8 b, f32x4 c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
 }

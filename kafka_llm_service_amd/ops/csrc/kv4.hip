@@ -133,16 +133,42 @@ __device__ __forceinline__ uint32_t rank_of(float x) {
   return a == 0u ? 0x80000000u : (b & 0x80000000u) ? ~b : b | 0x80000000u;
 }
 
-constexpr int KEEP_NT = 1024;
+constexpr int KEEP_NT = 1024, KEEP_NW = KEEP_NT / 64, KEEP_PER = 16;
+
+// Exclusive sum over the workgroup's threads, and the whole. ``ws`` holds KEEP_NW ints and is free again behind the next barrier.
+__device__ __forceinline__ int before_thread(int x, int* ws, int& all) {
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  int inc = x;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const int y = __shfl_up(inc, o, 64);
+    if (lane >= o) inc += y;
+  }
+  if (lane == 63) ws[w] = inc;
+  __syncthreads();
+  int at = inc - x;
+  all = 0;
+#pragma unroll
+  for (int i = 0; i < KEEP_NW; ++i) {
+    if (i < w) at += ws[i];
+    all += ws[i];
+  }
+  return at;
+}
 
 // Kept keys of one (sequence, head), ascending: the first ones, the most recent ones, and of those between them the ``room`` largest, ties to
-// the lowest index. Radix select: four counts of a byte each narrow the threshold down, then one ordered pass writes.
+// the lowest index. Radix select: four counts of a byte each narrow the threshold down, then the keys are numbered in order. A thread
+// holds KEEP_PER neighbouring keys; of longer sequences (REG false) they are read again, a chunk of KEEP_NT * KEEP_PER at a time. Each wave counts for
+// itself: the leading byte has few values, and 1024 threads at one counter wait for each other.
+template <bool REG>
 __global__ __launch_bounds__(KEEP_NT) void evict_keep_kernel(const float* __restrict__ mass, int64_t ms, int64_t mh, int N,
                                                              const int* __restrict__ lens, int budget, int first, int recent,
                                                              int* __restrict__ kept, int Hkv) {
-  __shared__ int hist[256];
+  constexpr int PER = KEEP_PER, CHUNK = KEEP_NT * PER;
+  __shared__ int hist[KEEP_NW][257];                                     // (a wave's counters a bank further than the last one's)
+  __shared__ int total[256];
   __shared__ int s_digit, s_above;
-  __shared__ int wsum[2][KEEP_NT / 64];
+  __shared__ int ws[2][KEEP_NW];
   const int h = blockIdx.x, r = blockIdx.y, tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
   const float* m = mass + r * ms + h * mh;
   int* out = kept + ((int64_t)r * Hkv + h) * budget;
@@ -152,19 +178,39 @@ __global__ __launch_bounds__(KEEP_NT) void evict_keep_kernel(const float* __rest
     return;
   }
   const int a = first, b = n - recent, room = budget - first - recent;   // (b - a = n - budget + room > room)
+  const int per = REG ? (n + KEEP_NT - 1) / KEEP_NT : PER;               // keys a thread, up to PER
+  uint32_t key[PER];
+  auto load = [&](int i0) {
+#pragma unroll
+    for (int k = 0; k < PER; ++k) {
+      const int i = i0 + tid * per + k;
+      key[k] = k < per && i >= a && i < b ? rank_of(m[i]) : 0u;
+    }
+  };
+  if (REG) load(0);
   uint32_t lead = 0, known = 0;
   int need = room;                                                       // of those with the leading digits of the threshold
   for (int shift = 24; shift >= 0 && need > 0; shift -= 8) {
-    if (tid < 256) hist[tid] = 0;
+    for (int i = lane; i < 256; i += 64) hist[w][i] = 0;                 // (a wave's own: no barrier)
+    for (int i0 = 0; i0 < (REG ? 1 : n); i0 += CHUNK) {
+      if (!REG) load(i0);
+#pragma unroll
+      for (int k = 0; k < PER; ++k) {
+        const int i = i0 + tid * per + k;
+        if (k < per && i >= a && i < b && (key[k] & known) == lead) atomicAdd(&hist[w][(key[k] >> shift) & 255], 1);
+      }
+    }
     __syncthreads();
-    for (int i = a + tid; i < b; i += KEEP_NT) {
-      const uint32_t k = rank_of(m[i]);
-      if ((k & known) == lead) atomicAdd(&hist[(k >> shift) & 255], 1);
+    if (tid < 256) {
+      int c = 0;
+#pragma unroll
+      for (int i = 0; i < KEEP_NW; ++i) c += hist[i][tid];
+      total[tid] = c;
     }
     __syncthreads();
     if (w == 0) {                                                        // four digits a lane, from the largest down
       const int d0 = 255 - 4 * lane;
-      const int c0 = hist[d0], c1 = hist[d0 - 1], c2 = hist[d0 - 2], c3 = hist[d0 - 3];
+      const int c0 = total[d0], c1 = total[d0 - 1], c2 = total[d0 - 2], c3 = total[d0 - 3];
       int inc = c0 + c1 + c2 + c3;
       for (int o = 1; o < 64; o <<= 1) {
         const int y = __shfl_up(inc, o, 64);
@@ -193,95 +239,115 @@ __global__ __launch_bounds__(KEEP_NT) void evict_keep_kernel(const float* __rest
     lead |= (uint32_t)s_digit << shift;
     known |= 255u << shift;
     need -= s_above;
-    __syncthreads();
   }
   // ``lead`` is the threshold: everything above it stays, and the first ``need`` of its equals (room 0: nothing between the two ends)
-  int ties = 0, done = 0;                                                // before this chunk
-  for (int i0 = 0; i0 < n; i0 += KEEP_NT) {
-    const int i = i0 + tid;
-    const bool fixed = i < a || (i >= b && i < n), mid = i >= a && i < b && room > 0;
-    const uint32_t k = mid ? rank_of(m[i]) : 0u;
-    const bool above = mid && k > lead, tie = mid && k == lead;
-    const uint64_t tb = __ballot(tie);
-    if (lane == 0) wsum[0][w] = __popcll(tb);
-    __syncthreads();
-    int tr = ties, tall = 0;
-    for (int x = 0; x < KEEP_NT / 64; ++x) {
-      if (x < w) tr += wsum[0][x];
-      tall += wsum[0][x];
+  int ties = 0, done = 0;                                                // in front of this chunk
+  for (int i0 = 0; i0 < n; i0 += CHUNK) {
+    if (!REG) load(i0);
+    int mine = 0, all;
+#pragma unroll
+    for (int k = 0; k < PER; ++k) {
+      const int i = i0 + tid * per + k;
+      mine += k < per && room > 0 && i >= a && i < b && key[k] == lead;
     }
-    tr += __popcll(tb & ((1ull << lane) - 1));
-    const bool keep = fixed || above || (tie && tr < need);
-    const uint64_t kb = __ballot(keep);
-    if (lane == 0) wsum[1][w] = __popcll(kb);
-    __syncthreads();
-    int at = done, kall = 0;
-    for (int x = 0; x < KEEP_NT / 64; ++x) {
-      if (x < w) at += wsum[1][x];
-      kall += wsum[1][x];
+    int rank = ties + before_thread(mine, ws[0], all);
+    ties += all;
+    uint32_t keep = 0;
+    int count = 0;
+#pragma unroll
+    for (int k = 0; k < PER; ++k) {
+      const int i = i0 + tid * per + k;
+      if (k >= per || i >= n) continue;
+      const bool mid = i >= a && i < b;
+      bool yes = !mid;
+      if (mid && room > 0) {
+        yes = key[k] > lead || (key[k] == lead && rank < need);
+        rank += key[k] == lead;
+      }
+      keep |= (uint32_t)yes << k;
+      count += yes;
     }
-    at += __popcll(kb & ((1ull << lane) - 1));
-    if (keep && at < budget) out[at] = i;
-    ties += tall;
-    done += kall;
+    int at = done + before_thread(count, ws[1], all);
+    done += all;
+#pragma unroll
+    for (int k = 0; k < PER; ++k)
+      if ((keep >> k) & 1) {
+        if (at < budget) out[at] = i0 + tid * per + k;
+        ++at;
+      }
   }
 }
 
-// Kept keys, values and masses into new pages, a wave per new page and head. K goes by 16-byte pieces, V by the words of its keys.
-// Keys outside of their table or cache leave their place in the new page as it was.
+// Kept keys, values and masses into new pages, a wave for four new pages of a head. K goes by
+// 16-byte pieces, V by the words of its keys. Keys outside of their table or cache leave their place in the new page as it was.
 template <int D>
 __global__ __launch_bounds__(256) void evict_copy_kernel(uint8_t* __restrict__ kc, uint8_t* __restrict__ vc, int64_t n_pages,
                                                          const int* __restrict__ tables, int tw, int64_t ts, const int* __restrict__ kept,
                                                          int budget, const int* __restrict__ new_tables, int nw, int64_t ns, int Hkv,
                                                          const float* __restrict__ mass, int64_t ms, int64_t mh, int N,
                                                          float* __restrict__ new_mass) {
-  constexpr int U = D / 8, KP = D / 32;     // words of a key; 16-byte pieces of it
+  constexpr int U = D / 8, KP = D / 32, BYTES = Page<D>::BYTES, DATA = Page<D>::DATA;   // words of a key; 16-byte pieces of it
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-  const int h = blockIdx.y, r = blockIdx.z, pg = blockIdx.x * 4 + w;
-  const int i0 = pg * PAGE;
+  const int h = blockIdx.y, r = blockIdx.z, i0 = (blockIdx.x * 4 + w) * 64;
   if (i0 >= budget) return;
-  const int* kp = kept + ((int64_t)r * Hkv + h) * budget + i0;
-  const int o = lane & 15;
-  int src = i0 + o < budget ? kp[o] : -1;   // lane o: the page's key o
-  if (new_mass && lane < 16 && i0 + o < budget)
-    new_mass[((int64_t)r * Hkv + h) * budget + i0 + o] = src >= 0 && src < N ? mass[r * ms + h * mh + src] : 0.f;
-  int64_t from = -1;                        // its page and head, in pages
+  const int64_t row = ((int64_t)r * Hkv + h) * budget;
+  // lane = key: where it is and where its page goes (-1: nowhere), in pages and heads
+  const int src = i0 + lane < budget ? kept[row + i0 + lane] : -1;
+  const int np = (i0 + lane) / PAGE < nw && i0 + lane < budget ? new_tables[r * ns + (i0 + lane) / PAGE] : -1;
+  int64_t from = -1;
   if (src >= 0 && (src >> 4) < tw) {
     const int p = tables[r * ts + (src >> 4)];
     if (p >= 0 && p < n_pages) from = (int64_t)p * Hkv + h;
   }
-  if (pg >= nw) return;
-  const int np = new_tables[r * ns + pg];
-  if (np < 0 || np >= n_pages) return;
-  const int so = src & 15;
-  uint8_t* kd = kc + ((int64_t)np * Hkv + h) * Page<D>::BYTES;
-  uint8_t* vd = vc + ((int64_t)np * Hkv + h) * Page<D>::BYTES;
+  if (np < 0 || np >= n_pages) from = -1;
+  const int64_t to = (int64_t)np * Hkv + h;
+  const int so = src & 15, o = lane & 15;
+  if (new_mass && i0 + lane < budget) new_mass[row + i0 + lane] = src >= 0 && src < N ? mass[r * ms + h * mh + src] : 0.f;
   auto of = [&](int64_t x, int l) {
     return (int64_t)(uint32_t)__shfl((int)(uint32_t)x, l, 64) | (int64_t)__shfl((int)(x >> 32), l, 64) << 32;
   };
-  // K: lane = (key, piece)
-  const int key = lane / KP, pc = lane % KP;
-  const int64_t kf = of(from, key & 15);
-  const int ko = __shfl(so, key & 15, 64);
-  if (key < 16 && kf >= 0)
-    *reinterpret_cast<u32x4*>(kd + key * (D / 2) + pc * 16) =
-        *reinterpret_cast<const u32x4*>(kc + kf * Page<D>::BYTES + ko * (D / 2) + pc * 16);
-  // V: lane = (four keys, eight elements)
-  const int c = lane / U, p = lane % U;
+  const int kk = lane / KP, kp = lane % KP, c = lane / U, p = lane % U;
+#pragma unroll 2
+  for (int g = 0; g < 4; ++g) {
+    const int64_t t = of(to, 16 * g) * BYTES;   // (the page of the group's first key)
+    u32x4 k, v;
+    int there = 0;
+    {                                           // K: lane = (key, piece)
+      const int l = 16 * g + (kk & 15), s = __shfl(so, l, 64);
+      const int64_t f = of(from, l);
+      if (kk < 16 && f >= 0) {
+        k = *reinterpret_cast<const u32x4*>(kc + f * BYTES + s * (D / 2) + kp * 16);
+        there = 16;
+      }
+    }
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int k4 = (4 * c + i) & 15;
-    const int64_t vf = of(from, k4);
-    const int vo = __shfl(so, k4, 64);
-    if (c < 4 && vf >= 0)
-      *reinterpret_cast<uint32_t*>(vd + (c * U + p) * 16 + i * 4) =
-          *reinterpret_cast<const uint32_t*>(vc + vf * Page<D>::BYTES + ((vo >> 2) * U + p) * 16 + (vo & 3) * 4);
+    for (int i = 0; i < 4; ++i) {               // V: lane = (four keys, eight elements)
+      const int l = 16 * g + ((4 * c + i) & 15), s = __shfl(so, l, 64);
+      const int64_t f = of(from, l);
+      if (c < 4 && f >= 0) {
+        v[i] = *reinterpret_cast<const uint32_t*>(vc + f * BYTES + ((s >> 2) * U + p) * 16 + (s & 3) * 4);
+        there |= 1 << i;
+      }
+    }
+    if (there & 16) *reinterpret_cast<u32x4*>(kc + t + kk * (D / 2) + kp * 16) = k;
+    uint8_t* vd = vc + t + (c * U + p) * 16;
+    if ((there & 15) == 15) *reinterpret_cast<u32x4*>(vd) = v;
+    else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if ((there >> i) & 1) *reinterpret_cast<uint32_t*>(vd + 4 * i) = v[i];
+    }
   }
-  // scales: lane = (group, key)
-  const int g = lane >> 4;
-  if (g < D / 32 && from >= 0) {
-    kd[Page<D>::DATA + o * (D / 32) + g] = kc[from * Page<D>::BYTES + Page<D>::DATA + so * (D / 32) + g];
-    vd[Page<D>::DATA + g * 16 + o] = vc[from * Page<D>::BYTES + Page<D>::DATA + g * 16 + so];
+  if (from >= 0) {                              // scales: lane = key
+    const uint8_t *kf = kc + from * BYTES + DATA, *vf = vc + from * BYTES + DATA;
+    uint8_t *kd = kc + to * BYTES + DATA, *vd = vc + to * BYTES + DATA;
+    if constexpr (D == 128) *reinterpret_cast<uint32_t*>(kd + o * 4) = *reinterpret_cast<const uint32_t*>(kf + so * 4);
+    else *reinterpret_cast<uint16_t*>(kd + o * 2) = *reinterpret_cast<const uint16_t*>(kf + so * 2);
+    uint8_t vs[KP];
+#pragma unroll
+    for (int g = 0; g < KP; ++g) vs[g] = vf[g * 16 + so];
+#pragma unroll
+    for (int g = 0; g < KP; ++g) vd[g * 16 + o] = vs[g];
   }
 }
 
@@ -319,7 +385,10 @@ extern "C" hipError_t kafka_kv4_evict_keep(const float* mass, int64_t ms, int64_
                                            int first, int recent, int* kept, hipStream_t st) {
   if (R == 0 || budget == 0) return hipSuccess;
   if (first < 0 || recent < 0 || (int64_t)first + recent > budget || R > 65535) return hipErrorInvalidValue;
-  evict_keep_kernel<<<dim3(Hkv, R), KEEP_NT, 0, st>>>(mass, ms, mh, N, lens, budget, first, recent, kept, Hkv);
+  if (N <= KEEP_NT * KEEP_PER)
+    evict_keep_kernel<true><<<dim3(Hkv, R), KEEP_NT, 0, st>>>(mass, ms, mh, N, lens, budget, first, recent, kept, Hkv);
+  else
+    evict_keep_kernel<false><<<dim3(Hkv, R), KEEP_NT, 0, st>>>(mass, ms, mh, N, lens, budget, first, recent, kept, Hkv);
   return hipGetLastError();
 }
 
@@ -329,7 +398,7 @@ extern "C" hipError_t kafka_kv4_evict_copy(uint8_t* kc, uint8_t* vc, int64_t n_p
   if (R == 0 || budget == 0) return hipSuccess;
   if ((D != 64 && D != 128) || R > 65535 || Hkv > 65535) return hipErrorInvalidValue;
   auto go = [&](auto kern) {
-    kern<<<dim3((budget + 63) / 64, Hkv, R), 256, 0, st>>>(kc, vc, n_pages, tables, tw, ts, kept, budget, new_tables, nw, ns, Hkv, mass, ms,
+    kern<<<dim3((budget + 255) / 256, Hkv, R), 256, 0, st>>>(kc, vc, n_pages, tables, tw, ts, kept, budget, new_tables, nw, ns, Hkv, mass, ms,
                                                            mh, N, new_mass);
     return hipGetLastError();
   };

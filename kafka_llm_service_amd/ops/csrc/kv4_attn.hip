@@ -63,9 +63,8 @@ struct Blocks {
   __device__ __forceinline__ int operator[](int v) const { return v < head ? v : v - head + tail; }
 };
 
-template <int D>
 struct KFrag {
-  uint32_t d[4][D / 32];   // a lane's words of four tiles of 16 keys
+  uint32_t d[4][4];        // a lane's 32 elements in each of four tiles of 16 keys
   uint32_t s[4];
 };
 struct VFrag {
@@ -73,34 +72,36 @@ struct VFrag {
   uint32_t s[4];
 };
 
-// Page ids of block b; keys behind ``last`` take its page (they are masked). An id that is not of the cache counts as page 0 and
-// sets ``bad``: such rows come out as no numbers.
-__device__ __forceinline__ void block_pages(const int* bt, int b, int last, int64_t n_pages, int (&pg)[4], bool& bad) {
+// Page ids of 16 blocks of 4 pages, a lane each (keys behind ``last`` take its page: they are masked). One load for them all, ahead of
+// their use: an id that is fetched in front of its page's loads adds a round trip to every block.
+struct PageIds {
+  int v = 0;
+  __device__ __forceinline__ PageIds() {}
+  template <class Of>
+  __device__ __forceinline__ PageIds(const int* bt, int last, int lane, Of block) : v(bt[min(block(lane >> 2) * 4 + (lane & 3), last >> 4)]) {}
+  // Those of the k-th block. An id that is not of the cache counts as page 0 and sets ``bad``: such rows come out as no numbers.
+  __device__ __forceinline__ void get(int k, int64_t n_pages, int (&pg)[4], bool& bad) const {
 #pragma unroll
-  for (int t = 0; t < 4; ++t) {
-    const int p = bt[min(b * 4 + t, last >> 4)];
-    const bool ok = p >= 0 && p < n_pages;
-    bad |= !ok;
-    pg[t] = ok ? p : 0;
+    for (int t = 0; t < 4; ++t) {
+      const int p = __builtin_amdgcn_readlane(v, k * 4 + t);
+      const bool ok = p >= 0 && p < n_pages;
+      bad |= !ok;
+      pg[t] = ok ? p : 0;
+    }
   }
-}
+};
 
+// (heads of 64: both halves of the lanes hold the key, for the two parts of Q)
 template <int D>
-__device__ __forceinline__ void load_k(KFrag<D>& f, const uint8_t* kc, int Hkv, int h, const int (&pg)[4], int lane) {
-  const int key = lane & 15, c = lane >> 4;
+__device__ __forceinline__ void load_k(KFrag& f, const uint8_t* kc, int Hkv, int h, const int (&pg)[4], int lane) {
+  const int key = lane & 15, g = (lane >> 4) & (D / 32 - 1);
 #pragma unroll
   for (int t = 0; t < 4; ++t) {
     const uint8_t* p = kc + ((int64_t)pg[t] * Hkv + h) * Page<D>::BYTES;
-    if constexpr (D == 128) {
-      const u32x4 x = *reinterpret_cast<const u32x4*>(p + key * 64 + c * 16);
+    const u32x4 x = *reinterpret_cast<const u32x4*>(p + key * (D / 2) + g * 16);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) f.d[t][i] = x[i];
-    } else {
-      const u32x2 x = *reinterpret_cast<const u32x2*>(p + key * 32 + c * 8);
-      f.d[t][0] = x[0];
-      f.d[t][1] = x[1];
-    }
-    f.s[t] = p[Page<D>::DATA + key * (D / 32) + c * (D / 32) / 4];
+    for (int i = 0; i < 4; ++i) f.d[t][i] = x[i];
+    f.s[t] = p[Page<D>::DATA + key * (D / 32) + g];
   }
 }
 
@@ -115,50 +116,100 @@ __device__ __forceinline__ void load_v(VFrag& f, const uint8_t* vc, int Hkv, int
   }
 }
 
+// Q in e4m3, so that the matrix cores take the keys in four bits as they lie: 2^-u q = hi + lo / 16, hi the nearest e4m3, u so that the row's
+// largest element comes to 128 .. 256. A bf16 number has eight bits of mantissa, hi takes four of them and lo the rest, so the
+// sum is exact down to 2^-14 of the largest element, and off by at most 2^-21 of it below.
+template <int D>
+struct QFrag {
+  i32x8 x[D / 64];          // heads of 128: hi, lo; of 64: both in one, a half of k each
+  uint32_t s[D / 64];
+};
+
 template <int D, int NQ>
 struct Rows {
-  bf16x8 q[NQ][D / 32];
+  QFrag<D> q[NQ];
   int lim[NQ];              // a column's position; -1: no row
   f32x4 o[NQ][D / 16];      // register i of tile n: d = (D / 16) (4 c + i) + n
   float m[NQ], l[NQ];       // maximum so far (times scale, log2), this lane's part of the sum
 };
 
-// Q's fragments of 16 columns from column R0 of the tile on
+// 16 columns from column R0 of the tile on
 template <int D>
-__device__ __forceinline__ int load_q(bf16x8 (&q)[D / 32], const Args& a, int row, int tokens, int pos, int h, int R0, int lane) {
-  const int R = R0 + (lane & 15), tok = R / a.G, g = R - tok * a.G;
+__device__ __forceinline__ int load_q(QFrag<D>& f, const Args& a, int row, int tokens, int pos, int h, int R0, int lane) {
+  constexpr int N = D / 32;                                  // pieces of eight elements a lane
+  const int R = R0 + (lane & 15), tok = R / a.G, g = R - tok * a.G, c = lane >> 4;
   const bool there = tok < tokens;
-  const bf16* p = a.q + (int64_t)(row + (there ? tok : 0)) * a.qs + (int64_t)(h * a.G + g) * D + (lane >> 4) * (D / 4);
+  const bf16* p = a.q + (int64_t)(row + (there ? tok : 0)) * a.qs + (int64_t)(h * a.G + g) * D + 16 * c;
+  bf16x8 q[N];
 #pragma unroll
-  for (int s = 0; s < D / 32; ++s) {
-    q[s] = load_bf16x8(p + 8 * s);
-    if (!there) q[s] = bf16x8{};
+  for (int i = 0; i < N; ++i) q[i] = load_bf16x8(p + 64 * (i >> 1) + 8 * (i & 1));
+  uint32_t m = 0;                                            // the largest element's bits
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const u32x4 b = __builtin_bit_cast(u32x4, q[i]);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) m = max(m, max(b[j] & 0x7fffu, (b[j] >> 16) & 0x7fffu));
+  }
+  m = max(m, (uint32_t)__shfl_xor((int)m, 16, 64));
+  m = max(m, (uint32_t)__shfl_xor((int)m, 32, 64));
+  const bool finite = m < 0x7f80u;
+  const int e = max((int)(m >> 7), 30) - 7;                  // (its exponent) - 7, biased: 2^(e - 127) is 2^u
+  const float s = there ? __uint_as_float((uint32_t)(254 - e) << 23) : 0.f;
+  uint32_t hi[2 * N], lo[2 * N];
+#pragma unroll
+  for (int i = 0; i < 2 * N; ++i) {
+    float x[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) x[j] = (float)q[i >> 1][4 * (i & 1) + j] * s;
+    int w = __builtin_amdgcn_cvt_pk_fp8_f32(x[0], x[1], 0, false);
+    w = __builtin_amdgcn_cvt_pk_fp8_f32(x[2], x[3], w, true);
+    const auto y0 = __builtin_amdgcn_cvt_pk_f32_fp8(w, false), y1 = __builtin_amdgcn_cvt_pk_f32_fp8(w, true);
+    int v = __builtin_amdgcn_cvt_pk_fp8_f32(16.f * (x[0] - y0[0]), 16.f * (x[1] - y0[1]), 0, false);
+    v = __builtin_amdgcn_cvt_pk_fp8_f32(16.f * (x[2] - y1[0]), 16.f * (x[3] - y1[1]), v, true);
+    hi[i] = finite ? (uint32_t)w : 0x7f7f7f7fu;              // (a row with an infinity or no number in it is no numbers)
+    lo[i] = finite ? (uint32_t)v : 0x7f7f7f7fu;
+  }
+  if constexpr (D == 128) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      f.x[0][i] = (int)hi[i];
+      f.x[1][i] = (int)lo[i];
+    }
+    f.s[0] = (uint32_t)e;
+    f.s[1] = (uint32_t)e - 4u;
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      f.x[0][i] = (int)hi[i];
+      f.x[0][4 + i] = (int)lo[i];
+    }
+    f.s[0] = c < 2 ? (uint32_t)e : (uint32_t)e - 4u;
   }
   return there ? pos + tok : -1;
 }
 
 // Scores of 64 keys
 template <int D, int NQ>
-__device__ __forceinline__ void scores(const KFrag<D>& f, const bf16x8 (&q)[NQ][D / 32], f32x4 (&s)[4][NQ]) {
+__device__ __forceinline__ void scores(const KFrag& f, const QFrag<D> (&q)[NQ], f32x4 (&s)[4][NQ]) {
 #pragma unroll
-  for (int t = 0; t < 4; ++t) {
-    const float sc = scale_of(f.s[t]);
+  for (int t = 0; t < 4; ++t)
 #pragma unroll
-    for (int n = 0; n < NQ; ++n) s[t][n] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int n = 0; n < NQ; ++n) {
+      s[t][n] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int i = 0; i < D / 32; ++i) {
-      const bf16x8 k = widen8(f.d[t][i], sc);
-#pragma unroll
-      for (int n = 0; n < NQ; ++n) s[t][n] = mfma16(k, q[n][i], s[t][n]);
+      for (int i = 0; i < D / 64; ++i) s[t][n] = mfma4x8(f.d[t], f.s[t], q[n].x[i], q[n].s[i], s[t][n]);
     }
-  }
+#pragma unroll
+  for (int t = 0; t < 4; ++t)
+#pragma unroll
+    for (int n = 0; n < NQ; ++n) asm volatile("" : "+v"(s[t][n]));
 }
 
 __device__ __forceinline__ bool sees(int key, int lim, int window, int first) { return key <= lim && (key > lim - window || key < first); }
 
 // One block of keys: scores, softmax, values
 template <int D, int NQ>
-__device__ __forceinline__ void block_step(const KFrag<D>& kf, const VFrag& vf, Rows<D, NQ>& r, int key0, int pmin, int pmax, int window,
+__device__ __forceinline__ void block_step(const KFrag& kf, const VFrag& vf, Rows<D, NQ>& r, int key0, int pmin, int pmax, int window,
                                            int first, float scale2, int lane) {
   const int c = lane >> 4;
   f32x4 s[4][NQ];
@@ -179,15 +230,16 @@ __device__ __forceinline__ void block_step(const KFrag<D>& kf, const VFrag& vf, 
     float mx = vmax(vmax(s[0][n][0], s[0][n][1]), vmax(s[0][n][2], s[0][n][3]));
 #pragma unroll
     for (int t = 1; t < 4; ++t) mx = vmax(vmax(vmax(mx, s[t][n][0]), s[t][n][1]), vmax(s[t][n][2], s[t][n][3]));
-    mx = vmax(r.m[n], over_quarters_max(mx) * scale2);
-    const float use = mx == -INFINITY ? 0.f : mx;
-    if (!__all(mx == r.m[n])) {
-      const float f = fast_exp2(r.m[n] - use);
+    // (the maximum is raised only where it has grown by 2^24, which sums of fp32 hold: most blocks have nothing to exchange or scale)
+    if (__any(!(mx * scale2 <= r.m[n] + 24.f))) {
+      mx = vmax(r.m[n], over_quarters_max(mx) * scale2);
+      const float f = mx == -INFINITY ? 1.f : fast_exp2(r.m[n] - mx);
       r.l[n] *= f;
 #pragma unroll
       for (int d = 0; d < D / 16; ++d) r.o[n][d] *= f;
+      r.m[n] = mx;
     }
-    r.m[n] = mx;
+    const float use = r.m[n] == -INFINITY ? 0.f : r.m[n];
     float sum = 0.f;
 #pragma unroll
     for (int t = 0; t < 4; ++t)
@@ -237,9 +289,10 @@ __device__ __forceinline__ void block_step(const KFrag<D>& kf, const VFrag& vf, 
   }
 }
 
-// NW waves take a tile of 16 NQ rows, every NW-th block each; their results meet in LDS.
-template <int D, int NQ, int NW>
-__global__ __launch_bounds__(64 * NW) void attn_kernel(Args a) {
+// NW waves take a tile of 16 NQ rows, every NW-th block each; their results meet in LDS. A wave has NB blocks in registers: one that it works
+// on, the others on their way. (The loop's first form fetches without a condition, so that the waits count what is on its way.)
+template <int D, int NQ, int NW, int NB>
+__global__ __launch_bounds__(64 * NW, NQ == 1 ? 2 : 1) void attn_kernel(Args a) {
   constexpr int LD = D + 4;                                     // (16 lanes a quarter write 16 rows: other banks each)
   __shared__ float sO[NW][16][LD];
   __shared__ float sM[NW][16], sL[NW][16];
@@ -262,27 +315,44 @@ __global__ __launch_bounds__(64 * NW) void attn_kernel(Args a) {
     for (int d = 0; d < D / 16; ++d) r.o[n][d] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
   bool bad = false;
-  int v = it.lo + w;
-  if (v < hi) {
-    int pg[4];
-    KFrag<D> kf;
-    VFrag vf;
-    block_pages(bt, list[v], pmax, a.n_pages, pg, bad);
-    load_k<D>(kf, a.kc, a.Hkv, h, pg, lane);
-    load_v<D>(vf, a.vc, a.Hkv, h, pg, lane);
+  const int v0 = it.lo + w, n = (hi - v0 + NW - 1) / NW;        // this wave's blocks: v0, v0 + NW, ..
+  if (n > 0) {
+    auto ids = [&](int k) { return PageIds(bt, pmax, lane, [&](int i) { return list[min(v0 + NW * (k + i), hi - 1)]; }); };
+    PageIds id = ids(0), idn = ids(16);
+    KFrag kf[NB];
+    VFrag vf[NB];
+    auto fetch = [&](int x, int k) {
+      if (k && k % 16 == 0) {
+        id = idn;
+        idn = ids(k + 16);
+      }
+      int pg[4];
+      id.get(k % 16, a.n_pages, pg, bad);
+      load_k<D>(kf[x], a.kc, a.Hkv, h, pg, lane);
+      load_v<D>(vf[x], a.vc, a.Hkv, h, pg, lane);
+    };
+    auto step = [&](int x, int k) {
+      block_step<D, NQ>(kf[x], vf[x], r, list[v0 + NW * k] * KB, pmin, pmax, a.window, a.first, a.scale2, lane);
+    };
 #pragma unroll
-    for (int n = 0; n < NQ; ++n) r.lim[n] = load_q<D>(r.q[n], a, it.row, it.tokens, it.pos, h, 16 * n, lane);
-    for (; v < hi; v += NW) {
-      const int nv = v + NW < hi ? v + NW : v;
-      KFrag<D> kn;
-      VFrag vn;
-      block_pages(bt, list[nv], pmax, a.n_pages, pg, bad);
-      load_k<D>(kn, a.kc, a.Hkv, h, pg, lane);
-      load_v<D>(vn, a.vc, a.Hkv, h, pg, lane);
-      block_step<D, NQ>(kf, vf, r, list[v] * KB, pmin, pmax, a.window, a.first, a.scale2, lane);
-      kf = kn;
-      vf = vn;
-    }
+    for (int x = 0; x < NB; ++x)
+      if (x < n) fetch(x, x);
+#pragma unroll
+    for (int m = 0; m < NQ; ++m) r.lim[m] = load_q<D>(r.q[m], a, it.row, it.tokens, it.pos, h, 16 * m, lane);
+    int k = 0;
+    for (; k + 2 * NB <= n; k += NB)
+#pragma unroll
+      for (int x = 0; x < NB; ++x) {
+        step(x, k + x);
+        fetch(x, k + x + NB);
+      }
+    for (; k < n; k += NB)
+#pragma unroll
+      for (int x = 0; x < NB; ++x)
+        if (k + x < n) {
+          step(x, k + x);
+          if (k + x + NB < n) fetch(x, k + x + NB);
+        }
   }
   const int Hq = a.Hkv * a.G;
 #pragma unroll
@@ -398,6 +468,20 @@ __device__ __forceinline__ float over_columns(float x) {
   return x + __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(x), 0x121, 0xf, 0xf, true));
 }
 
+// Q of 16 columns in bf16, elements as the lanes hold those of the keys (heads of 64: the two lanes of a half share it)
+template <int D>
+__device__ __forceinline__ int load_q16(bf16x8 (&q)[D / 32], const Args& a, int row, int tokens, int pos, int h, int R0, int lane) {
+  const int R = R0 + (lane & 15), tok = R / a.G, g = R - tok * a.G, c = lane >> 4;
+  const bool there = tok < tokens;
+  const bf16* p = a.q + (int64_t)(row + (there ? tok : 0)) * a.qs + (int64_t)(h * a.G + g) * D + (D == 128 ? 32 * c : 32 * (c & 1) + 16 * (c >> 1));
+#pragma unroll
+  for (int s = 0; s < D / 32; ++s) {
+    q[s] = load_bf16x8(p + 8 * s);
+    if (!there) q[s] = bf16x8{};
+  }
+  return there ? pos + tok : -1;
+}
+
 // lse of 16 columns from R0 on; +infinity where there is no row or the row sees nothing (its weights are zero)
 __device__ __forceinline__ float load_lse(const Args& a, int row, int tokens, int h, int R0, int lane) {
   const int R = R0 + (lane & 15), tok = R / a.G, g = R - tok * a.G;
@@ -434,7 +518,7 @@ __global__ __launch_bounds__(256) void mass_few_kernel(MassArgs ma) {
   const int row = it[0], rows = it[1], pos = it[2], table = it[3], seg = it[4], end = it[6];
   const int h = blockIdx.x % a.Hkv, lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int c = lane >> 4, last = pos + rows - 1;
-  if (row < 0 || rows < 0 || row + rows > a.T || rows * a.G > 16 * NQ) return;
+  if (row < 0 || rows < 0 || row + rows > a.T || rows * a.G > 16 * NQ || end - it[5] > 32) return;
   const int* bt = a.tables + table * a.ts;
   const Blocks list(pos, last, a.window, a.first);
   // blocks that no row sees give nothing: behind the last key, between the first ones and the window
@@ -442,13 +526,15 @@ __global__ __launch_bounds__(256) void mass_few_kernel(MassArgs ma) {
   int b = it[5] + w;
   if (b >= end) return;
   bool bad = false, badn = false;
-  int pg[4];
-  KFrag<D> kf, kn;
+  int pg[4], k = 0;
+  KFrag kf, kn;
+  PageIds id;
+  if (rows > 0) id = PageIds(bt, last, lane, [&](int i) { return b + 4 * min(i, 7); });   // (at most eight blocks a wave)
   if (seen(b)) {
-    block_pages(bt, b, last, a.n_pages, pg, bad);
+    id.get(0, a.n_pages, pg, bad);
     load_k<D>(kf, a.kc, a.Hkv, h, pg, lane);
   }
-  bf16x8 qf[NQ][D / 32];
+  QFrag<D> qf[NQ];
   int lim[NQ];
   float ls[NQ];
 #pragma unroll
@@ -459,9 +545,10 @@ __global__ __launch_bounds__(256) void mass_few_kernel(MassArgs ma) {
     }
   for (; b < end; b += 4) {
     const int nb = b + 4;
+    ++k;
     if (nb < end && seen(nb)) {
       badn = false;
-      block_pages(bt, nb, last, a.n_pages, pg, badn);
+      id.get(k, a.n_pages, pg, badn);
       load_k<D>(kn, a.kc, a.Hkv, h, pg, lane);
     }
     float mine = 0.f;
@@ -507,19 +594,19 @@ __global__ __launch_bounds__(64 * NW) void mass_many_kernel(MassArgs ma) {
   bool bad = false;
   if (rows > 0 && key0 <= last && (b < list.head || b >= list.tail)) {
     int pg[4];
-    KFrag<D> kf;
-    block_pages(a.tables + table * a.ts, b, last, a.n_pages, pg, bad);
+    KFrag kf;
+    PageIds(a.tables + table * a.ts, last, lane, [&](int) { return b; }).get(0, a.n_pages, pg, bad);
     load_k<D>(kf, a.kc, a.Hkv, h, pg, lane);
     const int R1 = rows * a.G;
     int R = (max(0, (key0 - pos) * a.G) & ~15) + 16 * w;                 // rows that may see the block: from its first key's position on
     bf16x8 qf[D / 32];
-    int lim = load_q<D>(qf, a, row, rows, pos, h, R, lane);
+    int lim = load_q16<D>(qf, a, row, rows, pos, h, R, lane);
     float ls = load_lse(a, row, rows, h, R, lane);
     bf16x8 k[4][D / 32];
 #pragma unroll
     for (int t = 0; t < 4; ++t)
 #pragma unroll
-      for (int i = 0; i < D / 32; ++i) k[t][i] = widen8(kf.d[t][i], scale_of(kf.s[t]));
+      for (int i = 0; i < D / 32; ++i) k[t][i] = widen8(D == 64 && c > 1 ? kf.d[t][2 + i] : kf.d[t][i], scale_of(kf.s[t]));
     for (; R < R1; R += 16 * NW) {
       const int pmin = pos + R / a.G, pmax = min(pos + (R + 15) / a.G, last);
       if (key0 + KB <= pmin - a.window + 1 && key0 >= a.first) break;    // (so do all rows after these)
@@ -532,7 +619,7 @@ __global__ __launch_bounds__(64 * NW) void mass_many_kernel(MassArgs ma) {
       }
       const int lim0 = lim;
       const float ls0 = ls;
-      lim = load_q<D>(qf, a, row, rows, pos, h, R + 16 * NW, lane);      // (behind the last row: the first one again)
+      lim = load_q16<D>(qf, a, row, rows, pos, h, R + 16 * NW, lane);      // (behind the last row: the first one again)
       ls = load_lse(a, row, rows, h, R + 16 * NW, lane);
       const bool masked = key0 + KB - 1 > pmin || (key0 <= pmax - a.window && key0 + KB > a.first);
       add_weights<1>(acc, s, 0, ls0, masked, key0, lim0, a, lane);
@@ -590,9 +677,9 @@ extern "C" hipError_t kafka_kv4_attn(const bf16* q, int64_t qs, const uint8_t* k
   auto go = [&](auto kern) { kern<<<(unsigned)wgs, 64 * nw, 0, st>>>(a); };
   auto dim = [&](auto d) {
     constexpr int DD = decltype(d)::value;
-    if (nq == 1 && nw == 4) go(attn_kernel<DD, 1, 4>);
-    else if (nq == 1 && nw == 8) go(attn_kernel<DD, 1, 8>);
-    else if (nq == 2 && nw == 4) go(attn_kernel<DD, 2, 4>);
+    if (nq == 1 && nw == 4) go(attn_kernel<DD, 1, 4, 3>);
+    else if (nq == 1 && nw == 8) go(attn_kernel<DD, 1, 8, 3>);
+    else if (nq == 2 && nw == 4) go(attn_kernel<DD, 2, 4, 2>);
     else return false;
     return true;
   };
@@ -603,7 +690,7 @@ extern "C" hipError_t kafka_kv4_attn(const bf16* q, int64_t qs, const uint8_t* k
 
 constexpr int MASS_NW = 8;
 
-// items of segments of at most 32 rows, then of those of more
+// items of segments of at most 16 rows, then of those of more
 extern "C" hipError_t kafka_kv4_mass(const bf16* q, int64_t qs, const float* lse, const uint8_t* kc, int64_t n_pages, const int* tables,
                                      int64_t ts, const int* items, int n_few, int n_many, int T, int Hkv, int G, int D, int window,
                                      int first, float scale, const float* base, float* out, int N, hipStream_t st) {
@@ -617,9 +704,9 @@ extern "C" hipError_t kafka_kv4_mass(const bf16* q, int64_t qs, const float* lse
   if (n_few) {
     const MassArgs m = args(items);
     if (D == 128)
-      mass_few_kernel<128, 2><<<Hkv * n_few, 256, 0, st>>>(m);
+      mass_few_kernel<128, 1><<<Hkv * n_few, 256, 0, st>>>(m);
     else
-      mass_few_kernel<64, 2><<<Hkv * n_few, 256, 0, st>>>(m);
+      mass_few_kernel<64, 1><<<Hkv * n_few, 256, 0, st>>>(m);
   }
   if (n_many) {
     const MassArgs m = args(items + 8 * (int64_t)n_few);

@@ -61,7 +61,7 @@ SHORT_BLOCKS = 32          # blocks a CU up to which a launch is short: workgrou
 SHORT_PIECE = 16           # blocks of a piece in it: two for each wave
 LONG_WGS = 1024            # workgroups of four waves that a longer launch is split towards
 LONG_PIECE = 4
-MASS_FEW = 32              # rows of a segment up to which a wave takes them all for its block of keys
+MASS_FEW = 16              # rows of a segment up to which a wave takes them all for its block of keys
 MASS_WGS = 1024
 
 

@@ -3,8 +3,10 @@
 Tolerances. Stored numbers, kept keys and moved pages are compared bit for bit: rounding to a code is decided by comparisons of
 numbers that 32 bits hold exactly (the rotation's products are rounded one by one in both). Attention, for weights w (their sum 1), with
 A the largest sum_d |scale q_d k_d| of a row: a score is a sum of D exact products in fp32 and a product by the scale, off by at
-most (D + 4) 2^-24 A; the exponential and its argument add 2^-22 (1 + A): EW = 2 ((D + 4) 2^-24 A + 2^-22 (1 + A)) bounds
-a weight's relative error with its sum's. P is rounded to bf16 (2^-8), the output too: |do| <= (2^-8 + EW + n 2^-24) sum w |v| + 2^-8 |o|.
+most (D + 4) 2^-24 A, and where Q goes in two parts of e4m3 by 2^-21 B, B the largest scale max |q| sum_d |k_d| (a part's
+step is 2^-9, its factor 2^-4, and the largest element comes to at least 128: an element is off by half of 2^-13 / 128 of that); the
+exponential and its argument add 2^-22 (1 + A): EW = 2 ((D + 4) 2^-24 A + 2^-21 B + 2^-22 (1 + A)) bounds a weight's relative error with its
+sum's. P is rounded to bf16 (2^-8), the output too: |do| <= (2^-8 + EW + n 2^-24) sum w |v| + 2^-8 |o|.
 The logarithm is off by (EW + n 2^-24) / ln 2 and its own rounding; a key's weight, from R rows, by the weights' errors, that of
 the logarithm and R additions: (2 EW + (n + R + 2) 2^-24 + 2^-23 |lse|) of itself."""
 import math
@@ -70,7 +72,8 @@ def oracle(q, kc, vc, tables, segs, window, first, scale):
             x, kh, vh = q[t0:t0 + rows, h].double(), k[:, h // G], v[:, h // G]
             s = (x @ kh.T * scale).masked_fill(~see, -math.inf)
             A = (x.abs() @ kh.abs().T * scale).masked_fill(~see, 0).amax(-1, keepdim=True)
-            EW = 2 * ((D + 4) * 2.0 ** -24 * A + 2.0 ** -22 * (1 + A))
+            B = x.abs().amax(-1, keepdim=True) * kh.abs().sum(-1).max() * scale
+            EW = 2 * ((D + 4) * 2.0 ** -24 * A + 2.0 ** -21 * B + 2.0 ** -22 * (1 + A))
             ls = torch.logsumexp(s, -1, keepdim=True)
             w = torch.exp(s - ls)
             o = w @ vh
@@ -306,7 +309,8 @@ def _masses(R, H, N, kind, seed=0):
 
 KEEPS = [(3, 2, 200, 64, 4, 16, "plain"), (2, 2, 3000, 1024, 4, 256, "ties"), (1, 3, 1500, 1000, 0, 0, "same"), (2, 1, 1025, 64, 32, 32, "plain"),
          (2, 2, 2500, 1500, 1, 100, "special"), (1, 1, 5, 1, 0, 0, "plain"), (2, 2, 30, 64, 4, 16, "plain"), (1, 2, 9000, 4097, 16, 1, "plain"),
-         (2, 1, 700, 1, 1, 0, "ties"), (1, 1, 2000, 300, 0, 300, "special")]
+         (2, 1, 700, 1, 1, 0, "ties"), (1, 1, 2000, 300, 0, 300, "special"),
+         (2, 2, 40000, 9000, 4, 1000, "plain"), (1, 1, 40000, 20000, 0, 7, "ties"), (1, 2, 16385, 500, 3, 0, "special"), (1, 1, 16384, 16383, 0, 0, "same")]
 
 
 def _lens(R, N):
