@@ -21,8 +21,8 @@ struct Item {
   int pos;               // position of the first
   int table;             // row of the block table
   int lo, hi;            // blocks of its list
-  int slot;              // < 0: the rows are written, else partial results number ``slot``
-  int pad;
+  int slot;              // < 0: the rows are written here, else the first of the tile's partial results,
+  int part;              // of which this is number part & 0xffff of part >> 16
 };
 
 struct Args {
@@ -39,7 +39,8 @@ struct Args {
   bf16* out;
   int64_t os;
   float* lse;            // [T][Hq], may be null
-  float *part, *plse;    // [slots][Hkv][rows of a tile][D], [slots][Hkv][rows of a tile]
+  float *part, *plse;    // partial results: from slot Hkv + head * parts on of every split tile [parts][rows of a tile][D], [..][rows of a tile]
+  int* counters;         // [slots][Hkv] zeros, and zeros again when the launch has ended
 };
 
 __device__ __forceinline__ float vmax(float a, float b) { return __builtin_elementwise_maximum(a, b); }
@@ -289,6 +290,25 @@ __device__ __forceinline__ void block_step(const KFrag& kf, const VFrag& vf, Row
   }
 }
 
+// Partial results (normalised, with their sums' logarithms) joined to what (M, L, o) holds: the first n of B
+template <int B>
+__device__ __forceinline__ void join(float& M, float& L, f32x4& o, const float (&l)[B], const f32x4 (&p)[B], int n) {
+  float mx = M;
+#pragma unroll
+  for (int s = 0; s < B; ++s) mx = vmax(mx, l[s]);              // (those behind the last are the last once more)
+  const float use = mx == -INFINITY ? 0.f : mx, f0 = fast_exp2(M - use);
+  M = mx;
+  L *= f0;
+  o *= f0;
+#pragma unroll
+  for (int s = 0; s < B; ++s) {
+    const float f = s < n ? fast_exp2(l[s] - use) : 0.f;
+    L += f;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) o[j] = fmaf(p[s][j], f, o[j]);
+  }
+}
+
 // NW waves take a tile of 16 NQ rows, every NW-th block each; their results meet in LDS. A wave has NB blocks in registers: one that it works
 // on, the others on their way. (The loop's first form fetches without a condition, so that the waits count what is on its way.)
 template <int D, int NQ, int NW, int NB>
@@ -296,6 +316,7 @@ __global__ __launch_bounds__(64 * NW, NQ == 1 ? 2 : 1) void attn_kernel(Args a) 
   constexpr int LD = D + 4;                                     // (16 lanes a quarter write 16 rows: other banks each)
   __shared__ float sO[NW][16][LD];
   __shared__ float sM[NW][16], sL[NW][16];
+  __shared__ bool s_last;
   const Item it = a.items[blockIdx.x / a.Hkv];
   const int h = blockIdx.x % a.Hkv, lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int q = lane & 15, c = lane >> 4;
@@ -354,7 +375,7 @@ __global__ __launch_bounds__(64 * NW, NQ == 1 ? 2 : 1) void attn_kernel(Args a) 
           if (k + x + NB < n) fetch(x, k + x + NB);
         }
   }
-  const int Hq = a.Hkv * a.G;
+  const int Hq = a.Hkv * a.G, parts = it.part >> 16;
 #pragma unroll
   for (int n = 0; n < NQ; ++n) {
     const int live = min(16, it.tokens * a.G - 16 * n);         // columns of the tile that are rows
@@ -396,16 +417,52 @@ __global__ __launch_bounds__(64 * NW, NQ == 1 ? 2 : 1) void attn_kernel(Args a) 
         *reinterpret_cast<bf16x4*>(a.out + (int64_t)(it.row + tok) * a.os + (int64_t)(h * a.G + g) * D + d0) =
             bf16x4{(bf16)o[0], (bf16)o[1], (bf16)o[2], (bf16)o[3]};
         if (a.lse && d0 == 0) a.lse[(int64_t)(it.row + tok) * Hq + h * a.G + g] = lse;
-      } else {
-        const int64_t at = ((int64_t)it.slot * a.Hkv + h) * (16 * NQ) + R;
-        *reinterpret_cast<f32x4*>(a.part + at * D + d0) = o;
-        if (d0 == 0) a.plse[at] = lse;
+      } else {                                                  // (through to where the other XCDs see it)
+        const int64_t at = ((int64_t)it.slot * a.Hkv + h * parts + (it.part & 0xffff)) * (16 * NQ) + R;
+        store16_slab(a.part + at * D + d0, o);
+        if (d0 == 0) __hip_atomic_store(a.plse + at, lse, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
       }
     }
   }
+  if (it.slot < 0) return;
+  // ---- the last workgroup of a split tile joins its parts: each has waited for its stores before it counts itself, and the last one's loads go
+  // past this XCD's cache; it leaves the counter zero
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    int* n = a.counters + (int64_t)it.slot * a.Hkv + h;
+    const bool last = __hip_atomic_fetch_add(n, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == parts - 1;
+    if (last) __hip_atomic_store(n, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    s_last = last;
+  }
+  __syncthreads();
+  if (!s_last) return;
+  constexpr int B = 8;                                          // parts on their way at a time
+  const int64_t at = ((int64_t)it.slot * a.Hkv + h * parts) * (16 * NQ);
+  const auto rp = buf_rsrc(a.part + at * D);                    // (at most 2^16 parts of 16 KiB)
+  for (int x = threadIdx.x; x < it.tokens * a.G * (D / 4); x += 64 * NW) {
+    const int R = x / (D / 4), d0 = (x % (D / 4)) * 4, tok = R / a.G, g = R - tok * a.G;
+    float M = -INFINITY, L = 0.f;
+    f32x4 o = {0.f, 0.f, 0.f, 0.f};
+    for (int s0 = 0; s0 < parts; s0 += B) {
+      float l[B];
+      f32x4 p[B];
+#pragma unroll
+      for (int s = 0; s < B; ++s) {
+        const int i = min(s0 + s, parts - 1) * (16 * NQ) + R;
+        l[s] = __hip_atomic_load(a.plse + at + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        p[s] = load16_sc1(rp, (i * D + d0) * 4);
+      }
+      join<B>(M, L, o, l, p, parts - s0);
+    }
+    const float inv = L == 0.f ? 0.f : 1.f / L;
+    *reinterpret_cast<bf16x4*>(a.out + (int64_t)(it.row + tok) * a.os + (int64_t)(h * a.G + g) * D + d0) =
+        bf16x4{(bf16)(o[0] * inv), (bf16)(o[1] * inv), (bf16)(o[2] * inv), (bf16)(o[3] * inv)};
+    if (a.lse && d0 == 0) a.lse[(int64_t)(it.row + tok) * Hq + h * a.G + g] = L == 0.f ? -INFINITY : M + log2f(L);
+  }
 }
 
-// Partial results of split tiles, eight on their way at a time. Merge items: first row, rows, first slot, slots.
+// Partial results of wide tiles (kv4_tile.hip). Merge items: first row, rows, first slot, slots.
 template <int D>
 __global__ __launch_bounds__(256) void merge_kernel(Args a, const int* __restrict__ merges, int tile_rows) {
   constexpr int B = 8;
@@ -426,20 +483,7 @@ __global__ __launch_bounds__(256) void merge_kernel(Args a, const int* __restric
       l[s] = a.plse[i];
       p[s] = *reinterpret_cast<const f32x4*>(a.part + i * D + d0);
     }
-    float mx = M;
-#pragma unroll
-    for (int s = 0; s < B; ++s) mx = vmax(mx, l[s]);
-    const float use = mx == -INFINITY ? 0.f : mx, f0 = fast_exp2(M - use);
-    M = mx;
-    L *= f0;
-    o *= f0;
-#pragma unroll
-    for (int s = 0; s < B; ++s) {
-      const float f = s0 + s < n ? fast_exp2(l[s] - use) : 0.f;
-      L += f;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) o[j] = fmaf(p[s][j], f, o[j]);
-    }
+    join<B>(M, L, o, l, p, n - s0);
   }
   const float inv = L == 0.f ? 0.f : 1.f / L;
   bf16x4 y;
@@ -646,9 +690,9 @@ using namespace kv4;
 
 static Args make_args(const bf16* q, int64_t qs, const uint8_t* kc, const uint8_t* vc, int64_t n_pages, const int* tables, int64_t ts,
                       const int* items, int T, int Hkv, int G, int window, int first, float scale, bf16* out, int64_t os, float* lse,
-                      float* part, float* plse) {
+                      float* part, float* plse, int* counters = nullptr) {
   return Args{q,   qs, kc,  vc,   n_pages, tables, ts, reinterpret_cast<const Item*>(items), T, Hkv, G, window > 0 ? window : 1 << 30,
-              first, scale * 1.4426950408889634f, out, os, lse, part, plse};
+              first, scale * 1.4426950408889634f, out, os, lse, part, plse, counters};
 }
 
 extern "C" hipError_t kafka_kv4_merge(const int* merges, int n_merges, int tile_rows, int T, int Hkv, int G, int D, bf16* out, int64_t os,
@@ -667,13 +711,12 @@ extern "C" hipError_t kafka_kv4_merge(const int* merges, int n_merges, int tile_
 
 // tiles of 16 nq rows, nw waves each
 extern "C" hipError_t kafka_kv4_attn(const bf16* q, int64_t qs, const uint8_t* kc, const uint8_t* vc, int64_t n_pages, const int* tables,
-                                     int64_t ts, const int* items, int n_items, int nq, int nw, const int* merges, int n_merges, int T,
-                                     int Hkv, int G, int D, int window, int first, float scale, bf16* out, int64_t os, float* lse,
-                                     float* part, float* plse, hipStream_t st) {
+                                     int64_t ts, const int* items, int n_items, int nq, int nw, int T, int Hkv, int G, int D, int window, int first, float scale, bf16* out, int64_t os, float* lse,
+                                     float* part, float* plse, int* counters, hipStream_t st) {
   if (n_items == 0) return hipSuccess;
   const int64_t wgs = (int64_t)Hkv * n_items;
   if ((D != 64 && D != 128) || G < 1 || G > 16 || wgs >= 1 << 24) return hipErrorInvalidValue;
-  const Args a = make_args(q, qs, kc, vc, n_pages, tables, ts, items, T, Hkv, G, window, first, scale, out, os, lse, part, plse);
+  const Args a = make_args(q, qs, kc, vc, n_pages, tables, ts, items, T, Hkv, G, window, first, scale, out, os, lse, part, plse, counters);
   auto go = [&](auto kern) { kern<<<(unsigned)wgs, 64 * nw, 0, st>>>(a); };
   auto dim = [&](auto d) {
     constexpr int DD = decltype(d)::value;
@@ -684,7 +727,6 @@ extern "C" hipError_t kafka_kv4_attn(const bf16* q, int64_t qs, const uint8_t* k
     return true;
   };
   if (!(D == 128 ? dim(std::integral_constant<int, 128>{}) : dim(std::integral_constant<int, 64>{}))) return hipErrorInvalidValue;
-  if (n_merges) return kafka_kv4_merge(merges, n_merges, 16 * nq, T, Hkv, G, D, out, os, lse, part, plse, st);
   return hipGetLastError();
 }
 

@@ -17,8 +17,8 @@ hipError_t kafka_kv4_evict_copy(uint8_t* kc, uint8_t* vc, int64_t n_pages, const
                                 int Hkv, int budget, const int* new_tables, int nw, int64_t ns, const float* mass, int64_t ms, int64_t mh,
                                 int N, float* new_mass, int D, hipStream_t st);
 hipError_t kafka_kv4_attn(const void* q, int64_t qs, const uint8_t* kc, const uint8_t* vc, int64_t n_pages, const int* tables, int64_t ts,
-                          const int* items, int n_items, int nq, int nw, const int* merges, int n_merges, int T, int Hkv, int G, int D, int window,
-                          int first, float scale, void* out, int64_t os, float* lse, float* part, float* plse, hipStream_t st);
+                          const int* items, int n_items, int nq, int nw, int T, int Hkv, int G, int D, int window, int first, float scale, void* out,
+                          int64_t os, float* lse, float* part, float* plse, int* counters, hipStream_t st);
 hipError_t kafka_kv4_tiles(const void* q, int64_t qs, const uint8_t* kc, const uint8_t* vc, int64_t n_pages, const int* tables, int64_t ts,
                            int rows, const int* items, int n_items, const int* wtiles, int n_wtiles, const int* merges, int n_merges, int T, int Hkv,
                            int G, int D, int window, int first, float scale, void* out, int64_t os, float* lse, float* part, float* plse,
@@ -125,6 +125,23 @@ struct Plan {
   std::vector<Part> parts;
   OptT mass;
 
+  // Counters of split tiles, which every launch leaves zero: one set for each stream that the plan is used on. A captured call has a set of its
+  // own, cleared in its graph, since the graph may be replayed beside anything.
+  mutable std::vector<std::pair<hipStream_t, Tensor>> counters;
+  int* zeros(int64_t n, Tensor& held) const {
+    const auto opt = parts[0].items.options();
+    hipStreamCaptureStatus status;
+    KV4_HIP(hipStreamIsCapturing(stream(), &status));
+    if (status != hipStreamCaptureStatusNone) {
+      held = at::zeros({n}, opt);
+      return held.data_ptr<int>();
+    }
+    for (auto& c : counters)
+      if (c.first == stream() && c.second.numel() >= n) return c.second.data_ptr<int>();
+    counters.emplace_back(stream(), at::zeros({n}, opt));
+    return counters.back().second.data_ptr<int>();
+  }
+
   void add(int64_t r, int64_t w, int64_t slots, Tensor items, Tensor merges, Tensor keys) {
     auto ok = [&](const Tensor& t, int64_t cols) {
       return t.is_cuda() && t.scalar_type() == at::kInt && t.dim() == 2 && t.size(1) == cols && t.is_contiguous() && t.size(0) < 1 << 24;
@@ -175,7 +192,7 @@ Tensor attn(Tensor q, Tensor kc, Tensor vc, Tensor tables, const Plan& p, double
   float* lp = row_values(lse, q, kc);
   for (const Part& t : p.parts) {
     TORCH_CHECK_VALUE(t.items.device() == kc.device(), "kv4: the plan was made for another device");
-    Tensor part, ws;                // (the caching allocator orders them with the stream)
+    Tensor part, ws, held;          // (the caching allocator orders them with the stream)
     float *pp = nullptr, *pl = nullptr;
     if (t.slots > 0) {
       const int64_t n = t.slots * H * t.rows;
@@ -187,8 +204,8 @@ Tensor attn(Tensor q, Tensor kc, Tensor vc, Tensor tables, const Plan& p, double
     const int ni = (int)t.items.size(0), nm = (int)t.merges.size(0);
     if (t.keys.size(0) == 0) {
       KV4_HIP(kafka_kv4_attn(q.data_ptr(), q.stride(0), kc.data_ptr<uint8_t>(), vc.data_ptr<uint8_t>(), kc.size(0), tp, tables.stride(0), ip, ni,
-                             (int)(t.rows / 16), (int)t.waves, mp, nm, (int)T, (int)H, (int)(Hq / H), D, (int)p.window, (int)p.first,
-                             (float)scale, out.data_ptr(), out.stride(0), lp, pp, pl, stream()));
+                             (int)(t.rows / 16), (int)t.waves, (int)T, (int)H, (int)(Hq / H), D, (int)p.window, (int)p.first, (float)scale,
+                             out.data_ptr(), out.stride(0), lp, pp, pl, t.slots > 0 ? p.zeros(t.slots * H, held) : nullptr, stream()));
     } else {
       ws = at::empty({t.keys.size(0) * H * 256 * D}, kc.options());
       KV4_HIP(kafka_kv4_tiles(q.data_ptr(), q.stride(0), kc.data_ptr<uint8_t>(), vc.data_ptr<uint8_t>(), kc.size(0), tp, tables.stride(0),

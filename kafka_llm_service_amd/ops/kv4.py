@@ -91,8 +91,8 @@ def _tiles(segs: np.ndarray, tokens: int):
 
 
 def _pieces(tiles: np.ndarray, count: np.ndarray, n: np.ndarray):
-    """(tile, first block, last + 1, slot) int64 [n, 4], merges int64 [m, 4], slots: tiles of ``count`` blocks in ``n`` pieces each (or fewer), the
-    longest first."""
+    """(tile, first block, last + 1, first slot of the tile's partial results, number among them, how many) int64 [n, 6], merges int64 [m, 4],
+    slots: tiles of ``count`` blocks in ``n`` pieces each (or fewer), the longest first. The slot of a tile in one piece is -1."""
     each = (count + n - 1) // n
     n = np.maximum(1, (count + each - 1) // each)
     t = np.repeat(np.arange(len(tiles)), n)
@@ -101,7 +101,7 @@ def _pieces(tiles: np.ndarray, count: np.ndarray, n: np.ndarray):
     split = n > 1
     base = np.cumsum(np.where(split, n, 0)) - np.where(split, n, 0)
     lo = i * each[t]
-    pieces = np.stack([t, lo, np.minimum(lo + each[t], count[t]), np.where(split[t], base[t] + i, -1)], 1)
+    pieces = np.stack([t, lo, np.minimum(lo + each[t], count[t]), np.where(split[t], base[t], -1), i, n[t]], 1)
     merges = np.stack([tiles[split, 0], tiles[split, 1], base[split], n[split]], 1)
     return pieces[np.argsort(pieces[:, 1] - pieces[:, 2], kind="stable")], merges, int(n[split].sum())
 
@@ -149,13 +149,15 @@ def _tables(full: np.ndarray, heads: int, kv_heads: int, dim: int, window: int, 
             i = np.arange(len(s)) - base[s]
             keys = np.stack([part[s, 3], np.where(i < head[s], i, i - head[s] + tail[s]), (part[:, 2] + part[:, 1] - 1)[s], np.zeros_like(s)], 1)
             s = t[:, 4]
-            cols = [t[:, 0], t[:, 1], t[:, 2], base[s], head[s], tail[s]]
+            cols = [t[:, 0], t[:, 1], t[:, 2], base[s], head[s], tail[s], pieces[:, 1], pieces[:, 2],
+                    np.where(pieces[:, 3] < 0, -1, pieces[:, 3] + pieces[:, 4])]
         else:
             waves, n = _narrow_split(count, kv_heads, size)
             pieces, merges, slots = _pieces(tiles, count, n)
             t = tiles[pieces[:, 0]]
-            keys, cols = np.zeros((0, 4)), [t[:, 0], t[:, 1], t[:, 2], t[:, 3]]
-        cols += [pieces[:, 1], pieces[:, 2], pieces[:, 3]]
+            keys = np.zeros((0, 4))
+            cols = [t[:, 0], t[:, 1], t[:, 2], t[:, 3], pieces[:, 1], pieces[:, 2], pieces[:, 3], pieces[:, 5] << 16 | pieces[:, 4]]
+            merges = merges[:0]                                            # (the last piece to end joins them)
         items = np.stack(cols + [np.zeros_like(t[:, 0])] * ((12 if len(keys) else 8) - len(cols)), 1)
         shapes.append((size, waves, slots, len(items), len(merges), len(keys)))
         arrays += [x.astype(np.int32) for x in (items, merges, keys)]

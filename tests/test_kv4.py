@@ -449,9 +449,9 @@ def test_plan_covers_every_block_once():
         n = (kv4._narrow_split(count, 2, 16 + 16 * r(2))[1], kv4._wide_split(count, 2, 256), np.array([1 + r(9) for _ in tiles]))[r(3)]
         pieces, merges, slots = kv4._pieces(tiles, count, n)
         seen = {}
-        for t, lo, hi, slot in pieces.tolist():
-            assert lo < hi
-            seen.setdefault(int(tiles[t, 0]), []).append((lo, hi, slot))
+        for t, lo, hi, slot, i, of in pieces.tolist():
+            assert lo < hi and 0 <= i < of and (slot >= 0) == (of > 1)
+            seen.setdefault(int(tiles[t, 0]), []).append((lo, hi, slot + i))
         for row, n, pos, tab, _ in tiles.tolist():
             parts = sorted(seen[row])
             need = {j // 64 for p in range(pos, pos + n) for j in range(p + 1) if not window or j > p - window or j < first}
@@ -768,3 +768,39 @@ def test_widened_keys_are_those_that_a_tile_sees(monkeypatch):
                 k = keys[base + (b if b < head else b - tail + head)].tolist()
                 seg = segs[row // 1000]
                 assert k[:3] == [seg[3], b, seg[1] + seg[2] - 1]
+
+
+@pytest.mark.gpu
+def test_split_tiles_side_by_side(cuda):
+    """Tiles in several pieces whose last one joins them: the same plan eager on two streams and in two graphs, all at once and again."""
+    segs = [(0, 1, 4000, 0), (1, 1, 9000, 1), (2, 2, 2500, 2)]
+    kc, vc, tables = world(segs, 2, 128, 0, cuda)
+    q = queries(4, 8, 128, 1, cuda)
+    plan = kv4.attn_plan(segs, 8, 2, 128, device=cuda)
+    p, a = kv4._plan(segs, 8, 2, 128, 0, 0)
+    assert kv4._tables(a, 8, 2, 128, 0, 0)[0][0][2] > 3                     # (slots of partial results)
+    lse = torch.empty(4, 8, device=cuda)
+    want = kv4.attn(q, kc, vc, tables, plan, 0.1, lse=lse)
+    streams, runs = [torch.cuda.Stream() for _ in range(4)], []
+    for s in streams[:2]:
+        s.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(s):
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph, stream=s):
+                l = torch.empty_like(lse)
+                o = kv4.attn(q, kc, vc, tables, plan, 0.1, lse=l)
+            runs.append((graph, o, l))
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    eager = []
+    for _ in range(10):
+        for s, (graph, o, l) in zip(streams, runs):
+            with torch.cuda.stream(s):
+                graph.replay()
+        for s in streams[2:]:
+            with torch.cuda.stream(s):
+                l = torch.empty_like(lse)
+                eager.append((kv4.attn(q, kc, vc, tables, plan, 0.1, lse=l), l))
+    torch.cuda.synchronize()
+    for o, l in eager + [r[1:] for r in runs]:
+        assert torch.equal(o, want) and torch.equal(l, lse)
