@@ -4,8 +4,9 @@
 // those with j > p - window or j < first. A work item is a tile of a segment's tokens and a range of the blocks of 64 keys that
 // any of them sees (the first ones, then those from the window's start on: a block in the range is a place in this list).
 //
-//   S^T[key][row] = K . Q^T    A: a lane's key and quarter of its elements, widened to bf16 (exactly), B: Q's fragments in registers
-//   O^T[d][row]  += V^T . P    A: a lane's eight d's, widened and turned by v_perm to pairs of keys, B: P as S^T's registers hold it
+//   S^T[key][row] = K . Q^T    A: K in four bits as it lies, B: Q in two parts of e4m3
+//   O^T[d][row]  += V^T . P    A: a lane's values of four keys, two neighbouring d's a register as they are widened (exactly), B: P as S^T's
+//                              registers hold it, beside zeros for the other d: twice the products, but no register is turned
 // The softmax runs in one pass with a running maximum per row; its sums and maxima are fp32, P is rounded to bf16 for the product.
 #include "kv4.h"
 
@@ -64,13 +65,15 @@ struct Blocks {
   __device__ __forceinline__ int operator[](int v) const { return v < head ? v : v - head + tail; }
 };
 
+template <int NP>          // of NP pages
 struct KFrag {
-  uint32_t d[4][4];        // a lane's 32 elements in each of four tiles of 16 keys
-  uint32_t s[4];
+  uint32_t d[NP][4];       // a lane's 32 elements of a key
+  uint32_t s[NP];
 };
+template <int NP>
 struct VFrag {
-  u32x4 d[4];              // a word for each of four keys, of four pages
-  uint32_t s[4];
+  u32x4 d[NP];             // a word for each of four keys
+  uint32_t s[NP];
 };
 
 // Page ids of 16 blocks of 4 pages, a lane each (keys behind ``last`` take its page: they are masked). One load for them all, ahead of
@@ -80,11 +83,12 @@ struct PageIds {
   __device__ __forceinline__ PageIds() {}
   template <class Of>
   __device__ __forceinline__ PageIds(const int* bt, int last, int lane, Of block) : v(bt[min(block(lane >> 2) * 4 + (lane & 3), last >> 4)]) {}
-  // Those of the k-th block. An id that is not of the cache counts as page 0 and sets ``bad``: such rows come out as no numbers.
-  __device__ __forceinline__ void get(int k, int64_t n_pages, int (&pg)[4], bool& bad) const {
+  // NP of them from lane ``at`` on. An id that is not of the cache counts as page 0 and sets ``bad``: such rows come out as no numbers.
+  template <int NP>
+  __device__ __forceinline__ void get(int at, int64_t n_pages, int (&pg)[NP], bool& bad) const {
 #pragma unroll
-    for (int t = 0; t < 4; ++t) {
-      const int p = __builtin_amdgcn_readlane(v, k * 4 + t);
+    for (int t = 0; t < NP; ++t) {
+      const int p = __builtin_amdgcn_readlane(v, at + t);
       const bool ok = p >= 0 && p < n_pages;
       bad |= !ok;
       pg[t] = ok ? p : 0;
@@ -93,11 +97,11 @@ struct PageIds {
 };
 
 // (heads of 64: both halves of the lanes hold the key, for the two parts of Q)
-template <int D>
-__device__ __forceinline__ void load_k(KFrag& f, const uint8_t* kc, int Hkv, int h, const int (&pg)[4], int lane) {
-  const int key = lane & 15, g = (lane >> 4) & (D / 32 - 1);
+template <int D, int NP>
+__device__ __forceinline__ void load_k(KFrag<NP>& f, const uint8_t* kc, int Hkv, int h, const int (&pg)[NP], int lane) {
+  const uint32_t key = lane & 15, g = (lane >> 4) & (D / 32 - 1);
 #pragma unroll
-  for (int t = 0; t < 4; ++t) {
+  for (int t = 0; t < NP; ++t) {
     const uint8_t* p = kc + ((int64_t)pg[t] * Hkv + h) * Page<D>::BYTES;
     const u32x4 x = *reinterpret_cast<const u32x4*>(p + key * (D / 2) + g * 16);
 #pragma unroll
@@ -106,11 +110,11 @@ __device__ __forceinline__ void load_k(KFrag& f, const uint8_t* kc, int Hkv, int
   }
 }
 
-template <int D>
-__device__ __forceinline__ void load_v(VFrag& f, const uint8_t* vc, int Hkv, int h, const int (&pg)[4], int lane) {
-  const int dl = lane & 15, c = lane >> 4;
+template <int D, int NP>
+__device__ __forceinline__ void load_v(VFrag<NP>& f, const uint8_t* vc, int Hkv, int h, const int (&pg)[NP], int lane) {
+  const uint32_t dl = lane & 15, c = lane >> 4;
 #pragma unroll
-  for (int t = 0; t < 4; ++t) {
+  for (int t = 0; t < NP; ++t) {
     const uint8_t* p = vc + ((int64_t)pg[t] * Hkv + h) * Page<D>::BYTES;
     f.d[t] = *reinterpret_cast<const u32x4*>(p + (c * (D / 8) + dl * (D / 8) / 16) * 16);
     f.s[t] = *reinterpret_cast<const uint32_t*>(p + Page<D>::DATA + (dl * (D / 16) / 32) * 16 + c * 4);
@@ -189,11 +193,11 @@ __device__ __forceinline__ int load_q(QFrag<D>& f, const Args& a, int row, int t
   return there ? pos + tok : -1;
 }
 
-// Scores of 64 keys
-template <int D, int NQ>
-__device__ __forceinline__ void scores(const KFrag& f, const QFrag<D> (&q)[NQ], f32x4 (&s)[4][NQ]) {
+// Scores of 16 NP keys
+template <int D, int NQ, int NP>
+__device__ __forceinline__ void scores(const KFrag<NP>& f, const QFrag<D> (&q)[NQ], f32x4 (&s)[NP][NQ]) {
 #pragma unroll
-  for (int t = 0; t < 4; ++t)
+  for (int t = 0; t < NP; ++t)
 #pragma unroll
     for (int n = 0; n < NQ; ++n) {
       s[t][n] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -201,37 +205,46 @@ __device__ __forceinline__ void scores(const KFrag& f, const QFrag<D> (&q)[NQ], 
       for (int i = 0; i < D / 64; ++i) s[t][n] = mfma4x8(f.d[t], f.s[t], q[n].x[i], q[n].s[i], s[t][n]);
     }
 #pragma unroll
-  for (int t = 0; t < 4; ++t)
+  for (int t = 0; t < NP; ++t)
 #pragma unroll
     for (int n = 0; n < NQ; ++n) asm volatile("" : "+v"(s[t][n]));
 }
 
 __device__ __forceinline__ bool sees(int key, int lim, int window, int first) { return key <= lim && (key > lim - window || key < first); }
 
-// One block of keys: scores, softmax, values
-template <int D, int NQ>
-__device__ __forceinline__ void block_step(const KFrag& kf, const VFrag& vf, Rows<D, NQ>& r, int key0, int pmin, int pmax, int window,
-                                           int first, float scale2, int lane) {
+// 16 NP keys from key0 on: scores, softmax, values
+template <int D, int NQ, int NP>
+__device__ __forceinline__ void keys_step(const KFrag<NP>& kf, VFrag<NP>& vf, Rows<D, NQ>& r, int key0, int pmin, int pmax, int window, int first,
+                                          float scale2, int lane) {
   const int c = lane >> 4;
-  f32x4 s[4][NQ];
-  scores<D, NQ>(kf, r.q, s);
-  const bool masked = key0 + KB - 1 > pmin || (key0 <= pmax - window && key0 + KB > first);
-  if (masked) {
+  f32x4 s[NP][NQ];
+  scores<D, NQ, NP>(kf, r.q, s);
+  if (key0 + 16 * NP - 1 > pmin || (key0 <= pmax - window && key0 + 16 * NP > first)) {
 #pragma unroll
     for (int n = 0; n < NQ; ++n)
 #pragma unroll
-      for (int t = 0; t < 4; ++t)
+      for (int t = 0; t < NP; ++t)
 #pragma unroll
         for (int i = 0; i < 4; ++i)
           if (!sees(key0 + 16 * t + 4 * c + i, r.lim[n], window, first)) s[t][n][i] = -INFINITY;
+    // behind the last position the page may hold anything, also scales that are no numbers: their weight is zero, so must they be
+    if (key0 + 16 * NP - 1 > pmax) {
+#pragma unroll
+      for (int t = 0; t < NP; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (key0 + 16 * t + 4 * c + i > pmax) {
+            vf.d[t][i] = 0u;
+            vf.s[t] &= ~(255u << (8 * i));
+          }
+    }
   }
-  bf16x8 p[NQ][2];
 #pragma unroll
   for (int n = 0; n < NQ; ++n) {
     float mx = vmax(vmax(s[0][n][0], s[0][n][1]), vmax(s[0][n][2], s[0][n][3]));
 #pragma unroll
-    for (int t = 1; t < 4; ++t) mx = vmax(vmax(vmax(mx, s[t][n][0]), s[t][n][1]), vmax(s[t][n][2], s[t][n][3]));
-    // (the maximum is raised only where it has grown by 2^24, which sums of fp32 hold: most blocks have nothing to exchange or scale)
+    for (int t = 1; t < NP; ++t) mx = vmax(vmax(vmax(mx, s[t][n][0]), s[t][n][1]), vmax(s[t][n][2], s[t][n][3]));
+    // (the maximum is raised only where it has grown by 2^24, which sums of fp32 hold: most steps have nothing to exchange or scale)
     if (__any(!(mx * scale2 <= r.m[n] + 24.f))) {
       mx = vmax(r.m[n], over_quarters_max(mx) * scale2);
       const float f = mx == -INFINITY ? 1.f : fast_exp2(r.m[n] - mx);
@@ -240,53 +253,44 @@ __device__ __forceinline__ void block_step(const KFrag& kf, const VFrag& vf, Row
       for (int d = 0; d < D / 16; ++d) r.o[n][d] *= f;
       r.m[n] = mx;
     }
-    const float use = r.m[n] == -INFINITY ? 0.f : r.m[n];
-    float sum = 0.f;
+  }
 #pragma unroll
-    for (int t = 0; t < 4; ++t)
+  for (int t = 0; t < NP; ++t) {
+    bf16x8 p[NQ][2];                                            // weights of four keys, each beside a zero: for even d's, for odd ones
+#pragma unroll
+    for (int n = 0; n < NQ; ++n) {
+      const float use = r.m[n] == -INFINITY ? 0.f : r.m[n];
+      u32x4 x, y;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const float e = fast_exp2(fmaf(s[t][n][i], scale2, -use));
-        sum += e;
-        p[n][t >> 1][4 * (t & 1) + i] = (bf16)e;
+        r.l[n] += e;
+        x[i] = __builtin_bit_cast(uint32_t, bf16x2{(bf16)e, (bf16)0.f});
+        y[i] = x[i] << 16;
       }
-    r.l[n] += sum;
-  }
-  constexpr int W = D / 32;                                     // pairs of d a lane
-  const int dl = lane & 15;
+      p[n][0] = __builtin_bit_cast(bf16x8, x);
+      p[n][1] = __builtin_bit_cast(bf16x8, y);
+    }
+    constexpr int W = D / 32;                                   // pairs of d a lane
+    u32x4 x[W];
 #pragma unroll
-  for (int u = 0; u < 2; ++u) {
-    uint32_t x[W][8];
-#pragma unroll
-    for (int t = 0; t < 2; ++t)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        uint32_t w = vf.d[2 * u + t][i], e = (vf.s[2 * u + t] >> (8 * i)) & 255u;
-        if (D == 64) w >>= 16 * (dl & 1);
-        // (behind the last position the page may hold anything, also scales that are no numbers: their weight is zero, so must they be)
-        if (masked && key0 + 32 * u + 16 * t + 4 * c + i > pmax) w = 0u, e = 0u;
-        const float sc = scale_of(e);
-        x[0][4 * t + i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, sc, 0));
-        x[1][4 * t + i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, sc, 1));
-        if constexpr (D == 128) {
-          x[2][4 * t + i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, sc, 2));
-          x[3][4 * t + i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, sc, 3));
-        }
-      }
-#pragma unroll
-    for (int m = 0; m < W; ++m) {
-      u32x4 lo, hi;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        lo[j] = __builtin_amdgcn_perm(x[m][2 * j + 1], x[m][2 * j], 0x05040100u);
-        hi[j] = __builtin_amdgcn_perm(x[m][2 * j + 1], x[m][2 * j], 0x07060302u);
-      }
-#pragma unroll
-      for (int n = 0; n < NQ; ++n) {
-        r.o[n][2 * m] = mfma16(__builtin_bit_cast(bf16x8, lo), p[n][u], r.o[n][2 * m]);
-        r.o[n][2 * m + 1] = mfma16(__builtin_bit_cast(bf16x8, hi), p[n][u], r.o[n][2 * m + 1]);
+    for (int i = 0; i < 4; ++i) {
+      uint32_t w = vf.d[t][i];
+      if (D == 64) w >>= 16 * (lane & 1);
+      const float sc = __uint_as_float(i < 3 ? vf.s[t] << (23 - 8 * i) : vf.s[t] >> 1);   // (only its exponent counts)
+      x[0][i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, sc, 0));
+      x[1][i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, sc, 1));
+      if constexpr (D == 128) {
+        x[2][i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, sc, 2));
+        x[3][i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, sc, 3));
       }
     }
+#pragma unroll
+    for (int m = 0; m < W; ++m)
+#pragma unroll
+      for (int n = 0; n < NQ; ++n)
+#pragma unroll
+        for (int b = 0; b < 2; ++b) r.o[n][2 * m + b] = mfma16(__builtin_bit_cast(bf16x8, x[m]), p[n][b], r.o[n][2 * m + b]);
   }
 }
 
@@ -309,10 +313,10 @@ __device__ __forceinline__ void join(float& M, float& L, f32x4& o, const float (
   }
 }
 
-// NW waves take a tile of 16 NQ rows, every NW-th block each; their results meet in LDS. A wave has NB blocks in registers: one that it works
-// on, the others on their way. (The loop's first form fetches without a condition, so that the waits count what is on its way.)
+// NW waves take a tile of 16 NQ rows, every NW-th block each; their results meet in LDS. A wave has NB half blocks in registers: one that it
+// works on, the others on their way. (The loop's first form fetches without a condition, so that the waits count what is on its way.)
 template <int D, int NQ, int NW, int NB>
-__global__ __launch_bounds__(64 * NW, NQ == 1 ? 2 : 1) void attn_kernel(Args a) {
+__global__ __launch_bounds__(64 * NW, NQ == 1 ? 3 : 2) void attn_kernel(Args a) {
   constexpr int LD = D + 4;                                     // (16 lanes a quarter write 16 rows: other banks each)
   __shared__ float sO[NW][16][LD];
   __shared__ float sM[NW][16], sL[NW][16];
@@ -336,24 +340,24 @@ __global__ __launch_bounds__(64 * NW, NQ == 1 ? 2 : 1) void attn_kernel(Args a) 
     for (int d = 0; d < D / 16; ++d) r.o[n][d] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
   bool bad = false;
-  const int v0 = it.lo + w, n = (hi - v0 + NW - 1) / NW;        // this wave's blocks: v0, v0 + NW, ..
-  if (n > 0) {
-    auto ids = [&](int k) { return PageIds(bt, pmax, lane, [&](int i) { return list[min(v0 + NW * (k + i), hi - 1)]; }); };
-    PageIds id = ids(0), idn = ids(16);
-    KFrag kf[NB];
-    VFrag vf[NB];
+  const int v0 = it.lo + w, n = (hi - v0 + NW - 1) / NW * 2;    // halves of this wave's blocks: v0, v0 + NW, ..
+  if (hi > v0) {
+    auto ids = [&](int k) { return PageIds(bt, pmax, lane, [&](int i) { return list[min(v0 + NW * (k / 2 + i), hi - 1)]; }); };
+    PageIds id = ids(0), idn = ids(32);
+    KFrag<2> kf[NB];
+    VFrag<2> vf[NB];
     auto fetch = [&](int x, int k) {
-      if (k && k % 16 == 0) {
+      if (k && k % 32 == 0) {
         id = idn;
-        idn = ids(k + 16);
+        idn = ids(k + 32);
       }
-      int pg[4];
-      id.get(k % 16, a.n_pages, pg, bad);
-      load_k<D>(kf[x], a.kc, a.Hkv, h, pg, lane);
-      load_v<D>(vf[x], a.vc, a.Hkv, h, pg, lane);
+      int pg[2];
+      id.get<2>(k % 32 * 2, a.n_pages, pg, bad);
+      load_k<D, 2>(kf[x], a.kc, a.Hkv, h, pg, lane);
+      load_v<D, 2>(vf[x], a.vc, a.Hkv, h, pg, lane);
     };
     auto step = [&](int x, int k) {
-      block_step<D, NQ>(kf[x], vf[x], r, list[v0 + NW * k] * KB, pmin, pmax, a.window, a.first, a.scale2, lane);
+      keys_step<D, NQ, 2>(kf[x], vf[x], r, list[v0 + NW * (k >> 1)] * KB + 32 * (k & 1), pmin, pmax, a.window, a.first, a.scale2, lane);
     };
 #pragma unroll
     for (int x = 0; x < NB; ++x)
@@ -571,12 +575,12 @@ __global__ __launch_bounds__(256) void mass_few_kernel(MassArgs ma) {
   if (b >= end) return;
   bool bad = false, badn = false;
   int pg[4], k = 0;
-  KFrag kf, kn;
+  KFrag<4> kf, kn;
   PageIds id;
   if (rows > 0) id = PageIds(bt, last, lane, [&](int i) { return b + 4 * min(i, 7); });   // (at most eight blocks a wave)
   if (seen(b)) {
-    id.get(0, a.n_pages, pg, bad);
-    load_k<D>(kf, a.kc, a.Hkv, h, pg, lane);
+    id.get<4>(0, a.n_pages, pg, bad);
+    load_k<D, 4>(kf, a.kc, a.Hkv, h, pg, lane);
   }
   QFrag<D> qf[NQ];
   int lim[NQ];
@@ -592,15 +596,15 @@ __global__ __launch_bounds__(256) void mass_few_kernel(MassArgs ma) {
     ++k;
     if (nb < end && seen(nb)) {
       badn = false;
-      id.get(k, a.n_pages, pg, badn);
-      load_k<D>(kn, a.kc, a.Hkv, h, pg, lane);
+      id.get<4>(4 * k, a.n_pages, pg, badn);
+      load_k<D, 4>(kn, a.kc, a.Hkv, h, pg, lane);
     }
     float mine = 0.f;
     const int key0 = b * KB;
     if (seen(b)) {
       float acc[4][4] = {};
       f32x4 s[4][NQ];
-      scores<D, NQ>(kf, qf, s);
+      scores<D, NQ, 4>(kf, qf, s);
       const bool masked = key0 + KB - 1 > pos || (key0 <= last - a.window && key0 + KB > a.first);
 #pragma unroll
       for (int n = 0; n < NQ; ++n) add_weights<NQ>(acc, s, n, ls[n], masked, key0, lim[n], a, lane);
@@ -638,9 +642,9 @@ __global__ __launch_bounds__(64 * NW) void mass_many_kernel(MassArgs ma) {
   bool bad = false;
   if (rows > 0 && key0 <= last && (b < list.head || b >= list.tail)) {
     int pg[4];
-    KFrag kf;
-    PageIds(a.tables + table * a.ts, last, lane, [&](int) { return b; }).get(0, a.n_pages, pg, bad);
-    load_k<D>(kf, a.kc, a.Hkv, h, pg, lane);
+    KFrag<4> kf;
+    PageIds(a.tables + table * a.ts, last, lane, [&](int) { return b; }).get<4>(0, a.n_pages, pg, bad);
+    load_k<D, 4>(kf, a.kc, a.Hkv, h, pg, lane);
     const int R1 = rows * a.G;
     int R = (max(0, (key0 - pos) * a.G) & ~15) + 16 * w;                 // rows that may see the block: from its first key's position on
     bf16x8 qf[D / 32];
@@ -720,8 +724,8 @@ extern "C" hipError_t kafka_kv4_attn(const bf16* q, int64_t qs, const uint8_t* k
   auto go = [&](auto kern) { kern<<<(unsigned)wgs, 64 * nw, 0, st>>>(a); };
   auto dim = [&](auto d) {
     constexpr int DD = decltype(d)::value;
-    if (nq == 1 && nw == 4) go(attn_kernel<DD, 1, 4, 3>);
-    else if (nq == 1 && nw == 8) go(attn_kernel<DD, 1, 8, 3>);
+    if (nq == 1 && nw == 4) go(attn_kernel<DD, 1, 4, 2>);
+    else if (nq == 1 && nw == 8) go(attn_kernel<DD, 1, 8, 2>);
     else if (nq == 2 && nw == 4) go(attn_kernel<DD, 2, 4, 2>);
     else return false;
     return true;
