@@ -54,6 +54,12 @@ __device__ __forceinline__ f32x4 mfma4x8(const uint32_t* a, uint32_t sa, i32x8 b
   return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(x, b, c, 4, 0, 0, (int)sa, 0, (int)sb);
 }
 
+// The same with the operands in each other's place: a [16 rows][128] in e4m3, b [128][16 columns] in e2m1
+__device__ __forceinline__ f32x4 mfma8x4(i32x8 a, uint32_t sa, const uint32_t* b, uint32_t sb, f32x4 c) {
+  const i32x8 x = {(int)b[0], (int)b[1], (int)b[2], (int)b[3], 0, 0, 0, 0};
+  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, x, c, 0, 4, 0, (int)sa, 0, (int)sb);
+}
+
 __device__ __forceinline__ f32x4 mfma16(bf16x8 a, bf16x8 b, f32x4 c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
 }

@@ -498,9 +498,8 @@ __global__ __launch_bounds__(256) void merge_kernel(Args a, const int* __restric
 }
 
 // ---- weights of the keys ------------------------------------------------------------------------------------------------
-// out[segment][head][key] = base + sum over the segment's rows and the head's queries of 2^(s - lse). Every key is one wave's or one
-// workgroup's, so that no sums meet in memory and a call's result does not depend on their order.
-// Items: first row, rows, position, table row, segment, first block, last block + 1, 0.
+// out[segment][head][key] = base + sum over the segment's rows and the head's queries of 2^(s - lse). Sums meet in a fixed order, so that a
+// call's result does not depend on who ends first. Items of few rows: first row, rows, position, table row, segment, first block, behind the last, 0.
 struct MassArgs {
   Args a;
   const float* base;      // may be null, or out
@@ -508,184 +507,248 @@ struct MassArgs {
   int N;
 };
 
-// sum over the 16 lanes of a quarter, in every one of them
-__device__ __forceinline__ float over_columns(float x) {
-  x += __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(x), 0x128, 0xf, 0xf, true));   // row_ror 8, 4, 2, 1
-  x += __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(x), 0x124, 0xf, 0xf, true));
-  x += __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(x), 0x122, 0xf, 0xf, true));
-  return x + __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(x), 0x121, 0xf, 0xf, true));
-}
+// Here Q is the first operand: a lane has one key and the rows 4 c + i, so its weights add up in registers, and only the four quarters' sums
+// meet at the end.
 
-// Q of 16 columns in bf16, elements as the lanes hold those of the keys (heads of 64: the two lanes of a half share it)
-template <int D>
-__device__ __forceinline__ int load_q16(bf16x8 (&q)[D / 32], const Args& a, int row, int tokens, int pos, int h, int R0, int lane) {
-  const int R = R0 + (lane & 15), tok = R / a.G, g = R - tok * a.G, c = lane >> 4;
-  const bool there = tok < tokens;
-  const bf16* p = a.q + (int64_t)(row + (there ? tok : 0)) * a.qs + (int64_t)(h * a.G + g) * D + (D == 128 ? 32 * c : 32 * (c & 1) + 16 * (c >> 1));
+// acc[t] += weights of the block's key 16 t + (l & 15) in 16 rows, of which the lane has those whose lse and positions are ls and lim
+__device__ __forceinline__ void add_weights(float (&acc)[4], f32x4 (&s)[4], const f32x4& ls, bool masked, int key0, const int (&lim)[4],
+                                            const Args& a, int lane) {
 #pragma unroll
-  for (int s = 0; s < D / 32; ++s) {
-    q[s] = load_bf16x8(p + 8 * s);
-    if (!there) q[s] = bf16x8{};
+  for (int t = 0; t < 4; ++t) asm volatile("" : "+v"(s[t]));
+  if (masked) {
+#pragma unroll
+    for (int t = 0; t < 4; ++t)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (!sees(key0 + 16 * t + (lane & 15), lim[i], a.window, a.first)) s[t][i] = -INFINITY;
   }
-  return there ? pos + tok : -1;
+#pragma unroll
+  for (int t = 0; t < 4; ++t)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) acc[t] += fast_exp2(fmaf(s[t][i], a.scale2, -ls[i]));
 }
 
-// lse of 16 columns from R0 on; +infinity where there is no row or the row sees nothing (its weights are zero)
+// Q of 16 rows (of a token and a query head) in bf16 and their lse, step s of the products the elements 32 s .. 32 s + 31 (quarters of a
+// lane's own, as single tokens take them, would be four times the cache lines a load); then of the rows ``step`` further. Row and head move on by additions: a division in the loop takes as long as its exponentials.
+template <int D>
+struct Columns {
+  const bf16 *q, *q0;
+  const float *l, *l0;
+  int64_t dq, back_q;       // elements of a step; of a carry from the group's last head to the next row
+  int tok, g, G, rows, dt, dg, dl, back_l;
+  __device__ __forceinline__ Columns(const Args& a, int row, int rows_, int h, int R0, int step, int lane) : G(a.G), rows(rows_) {
+    const int R = R0 + (lane & 15), c = lane >> 4, Hq = a.Hkv * G;
+    tok = R / G, g = R - tok * G;
+    dt = step / G, dg = step - dt * G;
+    q0 = a.q + (int64_t)row * a.qs + (int64_t)h * G * D + 8 * c;
+    l0 = a.lse + (int64_t)row * Hq + h * G;
+    q = q0 + (int64_t)tok * a.qs + (int64_t)g * D;
+    l = l0 + (int64_t)tok * Hq + g;
+    dq = (int64_t)dt * a.qs + (int64_t)dg * D, back_q = a.qs - (int64_t)G * D;
+    dl = dt * Hq + dg, back_l = Hq - G;
+  }
+  __device__ __forceinline__ void next() {
+    tok += dt, g += dg, q += dq, l += dl;
+    if (g >= G) ++tok, g -= G, q += back_q, l += back_l;
+  }
+  // lse; +infinity where there is no row (whose q is the first one's) or the row sees nothing: its weights are zero
+  __device__ __forceinline__ float load(bf16x8 (&x)[D / 32]) const {
+    const bool there = tok < rows;
+    const bf16* p = there ? q : q0;
+#pragma unroll
+    for (int s = 0; s < D / 32; ++s) x[s] = load_bf16x8(p + 32 * s);
+    const float y = *(there ? l : l0);
+    return there && y != -INFINITY ? y : INFINITY;
+  }
+};
+
+// lse of 16 rows from R0 on
 __device__ __forceinline__ float load_lse(const Args& a, int row, int tokens, int h, int R0, int lane) {
   const int R = R0 + (lane & 15), tok = R / a.G, g = R - tok * a.G;
   const float x = a.lse[(int64_t)(row + min(tok, tokens - 1)) * (a.Hkv * a.G) + h * a.G + g];
   return tok >= tokens || x == -INFINITY ? INFINITY : x;
 }
 
-// acc[t][i] += weights of the block's keys 16 t + 4 c + i in 16 columns
-template <int NQ>
-__device__ __forceinline__ void add_weights(float (&acc)[4][4], const f32x4 (&s)[4][NQ], int n, float ls, bool masked, int key0, int lim,
-                                            const Args& a, int lane) {
+// what the lanes l & 15 have of the rows 4 c + i
+template <class T>
+__device__ __forceinline__ void of_rows(T x, T (&y)[4], int lane) {
 #pragma unroll
-  for (int t = 0; t < 4; ++t)
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      float e = fast_exp2(fmaf(s[t][n][i], a.scale2, -ls));
-      if (masked && !sees(key0 + 16 * t + 4 * (lane >> 4) + i, lim, a.window, a.first)) e = 0.f;
-      acc[t][i] += e;
-    }
+  for (int i = 0; i < 4; ++i) y[i] = __shfl(x, 4 * (lane >> 4) + i, 64);
 }
 
-__device__ __forceinline__ void store_mass(const MassArgs& ma, int seg, int h, int key, float x) {
-  if (key >= ma.N) return;
-  const int64_t at = ((int64_t)seg * ma.a.Hkv + h) * ma.N + key;
-  ma.out[at] = (ma.base ? ma.base[at] : 0.f) + x;
-}
-
-// Segments of at most 16 NQ rows: four waves take every fourth block of an item's, its keys widened as they come.
-template <int D, int NQ>
+// Segments of at most 16 rows: four waves take every fourth block of an item's (at most 32), NB of them in registers. What a key had before
+// comes with it: a load that is asked for when its sum is there holds up those of the next keys.
+template <int D, int NB>
 __global__ __launch_bounds__(256) void mass_few_kernel(MassArgs ma) {
   const Args& a = ma.a;
-  __shared__ float sum[4][KB];
   const int* it = reinterpret_cast<const int*>(a.items) + 8 * (blockIdx.x / a.Hkv);
   const int row = it[0], rows = it[1], pos = it[2], table = it[3], seg = it[4], end = it[6];
   const int h = blockIdx.x % a.Hkv, lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int c = lane >> 4, last = pos + rows - 1;
-  if (row < 0 || rows < 0 || row + rows > a.T || rows * a.G > 16 * NQ || end - it[5] > 32) return;
-  const int* bt = a.tables + table * a.ts;
+  const int c = lane >> 4, last = pos + rows - 1, b0 = it[5] + w;
+  if (row < 0 || rows < 0 || row + rows > a.T || rows * a.G > 16 || end - it[5] > 32 || b0 >= end) return;
   const Blocks list(pos, last, a.window, a.first);
   // blocks that no row sees give nothing: behind the last key, between the first ones and the window
   auto seen = [&](int b) { return rows > 0 && b * KB <= last && (b < list.head || b >= list.tail); };
-  int b = it[5] + w;
-  if (b >= end) return;
-  bool bad = false, badn = false;
-  int pg[4], k = 0;
-  KFrag<4> kf, kn;
-  PageIds id;
-  if (rows > 0) id = PageIds(bt, last, lane, [&](int i) { return b + 4 * min(i, 7); });   // (at most eight blocks a wave)
-  if (seen(b)) {
-    id.get<4>(0, a.n_pages, pg, bad);
-    load_k<D, 4>(kf, a.kc, a.Hkv, h, pg, lane);
+  const int64_t at = ((int64_t)seg * a.Hkv + h) * ma.N;
+  float* out = ma.out + at;
+  const float* base = ma.base ? ma.base + at : out;
+  const int n = (end - b0 + 3) / 4;
+  if (rows == 0) {
+    for (int k = 0; k < n; ++k) {
+      const int key = (b0 + 4 * k) * KB + lane;
+      if (key < ma.N) out[key] = ma.base ? base[key] : 0.f;
+    }
+    return;
   }
-  QFrag<D> qf[NQ];
-  int lim[NQ];
-  float ls[NQ];
+  const PageIds id(a.tables + table * a.ts, last, lane, [&](int i) { return b0 + 4 * min(i, 7); });
+  bool bad[NB];
+  KFrag<4> kf[NB];
+  float had[NB];
+  // (without conditions, so that the waits count what is on its way: behind the last block that one again, of no row some page)
+  auto fetch = [&](int x, int k) {
+    k = min(k, n - 1);
+    int pg[4];
+    bad[x] = false;
+    id.get<4>(4 * k, a.n_pages, pg, bad[x]);
+    load_k<D, 4>(kf[x], a.kc, a.Hkv, h, pg, lane);
+    had[x] = base[min((b0 + 4 * k) * KB + lane, ma.N - 1)];
+  };
 #pragma unroll
-  for (int n = 0; n < NQ; ++n)
-    if (rows > 0) {
-      lim[n] = load_q<D>(qf[n], a, row, rows, pos, h, 16 * n, lane);
-      ls[n] = load_lse(a, row, rows, h, 16 * n, lane);
+  for (int x = 0; x < NB; ++x) fetch(x, x);
+  QFrag<D> qf;
+  int lim[4];
+  of_rows(load_q<D>(qf, a, row, rows, pos, h, 0, lane), lim, lane);
+  float l4[4];
+  of_rows(load_lse(a, row, rows, h, 0, lane), l4, lane);
+  const f32x4 ls = {l4[0], l4[1], l4[2], l4[3]};
+  for (int k = 0; k < n; k += NB)
+#pragma unroll
+    for (int x = 0; x < NB; ++x) {
+      const int b = b0 + 4 * (k + x), key0 = b * KB;
+      float acc[4] = {};
+      f32x4 s[4];
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+        s[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int i = 0; i < D / 64; ++i) s[t] = mfma8x4(qf.x[i], qf.s[i], kf[x].d[t], kf[x].s[t], s[t]);
+      }
+      add_weights(acc, s, ls, key0 + KB - 1 > pos || (key0 <= last - a.window && key0 + KB > a.first), key0, lim, a, lane);
+      // lane = key: that of tile c, whose sum every quarter has then
+      float mine = 0.f;
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+        const float y = over_quarters_sum(acc[t]);
+        if (c == t) mine = y;
+      }
+      if (bad[x]) mine = __builtin_nanf("");
+      if (!seen(b)) mine = 0.f;
+      if (k + x < n && key0 + lane < ma.N) out[key0 + lane] = (ma.base ? had[x] : 0.f) + mine;
+      fetch(x, k + x + NB);
     }
-  for (; b < end; b += 4) {
-    const int nb = b + 4;
-    ++k;
-    if (nb < end && seen(nb)) {
-      badn = false;
-      id.get<4>(4 * k, a.n_pages, pg, badn);
-      load_k<D, 4>(kn, a.kc, a.Hkv, h, pg, lane);
-    }
-    float mine = 0.f;
-    const int key0 = b * KB;
-    if (seen(b)) {
-      float acc[4][4] = {};
-      f32x4 s[4][NQ];
-      scores<D, NQ, 4>(kf, qf, s);
-      const bool masked = key0 + KB - 1 > pos || (key0 <= last - a.window && key0 + KB > a.first);
-#pragma unroll
-      for (int n = 0; n < NQ; ++n) add_weights<NQ>(acc, s, n, ls[n], masked, key0, lim[n], a, lane);
-#pragma unroll
-      for (int t = 0; t < 4; ++t)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float x = over_columns(acc[t][i]);
-          if ((lane & 15) == 0) sum[w][16 * t + 4 * c + i] = bad ? __builtin_nanf("") : x;
-        }
-      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-      __builtin_amdgcn_wave_barrier();
-      mine = sum[w][lane];
-      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-      __builtin_amdgcn_wave_barrier();
-    }
-    store_mass(ma, seg, h, key0 + lane, mine);
-    kf = kn;
-    bad = badn;
-  }
 }
 
-// Longer segments: NW waves share the rows that may see a block, whose keys stay widened in registers.
+// Longer segments: NW waves share the rows that may see a block, or a part of them, whose keys stay widened in registers. Parts of a block's
+// rows are joined in their order by the last workgroup of them to end (attn_kernel).
+// Items: first row, rows, position, table row, segment, block, first column, behind the last, first slot or -1, part | parts << 16, 0, 0.
 template <int D, int NW>
 __global__ __launch_bounds__(64 * NW) void mass_many_kernel(MassArgs ma) {
   const Args& a = ma.a;
   __shared__ float sum[NW][KB];
-  const int* it = reinterpret_cast<const int*>(a.items) + 8 * (blockIdx.x / a.Hkv);
-  const int row = it[0], rows = it[1], pos = it[2], table = it[3], seg = it[4], b = it[5], key0 = b * KB;
+  const int* it = reinterpret_cast<const int*>(a.items) + 12 * (blockIdx.x / a.Hkv);
+  const int row = it[0], rows = it[1], pos = it[2], table = it[3], seg = it[4], b = it[5], key0 = b * KB, slot = it[8], parts = it[9] >> 16;
   const int h = blockIdx.x % a.Hkv, lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int c = lane >> 4, last = pos + rows - 1;
   if (row < 0 || rows < 0 || row + rows > a.T) return;
-  const Blocks list(pos, last, a.window, a.first);
-  float acc[4][4] = {};
+  float acc[4] = {};
   bool bad = false;
-  if (rows > 0 && key0 <= last && (b < list.head || b >= list.tail)) {
+  int R = it[6] + 16 * w;
+  const int R1 = min(it[7], rows * a.G);
+  if (it[6] < R1) {
     int pg[4];
-    KFrag<4> kf;
+    uint32_t kw[4][D / 32], ks[4][D / 32];
     PageIds(a.tables + table * a.ts, last, lane, [&](int) { return b; }).get<4>(0, a.n_pages, pg, bad);
-    load_k<D, 4>(kf, a.kc, a.Hkv, h, pg, lane);
-    const int R1 = rows * a.G;
-    int R = (max(0, (key0 - pos) * a.G) & ~15) + 16 * w;                 // rows that may see the block: from its first key's position on
-    bf16x8 qf[D / 32];
-    int lim = load_q16<D>(qf, a, row, rows, pos, h, R, lane);
-    float ls = load_lse(a, row, rows, h, R, lane);
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+      const uint8_t* p = a.kc + ((int64_t)pg[t] * a.Hkv + h) * Page<D>::BYTES;
+#pragma unroll
+      for (int i = 0; i < D / 32; ++i) {
+        kw[t][i] = *reinterpret_cast<const uint32_t*>(p + (lane & 15) * (D / 2) + 16 * i + 4 * c);
+        ks[t][i] = p[Page<D>::DATA + (lane & 15) * (D / 32) + i];
+      }
+    }
+    Columns<D> col(a, row, rows, h, R, 16 * NW, lane);
+    bf16x8 qf[2][D / 32];                                  // of this tile of rows and the next
+    float ls[2];
+    int tok[2];
+    auto fetch = [&](int x) {
+      tok[x] = col.tok;
+      ls[x] = col.load(qf[x]);
+      col.next();
+    };
+    fetch(0);
+    fetch(1);
     bf16x8 k[4][D / 32];
 #pragma unroll
     for (int t = 0; t < 4; ++t)
 #pragma unroll
-      for (int i = 0; i < D / 32; ++i) k[t][i] = widen8(D == 64 && c > 1 ? kf.d[t][2 + i] : kf.d[t][i], scale_of(kf.s[t]));
-    for (; R < R1; R += 16 * NW) {
-      const int pmin = pos + R / a.G, pmax = min(pos + (R + 15) / a.G, last);
-      if (key0 + KB <= pmin - a.window + 1 && key0 >= a.first) break;    // (so do all rows after these)
-      f32x4 s[4][1];
+      for (int i = 0; i < D / 32; ++i) k[t][i] = widen8(kw[t][i], scale_of(ks[t][i]));
+    auto step = [&](int x) {
+      f32x4 s[4];
 #pragma unroll
       for (int t = 0; t < 4; ++t) {
-        s[t][0] = f32x4{0.f, 0.f, 0.f, 0.f};
+        s[t] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int i = 0; i < D / 32; ++i) s[t][0] = mfma16(k[t][i], qf[i], s[t][0]);
+        for (int i = 0; i < D / 32; ++i) s[t] = mfma16(qf[x][i], k[t][i], s[t]);
       }
-      const int lim0 = lim;
-      const float ls0 = ls;
-      lim = load_q16<D>(qf, a, row, rows, pos, h, R + 16 * NW, lane);      // (behind the last row: the first one again)
-      ls = load_lse(a, row, rows, h, R + 16 * NW, lane);
-      const bool masked = key0 + KB - 1 > pmin || (key0 <= pmax - a.window && key0 + KB > a.first);
-      add_weights<1>(acc, s, 0, ls0, masked, key0, lim0, a, lane);
+      float l4[4];
+      of_rows(ls[x], l4, lane);
+      const f32x4 ls4 = {l4[0], l4[1], l4[2], l4[3]};
+      const int pmin = pos + __builtin_amdgcn_readlane(tok[x], 0), pmax = pos + __builtin_amdgcn_readlane(tok[x], 15);
+      const bool masked = key0 + KB - 1 > pmin || pmax > last || (key0 <= pmax - a.window && key0 + KB > a.first);
+      int lim[4];
+      if (masked) of_rows(tok[x] < rows ? pos + tok[x] : -1, lim, lane);
+      fetch(x);                                            // (behind the last row: the first one again)
+      add_weights(acc, s, ls4, masked, key0, lim, a, lane);
+    };
+    for (; R + 16 * NW < R1; R += 32 * NW) {
+      step(0);
+      step(1);
     }
+    if (R < R1) step(0);
   }
 #pragma unroll
-  for (int t = 0; t < 4; ++t)
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float x = over_columns(acc[t][i]);
-      if ((lane & 15) == 0) sum[w][16 * t + 4 * c + i] = bad ? __builtin_nanf("") : x;
-    }
+  for (int t = 0; t < 4; ++t) {
+    const float x = over_quarters_sum(acc[t]);
+    if (c == t) sum[w][lane] = bad ? __builtin_nanf("") : x;
+  }
   __syncthreads();
   if (w) return;
   float mine = 0.f;
 #pragma unroll
   for (int i = 0; i < NW; ++i) mine += sum[i][lane];
-  store_mass(ma, seg, h, key0 + lane, mine);
+  if (slot >= 0) {
+    float* p = a.part + ((int64_t)slot * a.Hkv + h * parts) * KB + lane;
+    __hip_atomic_store(p + (it[9] & 0xffff) * KB, mine, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    int* n = a.counters + (int64_t)slot * a.Hkv + h;
+    int before = 0;
+    if (lane == 0) before = __hip_atomic_fetch_add(n, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    if (__builtin_amdgcn_readfirstlane(before) != parts - 1) return;
+    if (lane == 0) __hip_atomic_store(n, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    mine = 0.f;
+    for (int i0 = 0; i0 < parts; i0 += 8) {
+      float x[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[i] = __hip_atomic_load(p + min(i0 + i, parts - 1) * KB, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) mine += i0 + i < parts ? x[i] : 0.f;
+    }
+  }
+  if (key0 + lane < ma.N) {
+    const int64_t at = ((int64_t)seg * a.Hkv + h) * ma.N + key0 + lane;
+    ma.out[at] = (ma.base ? ma.base[at] : 0.f) + mine;
+  }
 }
 
 }  // namespace kv4
@@ -734,32 +797,31 @@ extern "C" hipError_t kafka_kv4_attn(const bf16* q, int64_t qs, const uint8_t* k
   return hipGetLastError();
 }
 
-constexpr int MASS_NW = 8;
-
-// items of segments of at most 16 rows, then of those of more
+// few: items of segments of at most 16 rows; many: of those of more
 extern "C" hipError_t kafka_kv4_mass(const bf16* q, int64_t qs, const float* lse, const uint8_t* kc, int64_t n_pages, const int* tables,
-                                     int64_t ts, const int* items, int n_few, int n_many, int T, int Hkv, int G, int D, int window,
-                                     int first, float scale, const float* base, float* out, int N, hipStream_t st) {
+                                     int64_t ts, const int* few, int n_few, const int* many, int n_many, int T, int Hkv, int G, int D,
+                                     int window, int first, float scale, const float* base, float* out, int N, float* part, int* counters,
+                                     hipStream_t st) {
   if ((D != 64 && D != 128) || G < 1 || G > 16 || (int64_t)Hkv * n_few >= 1 << 24 || (int64_t)Hkv * n_many >= 1 << 24)
     return hipErrorInvalidValue;
-  auto args = [&](const int* at) {
-    return MassArgs{make_args(q, qs, kc, nullptr, n_pages, tables, ts, at, T, Hkv, G, window, first, scale, nullptr, 0,
-                              const_cast<float*>(lse), nullptr, nullptr),
+  auto args = [&](const int* items) {
+    return MassArgs{make_args(q, qs, kc, nullptr, n_pages, tables, ts, items, T, Hkv, G, window, first, scale, nullptr, 0,
+                              const_cast<float*>(lse), part, nullptr, counters),
                     base, out, N};
   };
   if (n_few) {
-    const MassArgs m = args(items);
+    const MassArgs m = args(few);
     if (D == 128)
-      mass_few_kernel<128, 1><<<Hkv * n_few, 256, 0, st>>>(m);
+      mass_few_kernel<128, 3><<<Hkv * n_few, 256, 0, st>>>(m);
     else
-      mass_few_kernel<64, 1><<<Hkv * n_few, 256, 0, st>>>(m);
+      mass_few_kernel<64, 3><<<Hkv * n_few, 256, 0, st>>>(m);
   }
   if (n_many) {
-    const MassArgs m = args(items + 8 * (int64_t)n_few);
+    const MassArgs m = args(many);
     if (D == 128)
-      mass_many_kernel<128, MASS_NW><<<Hkv * n_many, 64 * MASS_NW, 0, st>>>(m);
+      mass_many_kernel<128, 4><<<Hkv * n_many, 256, 0, st>>>(m);
     else
-      mass_many_kernel<64, MASS_NW><<<Hkv * n_many, 64 * MASS_NW, 0, st>>>(m);
+      mass_many_kernel<64, 4><<<Hkv * n_many, 256, 0, st>>>(m);
   }
   return hipGetLastError();
 }

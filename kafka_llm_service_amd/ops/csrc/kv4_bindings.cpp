@@ -24,8 +24,8 @@ hipError_t kafka_kv4_tiles(const void* q, int64_t qs, const uint8_t* kc, const u
                            int G, int D, int window, int first, float scale, void* out, int64_t os, float* lse, float* part, float* plse,
                            char* ws, hipStream_t st);
 hipError_t kafka_kv4_mass(const void* q, int64_t qs, const float* lse, const uint8_t* kc, int64_t n_pages, const int* tables, int64_t ts,
-                          const int* items, int n_few, int n_many, int T, int Hkv, int G, int D, int window, int first, float scale,
-                          const float* base, float* out, int N, hipStream_t st);
+                          const int* few, int n_few, const int* many, int n_many, int T, int Hkv, int G, int D, int window, int first,
+                          float scale, const float* base, float* out, int N, float* part, int* counters, hipStream_t st);
 }
 
 namespace {
@@ -121,15 +121,15 @@ struct Part {
 };
 struct Plan {
   int64_t heads, kv_heads, dim, window, first, rows, covered, keys, tables;
-  int64_t segments = 0, mass_few = 0;
+  int64_t segments = 0, mass_slots = 0;
   std::vector<Part> parts;
-  OptT mass;
+  OptT few, many;                 // items of attn_mass
 
   // Counters of split tiles, which every launch leaves zero: one set for each stream that the plan is used on. A captured call has a set of its
   // own, cleared in its graph, since the graph may be replayed beside anything.
   mutable std::vector<std::pair<hipStream_t, Tensor>> counters;
   int* zeros(int64_t n, Tensor& held) const {
-    const auto opt = parts[0].items.options();
+    const auto opt = (parts.empty() ? *many : parts[0].items).options();
     hipStreamCaptureStatus status;
     KV4_HIP(hipStreamIsCapturing(stream(), &status));
     if (status != hipStreamCaptureStatusNone) {
@@ -150,11 +150,14 @@ struct Plan {
     TORCH_CHECK_VALUE(ok(items, wide ? 12 : 8) && ok(merges, 4) && ok(keys, 4) && r > 0 && r <= 256 && slots >= 0 && slots < 1 << 24, "kv4: plan");
     parts.push_back({r, w, slots, items, merges, keys});
   }
-  void weigh(Tensor items, int64_t few, int64_t n) {
-    TORCH_CHECK_VALUE(items.is_cuda() && items.scalar_type() == at::kInt && items.dim() == 2 && items.size(1) == 8 && items.is_contiguous() &&
-                          few >= 0 && few <= items.size(0) && items.size(0) < 1 << 24, "kv4: plan");
-    mass = items;
-    mass_few = few;
+  void weigh(Tensor f, Tensor m, int64_t slots, int64_t n) {
+    auto ok = [&](const Tensor& t, int64_t cols) {
+      return t.is_cuda() && t.scalar_type() == at::kInt && t.dim() == 2 && t.size(1) == cols && t.is_contiguous() && t.size(0) < 1 << 24;
+    };
+    TORCH_CHECK_VALUE(ok(f, 8) && ok(m, 12) && f.device() == m.device() && slots >= 0 && slots < 1 << 24, "kv4: plan");
+    few = f;
+    many = m;
+    mass_slots = slots;
     segments = n;
   }
 };
@@ -227,7 +230,7 @@ Tensor attn_mass(Tensor q, Tensor lse, Tensor kc, Tensor tables, const Plan& p, 
   const int D = cache(kc, "k_cache");
   const c10::DeviceGuard guard(kc.device());
   const int* tp = call(p, q, kc, D, tables);
-  TORCH_CHECK_VALUE(p.mass.has_value() && p.mass->device() == kc.device(), "attn_mass: a plan of attn_plan for this device expected");
+  TORCH_CHECK_VALUE(p.few.has_value() && p.few->device() == kc.device(), "attn_mass: a plan of attn_plan for this device expected");
   const float* lp = row_values(lse, q, kc);
   const int64_t S = p.segments, H = p.kv_heads;
   int64_t N = p.keys;
@@ -246,10 +249,18 @@ Tensor attn_mass(Tensor q, Tensor lse, Tensor kc, Tensor tables, const Plan& p, 
     if (base.has_value()) rest.copy_(base->narrow(2, done, N - done));
     else rest.zero_();
   }
-  KV4_HIP(kafka_kv4_mass(q.data_ptr(), q.stride(0), lp, kc.data_ptr<uint8_t>(), kc.size(0), tp, tables.stride(0), p.mass->data_ptr<int>(),
-                         (int)p.mass_few, (int)(p.mass->size(0) - p.mass_few), (int)q.size(0), (int)H, (int)(p.heads / H), D, (int)p.window,
-                         (int)p.first, (float)scale, base.has_value() ? base->data_ptr<float>() : nullptr, out.data_ptr<float>(), (int)N,
-                         stream()));
+  Tensor part, held;
+  float* pp = nullptr;
+  int* counters = nullptr;
+  if (p.mass_slots > 0) {
+    part = at::empty({p.mass_slots * H * 64}, lse.options());
+    pp = part.data_ptr<float>();
+    counters = p.zeros(p.mass_slots * H, held);
+  }
+  KV4_HIP(kafka_kv4_mass(q.data_ptr(), q.stride(0), lp, kc.data_ptr<uint8_t>(), kc.size(0), tp, tables.stride(0), p.few->data_ptr<int>(),
+                         (int)p.few->size(0), p.many->data_ptr<int>(), (int)p.many->size(0), (int)q.size(0), (int)H, (int)(p.heads / H), D,
+                         (int)p.window, (int)p.first, (float)scale, base.has_value() ? base->data_ptr<float>() : nullptr,
+                         out.data_ptr<float>(), (int)N, pp, counters, stream()));
   return out;
 }
 

@@ -57,12 +57,14 @@ MANY_MIN = 128             # rows of a segment from which on its keys may be wid
 MANY_WORK = 1 << 29        # and work (pairs of rows and keys, times heads, times dim) of all such segments from which on they are
 MANY_BLOCKS = 8            # blocks of a piece of a wide tile
 CUS = 256
-SHORT_BLOCKS = 32          # blocks a CU up to which a launch is short: workgroups of eight waves, tiles whole
-SHORT_PIECE = 16           # blocks of a piece in it: two for each wave
+LEAST_SHARE = 4            # blocks a CU up to which every four of them are a workgroup, one for each wave
+SHORT_TILE = 16            # blocks of a tile on average below which four waves take it, else eight
 LONG_WGS = 1024            # workgroups of four waves that a longer launch is split towards
 LONG_PIECE = 4
 MASS_FEW = 16              # rows of a segment up to which a wave takes them all for its block of keys
-MASS_WGS = 1024
+MASS_WGS = 1024            # workgroups that a launch of few rows is split towards
+MASS_MANY_WGS = 768        # ... of portions (as many as the CUs hold)
+MASS_TILES = 16            # tiles of 16 rows of a part: four for each of its waves
 
 
 class AttnPlan:
@@ -109,8 +111,10 @@ def _pieces(tiles: np.ndarray, count: np.ndarray, n: np.ndarray):
 def _narrow_split(count: np.ndarray, kv_heads: int, rows: int) -> tuple[int, np.ndarray]:
     """(waves of a workgroup, pieces of every tile) for tiles of ``rows`` rows that see ``count`` blocks."""
     total = int(count.sum()) * kv_heads
-    if rows == FEW_ROWS and total <= SHORT_BLOCKS * CUS:
-        return 8, np.maximum(1, count // max(SHORT_PIECE, -(-total // CUS)))
+    share = -(-total // CUS)
+    if rows == FEW_ROWS and share > LEAST_SHARE:
+        waves = 4 if int(count.sum()) < SHORT_TILE * len(count) else 8
+        return waves, np.maximum(1, count // max(2 * waves if waves == 4 else waves, share))
     size = max(LONG_PIECE, -(-total // LONG_WGS))
     return 4, np.maximum(1, (count + size - 1) // size)
 
@@ -164,6 +168,39 @@ def _tables(full: np.ndarray, heads: int, kv_heads: int, dim: int, window: int, 
     return shapes, arrays
 
 
+def _mass_tables(a: np.ndarray, G: int, kv_heads: int, keys: int, window: int, first: int):
+    """Items of ``attn_mass`` for single tokens, for portions, and their partial results: every block of 64 of the plan's ``keys`` of every
+    segment once, or in parts of the rows that see it where the blocks by themselves are too few workgroups."""
+    nb = (keys + BLOCK - 1) // BLOCK
+    few = a[:, 1] * G <= MASS_FEW
+    idx = np.nonzero(few)[0]
+    step = min(32, max(4, -(-nb * len(idx) * kv_heads // MASS_WGS // 4) * 4))
+    b = np.arange(0, nb, step)
+    s, b = np.repeat(idx, len(b)), np.tile(b, len(idx))
+    out = [np.stack([a[s, 0], a[s, 1], a[s, 2], a[s, 3], s, b, np.minimum(b + step, nb), np.zeros_like(s)], 1).astype(np.int32)]
+    idx = np.nonzero(~few)[0]
+    s, b = np.repeat(idx, nb), np.tile(np.arange(nb), len(idx))
+    # columns (row, query head) that may see the block: rows from its first key's position on, to the last whose window has its last key
+    lo = np.minimum(np.maximum(0, (b * BLOCK - a[s, 2]) * G) // 16 * 16, a[s, 1] * G)
+    hi = a[s, 1] * G
+    if window:
+        end = np.clip((b * BLOCK + BLOCK - 1 + window - a[s, 2]) * G, 0, hi)
+        hi = np.where(b * BLOCK < first, hi, end)
+    tiles = np.maximum(0, hi - lo + 15) // 16
+    size = max(MASS_TILES, -(-int(tiles.sum()) * kv_heads // MASS_MANY_WGS))
+    n = np.maximum(1, (tiles + size // 2) // size)
+    each = np.maximum(1, (tiles + n - 1) // n)
+    n = np.maximum(1, (tiles + each - 1) // each)
+    t = np.repeat(np.arange(len(s)), n)
+    i = np.arange(len(t)) - np.repeat(np.cumsum(n) - n, n)
+    split = np.where(n > 1, n, 0)
+    slot = np.where(n > 1, np.cumsum(split) - split, -1)
+    s, b, at = s[t], b[t], lo[t] + 16 * each[t] * i
+    z = np.zeros_like(s)
+    many = np.stack([a[s, 0], a[s, 1], a[s, 2], a[s, 3], s, b, at, np.minimum(at + 16 * each[t], hi[t]), slot[t], n[t] << 16 | i, z, z], 1)
+    return out[0], many[np.argsort(many[:, 6] - many[:, 7], kind="stable")].astype(np.int32), int(split.sum())
+
+
 class _Take:
     """Tables one behind the other in a flat int32 tensor."""
 
@@ -212,16 +249,10 @@ def attn_plan(segs, heads: int, kv_heads: int, dim: int, window: int = 0, first:
     if dev.type != "cuda":
         return p
     shapes, arrays = _tables(a[a[:, 1] > 0], heads, kv_heads, dim, p.window, p.first)
-    few = a[:, 1] * (heads // kv_heads) <= MASS_FEW
-    nb = (p.keys + BLOCK - 1) // BLOCK
-    mass = []
-    for pick, step in ((few, min(32, max(4, -(-nb * int(few.sum()) * kv_heads // MASS_WGS // 4) * 4))), (~few, 1)):
-        idx, b = np.nonzero(pick)[0], np.arange(0, nb, step)
-        s, b = np.repeat(idx, len(b)), np.tile(b, len(idx))
-        mass.append(np.stack([a[s, 0], a[s, 1], a[s, 2], a[s, 3], s, b, np.minimum(b + step, nb), np.zeros_like(s)], 1).astype(np.int32))
-    take = _Take(torch.from_numpy(np.concatenate([t.reshape(-1) for t in arrays + mass])).to(dev))
+    few, many, slots = _mass_tables(a, heads // kv_heads, kv_heads, p.keys, p.window, p.first)
+    take = _Take(torch.from_numpy(np.concatenate([t.reshape(-1) for t in arrays + [few, many]])).to(dev))
     _native(p, take, shapes)
-    p.native.weigh(take(len(mass[0]) + len(mass[1]), 8), len(mass[0]), len(a))
+    p.native.weigh(take(len(few), 8), take(len(many), 12), slots, len(a))
     return p
 
 

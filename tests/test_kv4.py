@@ -513,7 +513,8 @@ def test_attention_on_the_gpu(cuda, monkeypatch, case, wide):
     """Every kind of tile, whatever the sizes from which on a plan takes it."""
     if wide:
         monkeypatch.setattr(kv4, "MANY_WORK", 0)
-        monkeypatch.setattr(kv4, "SHORT_BLOCKS", 0)
+        monkeypatch.setattr(kv4, "LEAST_SHARE", 0)
+        monkeypatch.setattr(kv4, "MASS_TILES", 1)
     else:
         monkeypatch.setattr(kv4, "MANY_WORK", 1 << 60)
     _check_attention(case, cuda)
