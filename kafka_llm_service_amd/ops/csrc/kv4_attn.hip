@@ -8,6 +8,7 @@
 //   O^T[d][row]  += V^T . P    A: a lane's values of four keys, two neighbouring d's a register as they are widened (exactly), B: P as S^T's
 //                              registers hold it, beside zeros for the other d: twice the products, but no register is turned
 // The softmax runs in one pass with a running maximum per row; its sums and maxima are fp32, P is rounded to bf16 for the product.
+#include "attn_tile.h"
 #include "kv4.h"
 
 #include <type_traits>
@@ -528,40 +529,6 @@ __device__ __forceinline__ void add_weights(float (&acc)[4], f32x4 (&s)[4], cons
     for (int i = 0; i < 4; ++i) acc[t] += fast_exp2(fmaf(s[t][i], a.scale2, -ls[i]));
 }
 
-// Q of 16 rows (of a token and a query head) in bf16 and their lse, step s of the products the elements 32 s .. 32 s + 31 (quarters of a
-// lane's own, as single tokens take them, would be four times the cache lines a load); then of the rows ``step`` further. Row and head move on by additions: a division in the loop takes as long as its exponentials.
-template <int D>
-struct Columns {
-  const bf16 *q, *q0;
-  const float *l, *l0;
-  int64_t dq, back_q;       // elements of a step; of a carry from the group's last head to the next row
-  int tok, g, G, rows, dt, dg, dl, back_l;
-  __device__ __forceinline__ Columns(const Args& a, int row, int rows_, int h, int R0, int step, int lane) : G(a.G), rows(rows_) {
-    const int R = R0 + (lane & 15), c = lane >> 4, Hq = a.Hkv * G;
-    tok = R / G, g = R - tok * G;
-    dt = step / G, dg = step - dt * G;
-    q0 = a.q + (int64_t)row * a.qs + (int64_t)h * G * D + 8 * c;
-    l0 = a.lse + (int64_t)row * Hq + h * G;
-    q = q0 + (int64_t)tok * a.qs + (int64_t)g * D;
-    l = l0 + (int64_t)tok * Hq + g;
-    dq = (int64_t)dt * a.qs + (int64_t)dg * D, back_q = a.qs - (int64_t)G * D;
-    dl = dt * Hq + dg, back_l = Hq - G;
-  }
-  __device__ __forceinline__ void next() {
-    tok += dt, g += dg, q += dq, l += dl;
-    if (g >= G) ++tok, g -= G, q += back_q, l += back_l;
-  }
-  // lse; +infinity where there is no row (whose q is the first one's) or the row sees nothing: its weights are zero
-  __device__ __forceinline__ float load(bf16x8 (&x)[D / 32]) const {
-    const bool there = tok < rows;
-    const bf16* p = there ? q : q0;
-#pragma unroll
-    for (int s = 0; s < D / 32; ++s) x[s] = load_bf16x8(p + 32 * s);
-    const float y = *(there ? l : l0);
-    return there && y != -INFINITY ? y : INFINITY;
-  }
-};
-
 // lse of 16 rows from R0 on
 __device__ __forceinline__ float load_lse(const Args& a, int row, int tokens, int h, int R0, int lane) {
   const int R = R0 + (lane & 15), tok = R / a.G, g = R - tok * a.G;
@@ -648,105 +615,160 @@ __global__ __launch_bounds__(256) void mass_few_kernel(MassArgs ma) {
     }
 }
 
-// Longer segments: NW waves share the rows that may see a block, or a part of them, whose keys stay widened in registers. Parts of a block's
-// rows are joined in their order by the last workgroup of them to end (attn_kernel).
+// Longer segments: four waves, a block of keys each, its keys widened in registers, go through the same rows, all that may see one of the
+// blocks or a part of them, in stages of 64 that stay in LDS for all four (each wave's own loads of 16 rows, 256 bytes apart, would take
+// 64 cycles a load of what the CU has for all its waves, four times what they need to be computed). A lane has one of 16 rows and a quarter of
+// the keys, each key's sum by itself: no lane asks another for anything until the rows end. Parts of a block's rows are joined in their
+// order by the last workgroup of them to end (attn_kernel).
 // Items: first row, rows, position, table row, segment, block, first column, behind the last, first slot or -1, part | parts << 16, 0, 0.
-template <int D, int NW>
-__global__ __launch_bounds__(64 * NW) void mass_many_kernel(MassArgs ma) {
+template <int D>
+__global__ __launch_bounds__(256, 4) void mass_many_kernel(MassArgs ma) {
+  constexpr int CH = 64, STAGE = CH * D * 2, PIECES = STAGE / 4096;
   const Args& a = ma.a;
-  __shared__ float sum[NW][KB];
+  // (one object: of several the compiler knows which one a load fills, and waits for it ahead of every read)
+  __shared__ __attribute__((aligned(1024))) char smem[2 * STAGE + 2 * CH * 4];
+  char* const rows_q = smem;
+  char* const rows_l = smem + 2 * STAGE;
   const int* it = reinterpret_cast<const int*>(a.items) + 12 * (blockIdx.x / a.Hkv);
-  const int row = it[0], rows = it[1], pos = it[2], table = it[3], seg = it[4], b = it[5], key0 = b * KB, slot = it[8], parts = it[9] >> 16;
+  const int row = it[0], rows = it[1], pos = it[2], table = it[3], seg = it[4], slot = it[8], part = it[9] & 0xffff, parts = it[9] >> 16;
   const int h = blockIdx.x % a.Hkv, lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int c = lane >> 4, last = pos + rows - 1;
+  const int c = lane >> 4, last = pos + rows - 1, G = a.G, key0 = (it[5] + w) * KB;
   if (row < 0 || rows < 0 || row + rows > a.T) return;
-  float acc[4] = {};
-  bool bad = false;
-  int R = it[6] + 16 * w;
-  const int R1 = min(it[7], rows * a.G);
+  float acc[16] = {};
+  bool bad = false, any = false;
+  const int R1 = min(it[7], rows * G);
   if (it[6] < R1) {
-    int pg[4];
-    uint32_t kw[4][D / 32], ks[4][D / 32];
-    PageIds(a.tables + table * a.ts, last, lane, [&](int) { return b; }).get<4>(0, a.n_pages, pg, bad);
+    // x / G of x < 80
+    const uint32_t inv = 65536u / G + 1;
+    int tok = it[6] / G, rem = it[6] - tok * G;            // token and query head of the next stage's first column
+    const int Hq = a.Hkv * G;
+    const bf16* q0 = a.q + (int64_t)row * a.qs + (int64_t)h * G * D;
+    const float* l0 = a.lse + (int64_t)row * Hq + h * G;
+    // The 16 bytes k of row r lie at k ^ r (heads of 64: k ^ r / 2): 16 lanes read them without a bank taken twice. Behind the last row: some row.
+    auto stage = [&](int buf) {
+      const int t0 = min(tok, rows - 1);
+      auto of = [&](int r, uint32_t& dx, uint32_t& g) {    // row and head of column r, none behind the last
+        const uint32_t x = rem + r;
+        dx = x * inv >> 16, g = x - dx * G;
+        dx = min(dx, (uint32_t)(rows - 1 - t0));
+      };
+      uint32_t dx, g;
+      int ln = lane;
+      asm volatile("" : "+v"(ln));                         // (or its multiples of every piece stay in registers all the time)
 #pragma unroll
-    for (int t = 0; t < 4; ++t) {
-      const uint8_t* p = a.kc + ((int64_t)pg[t] * a.Hkv + h) * Page<D>::BYTES;
-#pragma unroll
-      for (int i = 0; i < D / 32; ++i) {
-        kw[t][i] = *reinterpret_cast<const uint32_t*>(p + (lane & 15) * (D / 2) + 16 * i + 4 * c);
-        ks[t][i] = p[Page<D>::DATA + (lane & 15) * (D / 32) + i];
+      for (int i = 0; i < PIECES; ++i) {
+        const int p = PIECES * w + i, n = D / 8, r = p * (64 / n) + ln / n, k = (ln & (n - 1)) ^ (D == 128 ? r & 15 : r >> 1 & 7);
+        of(r, dx, g);
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(buf_rsrc(q0 + t0 * a.qs), (lds_void_t*)(rows_q + buf * STAGE + 1024 * p), 16,
+                                                 2 * (dx * (uint32_t)a.qs + g * D) + 16 * k, 0, 0, 0);
       }
-    }
-    Columns<D> col(a, row, rows, h, R, 16 * NW, lane);
-    bf16x8 qf[2][D / 32];                                  // of this tile of rows and the next
-    float ls[2];
-    int tok[2];
-    auto fetch = [&](int x) {
-      tok[x] = col.tok;
-      ls[x] = col.load(qf[x]);
-      col.next();
+      if (w == 0) {
+        of(ln, dx, g);
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(buf_rsrc(l0 + (int64_t)t0 * Hq), (lds_void_t*)(rows_l + buf * (CH * 4)), 4, 4 * (dx * Hq + g), 0, 0, 0);
+      }
     };
-    fetch(0);
-    fetch(1);
+    stage(0);
     bf16x8 k[4][D / 32];
-#pragma unroll
-    for (int t = 0; t < 4; ++t)
-#pragma unroll
-      for (int i = 0; i < D / 32; ++i) k[t][i] = widen8(kw[t][i], scale_of(ks[t][i]));
-    auto step = [&](int x) {
-      f32x4 s[4];
+    {
+      int pg[4];
+      uint32_t kw[4][D / 32], ks[4][D / 32];
+      PageIds(a.tables + table * a.ts, last, lane, [&](int) { return it[5] + w; }).get<4>(0, a.n_pages, pg, bad);
 #pragma unroll
       for (int t = 0; t < 4; ++t) {
-        s[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+        const uint8_t* p = a.kc + ((int64_t)pg[t] * a.Hkv + h) * Page<D>::BYTES;
 #pragma unroll
-        for (int i = 0; i < D / 32; ++i) s[t] = mfma16(qf[x][i], k[t][i], s[t]);
+        for (int i = 0; i < D / 32; ++i) {
+          kw[t][i] = *reinterpret_cast<const uint32_t*>(p + (lane & 15) * (D / 2) + 16 * i + 4 * c);
+          ks[t][i] = p[Page<D>::DATA + (lane & 15) * (D / 32) + i];
+        }
       }
-      float l4[4];
-      of_rows(ls[x], l4, lane);
-      const f32x4 ls4 = {l4[0], l4[1], l4[2], l4[3]};
-      const int pmin = pos + __builtin_amdgcn_readlane(tok[x], 0), pmax = pos + __builtin_amdgcn_readlane(tok[x], 15);
-      const bool masked = key0 + KB - 1 > pmin || pmax > last || (key0 <= pmax - a.window && key0 + KB > a.first);
-      int lim[4];
-      if (masked) of_rows(tok[x] < rows ? pos + tok[x] : -1, lim, lane);
-      fetch(x);                                            // (behind the last row: the first one again)
-      add_weights(acc, s, ls4, masked, key0, lim, a, lane);
-    };
-    for (; R + 16 * NW < R1; R += 32 * NW) {
-      step(0);
-      step(1);
+#pragma unroll
+      for (int t = 0; t < 4; ++t)
+#pragma unroll
+        for (int i = 0; i < D / 32; ++i) k[t][i] = widen8(kw[t][i], scale_of(ks[t][i]));
     }
-    if (R < R1) step(0);
-  }
+    int buf = 0;
+    for (int R = it[6]; R < R1; R += CH, buf ^= 1) {
+      const int tok0 = tok, rem0 = rem;
+      rem += CH % G, tok += CH / G;
+      if (rem >= G) ++tok, rem -= G;
+      t3_wait_vmcnt<0>();                                  // this stage; and all have done with the one before the next takes its place
+      t3_barrier();
+      if (R + CH < R1) stage(buf ^ 1);
+      for (int j = 0; j < CH; j += 16) {
+        const int pmin = pos + tok0 + (int)((rem0 + j) * inv >> 16), pmax = pos + tok0 + (int)((rem0 + j + 15) * inv >> 16);
+        if (R + j >= R1 || pmax < key0 || (pmin - a.window >= key0 + KB - 1 && key0 >= a.first)) continue;
+        any = true;
+        const int r = j + (lane & 15);
+        bf16x8 q[D / 32];
 #pragma unroll
-  for (int t = 0; t < 4; ++t) {
-    const float x = over_quarters_sum(acc[t]);
-    if (c == t) sum[w][lane] = bad ? __builtin_nanf("") : x;
-  }
-  __syncthreads();
-  if (w) return;
-  float mine = 0.f;
+        for (int i = 0; i < D / 32; ++i)
+          q[i] = *reinterpret_cast<const bf16x8*>(rows_q + buf * STAGE + r * (2 * D) + 16 * ((4 * i + c) ^ (D == 128 ? lane & 15 : lane >> 1 & 7)));
+        const int t = tok0 + (int)((rem0 + r) * inv >> 16), lim = t < rows ? pos + t : -1;
+        float l = *reinterpret_cast<const float*>(rows_l + buf * (CH * 4) + 4 * r);
+        l = lim >= 0 && l != -INFINITY ? l : INFINITY;     // no row, or one that sees nothing: weights of zero
+        const bool masked = key0 + KB - 1 > pmin || pmax > last || (key0 <= pmax - a.window && key0 + KB > a.first);
 #pragma unroll
-  for (int i = 0; i < NW; ++i) mine += sum[i][lane];
+        for (int u = 0; u < 4; u += 2) {
+          f32x4 s[2];
+#pragma unroll
+          for (int t = 0; t < 2; ++t) {
+            s[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int i = 0; i < D / 32; ++i) s[t] = mfma16(k[u + t][i], q[i], s[t]);
+          }
+#pragma unroll
+          for (int t = 0; t < 2; ++t) asm volatile("" : "+v"(s[t]));
+          if (masked) {
+            int cc = c;
+            asm volatile("" : "+v"(cc));
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+#pragma unroll
+              for (int i = 0; i < 4; ++i)
+                if (!sees(key0 + 16 * (u + t) + 4 * cc + i, lim, a.window, a.first)) s[t][i] = -INFINITY;
+          }
+#pragma unroll
+          for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) acc[4 * (u + t) + i] += fast_exp2(fmaf(s[t][i], a.scale2, -l));
+        }
+      }
+    }
+  }
+  // over the 16 rows: halves of the sums change places until a lane has one of them
+#pragma unroll
+  for (int n = 8; n; n /= 2)
+#pragma unroll
+    for (int j = 0; j < n; ++j) {
+      const bool up = lane & n;
+      const float keep = up ? acc[j + n] : acc[j], give = up ? acc[j] : acc[j + n];
+      acc[j] = keep + __shfl_xor(give, n, 64);
+    }
+  float mine = bad && any ? __builtin_nanf("") : acc[0];
   if (slot >= 0) {
-    float* p = a.part + ((int64_t)slot * a.Hkv + h * parts) * KB + lane;
-    __hip_atomic_store(p + (it[9] & 0xffff) * KB, mine, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    float* p = a.part + (((int64_t)slot * a.Hkv + h * parts) * 4 + w) * KB + lane;
+    __hip_atomic_store(p + part * (4 * KB), mine, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
     int* n = a.counters + (int64_t)slot * a.Hkv + h;
-    int before = 0;
-    if (lane == 0) before = __hip_atomic_fetch_add(n, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    if (__builtin_amdgcn_readfirstlane(before) != parts - 1) return;
-    if (lane == 0) __hip_atomic_store(n, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    int* const before = reinterpret_cast<int*>(smem);      // (nobody reads rows any more)
+    if (threadIdx.x == 0) *before = __hip_atomic_fetch_add(n, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    __syncthreads();
+    if (*before != parts - 1) return;
+    if (threadIdx.x == 0) __hip_atomic_store(n, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     mine = 0.f;
     for (int i0 = 0; i0 < parts; i0 += 8) {
       float x[8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) x[i] = __hip_atomic_load(p + min(i0 + i, parts - 1) * KB, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      for (int i = 0; i < 8; ++i) x[i] = __hip_atomic_load(p + min(i0 + i, parts - 1) * (4 * KB), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 #pragma unroll
       for (int i = 0; i < 8; ++i) mine += i0 + i < parts ? x[i] : 0.f;
     }
   }
-  if (key0 + lane < ma.N) {
-    const int64_t at = ((int64_t)seg * a.Hkv + h) * ma.N + key0 + lane;
+  const int key = key0 + 16 * ((lane & 15) >> 2) + 4 * c + (lane & 3);
+  if (key < ma.N) {
+    const int64_t at = ((int64_t)seg * a.Hkv + h) * ma.N + key;
     ma.out[at] = (ma.base ? ma.base[at] : 0.f) + mine;
   }
 }
@@ -819,9 +841,9 @@ extern "C" hipError_t kafka_kv4_mass(const bf16* q, int64_t qs, const float* lse
   if (n_many) {
     const MassArgs m = args(many);
     if (D == 128)
-      mass_many_kernel<128, 4><<<Hkv * n_many, 256, 0, st>>>(m);
+      mass_many_kernel<128><<<Hkv * n_many, 256, 0, st>>>(m);
     else
-      mass_many_kernel<64, 4><<<Hkv * n_many, 256, 0, st>>>(m);
+      mass_many_kernel<64><<<Hkv * n_many, 256, 0, st>>>(m);
   }
   return hipGetLastError();
 }

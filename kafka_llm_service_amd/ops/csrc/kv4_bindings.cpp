@@ -231,6 +231,7 @@ Tensor attn_mass(Tensor q, Tensor lse, Tensor kc, Tensor tables, const Plan& p, 
   const c10::DeviceGuard guard(kc.device());
   const int* tp = call(p, q, kc, D, tables);
   TORCH_CHECK_VALUE(p.few.has_value() && p.few->device() == kc.device(), "attn_mass: a plan of attn_plan for this device expected");
+  TORCH_CHECK_VALUE(p.rows < 2 || q.stride(0) < 1 << 23, "attn_mass: q's rows less than 2^23 elements apart");
   const float* lp = row_values(lse, q, kc);
   const int64_t S = p.segments, H = p.kv_heads;
   int64_t N = p.keys;
@@ -253,7 +254,7 @@ Tensor attn_mass(Tensor q, Tensor lse, Tensor kc, Tensor tables, const Plan& p, 
   float* pp = nullptr;
   int* counters = nullptr;
   if (p.mass_slots > 0) {
-    part = at::empty({p.mass_slots * H * 64}, lse.options());
+    part = at::empty({p.mass_slots * H * 256}, lse.options());
     pp = part.data_ptr<float>();
     counters = p.zeros(p.mass_slots * H, held);
   }

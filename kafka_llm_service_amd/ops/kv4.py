@@ -63,7 +63,7 @@ LONG_WGS = 1024            # workgroups of four waves that a longer launch is sp
 LONG_PIECE = 4
 MASS_FEW = 16              # rows of a segment up to which a wave takes them all for its block of keys
 MASS_WGS = 1024            # workgroups that a launch of few rows is split towards
-MASS_MANY_WGS = 768        # ... of portions (as many as the CUs hold)
+MASS_MANY_WGS = 2048       # ... of portions (twice as many as the CUs hold: parts of rows are unequal; 1900 rows 45 us, with 1024 49, 512 62)
 MASS_TILES = 16            # tiles of 16 rows of a part: four for each of its waves
 
 
@@ -179,12 +179,13 @@ def _mass_tables(a: np.ndarray, G: int, kv_heads: int, keys: int, window: int, f
     s, b = np.repeat(idx, len(b)), np.tile(b, len(idx))
     out = [np.stack([a[s, 0], a[s, 1], a[s, 2], a[s, 3], s, b, np.minimum(b + step, nb), np.zeros_like(s)], 1).astype(np.int32)]
     idx = np.nonzero(~few)[0]
-    s, b = np.repeat(idx, nb), np.tile(np.arange(nb), len(idx))
-    # columns (row, query head) that may see the block: rows from its first key's position on, to the last whose window has its last key
+    nq = (nb + 3) // 4
+    s, b = np.repeat(idx, nq), np.tile(4 * np.arange(nq), len(idx))
+    # columns (row, query head) that may see one of four blocks: rows from its first key's position on, to the last whose window has its last
     lo = np.minimum(np.maximum(0, (b * BLOCK - a[s, 2]) * G) // 16 * 16, a[s, 1] * G)
     hi = a[s, 1] * G
     if window:
-        end = np.clip((b * BLOCK + BLOCK - 1 + window - a[s, 2]) * G, 0, hi)
+        end = np.clip((b * BLOCK + 4 * BLOCK - 1 + window - a[s, 2]) * G, 0, hi)
         hi = np.where(b * BLOCK < first, hi, end)
     tiles = np.maximum(0, hi - lo + 15) // 16
     size = max(MASS_TILES, -(-int(tiles.sum()) * kv_heads // MASS_MANY_WGS))
