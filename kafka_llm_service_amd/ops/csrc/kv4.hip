@@ -133,42 +133,42 @@ __device__ __forceinline__ uint32_t rank_of(float x) {
   return a == 0u ? 0x80000000u : (b & 0x80000000u) ? ~b : b | 0x80000000u;
 }
 
-constexpr int KEEP_NT = 1024, KEEP_NW = KEEP_NT / 64, KEEP_PER = 16;
+constexpr int KEEP_NT = 1024, KEEP_NW = KEEP_NT / 64;
+
+// Inclusive sum over a wave: shifts within rows of 16, then the last lane of a row to the next one, of the first half to the second.
+__device__ __forceinline__ int wave_sums(int x) {
+  x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);
+  return x;
+}
 
 // Exclusive sum over the workgroup's threads, and the whole. ``ws`` holds KEEP_NW ints and is free again behind the next barrier.
 __device__ __forceinline__ int before_thread(int x, int* ws, int& all) {
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-  int inc = x;
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const int y = __shfl_up(inc, o, 64);
-    if (lane >= o) inc += y;
-  }
+  const int inc = wave_sums(x);
   if (lane == 63) ws[w] = inc;
   __syncthreads();
-  int at = inc - x;
-  all = 0;
-#pragma unroll
-  for (int i = 0; i < KEEP_NW; ++i) {
-    if (i < w) at += ws[i];
-    all += ws[i];
-  }
-  return at;
+  const int sums = wave_sums(lane < KEEP_NW ? ws[lane] : 0);
+  all = __builtin_amdgcn_readlane(sums, 63);
+  return inc - x + (w ? __builtin_amdgcn_readlane(sums, w - 1) : 0);
 }
 
 // Kept keys of one (sequence, head), ascending: the first ones, the most recent ones, and of those between them the ``room`` largest, ties to
-// the lowest index. Radix select: four counts of a byte each narrow the threshold down, then the keys are numbered in order. A thread
-// holds KEEP_PER neighbouring keys; of longer sequences (REG false) they are read again, a chunk of KEEP_NT * KEEP_PER at a time. Each wave counts for
-// itself: the leading byte has few values, and 1024 threads at one counter wait for each other.
-template <bool REG>
+// the lowest index. Radix select: counts of 11 bits each narrow the threshold down (masses of one size share their leading byte: of 8 bits each
+// many threads would wait at one counter) until its equals are as many as are wanted, then the keys are numbered in order. A thread
+// holds PER neighbouring keys; of sequences that fit no such kernel (REG false) they are read again, KEEP_NT * PER at a time.
+template <int PER, bool REG>
 __global__ __launch_bounds__(KEEP_NT) void evict_keep_kernel(const float* __restrict__ mass, int64_t ms, int64_t mh, int N,
                                                              const int* __restrict__ lens, int budget, int first, int recent,
                                                              int* __restrict__ kept, int Hkv) {
-  constexpr int PER = KEEP_PER, CHUNK = KEEP_NT * PER;
-  __shared__ int hist[KEEP_NW][257];                                     // (a wave's counters a bank further than the last one's)
-  __shared__ int total[256];
-  __shared__ int s_digit, s_above;
-  __shared__ int ws[2][KEEP_NW];
+  constexpr int CHUNK = KEEP_NT * PER;
+  __shared__ int hist[2048];
+  __shared__ int s_digit, s_above, s_count;
+  __shared__ int ws[4][KEEP_NW];
   const int h = blockIdx.x, r = blockIdx.y, tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
   const float* m = mass + r * ms + h * mh;
   int* out = kept + ((int64_t)r * Hkv + h) * budget;
@@ -178,101 +178,83 @@ __global__ __launch_bounds__(KEEP_NT) void evict_keep_kernel(const float* __rest
     return;
   }
   const int a = first, b = n - recent, room = budget - first - recent;   // (b - a = n - budget + room > room)
-  const int per = REG ? (n + KEEP_NT - 1) / KEEP_NT : PER;               // keys a thread, up to PER
   uint32_t key[PER];
   auto load = [&](int i0) {
 #pragma unroll
     for (int k = 0; k < PER; ++k) {
-      const int i = i0 + tid * per + k;
-      key[k] = k < per && i >= a && i < b ? rank_of(m[i]) : 0u;
+      const int i = i0 + tid * PER + k;
+      key[k] = i >= a && i < b ? rank_of(m[i]) : 0u;
     }
   };
   if (REG) load(0);
+  // two counters a thread, from the largest digit down
+  const int d0 = 2047 - 2 * tid;
+  hist[d0] = hist[d0 - 1] = 0;
+  __syncthreads();
   uint32_t lead = 0, known = 0;
   int need = room;                                                       // of those with the leading digits of the threshold
-  for (int shift = 24; shift >= 0 && need > 0; shift -= 8) {
-    for (int i = lane; i < 256; i += 64) hist[w][i] = 0;                 // (a wave's own: no barrier)
+  for (int turn = 0; turn < 3 && need > 0; ++turn) {
+    const int shift = 21 - 11 * turn, left = max(0, -shift);             // (the last digit: 10 bits)
+    auto digit = [&](uint32_t x) { return (left ? x << left : x >> shift) & 2047; };
     for (int i0 = 0; i0 < (REG ? 1 : n); i0 += CHUNK) {
       if (!REG) load(i0);
 #pragma unroll
       for (int k = 0; k < PER; ++k) {
-        const int i = i0 + tid * per + k;
-        if (k < per && i >= a && i < b && (key[k] & known) == lead) atomicAdd(&hist[w][(key[k] >> shift) & 255], 1);
+        const int i = i0 + tid * PER + k;
+        if (i >= a && i < b && (key[k] & known) == lead) atomicAdd(&hist[digit(key[k])], 1);
       }
     }
     __syncthreads();
-    if (tid < 256) {
-      int c = 0;
-#pragma unroll
-      for (int i = 0; i < KEEP_NW; ++i) c += hist[i][tid];
-      total[tid] = c;
+    const int c0 = hist[d0], c1 = hist[d0 - 1];
+    hist[d0] = hist[d0 - 1] = 0;                                         // for the next turn
+    int all;
+    const int before = before_thread(c0 + c1, ws[turn & 1], all);
+    if (before < need && before + c0 + c1 >= need) {
+      const bool first_of = before + c0 >= need;
+      s_digit = first_of ? d0 : d0 - 1;
+      s_above = first_of ? before : before + c0;
+      s_count = first_of ? c0 : c1;
     }
     __syncthreads();
-    if (w == 0) {                                                        // four digits a lane, from the largest down
-      const int d0 = 255 - 4 * lane;
-      const int c0 = total[d0], c1 = total[d0 - 1], c2 = total[d0 - 2], c3 = total[d0 - 3];
-      int inc = c0 + c1 + c2 + c3;
-      for (int o = 1; o < 64; o <<= 1) {
-        const int y = __shfl_up(inc, o, 64);
-        if (lane >= o) inc += y;
-      }
-      int before = inc - (c0 + c1 + c2 + c3);
-      if (before < need && inc >= need) {
-        int d = d0;
-        if (before + c0 < need) {
-          before += c0;
-          d = d0 - 1;
-          if (before + c1 < need) {
-            before += c1;
-            d = d0 - 2;
-            if (before + c2 < need) {
-              before += c2;
-              d = d0 - 3;
-            }
-          }
-        }
-        s_digit = d;
-        s_above = before;
-      }
-    }
-    __syncthreads();
-    lead |= (uint32_t)s_digit << shift;
-    known |= 255u << shift;
+    lead |= left ? (uint32_t)s_digit >> left : (uint32_t)s_digit << shift;
+    known |= left ? 2047u >> left : 2047u << shift;
     need -= s_above;
+    if (s_count == need) break;
   }
-  // ``lead`` is the threshold: everything above it stays, and the first ``need`` of its equals (room 0: nothing between the two ends)
+  // ``lead`` is the threshold in its ``known`` bits: all above it stay, and the first ``need`` of its equals (room 0: nothing between the ends)
   int ties = 0, done = 0;                                                // in front of this chunk
   for (int i0 = 0; i0 < n; i0 += CHUNK) {
     if (!REG) load(i0);
     int mine = 0, all;
 #pragma unroll
     for (int k = 0; k < PER; ++k) {
-      const int i = i0 + tid * per + k;
-      mine += k < per && room > 0 && i >= a && i < b && key[k] == lead;
+      const int i = i0 + tid * PER + k;
+      mine += room > 0 && i >= a && i < b && (key[k] & known) == lead;
     }
-    int rank = ties + before_thread(mine, ws[0], all);
+    int rank = ties + before_thread(mine, ws[2], all);
     ties += all;
     uint32_t keep = 0;
     int count = 0;
 #pragma unroll
     for (int k = 0; k < PER; ++k) {
-      const int i = i0 + tid * per + k;
-      if (k >= per || i >= n) continue;
+      const int i = i0 + tid * PER + k;
+      if (i >= n) continue;
       const bool mid = i >= a && i < b;
       bool yes = !mid;
       if (mid && room > 0) {
-        yes = key[k] > lead || (key[k] == lead && rank < need);
-        rank += key[k] == lead;
+        const uint32_t x = key[k] & known;
+        yes = x > lead || (x == lead && rank < need);
+        rank += x == lead;
       }
       keep |= (uint32_t)yes << k;
       count += yes;
     }
-    int at = done + before_thread(count, ws[1], all);
+    int at = done + before_thread(count, ws[3], all);
     done += all;
 #pragma unroll
     for (int k = 0; k < PER; ++k)
       if ((keep >> k) & 1) {
-        if (at < budget) out[at] = i0 + tid * per + k;
+        if (at < budget) out[at] = i0 + tid * PER + k;
         ++at;
       }
   }
@@ -385,10 +367,11 @@ extern "C" hipError_t kafka_kv4_evict_keep(const float* mass, int64_t ms, int64_
                                            int first, int recent, int* kept, hipStream_t st) {
   if (R == 0 || budget == 0) return hipSuccess;
   if (first < 0 || recent < 0 || (int64_t)first + recent > budget || R > 65535) return hipErrorInvalidValue;
-  if (N <= KEEP_NT * KEEP_PER)
-    evict_keep_kernel<true><<<dim3(Hkv, R), KEEP_NT, 0, st>>>(mass, ms, mh, N, lens, budget, first, recent, kept, Hkv);
-  else
-    evict_keep_kernel<false><<<dim3(Hkv, R), KEEP_NT, 0, st>>>(mass, ms, mh, N, lens, budget, first, recent, kept, Hkv);
+  auto go = [&](auto kern) { kern<<<dim3(Hkv, R), KEEP_NT, 0, st>>>(mass, ms, mh, N, lens, budget, first, recent, kept, Hkv); };
+  if (N <= KEEP_NT * 4) go(evict_keep_kernel<4, true>);
+  else if (N <= KEEP_NT * 8) go(evict_keep_kernel<8, true>);
+  else if (N <= KEEP_NT * 16) go(evict_keep_kernel<16, true>);
+  else go(evict_keep_kernel<8, false>);
   return hipGetLastError();
 }
 
