@@ -53,14 +53,13 @@ FEW_ROWS = 16              # rows (tokens x query heads of a group) of a tile fo
 SOME_ROWS = 32             # of a tile for short portions
 MANY_ROWS = {128: 256, 64: 128}   # of a tile for portions whose keys are widened first, by head dim (csrc/kv4_tile.hip)
 MANY_WGS = {128: 256, 64: 768}    # workgroups of these that the CUs hold
-MANY_MIN = 128             # rows of a segment from which on its keys may be widened first,
-MANY_WORK = 1 << 29        # and work (pairs of rows and keys, times heads, times dim) of all such segments from which on they are
-MANY_BLOCKS = 8            # blocks of a piece of a wide tile
+MANY_MIN = 128             # rows of a segment from which on its keys may be widened first (_wide)
+MANY_BLOCKS = 4            # blocks of a piece of a wide tile
 CUS = 256
 LEAST_SHARE = 4            # blocks a CU up to which every four of them are a workgroup, one for each wave
 SHORT_TILE = 16            # blocks of a tile on average below which four waves take it, else eight
-LONG_WGS = 1024            # workgroups of four waves that a longer launch is split towards
-LONG_PIECE = 4
+SOME_WGS, SOME_PIECE = 256, 8     # workgroups that a launch of short portions is split towards, least blocks of a piece
+MANY_COST = 14.            # what two more launches and a workspace cost (_wide)
 MASS_FEW = 16              # rows of a segment up to which a wave takes them all for its block of keys
 MASS_WGS = 1024            # workgroups that a launch of few rows is split towards
 MASS_MANY_WGS = 2048       # ... of portions (twice as many as the CUs hold: parts of rows are unequal; 1900 rows 45 us, with 1024 49, 512 62)
@@ -115,8 +114,34 @@ def _narrow_split(count: np.ndarray, kv_heads: int, rows: int) -> tuple[int, np.
     if rows == FEW_ROWS and share > LEAST_SHARE:
         waves = 4 if int(count.sum()) < SHORT_TILE * len(count) else 8
         return waves, np.maximum(1, count // max(2 * waves if waves == 4 else waves, share))
-    size = max(LONG_PIECE, -(-total // LONG_WGS))
-    return 4, np.maximum(1, (count + size - 1) // size)
+    if rows == FEW_ROWS:
+        return 4, np.maximum(1, (count + 3) // 4)
+    # 90 sizes of 1 to 16 portions of 33 to 512 tokens behind 0 to 8000: 3% off the best split of each on average, in pieces of at least 4
+    # blocks and for 512 workgroups 7%, at most 47% (the last piece's join costs as much as 4 blocks)
+    return 4, np.maximum(1, count // max(SOME_PIECE, -(-total // SOME_WGS)))
+
+
+def _wide(full: np.ndarray, heads: int, kv_heads: int, dim: int, window: int, first: int) -> np.ndarray:
+    """Which segments are taken in wide tiles whose keys are widened first: none or all of MANY_MIN rows or more, by the microseconds that
+    both ways take. Measured (32/8 heads of 128 / 64/8 heads of 128 / 24/8 heads of 64): 512 rows cold 21 against 14 with tiles of 32 rows / 25
+    against 25 / 17 against 10, 300 rows behind 1000 keys 24 against 23 / 31 against 33 / 18 against 14, 8 portions of 200 cold 20 against
+    35 / - / -, three of 1100 behind 900 in a window of 512 75 against 99 / - / 43 against 61."""
+    G = heads // kv_heads
+    wide = full[:, 1] * G >= MANY_MIN
+    part = full[wide]
+    if len(part):
+        def work(rows):
+            t = _tiles(part, rows // G)
+            return len(t) * kv_heads, int(_blocks(t[:, 2], t[:, 1], window, first)[1].sum()) * kv_heads
+
+        wgs, blocks = work(SOME_ROWS)
+        few = 7. * max(1., wgs / 512) + blocks * dim / 128 * 0.9 / 512     # rounds of workgroups, and blocks
+        wgs, blocks = work(MANY_ROWS[dim])
+        keys = int(_blocks(part[:, 2], part[:, 1], window, first)[1].sum()) * BLOCK * kv_heads
+        many = MANY_COST + blocks * dim / 128 * 2.1 / 256 + keys * dim * 5 / 4.5e6
+        if few <= many:
+            wide[:] = False
+    return wide
 
 
 def _wide_split(count: np.ndarray, kv_heads: int, wgs: int) -> np.ndarray:
@@ -130,12 +155,7 @@ def _tables(full: np.ndarray, heads: int, kv_heads: int, dim: int, window: int, 
     keys."""
     G = heads // kv_heads
     rows = full[:, 1] * G
-    seen = full[:, 2] + (full[:, 1] + 1) // 2                              # keys of the segment's middle row
-    if window:
-        seen = np.minimum(seen, window + first)
-    wide = rows >= MANY_MIN
-    if int((full[:, 1] * seen)[wide].sum()) * heads * dim < MANY_WORK:
-        wide[:] = False
+    wide = _wide(full, heads, kv_heads, dim, window, first)
     shapes, arrays = [], []
     for size, part in ((FEW_ROWS, full[(rows <= FEW_ROWS) & ~wide]), (SOME_ROWS, full[(rows > FEW_ROWS) & ~wide]), (MANY_ROWS[dim], full[wide])):
         if not len(part):

@@ -512,18 +512,19 @@ def test_writer_on_the_gpu(cuda, T, Hq, H, D, slab, special):
 def test_attention_on_the_gpu(cuda, monkeypatch, case, wide):
     """Every kind of tile, whatever the sizes from which on a plan takes it."""
     if wide:
-        monkeypatch.setattr(kv4, "MANY_WORK", 0)
+        monkeypatch.setattr(kv4, "MANY_COST", -1e9)
         monkeypatch.setattr(kv4, "LEAST_SHARE", 0)
+        monkeypatch.setattr(kv4, "SOME_PIECE", 2)
         monkeypatch.setattr(kv4, "MASS_TILES", 1)
     else:
-        monkeypatch.setattr(kv4, "MANY_WORK", 1 << 60)
+        monkeypatch.setattr(kv4, "MANY_COST", 1e9)
     _check_attention(case, cuda)
 
 
 @pytest.mark.gpu
 def test_attention_again_is_the_same(cuda, monkeypatch):
     """Bit for bit, whatever ran in between; on another stream; as rows of a wider tensor."""
-    monkeypatch.setattr(kv4, "MANY_WORK", 0)
+    monkeypatch.setattr(kv4, "MANY_COST", -1e9)
     segs = [(0, 1, 3000, 0), (1, 40, 500, 1), (41, 1, 70, 2)]
     kc, vc, tables = world(segs, 2, 128, 0, cuda)
     q = queries(42, 8, 128, 1, cuda)
@@ -734,8 +735,9 @@ def test_engine_on_the_gpu(cuda):
 
 
 @pytest.mark.gpu
-def test_step_plan_is_the_plan(cuda):
+def test_step_plan_is_the_plan(cuda, monkeypatch):
     """An engine step's tables, as uploaded, give what attn_plan's give."""
+    monkeypatch.setattr(kv4, "MANY_COST", -1e9)
     segs = [(0, 1, 500, 0), (1, 1, 33, 1), (2, 177, 900, 2), (179, 3, 4000, 3), (182, 10, 70, 4)]
     flat = kv4.step_tables(segs, 32, 2, 128)
     p = kv4.step_plan(flat, torch.from_numpy(flat).to(cuda), 32, 2, 128)
@@ -755,7 +757,7 @@ def test_widened_keys_are_those_that_a_tile_sees(monkeypatch):
 
     g = torch.Generator().manual_seed(1)
     r = lambda hi: int(torch.randint(0, hi, (1,), generator=g))
-    monkeypatch.setattr(kv4, "MANY_WORK", 0)
+    monkeypatch.setattr(kv4, "MANY_COST", -1e9)
     for _ in range(100):
         segs = np.array([(1000 * i, 33 + r(400), r(6000), 10 + i) for i in range(1 + r(4))])
         window, first = (0, 0) if r(3) == 0 else (1 + r(1500), r(300))
