@@ -31,7 +31,7 @@ __device__ __forceinline__ bf16x8 numbers(bf16x8 x) {
 template <int D>
 __global__ __launch_bounds__(256) void rope_write_kernel(const bf16* __restrict__ qkv, const float* __restrict__ qp, int S, int64_t ps,
                                                          int64_t qkv_stride, const int64_t* __restrict__ positions,
-                                                         const float* __restrict__ cos_sin, bf16* __restrict__ q_out, int64_t q_stride,
+                                                         const float* __restrict__ cos_sin, int64_t n_pos, bf16* __restrict__ q_out, int64_t q_stride,
                                                          uint8_t* __restrict__ kc, uint8_t* __restrict__ vc,
                                                          const int64_t* __restrict__ slots, int64_t n_slots, int64_t total, int Hq, int Hkv) {
   constexpr int HALF = D / 2, RU = HALF / 8, VU = D / 8;
@@ -40,7 +40,9 @@ __global__ __launch_bounds__(256) void rope_write_kernel(const bf16* __restrict_
   if (i >= total) return;
   const int t = (int)(i / n_row), u = (int)(i - (int64_t)t * n_row);
   int64_t slot = slots ? slots[t] : -1;
-  if (slot >= n_slots) slot = -1;
+  const int64_t pos = positions[t];
+  const bool turns = pos >= 0 && pos < n_pos;                      // (a row of a position without angles: no numbers, and not into the cache)
+  if (slot >= n_slots || !turns) slot = -1;
   const int64_t row = (int64_t)t * qkv_stride;
   const int64_t page = slot >> 4;
   const int o = (int)(slot & 15);
@@ -49,7 +51,7 @@ __global__ __launch_bounds__(256) void rope_write_kernel(const bf16* __restrict_
     float x1[8], x2[8];
     load_in8(x1, qkv, qp, S, ps, row + head * D + c);
     load_in8(x2, qkv, qp, S, ps, row + head * D + HALF + c);
-    const float* cs = cos_sin + positions[t] * D + c;
+    const float* cs = cos_sin + (turns ? pos : 0) * D + c;
     bf16x8 y1, y2;
     {
 #pragma clang fp contract(off)
@@ -62,6 +64,10 @@ __global__ __launch_bounds__(256) void rope_write_kernel(const bf16* __restrict_
       }
     }
     if (head < Hq) {
+      if (!turns) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) y1[j] = y2[j] = (bf16)__builtin_nanf("");
+      }
       bf16* dst = q_out + t * q_stride + head * D + c;
       store_bf16x8(dst, y1);
       store_bf16x8(dst + HALF, y2);
@@ -338,13 +344,13 @@ __global__ __launch_bounds__(256) void evict_copy_kernel(uint8_t* __restrict__ k
 using namespace kv4;
 
 extern "C" hipError_t kafka_kv4_rope_write(const bf16* qkv, const float* qp, int S, int64_t ps, int64_t qkv_stride, const int64_t* positions,
-                                           const float* cos_sin, bf16* q_out, int64_t q_stride, uint8_t* kc, uint8_t* vc,
+                                           const float* cos_sin, int64_t n_pos, bf16* q_out, int64_t q_stride, uint8_t* kc, uint8_t* vc,
                                            const int64_t* slots, int64_t n_slots, int T, int Hq, int Hkv, int D, hipStream_t st) {
   if (T == 0) return hipSuccess;
   const int64_t total = (int64_t)T * ((Hq + Hkv) * (D / 16) + Hkv * (D / 8));
-  if ((D != 64 && D != 128) || total > 0xffffff00ll) return hipErrorInvalidValue;
+  if (n_pos < 1 || (D != 64 && D != 128) || total > 0xffffff00ll) return hipErrorInvalidValue;
   auto go = [&](auto kern) {
-    kern<<<(unsigned)((total + 255) / 256), 256, 0, st>>>(qkv, qp, S, ps, qkv_stride, positions, cos_sin, q_out, q_stride, kc, vc, slots,
+    kern<<<(unsigned)((total + 255) / 256), 256, 0, st>>>(qkv, qp, S, ps, qkv_stride, positions, cos_sin, n_pos, q_out, q_stride, kc, vc, slots,
                                                           n_slots, total, Hq, Hkv);
     return hipGetLastError();
   };

@@ -77,13 +77,18 @@ struct VFrag {
   uint32_t s[NP];
 };
 
-// Page ids of 16 blocks of 4 pages, a lane each (keys behind ``last`` take its page: they are masked). One load for them all, ahead of
-// their use: an id that is fetched in front of its page's loads adds a round trip to every block.
+// Page ids of 16 blocks of 4 pages, a lane each; of pages that no row at pmin .. pmax sees a key of, page 0 (the table may name anything
+// there: pages that a window has left behind are their owner's again). One load for them all, ahead of their use: an id that is fetched in
+// front of its page's loads adds a round trip to every block.
 struct PageIds {
   int v = 0;
   __device__ __forceinline__ PageIds() {}
   template <class Of>
-  __device__ __forceinline__ PageIds(const int* bt, int last, int lane, Of block) : v(bt[min(block(lane >> 2) * 4 + (lane & 3), last >> 4)]) {}
+  __device__ __forceinline__ PageIds(const int* bt, int pmin, int pmax, int window, int first, int lane, Of block) {
+    const int i = block(lane >> 2) * 4 + (lane & 3), key = 16 * i;
+    v = bt[min(i, pmax >> 4)];
+    if (key > pmax || (key + 15 <= pmin - window && key >= first)) v = 0;
+  }
   // NP of them from lane ``at`` on. An id that is not of the cache counts as page 0 and sets ``bad``: such rows come out as no numbers.
   template <int NP>
   __device__ __forceinline__ void get(int at, int64_t n_pages, int (&pg)[NP], bool& bad) const {
@@ -228,16 +233,18 @@ __device__ __forceinline__ void keys_step(const KFrag<NP>& kf, VFrag<NP>& vf, Ro
 #pragma unroll
         for (int i = 0; i < 4; ++i)
           if (!sees(key0 + 16 * t + 4 * c + i, r.lim[n], window, first)) s[t][n][i] = -INFINITY;
-    // behind the last position the page may hold anything, also scales that are no numbers: their weight is zero, so must they be
-    if (key0 + 16 * NP - 1 > pmax) {
+    // where no row sees a key the page may hold anything, also scales that are no numbers: their weight is zero, so must they be
+    if (key0 + 16 * NP - 1 > pmax || (key0 <= pmin - window && key0 + 16 * NP > first)) {
 #pragma unroll
       for (int t = 0; t < NP; ++t)
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-          if (key0 + 16 * t + 4 * c + i > pmax) {
+        for (int i = 0; i < 4; ++i) {
+          const int key = key0 + 16 * t + 4 * c + i;
+          if (key > pmax || (key <= pmin - window && key >= first)) {
             vf.d[t][i] = 0u;
             vf.s[t] &= ~(255u << (8 * i));
           }
+        }
     }
   }
 #pragma unroll
@@ -343,7 +350,7 @@ __global__ __launch_bounds__(64 * NW, NQ == 1 ? 3 : 2) void attn_kernel(Args a) 
   bool bad = false;
   const int v0 = it.lo + w, n = (hi - v0 + NW - 1) / NW * 2;    // halves of this wave's blocks: v0, v0 + NW, ..
   if (hi > v0) {
-    auto ids = [&](int k) { return PageIds(bt, pmax, lane, [&](int i) { return list[min(v0 + NW * (k / 2 + i), hi - 1)]; }); };
+    auto ids = [&](int k) { return PageIds(bt, pmin, pmax, a.window, a.first, lane, [&](int i) { return list[min(v0 + NW * (k / 2 + i), hi - 1)]; }); };
     PageIds id = ids(0), idn = ids(32);
     KFrag<2> kf[NB];
     VFrag<2> vf[NB];
@@ -567,7 +574,7 @@ __global__ __launch_bounds__(256) void mass_few_kernel(MassArgs ma) {
     }
     return;
   }
-  const PageIds id(a.tables + table * a.ts, last, lane, [&](int i) { return b0 + 4 * min(i, 7); });
+  const PageIds id(a.tables + table * a.ts, pos, last, a.window, a.first, lane, [&](int i) { return b0 + 4 * min(i, 7); });
   bool bad[NB];
   KFrag<4> kf[NB];
   float had[NB];
@@ -672,7 +679,7 @@ __global__ __launch_bounds__(256, 4) void mass_many_kernel(MassArgs ma) {
     {
       int pg[4];
       uint32_t kw[4][D / 32], ks[4][D / 32];
-      PageIds(a.tables + table * a.ts, last, lane, [&](int) { return it[5] + w; }).get<4>(0, a.n_pages, pg, bad);
+      PageIds(a.tables + table * a.ts, pos, last, a.window, a.first, lane, [&](int) { return it[5] + w; }).get<4>(0, a.n_pages, pg, bad);
 #pragma unroll
       for (int t = 0; t < 4; ++t) {
         const uint8_t* p = a.kc + ((int64_t)pg[t] * a.Hkv + h) * Page<D>::BYTES;

@@ -7,7 +7,7 @@
 
 extern "C" {
 hipError_t kafka_kv4_rope_write(const void* qkv, const float* qp, int S, int64_t ps, int64_t qkv_stride, const int64_t* positions,
-                                const float* cos_sin, void* q_out, int64_t q_stride, uint8_t* kc, uint8_t* vc, const int64_t* slots,
+                                const float* cos_sin, int64_t n_pos, void* q_out, int64_t q_stride, uint8_t* kc, uint8_t* vc, const int64_t* slots,
                                 int64_t n_slots, int T, int Hq, int Hkv, int D, hipStream_t st);
 hipError_t kafka_kv4_read(const uint8_t* kc, const uint8_t* vc, const int64_t* slots, int64_t n_slots, int64_t T, int Hkv, int D, void* k,
                           void* v, hipStream_t st);
@@ -50,7 +50,7 @@ void on(const Tensor& t, const Tensor& home, at::ScalarType type, const char* na
 // head dim of a K / V page pool
 int cache(const Tensor& c, const char* name) {
   TORCH_CHECK_VALUE(c.is_cuda() && c.scalar_type() == at::kByte && c.dim() == 4 && c.size(2) == 16 && c.is_contiguous() && aligned(c) &&
-                        (c.size(3) == 68 || c.size(3) == 34) && c.size(1) > 0 && c.size(1) < 1 << 12 && c.size(0) < 1ll << 27,
+                        (c.size(3) == 68 || c.size(3) == 34) && c.size(1) > 0 && c.size(1) < 1 << 12 && c.size(0) > 0 && c.size(0) < 1ll << 27,
                     name, ": a cache of kv_cache_shapes(..., \"mx4\") with head dim 64 or 128 expected");
   return c.size(3) == 68 ? 128 : 64;
 }
@@ -85,7 +85,8 @@ void rope_write(Tensor qkv, Tensor positions, Tensor cos_sin, Tensor q_out, Tens
               "rope_kv_write: qkv bf16 [T, (Hq + 2 Hkv) D] or contiguous fp32 slabs of it");
   on(positions, kc, at::kLong, "positions");
   on(cos_sin, kc, at::kFloat, "cos_sin");
-  TORCH_CHECK_VALUE(positions.is_contiguous() && positions.numel() == T && cos_sin.is_contiguous() && cos_sin.dim() == 2 && cos_sin.size(1) == D,
+  TORCH_CHECK_VALUE(positions.is_contiguous() && positions.numel() == T && cos_sin.is_contiguous() && cos_sin.dim() == 2 && cos_sin.size(1) == D &&
+                  (T == 0 || cos_sin.size(0) > 0),
               "rope_kv_write: positions [T], cos_sin [positions, D]");
   rows3(q_out, kc, T, Hq, D, "q_out");
   const int64_t* sp = nullptr;
@@ -95,7 +96,7 @@ void rope_write(Tensor qkv, Tensor positions, Tensor cos_sin, Tensor q_out, Tens
     sp = slots->data_ptr<int64_t>();
   }
   KV4_HIP(kafka_kv4_rope_write(slab ? nullptr : qkv.data_ptr(), slab ? qkv.data_ptr<float>() : nullptr, slab ? (int)qkv.size(0) : 0,
-                               slab ? T * W : 0, slab ? W : qkv.stride(0), positions.data_ptr<int64_t>(), cos_sin.data_ptr<float>(),
+                               slab ? T * W : 0, slab ? W : qkv.stride(0), positions.data_ptr<int64_t>(), cos_sin.data_ptr<float>(), cos_sin.size(0),
                                q_out.data_ptr(), q_out.stride(0), kc.data_ptr<uint8_t>(), vc.data_ptr<uint8_t>(), sp, kc.size(0) * 16,
                                (int)T, (int)Hq, (int)Hkv, D, stream()));
 }
@@ -163,7 +164,8 @@ struct Plan {
 };
 
 // q and the block tables of a call against its plan
-const int* call(const Plan& p, const Tensor& q, const Tensor& kc, int D, const Tensor& tables) {
+const int* call(const Plan& p, const Tensor& q, const Tensor& kc, int D, const Tensor& tables, double scale) {
+  TORCH_CHECK_VALUE(scale >= 1e-30 && scale <= 1e30, "kv4: a positive scale expected");   // (masked scores are -infinity times it)
   TORCH_CHECK_VALUE(q.dim() == 3 && q.size(1) == p.heads && D == p.dim && kc.size(1) == p.kv_heads,
                     "kv4: q bf16 [T, heads, dim] and a cache of the plan's heads expected");
   rows3(q, kc, q.size(0), p.heads, D, "q");
@@ -183,7 +185,7 @@ float* row_values(const OptT& t, const Tensor& q, const Tensor& home) {
 Tensor attn(Tensor q, Tensor kc, Tensor vc, Tensor tables, const Plan& p, double scale, OptT out_, OptT lse) {
   const int D = caches(kc, vc);
   const c10::DeviceGuard guard(kc.device());
-  const int* tp = call(p, q, kc, D, tables);
+  const int* tp = call(p, q, kc, D, tables, scale);
   const int64_t T = q.size(0), Hq = p.heads, H = p.kv_heads;
   Tensor out;
   if (out_.has_value()) {
@@ -229,7 +231,7 @@ void masses(const Tensor& m, const Tensor& home, int64_t R, int64_t H, const cha
 Tensor attn_mass(Tensor q, Tensor lse, Tensor kc, Tensor tables, const Plan& p, double scale, OptT base, OptT out_) {
   const int D = cache(kc, "k_cache");
   const c10::DeviceGuard guard(kc.device());
-  const int* tp = call(p, q, kc, D, tables);
+  const int* tp = call(p, q, kc, D, tables, scale);
   TORCH_CHECK_VALUE(p.few.has_value() && p.few->device() == kc.device(), "attn_mass: a plan of attn_plan for this device expected");
   TORCH_CHECK_VALUE(p.rows < 2 || q.stride(0) < 1 << 23, "attn_mass: q's rows less than 2^23 elements apart");
   const float* lp = row_values(lse, q, kc);

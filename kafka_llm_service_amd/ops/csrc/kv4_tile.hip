@@ -18,12 +18,13 @@ struct Image {                            // of 64 keys and one head
 
 // ---- widening -----------------------------------------------------------------------------------------------------------
 // A workgroup per tile and head, a wave per page. K: [page][d / 8][key][8], V: [page][d][16 keys: 0-3, 8-11, 4-7, 12-15], the two halves of
-// rows with d & 8 exchanged (attn_tile.h: reads of both without bank conflicts). Keys behind ``last`` become zeros, those of a page that
-// is none no numbers. Tiles: table row, block, last key, 0.
+// rows with d & 8 exchanged (attn_tile.h: reads of both without bank conflicts). Keys behind ``last`` become zeros, and whole pages of which
+// no row from ``pmin`` on sees a key (the table may name anything there); those of a page that is none no numbers. Tiles: table row,
+// block, last key, pmin.
 template <int D>
 __global__ __launch_bounds__(256) void widen_kernel(const uint8_t* __restrict__ kc, const uint8_t* __restrict__ vc, int64_t n_pages,
                                                     const int* __restrict__ tables, int64_t ts, const int* __restrict__ tiles, int Hkv,
-                                                    char* __restrict__ ws) {
+                                                    int window, int first, char* __restrict__ ws) {
   constexpr int KW = D / 32;               // words of K a lane: its quarter of a key
   const int t = blockIdx.x / Hkv, h = blockIdx.x % Hkv;
   const int* tl = tiles + 4 * (int64_t)t;
@@ -32,7 +33,7 @@ __global__ __launch_bounds__(256) void widen_kernel(const uint8_t* __restrict__ 
   char* kd = ws + ((int64_t)t * Hkv + h) * Image<D>::BYTES + w * Image<D>::PAGE_BYTES;
   char* vd = kd + Image<D>::KBYTES;
   const int o = lane & 15, c = lane >> 4;
-  const bool some = key0 <= last;
+  const bool some = key0 <= last && (key0 + PAGE - 1 > tl[3] - window || key0 < first);
   const int pid = some ? tables[tl[0] * ts + (key0 >> 4)] : 0;
   const bool bad = pid < 0 || pid >= n_pages;
   const int64_t at = ((int64_t)(bad ? 0 : pid) * Hkv + h) * Page<D>::BYTES;
@@ -366,10 +367,10 @@ extern "C" hipError_t kafka_kv4_tiles(const bf16* q, int64_t qs, const uint8_t* 
   const TileArgs a{q,  qs, ws, reinterpret_cast<const TileItem4*>(items), T, Hkv, G, window > 0 ? window : 1 << 30, first,
                    scale * 1.4426950408889634f, out, os, lse, part, plse};
   if (D == 128) {
-    widen_kernel<128><<<(unsigned)wws, 256, 0, st>>>(kc, vc, n_pages, tables, ts, wtiles, Hkv, ws);
+    widen_kernel<128><<<(unsigned)wws, 256, 0, st>>>(kc, vc, n_pages, tables, ts, wtiles, Hkv, a.window, first, ws);
     tile_kernel<128, 8, 3><<<(unsigned)wgs, 512, 0, st>>>(a);
   } else {
-    widen_kernel<64><<<(unsigned)wws, 256, 0, st>>>(kc, vc, n_pages, tables, ts, wtiles, Hkv, ws);
+    widen_kernel<64><<<(unsigned)wws, 256, 0, st>>>(kc, vc, n_pages, tables, ts, wtiles, Hkv, a.window, first, ws);
     tile_kernel<64, 4, 3><<<(unsigned)wgs, 256, 0, st>>>(a);
   }
   if (n_merges) return kafka_kv4_merge(merges, n_merges, rows, T, Hkv, G, D, out, os, lse, part, plse, st);

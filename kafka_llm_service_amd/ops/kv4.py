@@ -1,5 +1,5 @@
 """Operators of the 4-bit KV cache (``kv_cache_shapes(..., "mx4")``): elements e2m1, one power of two for every 32 elements of a key's or
-value's head vector, 4.25 bits each in all; a sixteenth of the bf16 cache's head dims of 64 and 128, pages of 16 keys (csrc/kv4.h).
+value's head vector, 4.25 bits each in all, a little over a quarter of the bf16 cache; head dims 64 and 128, pages of 16 keys (csrc/kv4.h).
 
   ops.rope_kv_write   writes a step's rows (a cache of this kind given)            csrc/kv4.hip
   read                keys and values of slots as numbers                          csrc/kv4.hip
@@ -11,7 +11,8 @@ value's head vector, 4.25 bits each in all; a sixteenth of the bf16 cache's head
 Rows of a call are described by segments (first row, rows, position of the first, row of the block table): consecutive tokens of
 one sequence, whose keys lie in the cache at their positions. GPU tensors run the HIP kernels on the caches' device and its current
 stream, CPU tensors the references of ``kv4_reference.py``. Workspaces are made per call, so calls on several streams and captured
-graphs do not meet; a plan holds only tables that the kernels read.
+graphs do not meet. A plan holds the tables that the kernels read and, for each stream that it is used on, counters that every
+call leaves at zero (a captured call has its own, in its graph); like a call's tensors it has to live until the stream is done with it.
 """
 from __future__ import annotations
 
@@ -33,7 +34,7 @@ def _gpu(t: torch.Tensor) -> bool:
 
 def _check_cache(k_cache, v_cache, who: str) -> None:
     for c in (k_cache, v_cache):
-        if c.dtype != torch.uint8 or c.dim() != 4 or c.shape[2] != PAGE or c.shape[3] not in (34, 68) or c.shape != k_cache.shape:
+        if c.dtype != torch.uint8 or c.dim() != 4 or c.shape[0] == 0 or c.shape[2] != PAGE or c.shape[3] not in (34, 68) or c.shape != k_cache.shape:
             raise ValueError(f"{who}: caches of kv_cache_shapes(..., \"mx4\") with head dim 64 or 128 expected")
 
 
@@ -171,7 +172,7 @@ def _tables(full: np.ndarray, heads: int, kv_heads: int, dim: int, window: int, 
             base = np.cumsum(count) - count
             s = np.repeat(np.arange(len(part)), count)
             i = np.arange(len(s)) - base[s]
-            keys = np.stack([part[s, 3], np.where(i < head[s], i, i - head[s] + tail[s]), (part[:, 2] + part[:, 1] - 1)[s], np.zeros_like(s)], 1)
+            keys = np.stack([part[s, 3], np.where(i < head[s], i, i - head[s] + tail[s]), (part[:, 2] + part[:, 1] - 1)[s], part[s, 2]], 1)
             s = t[:, 4]
             cols = [t[:, 0], t[:, 1], t[:, 2], base[s], head[s], tail[s], pieces[:, 1], pieces[:, 2],
                     np.where(pieces[:, 3] < 0, -1, pieces[:, 3] + pieces[:, 4])]
@@ -301,7 +302,9 @@ def step_plan(host: np.ndarray, device: torch.Tensor, heads: int, kv_heads: int,
     return p
 
 
-def _check_call(q, k_cache, block_tables, plan: AttnPlan, who: str) -> None:
+def _check_call(q, k_cache, block_tables, plan: AttnPlan, scale: float, who: str) -> None:
+    if not 1e-30 <= scale <= 1e30:
+        raise ValueError(f"{who}: a positive scale expected")
     if q.dim() != 3 or q.dtype != torch.bfloat16 or q.shape[1] != plan.heads or q.shape[2] != plan.dim or \
             k_cache.shape[1] != plan.kv_heads or ref.head_dim(k_cache) != plan.dim:
         raise ValueError(f"{who}: q bf16 [T, heads, dim] and a cache of the plan's heads expected")
@@ -315,13 +318,15 @@ def _check_call(q, k_cache, block_tables, plan: AttnPlan, who: str) -> None:
 def attn(q, k_cache, v_cache, block_tables, plan: AttnPlan, scale: float, out=None, lse=None) -> torch.Tensor:
     """softmax(scale q k^T) v of the plan's rows: q [T, heads, dim] bf16 -> out (a new tensor unless given), the same shape.
     ``lse`` fp32 [T, heads] gets the base-2 logarithm of each row's sum of 2^(scores in base 2). Rows of no segment are left as they
-    were (zeros in a new ``out``). Rows whose block table names a page outside of the cache come out as no numbers."""
+    were (zeros in a new ``out``). Of a page that no row of the segment sees a key of (behind the last one, or between the first ones
+    and the window) the table may name anything; where it names none of the cache's for one that is seen, the rows that see it come out
+    as no numbers, and rows of the segment next to them may."""
     if _gpu(q):
         if plan.native is None:
             raise ValueError("kv4.attn: the plan was made for another device")
         return ext().kv4_attn(q, k_cache, v_cache, block_tables, plan.native, scale, out, lse)
     _check_cache(k_cache, v_cache, "kv4.attn")
-    _check_call(q, k_cache, block_tables, plan, "kv4.attn")
+    _check_call(q, k_cache, block_tables, plan, scale, "kv4.attn")
     if out is None:
         out = torch.zeros(q.shape, dtype=q.dtype)
     elif out.shape != q.shape or out.dtype != q.dtype:
@@ -342,7 +347,7 @@ def attn_mass(q, lse, k_cache, block_tables, plan: AttnPlan, scale: float, base=
             raise ValueError("kv4.attn_mass: the plan was made for another device")
         return ext().kv4_mass(q, lse, k_cache, block_tables, plan.native, scale, base, out)
     _check_cache(k_cache, k_cache, "kv4.attn_mass")
-    _check_call(q, k_cache, block_tables, plan, "kv4.attn_mass")
+    _check_call(q, k_cache, block_tables, plan, scale, "kv4.attn_mass")
     if lse.shape != q.shape[:2] or lse.dtype != torch.float32:
         raise ValueError("kv4.attn_mass: lse fp32 [T, heads] expected")
     like = base if base is not None else out

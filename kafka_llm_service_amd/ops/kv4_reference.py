@@ -92,14 +92,20 @@ def read(k_cache, v_cache, slots):
     return tuple(out)
 
 
-def gather(k_cache, v_cache, table, n: int):
-    """fp32 K, V [n, heads, D] of a sequence's first n keys (no numbers where the table names a page outside of the cache)."""
+def gather(k_cache, v_cache, table, n: int, seen=None):
+    """fp32 K, V [n, heads, D] of a sequence's first n keys (no numbers where the table names a page outside of the cache); of pages
+    without a key that is ``seen``, bool [n], anything."""
     ids = table[:(n + PAGE - 1) // PAGE].long()
+    if seen is not None:
+        pages = torch.nn.functional.pad(seen, (0, -n % PAGE)).view(-1, PAGE).any(1)
+        ids = torch.where(pages, ids, torch.zeros_like(ids))
     there = (ids >= 0) & (ids < k_cache.shape[0])
     out = []
     for c, value in ((k_cache, False), (v_cache, True)):
         x = values(*unpack(c[torch.where(there, ids, torch.zeros_like(ids))], value))
         x[~there] = math.nan
+        if seen is not None:
+            x[~pages] = 0.0
         out.append(x.transpose(1, 2).flatten(0, 1)[:n])
     return tuple(out)
 
@@ -109,6 +115,12 @@ def visible(pos: torch.Tensor, n: int, window: int, first: int) -> torch.Tensor:
     j, p = torch.arange(n, device=pos.device), pos[:, None]
     see = j <= p
     return see & ((j > p - window) | (j < first)) if window else see
+
+
+def _seen(seg, window, first, device):
+    """bool [keys]: those that a row of the segment sees."""
+    _, rows, p0, _ = seg
+    return visible(p0 + torch.arange(rows, device=device), p0 + rows, window, first).any(0)
 
 
 def _scores(q, k, seg, window, first, scale):
@@ -125,7 +137,7 @@ def attn(q, k_cache, v_cache, tables, segs, window, first, scale, out, lse):
         t0, rows, p0, tr = seg
         if not rows:
             continue
-        k, v = gather(k_cache, v_cache, tables[tr], p0 + rows)
+        k, v = gather(k_cache, v_cache, tables[tr], p0 + rows, _seen(seg, window, first, q.device))
         s = _scores(q, k, seg, window, first, scale)
         ls = torch.logsumexp(s, -1)
         o = torch.matmul(torch.exp(s - ls[..., None]), v.transpose(0, 1)[:, None])
@@ -140,7 +152,7 @@ def attn_mass(q, lse, k_cache, tables, segs, window, first, scale, out):
         t0, rows, p0, tr = seg
         if not rows:
             continue
-        k, _ = gather(k_cache, k_cache, tables[tr], p0 + rows)
+        k, _ = gather(k_cache, k_cache, tables[tr], p0 + rows, _seen(seg, window, first, q.device))
         s = _scores(q, k, seg, window, first, scale)
         ls = (lse[t0:t0 + rows] / math.log2(math.e)).unflatten(1, (k.shape[1], -1)).permute(1, 2, 0)[..., None]
         w = torch.where(torch.isinf(ls) & (ls < 0), torch.zeros_like(s), torch.exp(s - ls))

@@ -387,6 +387,13 @@ def test_refusals():
                  (q, kc, vc, bt[:1]), (q, kc, vc, bt[:, :1]), (q, kc, vc, bt.long())):
         with pytest.raises(ValueError):
             kv4.attn(*args, p, 0.1)
+    for scale in (0.0, -0.1, math.inf, math.nan):
+        with pytest.raises(ValueError):
+            kv4.attn(q, kc, vc, bt, p, scale)
+        with pytest.raises(ValueError):
+            kv4.attn_mass(q, lse, kc, bt, p, scale)
+    with pytest.raises(ValueError):
+        kv4.attn(q, kc[:0], vc[:0], bt, p, 0.1)
     for kw in (dict(out=torch.zeros(2, 8, 64)), dict(lse=torch.zeros(2, 7)), dict(lse=lse.double())):
         with pytest.raises(ValueError):
             kv4.attn(q, kc, vc, bt, p, 0.1, **kw)
@@ -431,6 +438,44 @@ def _bad_pages(device):
 
 def test_bad_pages_reference():
     _bad_pages("cpu")
+
+
+def _pages_left_behind(device, D, segs):
+    """Pages that the window has passed, and the first keys do not reach, may be anything: no page, or one that nobody ever wrote."""
+    window, first = 100, 20
+    kc, vc, tables = world(segs, 2, D, 3, device, spare=3)
+    T = max(s[0] + s[1] for s in segs)
+    q = queries(T, 8, D, 1, device)
+    plan = kv4.attn_plan(segs, 8, 2, D, window, first, device=device)
+    lse, again = torch.zeros(T, 8, device=device), torch.zeros(T, 8, device=device)
+    out = kv4.attn(q, kc, vc, tables, plan, 0.1, lse=lse)
+    mass = kv4.attn_mass(q, lse, kc, tables, plan, 0.1)
+    assert not out.isnan().any()
+    used = set(tables.flatten().tolist())
+    free = [p for p in range(kc.shape[0]) if p not in used][0]
+    if 0 in used:                                            # page 0 too is one that nobody wrote
+        tables[tables == 0] = free
+        kc[free], vc[free] = kc[0], vc[0]
+        free = 0
+    kc[free], vc[free] = 255, 255
+    for what in (-1, kc.shape[0], free):
+        left = tables.clone()
+        for _, rows, p0, tr in segs:
+            for page in range(left.shape[1]):
+                if page * 16 >= first and (page * 16 + 15 <= p0 - window or page * 16 >= p0 + rows):
+                    left[tr, page] = what
+        assert (left != tables).sum() > 10
+        assert torch.equal(kv4.attn(q, kc, vc, left, plan, 0.1, lse=again), out) and torch.equal(lse, again)
+        assert torch.equal(kv4.attn_mass(q, lse, kc, left, plan, 0.1), mass)
+
+
+LEFT = [[(0, 1, 300, 0), (1, 1, 555, 1), (2, 1, 37, 2)], [(0, 9, 411, 0), (9, 1, 800, 1)], [(0, 300, 333, 0), (300, 140, 900, 1)]]
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("segs", LEFT, ids=["tokens", "short", "long"])
+def test_pages_left_behind_reference(D, segs):
+    _pages_left_behind("cpu", D, segs)
 
 
 def test_plan_covers_every_block_once():
@@ -626,6 +671,34 @@ def test_bad_pages_on_the_gpu(cuda):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("wide", [False, True])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("segs", LEFT, ids=["tokens", "short", "long"])
+def test_pages_left_behind_on_the_gpu(cuda, monkeypatch, D, segs, wide):
+    monkeypatch.setattr(kv4, "MANY_COST", -1e9 if wide else 1e9)
+    _pages_left_behind(cuda, D, segs)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("D", [64, 128])
+def test_rows_without_angles(cuda, D):
+    """A position that cos_sin does not have: the row's queries are no numbers, the cache stays as it is."""
+    n = 7
+    qkv = torch.randn(n, 4 * D + 4 * D, device=cuda).bfloat16()
+    pos = torch.tensor([0, 5, -1, 6, 2 ** 40, 1, -2 ** 50], device=cuda)
+    cs = torch.rand(6, D, device=cuda)
+    slots = torch.arange(3, 3 + n, device=cuda)
+    q = torch.zeros(n, 4, D, dtype=torch.bfloat16, device=cuda)
+    kc, vc = (torch.full((1, 2, 16, D // 2 + D // 32), 255, dtype=torch.uint8, device=cuda) for _ in range(2))
+    want = [t.clone() for t in (q, kc, vc)]
+    ok = (pos >= 0) & (pos < 6)
+    ops.rope_kv_write(qkv, pos, cs, q, kc, vc, slots, 4, 2)
+    ops.rope_kv_write(qkv[ok], pos[ok], cs, (some := want[0][ok].clone()), *want[1:], slots[ok], 4, 2)
+    assert torch.equal(q[ok], some) and q[~ok].isnan().all()
+    assert torch.equal(kc, want[1]) and torch.equal(vc, want[2])
+
+
+@pytest.mark.gpu
 def test_pages_far_behind(cuda):
     """Pages whose bytes lie beyond 4 GiB."""
     H, D = 8, 128
@@ -668,9 +741,14 @@ def test_refusals_on_the_gpu(cuda):
     with pytest.raises(ValueError):
         kv4.attn(q, kc, vc, bt, kv4.attn_plan([(0, 2, 30, 1)], 8, 2, 128, device="cpu"), 0.1)
     odd = torch.zeros(2 * 8 * 128 + 4, dtype=torch.bfloat16, device=cuda)[4:].view(2, 8, 128)
-    for args in ((odd, kc, vc, bt), (q, kc, vc, bt.cpu()), (q, kc, vc.cpu(), bt)):
+    for args in ((odd, kc, vc, bt), (q, kc, vc, bt.cpu()), (q, kc, vc.cpu(), bt), (q, kc[:0], vc[:0], bt)):
         with pytest.raises(ValueError):
             kv4.attn(*args, plan, 0.1)
+    for scale in (0.0, -0.1, math.inf, math.nan):
+        with pytest.raises(ValueError):
+            kv4.attn(q, kc, vc, bt, plan, scale)
+        with pytest.raises(ValueError):
+            kv4.attn_mass(q, torch.zeros(2, 8, device=cuda), kc, bt, plan, scale)
     with pytest.raises(ValueError):
         kv4.read(kc, vc, torch.zeros(3, dtype=torch.int64))
     with pytest.raises(ValueError):
