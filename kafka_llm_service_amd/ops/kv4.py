@@ -55,16 +55,16 @@ SOME_ROWS = 32             # of a tile for short portions
 MANY_ROWS = {128: 256, 64: 128}   # of a tile for portions whose keys are widened first, by head dim (csrc/kv4_tile.hip)
 MANY_WGS = {128: 256, 64: 768}    # workgroups of these that the CUs hold
 MANY_MIN = 128             # rows of a segment from which on its keys may be widened first (_wide)
-MANY_BLOCKS = 4            # blocks of a piece of a wide tile
+MANY_BLOCKS = 4            # least blocks of a piece of a wide tile (300 rows behind 1000 keys 25 us; of 8 blocks 30, of 16 40)
 CUS = 256
-LEAST_SHARE = 4            # blocks a CU up to which every four of them are a workgroup, one for each wave
-SHORT_TILE = 16            # blocks of a tile on average below which four waves take it, else eight
+LEAST_SHARE = 2            # blocks a CU up to which every four of them are a workgroup, one for each wave
+SHORT_TILE = 48            # blocks of a tile on average below which four waves take it, where there is more than a tile a CU (_narrow_split)
 SOME_WGS, SOME_PIECE = 256, 8     # workgroups that a launch of short portions is split towards, least blocks of a piece
 MANY_COST = 14.            # what two more launches and a workspace cost (_wide)
 MASS_FEW = 16              # rows of a segment up to which a wave takes them all for its block of keys
-MASS_WGS = 1024            # workgroups that a launch of few rows is split towards
+MASS_WGS = 1024            # workgroups that a launch of few rows is split towards (64 threads of 2000 23.5 us, 256 28, 4096 37)
 MASS_MANY_WGS = 2048       # ... of portions (twice as many as the CUs hold: parts of rows are unequal; 1900 rows 45 us, with 1024 49, 512 62)
-MASS_TILES = 16            # tiles of 16 rows of a part: four for each of its waves
+MASS_TILES = 8             # least tiles of 16 rows of a part (200 rows behind 1000 keys 12.2 us, of 16 tiles 16.9; 1900 rows 50.5 and 48.8)
 
 
 class AttnPlan:
@@ -113,9 +113,11 @@ def _narrow_split(count: np.ndarray, kv_heads: int, rows: int) -> tuple[int, np.
     total = int(count.sum()) * kv_heads
     share = -(-total // CUS)
     if rows == FEW_ROWS and share > LEAST_SHARE:
-        waves = 4 if int(count.sum()) < SHORT_TILE * len(count) else 8
-        return waves, np.maximum(1, count // max(2 * waves if waves == 4 else waves, share))
-    if rows == FEW_ROWS:
+        # 48 / 64 / 100 threads of 500 keys on four waves 10.4 / 11.4 / 18.1 us, on eight 13.8 / 15.7 / 27.5; of 3000 keys 32 / 39 / 62 and
+        # 33 / 38 / 70; 20 / 32 threads (a tile a CU or less) of 2000 keys 17 / 20 and 15 / 19 (32/8 heads of 128, 64/8 heads alike)
+        waves = 4 if len(count) * kv_heads > CUS and int(count.sum()) < SHORT_TILE * len(count) else 8
+        return waves, np.maximum(1, count // max(8, share))
+    if rows == FEW_ROWS:   # (one thread of 1500 keys 7.5 us, by its share on eight waves 9.2; of 8000 11.4 and 10.5)
         return 4, np.maximum(1, (count + 3) // 4)
     # 90 sizes of 1 to 16 portions of 33 to 512 tokens behind 0 to 8000: 3% off the best split of each on average, in pieces of at least 4
     # blocks and for 512 workgroups 7%, at most 47% (the last piece's join costs as much as 4 blocks)
