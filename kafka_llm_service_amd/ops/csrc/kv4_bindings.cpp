@@ -1,4 +1,4 @@
-// Python bindings of the 4-bit cache's kernels (kv4.hip, kv4_attn.hip). What the kernels assume of shapes, types, strides, alignment
+// Python bindings of the 4-bit cache's kernels (kv4.hip, kv4_attn.hip, kv4_tile.hip). What the kernels assume of shapes, types, strides, alignment
 // and devices is checked here; index values on the device (slots, page ids, kept keys) are checked by the kernels.
 #include <torch/extension.h>
 #include <c10/core/DeviceGuard.h>

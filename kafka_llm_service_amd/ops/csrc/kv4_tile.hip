@@ -17,7 +17,8 @@ struct Image {                            // of 64 keys and one head
 };
 
 // ---- widening -----------------------------------------------------------------------------------------------------------
-// A workgroup per tile and head, a wave per page. K: [page][d / 8][key][8], V: [page][d][16 keys: 0-3, 8-11, 4-7, 12-15], the two halves of
+// A workgroup per tile and head, a wave per page: 16048 keys of 8 heads of 128, 83 MB, 15.5 us (5.4 TB/s, most of it into the last-level
+// cache). K: [page][d / 8][key][8], V: [page][d][16 keys: 0-3, 8-11, 4-7, 12-15], the two halves of
 // rows with d & 8 exchanged (attn_tile.h: reads of both without bank conflicts). Keys behind ``last`` become zeros, and whole pages of which
 // no row from ``pmin`` on sees a key (the table may name anything there); those of a page that is none no numbers. Tiles: table row,
 // block, last key, pmin.
@@ -113,6 +114,9 @@ struct TileArgs {
 // exponentials of this one, between those of its values the rest of them and the next one's maxima, each product behind the LDS reads of the F
 // fragments after it; keys run a tile ahead of the values, and the slots that a step has read are filled again in its middle, behind one counted
 // wait and one barrier. The maximum is raised only where it has grown by more than 2^24 (sums of weights up to that are exact enough in fp32).
+// Products and exponentials bound it, in turn on the same issue slots: 8000 rows cold, 32/8 heads of 128, 1054 TFLOP/s (a large product of the
+// library 1379), of 64, which have half the products for an exponential, 759. Heads of 64: three workgroups of four waves a CU, of 128 one of
+// eight, whose ring of three slots (96 KiB) leaves no room for another. Below about 500 rows the tiles of 32 rows (kv4_attn.hip) are as fast.
 template <int D, int NW, int NSLOT>
 __global__ __launch_bounds__(64 * NW, D == 64 ? 3 : 1) void tile_kernel(TileArgs a) {
   constexpr int F = D / 16, NT = D / 32, KBYTES = Image<D>::KBYTES, PB = Image<D>::PAGE_BYTES;
