@@ -561,7 +561,7 @@ __device__ __forceinline__ void of_rows(T x, T (&y)[4], int lane) {
 // comes with it: a load that is asked for when its sum is there holds up those of the next keys. Bytes bound it, and the start and
 // end of workgroups of 28 blocks: 29 threads of 7900 tokens, 8 heads of 128, 140 MB, 39 us, 3.6 TB/s.
 template <int D, int NB>
-__global__ __launch_bounds__(256) void mass_few_kernel(MassArgs ma) {
+__global__ __launch_bounds__(256, 4) void mass_few_kernel(MassArgs ma) {
   const Args& a = ma.a;
   const int* it = reinterpret_cast<const int*>(a.items) + 8 * (blockIdx.x / a.Hkv);
   const int row = it[0], rows = it[1], pos = it[2], table = it[3], seg = it[4], end = it[6];
