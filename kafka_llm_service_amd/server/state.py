@@ -84,7 +84,7 @@ class ServerConfig:
 
 
 def _engine_kwargs(e) -> dict[str, Any]:
-    """Engine options from the environment: KAFKA_KV_DTYPE (bf16 | fp8 KV cache), KAFKA_DTYPE (bfloat16 | float32
+    """Engine options from the environment: KAFKA_KV_DTYPE (bf16 | fp8 | mx4 KV cache), KAFKA_DTYPE (bfloat16 | float32
     activations, the latter for the model families built for it), KAFKA_GRAPHS=1 (hipGraph decode steps),
     KAFKA_MAX_NUM_SEQS, KAFKA_MAX_BATCHED_TOKENS."""
     kw: dict[str, Any] = {}
