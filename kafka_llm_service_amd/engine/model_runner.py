@@ -569,6 +569,8 @@ class CascadePlan:
 
 
 class ModelRunner:
+    mx4 = False  # the cache in 4 bits, on a GPU
+
     def __init__(self, model: TransformerLM, k_caches, v_caches, kvm, max_num_seqs: int, max_blocks_per_seq: int,
                  cascade_min_prefix: int = 512, use_cascade: bool = True, target_wgs: int = 256,
                  prefill_kv_chunk: int = 1024, slots=None):
@@ -638,7 +640,7 @@ class ModelRunner:
 
     def _init_common(self, max_num_seqs: int) -> None:
         """The runner state every plan kind needs (a segment-planned model has no tile variants or cascade)."""
-        self.variant, self.pad_rows, self.use_cascade, self.graphs, self.mx4 = 0, False, False, None, False
+        self.variant, self.pad_rows, self.use_cascade, self.graphs = 0, False, False, None
         self.vocab = self.model.cfg.vocab_size
         self._pin = self.device.type == "cuda"
         self.last_stats = {}
