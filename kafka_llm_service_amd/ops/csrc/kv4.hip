@@ -271,10 +271,10 @@ __global__ __launch_bounds__(KEEP_NT) void evict_keep_kernel(const float* __rest
   }
 }
 
-// Kept keys, values and masses into new pages, a wave for four new pages of a head. K goes by
+// Kept keys, values and masses into new pages, a wave for a new page of a head. K goes by
 // 16-byte pieces, V by the words of its keys. Keys outside of their table or cache leave their place in the new page as it was.
-// Cache lines bound it: half of the keys kept, nearly every line of the old pages is read. 4096 of 8000 keys, 16 sequences, 8 heads of 128: 55 us,
-// 142 MB kept and written, 213 MB with the lines' other halves (3.9 TB/s). (More pages at once: all four in registers spill, 14 times the time.)
+// Cache lines bound it: half of the keys kept, nearly every line of the old pages is read. 4096 of 8000 keys, 16 sequences, 8 heads of 128: 52 us,
+// 142 MB kept and written, 213 MB with the lines' other halves (4.1 TB/s). Four pages a wave take 55, and one short sequence 6.4 us for 4.2.
 template <int D>
 __global__ __launch_bounds__(256) void evict_copy_kernel(uint8_t* __restrict__ kc, uint8_t* __restrict__ vc, int64_t n_pages,
                                                          const int* __restrict__ tables, int tw, int64_t ts, const int* __restrict__ kept,
@@ -282,60 +282,57 @@ __global__ __launch_bounds__(256) void evict_copy_kernel(uint8_t* __restrict__ k
                                                          const float* __restrict__ mass, int64_t ms, int64_t mh, int N,
                                                          float* __restrict__ new_mass) {
   constexpr int U = D / 8, KP = D / 32, BYTES = Page<D>::BYTES, DATA = Page<D>::DATA;   // words of a key; 16-byte pieces of it
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-  const int h = blockIdx.y, r = blockIdx.z, i0 = (blockIdx.x * 4 + w) * 64;
+  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int h = blockIdx.y, r = blockIdx.z, pg = blockIdx.x * 4 + w, i0 = pg * PAGE;
   if (i0 >= budget) return;
   const int64_t row = ((int64_t)r * Hkv + h) * budget;
-  // lane = key: where it is and where its page goes (-1: nowhere), in pages and heads
-  const int src = i0 + lane < budget ? kept[row + i0 + lane] : -1;
-  const int np = (i0 + lane) / PAGE < nw && i0 + lane < budget ? new_tables[r * ns + (i0 + lane) / PAGE] : -1;
+  const int np = pg < nw ? new_tables[r * ns + pg] : -1;
+  const bool page = np >= 0 && np < n_pages;
+  const int64_t to = ((int64_t)(page ? np : 0) * Hkv + h) * BYTES;
+  // lane = key: where it is (-1: nowhere), in pages and heads
+  const bool mine = lane < PAGE && i0 + lane < budget;
+  const int src = mine ? kept[row + i0 + lane] : -1;
   int64_t from = -1;
-  if (src >= 0 && (src >> 4) < tw) {
+  if (page && src >= 0 && (src >> 4) < tw) {
     const int p = tables[r * ts + (src >> 4)];
     if (p >= 0 && p < n_pages) from = (int64_t)p * Hkv + h;
   }
-  if (np < 0 || np >= n_pages) from = -1;
-  const int64_t to = (int64_t)np * Hkv + h;
   const int so = src & 15, o = lane & 15;
-  if (new_mass && i0 + lane < budget) new_mass[row + i0 + lane] = src >= 0 && src < N ? mass[r * ms + h * mh + src] : 0.f;
-  auto of = [&](int64_t x, int l) {
-    return (int64_t)(uint32_t)__shfl((int)(uint32_t)x, l, 64) | (int64_t)__shfl((int)(x >> 32), l, 64) << 32;
+  if (new_mass && mine) new_mass[row + i0 + lane] = src >= 0 && src < N ? mass[r * ms + h * mh + src] : 0.f;
+  auto of = [&](int l) {
+    return (int64_t)(uint32_t)__shfl((int)(uint32_t)from, l, 64) | (int64_t)__shfl((int)(from >> 32), l, 64) << 32;
   };
   const int kk = lane / KP, kp = lane % KP, c = lane / U, p = lane % U;
-#pragma unroll 2
-  for (int g = 0; g < 4; ++g) {
-    const int64_t t = of(to, 16 * g) * BYTES;   // (the page of the group's first key)
-    u32x4 k, v;
-    int there = 0;
-    {                                           // K: lane = (key, piece)
-      const int l = 16 * g + (kk & 15), s = __shfl(so, l, 64);
-      const int64_t f = of(from, l);
-      if (kk < 16 && f >= 0) {
-        k = *reinterpret_cast<const u32x4*>(kc + f * BYTES + s * (D / 2) + kp * 16);
-        there = 16;
-      }
+  u32x4 k, v;
+  int there = 0;
+  {                                             // K: lane = (key, piece)
+    const int l = kk & 15, s = __shfl(so, l, 64);
+    const int64_t f = of(l);
+    if (kk < 16 && f >= 0) {
+      k = *reinterpret_cast<const u32x4*>(kc + f * BYTES + s * (D / 2) + kp * 16);
+      there = 16;
     }
+  }
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {               // V: lane = (four keys, eight elements)
-      const int l = 16 * g + ((4 * c + i) & 15), s = __shfl(so, l, 64);
-      const int64_t f = of(from, l);
-      if (c < 4 && f >= 0) {
-        v[i] = *reinterpret_cast<const uint32_t*>(vc + f * BYTES + ((s >> 2) * U + p) * 16 + (s & 3) * 4);
-        there |= 1 << i;
-      }
+  for (int i = 0; i < 4; ++i) {                 // V: lane = (four keys, eight elements)
+    const int l = (4 * c + i) & 15, s = __shfl(so, l, 64);
+    const int64_t f = of(l);
+    if (c < 4 && f >= 0) {
+      v[i] = *reinterpret_cast<const uint32_t*>(vc + f * BYTES + ((s >> 2) * U + p) * 16 + (s & 3) * 4);
+      there |= 1 << i;
     }
-    if (there & 16) *reinterpret_cast<u32x4*>(kc + t + kk * (D / 2) + kp * 16) = k;
-    uint8_t* vd = vc + t + (c * U + p) * 16;
-    if ((there & 15) == 15) *reinterpret_cast<u32x4*>(vd) = v;
-    else {
+  }
+  if (there & 16) *reinterpret_cast<u32x4*>(kc + to + kk * (D / 2) + kp * 16) = k;
+  uint8_t* vd = vc + to + (c * U + p) * 16;
+  if ((there & 15) == 15) *reinterpret_cast<u32x4*>(vd) = v;
+  else {
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if ((there >> i) & 1) *reinterpret_cast<uint32_t*>(vd + 4 * i) = v[i];
-    }
+    for (int i = 0; i < 4; ++i)
+      if ((there >> i) & 1) *reinterpret_cast<uint32_t*>(vd + 4 * i) = v[i];
   }
   if (from >= 0) {                              // scales: lane = key
     const uint8_t *kf = kc + from * BYTES + DATA, *vf = vc + from * BYTES + DATA;
-    uint8_t *kd = kc + to * BYTES + DATA, *vd = vc + to * BYTES + DATA;
+    uint8_t *kd = kc + to + DATA, *vd = vc + to + DATA;
     if constexpr (D == 128) *reinterpret_cast<uint32_t*>(kd + o * 4) = *reinterpret_cast<const uint32_t*>(kf + so * 4);
     else *reinterpret_cast<uint16_t*>(kd + o * 2) = *reinterpret_cast<const uint16_t*>(kf + so * 2);
     uint8_t vs[KP];
@@ -378,7 +375,7 @@ extern "C" hipError_t kafka_kv4_read(const uint8_t* kc, const uint8_t* vc, const
 
 extern "C" hipError_t kafka_kv4_evict_keep(const float* mass, int64_t ms, int64_t mh, int N, const int* lens, int R, int Hkv, int budget,
                                            int first, int recent, int* kept, hipStream_t st) {
-  if (R == 0 || budget == 0) return hipSuccess;
+  if (R == 0 || Hkv == 0 || budget == 0) return hipSuccess;
   if (first < 0 || recent < 0 || (int64_t)first + recent > budget || R > 65535) return hipErrorInvalidValue;
   auto go = [&](auto kern) { kern<<<dim3(Hkv, R), KEEP_NT, 0, st>>>(mass, ms, mh, N, lens, budget, first, recent, kept, Hkv); };
   if (N <= KEEP_NT * 4) go(evict_keep_kernel<4, true>);
@@ -394,7 +391,7 @@ extern "C" hipError_t kafka_kv4_evict_copy(uint8_t* kc, uint8_t* vc, int64_t n_p
   if (R == 0 || budget == 0) return hipSuccess;
   if ((D != 64 && D != 128) || R > 65535 || Hkv > 65535) return hipErrorInvalidValue;
   auto go = [&](auto kern) {
-    kern<<<dim3((budget + 255) / 256, Hkv, R), 256, 0, st>>>(kc, vc, n_pages, tables, tw, ts, kept, budget, new_tables, nw, ns, Hkv, mass, ms,
+    kern<<<dim3((budget + 63) / 64, Hkv, R), 256, 0, st>>>(kc, vc, n_pages, tables, tw, ts, kept, budget, new_tables, nw, ns, Hkv, mass, ms,
                                                            mh, N, new_mass);
     return hipGetLastError();
   };
