@@ -171,7 +171,7 @@ __device__ __forceinline__ int before_thread(int x, int* ws, int& all) {
 // many threads would wait at one counter) until its equals are as many as are wanted, then the keys are numbered in order. A thread
 // holds PER neighbouring keys; of sequences that fit no such kernel (REG false) they are read again, KEEP_NT * PER at a time. Waiting bounds
 // it, for barriers and for instructions that nobody has fetched yet: 2500 keys of 8 heads take 5.9 us with 4 keys a thread and 10.2 with
-// 16, most of them not there; 16 sequences of 8000 keys 18 us.
+// 16, most of them not there; 16 sequences of 8000 keys 12 us.
 template <int PER, bool REG>
 __global__ __launch_bounds__(KEEP_NT) void evict_keep_kernel(const float* __restrict__ mass, int64_t ms, int64_t mh, int N,
                                                              const int* __restrict__ lens, int budget, int first, int recent,
@@ -378,10 +378,13 @@ extern "C" hipError_t kafka_kv4_evict_keep(const float* mass, int64_t ms, int64_
   if (R == 0 || Hkv == 0 || budget == 0) return hipSuccess;
   if (first < 0 || recent < 0 || (int64_t)first + recent > budget || R > 65535) return hipErrorInvalidValue;
   auto go = [&](auto kern) { kern<<<dim3(Hkv, R), KEEP_NT, 0, st>>>(mass, ms, mh, N, lens, budget, first, recent, kept, Hkv); };
+  // (16 sequences of 5000 / 8300 / 12000 keys, as few a thread as hold them, 9 / 12 / 14 us, 8300 with 16 a thread 18; read again, 4 a thread at a
+  // time, 12 / 16 / 19. One of 30000 keys, which no kernel holds, 4 a thread at a time 40, 16 at a time 49)
   if (N <= KEEP_NT * 4) go(evict_keep_kernel<4, true>);
   else if (N <= KEEP_NT * 8) go(evict_keep_kernel<8, true>);
+  else if (N <= KEEP_NT * 12) go(evict_keep_kernel<12, true>);
   else if (N <= KEEP_NT * 16) go(evict_keep_kernel<16, true>);
-  else go(evict_keep_kernel<8, false>);
+  else go(evict_keep_kernel<4, false>);
   return hipGetLastError();
 }
 

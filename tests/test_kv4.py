@@ -310,7 +310,8 @@ def _masses(R, H, N, kind, seed=0):
 KEEPS = [(3, 2, 200, 64, 4, 16, "plain"), (2, 2, 3000, 1024, 4, 256, "ties"), (1, 3, 1500, 1000, 0, 0, "same"), (2, 1, 1025, 64, 32, 32, "plain"),
          (2, 2, 2500, 1500, 1, 100, "special"), (1, 1, 5, 1, 0, 0, "plain"), (2, 2, 30, 64, 4, 16, "plain"), (1, 2, 9000, 4097, 16, 1, "plain"),
          (2, 1, 700, 1, 1, 0, "ties"), (1, 1, 2000, 300, 0, 300, "special"),
-         (2, 2, 40000, 9000, 4, 1000, "plain"), (1, 1, 40000, 20000, 0, 7, "ties"), (1, 2, 16385, 500, 3, 0, "special"), (1, 1, 16384, 16383, 0, 0, "same")]
+         (2, 2, 40000, 9000, 4, 1000, "plain"), (1, 1, 40000, 20000, 0, 7, "ties"), (1, 2, 16385, 500, 3, 0, "special"), (1, 1, 16384, 16383, 0, 0, "same"),
+         (2, 1, 4097, 1000, 4, 100, "plain"), (1, 2, 8193, 3000, 0, 9, "ties"), (2, 2, 12288, 5000, 5, 0, "special"), (1, 1, 12289, 700, 1, 1, "plain")]
 
 
 def _lens(R, N):
