@@ -638,7 +638,7 @@ __global__ __launch_bounds__(256, 4) void mass_few_kernel(MassArgs ma) {
 // heads of 128, 47 us, 430 TFLOP/s (each wave with rows of its own 85 us).
 // Items: first row, rows, position, table row, segment, block, first column, behind the last, first slot or -1, part | parts << 16, 0, 0.
 template <int D>
-__global__ __launch_bounds__(256, 4) void mass_many_kernel(MassArgs ma) {
+__global__ __launch_bounds__(256, 3) void mass_many_kernel(MassArgs ma) {
   constexpr int CH = 64, STAGE = CH * D * 2, PIECES = STAGE / 4096;
   const Args& a = ma.a;
   // (one object: of several the compiler knows which one a load fills, and waits for it ahead of every read)
@@ -687,21 +687,25 @@ __global__ __launch_bounds__(256, 4) void mass_many_kernel(MassArgs ma) {
     bf16x8 k[4][D / 32];
     {
       int pg[4];
-      uint32_t kw[4][D / 32], ks[4][D / 32];
+      u32x4 kw[4];
+      uint32_t ks[4];
       PageIds(a.tables + table * a.ts, pos, last, a.window, a.first, lane, [&](int) { return it[5] + w; }).get<4>(0, a.n_pages, pg, bad);
 #pragma unroll
-      for (int t = 0; t < 4; ++t) {
+      for (int t = 0; t < 4; ++t) {                        // a quarter of a key, D / 4 elements, is a lane's for all steps of the products
         const uint8_t* p = a.kc + ((int64_t)pg[t] * a.Hkv + h) * Page<D>::BYTES;
-#pragma unroll
-        for (int i = 0; i < D / 32; ++i) {
-          kw[t][i] = *reinterpret_cast<const uint32_t*>(p + (lane & 15) * (D / 2) + 16 * i + 4 * c);
-          ks[t][i] = p[Page<D>::DATA + (lane & 15) * (D / 32) + i];
+        const uint8_t* kp = p + (lane & 15) * (D / 2) + c * (D / 8);
+        if constexpr (D == 128) {
+          kw[t] = *reinterpret_cast<const u32x4*>(kp);
+        } else {
+          const u32x2 y = *reinterpret_cast<const u32x2*>(kp);
+          kw[t] = u32x4{y[0], y[1], 0, 0};
         }
+        ks[t] = p[Page<D>::DATA + (lane & 15) * (D / 32) + c * (D / 32) / 4];
       }
 #pragma unroll
       for (int t = 0; t < 4; ++t)
 #pragma unroll
-        for (int i = 0; i < D / 32; ++i) k[t][i] = widen8(kw[t][i], scale_of(ks[t][i]));
+        for (int i = 0; i < D / 32; ++i) k[t][i] = widen8(kw[t][i], scale_of(ks[t]));
     }
     int buf = 0;
     for (int R = it[6]; R < R1; R += CH, buf ^= 1) {
@@ -711,19 +715,15 @@ __global__ __launch_bounds__(256, 4) void mass_many_kernel(MassArgs ma) {
       t3_wait_vmcnt<0>();                                  // this stage; and all have done with the one before the next takes its place
       t3_barrier();
       if (R + CH < R1) stage(buf ^ 1);
-      for (int j = 0; j < CH; j += 16) {
-        const int pmin = pos + tok0 + (int)((rem0 + j) * inv >> 16), pmax = pos + tok0 + (int)((rem0 + j + 15) * inv >> 16);
-        if (R + j >= R1 || pmax < key0 || (pmin - a.window >= key0 + KB - 1 && key0 >= a.first)) continue;
-        any = true;
-        const int r = j + (lane & 15);
+      // scores of the 16 rows from j on, times 2^(- their lse)
+      const char* const qb = rows_q + buf * STAGE + (lane & 15) * (2 * D);
+      const char* const lb = rows_l + buf * (CH * 4) + 4 * (lane & 15);
+      auto tile = [&](int j, auto mask) {
         bf16x8 q[D / 32];
 #pragma unroll
         for (int i = 0; i < D / 32; ++i)
-          q[i] = *reinterpret_cast<const bf16x8*>(rows_q + buf * STAGE + r * (2 * D) + 16 * ((4 * i + c) ^ (D == 128 ? lane & 15 : lane >> 1 & 7)));
-        const int t = tok0 + (int)((rem0 + r) * inv >> 16), lim = t < rows ? pos + t : -1;
-        float l = *reinterpret_cast<const float*>(rows_l + buf * (CH * 4) + 4 * r);
-        l = lim >= 0 && l != -INFINITY ? l : INFINITY;     // no row, or one that sees nothing: weights of zero
-        const bool masked = key0 + KB - 1 > pmin || pmax > last || (key0 <= pmax - a.window && key0 + KB > a.first);
+          q[i] = *reinterpret_cast<const bf16x8*>(qb + j * (2 * D) + 16 * ((D / 32 * c + i) ^ (D == 128 ? lane & 15 : lane >> 1 & 7)));
+        const float x = *reinterpret_cast<const float*>(lb + 4 * j), l = x == -INFINITY ? INFINITY : x;   // (a row that sees nothing has no weights)
 #pragma unroll
         for (int u = 0; u < 4; u += 2) {
           f32x4 s[2];
@@ -735,20 +735,33 @@ __global__ __launch_bounds__(256, 4) void mass_many_kernel(MassArgs ma) {
           }
 #pragma unroll
           for (int t = 0; t < 2; ++t) asm volatile("" : "+v"(s[t]));
-          if (masked) {
-            int cc = c;
-            asm volatile("" : "+v"(cc));
-#pragma unroll
-            for (int t = 0; t < 2; ++t)
-#pragma unroll
-              for (int i = 0; i < 4; ++i)
-                if (!sees(key0 + 16 * (u + t) + 4 * cc + i, lim, a.window, a.first)) s[t][i] = -INFINITY;
-          }
+          mask(s, u);
 #pragma unroll
           for (int t = 0; t < 2; ++t)
 #pragma unroll
             for (int i = 0; i < 4; ++i) acc[4 * (u + t) + i] += fast_exp2(fmaf(s[t][i], a.scale2, -l));
         }
+      };
+      const int pmin = pos + tok0, pmax = pmin + (int)((rem0 + CH - 1) * inv >> 16);
+      if (R + CH <= R1 && pmin >= key0 + KB - 1 && pmax <= last && (pmax - a.window < key0 || key0 + KB <= a.first)) {
+        any = true;                                        // all of the rows see all of the keys
+#pragma unroll
+        for (int j = 0; j < CH; j += 16) tile(j, [](auto&, int) {});
+        continue;
+      }
+#pragma unroll 1
+      for (int j = 0; j < CH; j += 16) {
+        const int p0 = pos + tok0 + (int)((rem0 + j) * inv >> 16), p1 = pos + tok0 + (int)((rem0 + j + 15) * inv >> 16);
+        if (R + j >= R1 || p1 < key0 || (p0 - a.window >= key0 + KB - 1 && key0 >= a.first)) continue;
+        any = true;
+        const int t = tok0 + (int)((rem0 + j + (lane & 15)) * inv >> 16), lim = t < rows ? pos + t : -1;
+        tile(j, [&](f32x4(&s)[2], int u) {
+#pragma unroll
+          for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              if (!sees(key0 + 16 * (u + t) + 4 * c + i, lim, a.window, a.first)) s[t][i] = -INFINITY;
+        });
       }
     }
   }
