@@ -632,10 +632,10 @@ __global__ __launch_bounds__(256, 4) void mass_few_kernel(MassArgs ma) {
 
 // Longer segments: four waves, a block of keys each, its keys widened in registers, go through the same rows, all that may see one of the
 // blocks or a part of them, in stages of 64 that stay in LDS for all four (each wave's own loads of 16 rows, 256 bytes apart, would take
-// 64 cycles a load of what the CU has for all its waves, four times what they need to be computed). A lane has one of 16 rows and a quarter of
+// 64 cycles a load of what the CU has for all its waves). A lane has one of 16 rows and a quarter of
 // the keys, each key's sum by itself: no lane asks another for anything until the rows end. Parts of a block's rows are joined in their
-// order by the last workgroup of them to end (attn_kernel). Exponentials and the products' issue bound it: 1900 rows behind 1000 keys, 32/8
-// heads of 128, 47 us, 430 TFLOP/s (each wave with rows of its own 85 us).
+// order by the last workgroup of them to end (attn_kernel). Exponentials and products bound it, one after the other on a SIMD: 1900 rows behind 1000 keys, 32/8
+// heads of 128, 42 us, 480 TFLOP/s (each wave with rows of its own 85 us; 500 cycles for 16 rows and 64 keys, 256 of them products).
 // Items: first row, rows, position, table row, segment, block, first column, behind the last, first slot or -1, part | parts << 16, 0, 0.
 template <int D>
 __global__ __launch_bounds__(256, 3) void mass_many_kernel(MassArgs ma) {
