@@ -250,7 +250,10 @@ def _plan(segs, heads: int, kv_heads: int, dim: int, window: int, first: int) ->
     if first and not window:
         raise ValueError("kv4.attn_plan: first tokens stay visible beside a window")
     p = AttnPlan()
-    a = np.array([tuple(int(x) for x in s) for s in segs], dtype=np.int64).reshape(-1, 4)
+    a = np.array(list(segs), dtype=np.int64)
+    if a.size and (a.ndim != 2 or a.shape[1] != 4):
+        raise ValueError("kv4.attn_plan: segments of (first row, rows, position, table row)")
+    a = a.reshape(-1, 4)
     p.segs = [tuple(s) for s in a.tolist()]
     if (a < 0).any() or (a[:, 0] + a[:, 1] >= MAX_POS).any() or (a[:, 2] + a[:, 1] >= MAX_POS).any() or (a[:, 3] >= 1 << 30).any():
         raise ValueError("kv4.attn_plan: segments of (first row, rows, position, table row), none negative, positions below 2^26")

@@ -371,7 +371,7 @@ def test_refusals():
             ops.kv_cache_shapes(4, 2, bad, "mx4")
     plan = lambda *a, **k: kv4.attn_plan(*a, device="cpu", **k)
     for segs in ([(-1, 1, 0, 0)], [(0, 1, -1, 0)], [(0, -1, 0, 0)], [(0, 1, 0, -1)], [(0, 4, 0, 0), (3, 1, 0, 1)], [(0, 1, 1 << 26, 0)],
-                 [(1, 1, 0, 0), (1, 1, 0, 0)], [(1 << 26, 1, 0, 0)]):
+                 [(1, 1, 0, 0), (1, 1, 0, 0)], [(1 << 26, 1, 0, 0)], [(0, 1, 0)] * 4, [0, 1, 0, 0], [(0, 1, 0, 0), (1, 1)]):
         with pytest.raises(ValueError):
             plan(segs, 8, 2, 128)
     for heads in ((9, 2, 128), (34, 2, 128), (8, 2, 96), (8, 0, 128), (0, 2, 128)):
