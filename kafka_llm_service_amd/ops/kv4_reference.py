@@ -50,7 +50,7 @@ def pack(codes: torch.Tensor, e: torch.Tensor, value: bool) -> torch.Tensor:
 def unpack(pages: torch.Tensor, value: bool) -> tuple[torch.Tensor, torch.Tensor]:
     n, h = pages.shape[:2]
     D = head_dim(pages)
-    flat = pages.reshape(n, h, -1)
+    flat = pages.flatten(2)
     b, s = flat[..., :PAGE * D // 2], flat[..., PAGE * D // 2:]
     if value:
         b = b.reshape(n, h, 4, D // 8, 4, 4).transpose(3, 4).reshape(n, h, PAGE, D // 2)

@@ -479,6 +479,35 @@ def test_pages_left_behind_reference(D, segs):
     _pages_left_behind("cpu", D, segs)
 
 
+def _nothing(device):
+    """Plans without a segment, or without rows: nothing is written, masses stay what they were."""
+    kc, vc = (torch.zeros(2, 2, 16, 68, dtype=torch.uint8, device=device) for _ in range(2))
+    bt = torch.full((1, 1), -1, dtype=torch.int32, device=device)
+    q, lse = queries(3, 8, 128, device=device), torch.full((3, 8), 7.0, device=device)
+    for segs in ([], [(0, 0, 0, 0)], [(2, 0, 500, 9), (1, 0, 0, 0)]):
+        for kw in ({}, dict(window=5, first=2)):
+            plan = kv4.attn_plan(segs, 8, 2, 128, device=device, **kw)
+            out = torch.full_like(q, 3.0)
+            kv4.attn(q, kc, vc, bt, plan, 0.1, out=out, lse=lse)
+            assert (out == 3).all() and (lse == 7).all() and (kv4.attn(q, kc, vc, bt, plan, 0.1) == 0).all()
+            assert kv4.attn_mass(q, lse, kc, bt, plan, 0.1).shape == (len(segs), 2, 0)
+            base = torch.rand(len(segs), 2, 130, device=device)
+            assert torch.equal(kv4.attn_mass(q, lse, kc, bt, plan, 0.1, base=base), base)
+    none = torch.zeros(0, dtype=torch.int64, device=device)
+    assert kv4.read(kc, vc, none)[0].shape == (0, 2, 128)
+    ops.rope_kv_write(torch.zeros(0, 12 * 128, dtype=torch.bfloat16, device=device), none, torch.zeros(1, 128, device=device), q[:0], kc, vc, none, 8, 2)
+    kept = kv4.evict_keep(torch.zeros(2, 2, 0, device=device), torch.zeros(2, dtype=torch.int32, device=device), 5)
+    assert (kept == -1).all() and kept.shape == (2, 2, 5)
+    two = bt.expand(2, 1).contiguous()
+    assert (kv4.evict(kc, vc, two, kept, two, torch.zeros(2, 2, 0, device=device)) == 0).all()
+    assert kv4.evict_keep(torch.zeros(0, 2, 9, device=device), torch.zeros(0, dtype=torch.int32, device=device), 5).shape == (0, 2, 5)
+    assert (kc == 0).all() and (vc == 0).all()
+
+
+def test_nothing_reference():
+    _nothing("cpu")
+
+
 def test_plan_covers_every_block_once():
     """Pieces of tiles of any length and window cover the blocks that the tile sees, each once."""
     import numpy as np
@@ -664,6 +693,11 @@ def test_evict_on_the_gpu(cuda):
         a, b = _move("cpu", **kw), _move(cuda, **kw)
         for x, y in zip(a, b):
             assert torch.equal(x, y)
+
+
+@pytest.mark.gpu
+def test_nothing_on_the_gpu(cuda):
+    _nothing(cuda)
 
 
 @pytest.mark.gpu
