@@ -12,7 +12,8 @@ Rows of a call are described by segments (first row, rows, position of the first
 one sequence, whose keys lie in the cache at their positions. GPU tensors run the HIP kernels on the caches' device and its current
 stream, CPU tensors the references of ``kv4_reference.py``. Workspaces are made per call, so calls on several streams and captured
 graphs do not meet. A plan holds the tables that the kernels read and, for each stream that it is used on, counters that every
-call leaves at zero (a captured call has its own, in its graph); like a call's tensors it has to live until the stream is done with it.
+call leaves at zero (a captured call has its own, in its graph); like a call's tensors it has to live until the stream, or the graph, is
+done with it.
 """
 from __future__ import annotations
 

@@ -887,36 +887,45 @@ def test_widened_keys_are_those_that_a_tile_sees(monkeypatch):
 
 
 @pytest.mark.gpu
-def test_split_tiles_side_by_side(cuda):
-    """Tiles in several pieces whose last one joins them: the same plan eager on two streams and in two graphs, all at once and again."""
-    segs = [(0, 1, 4000, 0), (1, 1, 9000, 1), (2, 2, 2500, 2)]
+@pytest.mark.parametrize("wide", [False, True])
+def test_split_tiles_side_by_side(cuda, monkeypatch, wide):
+    """Work in several parts whose last one joins them: the same plan eager on two streams and in two graphs, all at once and again."""
+    monkeypatch.setattr(kv4, "MANY_COST", -1e9 if wide else 1e9)
+    monkeypatch.setattr(kv4, "SOME_PIECE", 2)
+    monkeypatch.setattr(kv4, "MASS_TILES", 1)
+    segs = [(0, 1, 4000, 0), (1, 1, 9000, 1), (2, 2, 2500, 2), (4, 90, 1500, 3)]
     kc, vc, tables = world(segs, 2, 128, 0, cuda)
-    q = queries(4, 8, 128, 1, cuda)
+    q = queries(94, 8, 128, 1, cuda)
     plan = kv4.attn_plan(segs, 8, 2, 128, device=cuda)
     p, a = kv4._plan(segs, 8, 2, 128, 0, 0)
-    assert kv4._tables(a, 8, 2, 128, 0, 0)[0][0][2] > 3                     # (slots of partial results)
-    lse = torch.empty(4, 8, device=cuda)
-    want = kv4.attn(q, kc, vc, tables, plan, 0.1, lse=lse)
+    shapes = kv4._tables(a, 8, 2, 128, 0, 0)[0]
+    assert [x[0] for x in shapes] == ([16, 256] if wide else [16, 32]) and all(x[2] > 3 for x in shapes)   # (slots of partial results)
+    assert kv4._mass_tables(a, 4, 2, p.keys, 0, 0)[2] > 3
+
+    def step():
+        l = torch.zeros(94, 8, device=cuda)
+        o = kv4.attn(q, kc, vc, tables, plan, 0.1, lse=l)
+        return o, l, kv4.attn_mass(q, l, kc, tables, plan, 0.1)
+
+    want = step()
     streams, runs = [torch.cuda.Stream() for _ in range(4)], []
     for s in streams[:2]:
         s.wait_stream(torch.cuda.current_stream())
         with torch.cuda.stream(s):
             graph = torch.cuda.CUDAGraph()
             with torch.cuda.graph(graph, stream=s):
-                l = torch.empty_like(lse)
-                o = kv4.attn(q, kc, vc, tables, plan, 0.1, lse=l)
-            runs.append((graph, o, l))
+                outs = step()
+            runs.append((graph, outs))
     for s in streams:
         s.wait_stream(torch.cuda.current_stream())
     eager = []
     for _ in range(10):
-        for s, (graph, o, l) in zip(streams, runs):
+        for s, (graph, _) in zip(streams, runs):
             with torch.cuda.stream(s):
                 graph.replay()
         for s in streams[2:]:
             with torch.cuda.stream(s):
-                l = torch.empty_like(lse)
-                eager.append((kv4.attn(q, kc, vc, tables, plan, 0.1, lse=l), l))
+                eager.append(step())
     torch.cuda.synchronize()
-    for o, l in eager + [r[1:] for r in runs]:
-        assert torch.equal(o, want) and torch.equal(l, lse)
+    for outs in eager + [r[1] for r in runs]:
+        assert all(torch.equal(x, y) for x, y in zip(outs, want))
