@@ -59,6 +59,16 @@ __device__ __forceinline__ float over_quarters_sum(float x) {
   return x + __shfl_xor(x, 32, 64);
 }
 
+// Of four numbers a lane the sums over the quarters, the c-th one in quarter c: halves, then rows of 16, of two registers change places
+__device__ __forceinline__ float quarters_sums(const float (&x)[4]) {
+  auto half = [](float a, float b) {
+    const auto y = __builtin_amdgcn_permlane32_swap(__float_as_uint(a), __float_as_uint(b), false, false);
+    return __uint_as_float(y[0]) + __uint_as_float(y[1]);
+  };
+  const auto y = __builtin_amdgcn_permlane16_swap(__float_as_uint(half(x[0], x[2])), __float_as_uint(half(x[1], x[3])), false, false);
+  return __uint_as_float(y[0]) + __uint_as_float(y[1]);
+}
+
 // The list of blocks that a tile of rows at positions [p0, p1] sees
 struct Blocks {
   int head, tail, count;   // blocks below ``head``, then from ``tail`` on
@@ -95,39 +105,38 @@ struct PageIds {
   }
   // NP of them from lane ``at`` on. An id that is not of the cache counts as page 0 and sets ``bad``: such rows come out as no numbers.
   template <int NP>
-  __device__ __forceinline__ void get(int at, int64_t n_pages, int (&pg)[NP], bool& bad) const {
+  __device__ __forceinline__ void get(int at, uint32_t n_pages, uint32_t (&pg)[NP], bool& bad) const {
 #pragma unroll
     for (int t = 0; t < NP; ++t) {
-      const int p = __builtin_amdgcn_readlane(v, at + t);
-      const bool ok = p >= 0 && p < n_pages;
-      bad |= !ok;
-      pg[t] = ok ? p : 0;
+      const uint32_t p = __builtin_amdgcn_readlane(v, at + t);
+      bad |= p >= n_pages;
+      pg[t] = p < n_pages ? p : 0;
     }
   }
 };
 
 // (heads of 64: both halves of the lanes hold the key, for the two parts of Q)
 template <int D, int NP>
-__device__ __forceinline__ void load_k(KFrag<NP>& f, const uint8_t* kc, int Hkv, int h, const int (&pg)[NP], int lane) {
-  const uint32_t key = lane & 15, g = (lane >> 4) & (D / 32 - 1);
+__device__ __forceinline__ void load_k(KFrag<NP>& f, const uint8_t* kh, uint32_t stride, const uint32_t (&pg)[NP], int lane) {
+  const uint32_t key = lane & 15, g = (lane >> 4) & (D / 32 - 1), at = key * (D / 2) + g * 16, sc = Page<D>::DATA + key * (D / 32) + g;
 #pragma unroll
   for (int t = 0; t < NP; ++t) {
-    const uint8_t* p = kc + ((int64_t)pg[t] * Hkv + h) * Page<D>::BYTES;
-    const u32x4 x = *reinterpret_cast<const u32x4*>(p + key * (D / 2) + g * 16);
+    const uint8_t* p = kh + (uint64_t)pg[t] * stride;
+    const u32x4 x = *reinterpret_cast<const u32x4*>(p + at);
 #pragma unroll
     for (int i = 0; i < 4; ++i) f.d[t][i] = x[i];
-    f.s[t] = p[Page<D>::DATA + key * (D / 32) + g];
+    f.s[t] = p[sc];
   }
 }
 
 template <int D, int NP>
-__device__ __forceinline__ void load_v(VFrag<NP>& f, const uint8_t* vc, int Hkv, int h, const int (&pg)[NP], int lane) {
-  const uint32_t dl = lane & 15, c = lane >> 4;
+__device__ __forceinline__ void load_v(VFrag<NP>& f, const uint8_t* vh, uint32_t stride, const uint32_t (&pg)[NP], int lane) {
+  const uint32_t dl = lane & 15, c = lane >> 4, at = (c * (D / 8) + dl * (D / 8) / 16) * 16, sc = Page<D>::DATA + (dl * (D / 16) / 32) * 16 + c * 4;
 #pragma unroll
   for (int t = 0; t < NP; ++t) {
-    const uint8_t* p = vc + ((int64_t)pg[t] * Hkv + h) * Page<D>::BYTES;
-    f.d[t] = *reinterpret_cast<const u32x4*>(p + (c * (D / 8) + dl * (D / 8) / 16) * 16);
-    f.s[t] = *reinterpret_cast<const uint32_t*>(p + Page<D>::DATA + (dl * (D / 16) / 32) * 16 + c * 4);
+    const uint8_t* p = vh + (uint64_t)pg[t] * stride;
+    f.d[t] = *reinterpret_cast<const u32x4*>(p + at);
+    f.s[t] = *reinterpret_cast<const uint32_t*>(p + sc);
   }
 }
 
@@ -358,6 +367,7 @@ __global__ __launch_bounds__(64 * NW, NQ == 1 ? 3 : 2) void attn_kernel(Args a) 
   if (hi > v0) {
     auto ids = [&](int k) { return PageIds(bt, pmin, pmax, a.window, a.first, lane, [&](int i) { return list[min(v0 + NW * (k / 2 + i), hi - 1)]; }); };
     PageIds id = ids(0), idn = ids(32);
+    const uint32_t stride = a.Hkv * Page<D>::BYTES;             // of a page of all heads
     KFrag<2> kf[NB];
     VFrag<2> vf[NB];
     auto fetch = [&](int x, int k) {
@@ -365,10 +375,10 @@ __global__ __launch_bounds__(64 * NW, NQ == 1 ? 3 : 2) void attn_kernel(Args a) 
         id = idn;
         idn = ids(k + 32);
       }
-      int pg[2];
-      id.get<2>(k % 32 * 2, a.n_pages, pg, bad);
-      load_k<D, 2>(kf[x], a.kc, a.Hkv, h, pg, lane);
-      load_v<D, 2>(vf[x], a.vc, a.Hkv, h, pg, lane);
+      uint32_t pg[2];
+      id.get<2>(k % 32 * 2, (uint32_t)a.n_pages, pg, bad);
+      load_k<D, 2>(kf[x], a.kc + h * Page<D>::BYTES, stride, pg, lane);
+      load_v<D, 2>(vf[x], a.vc + h * Page<D>::BYTES, stride, pg, lane);
     };
     auto step = [&](int x, int k) {
       keys_step<D, NQ, 2>(kf[x], vf[x], r, list[v0 + NW * (k >> 1)] * KB + 32 * (k & 1), pmin, pmax, a.window, a.first, a.scale2, lane);
@@ -559,7 +569,7 @@ __device__ __forceinline__ void of_rows(T x, T (&y)[4], int lane) {
 
 // Segments of at most 16 rows: four waves take every fourth block of an item's (at most 32), NB of them in registers. What a key had before
 // comes with it: a load that is asked for when its sum is there holds up those of the next keys. Bytes bound it, and the start and
-// end of workgroups of 28 blocks: 29 threads of 7900 tokens, 8 heads of 128, 140 MB, 39 us, 3.6 TB/s.
+// end of workgroups of 28 blocks: 29 threads of 7900 tokens, 8 heads of 128, 140 MB, 35 us, 4.0 TB/s.
 template <int D, int NB>
 __global__ __launch_bounds__(256, 4) void mass_few_kernel(MassArgs ma) {
   const Args& a = ma.a;
@@ -589,10 +599,10 @@ __global__ __launch_bounds__(256, 4) void mass_few_kernel(MassArgs ma) {
   // (without conditions, so that the waits count what is on its way: behind the last block that one again, of no row some page)
   auto fetch = [&](int x, int k) {
     k = min(k, n - 1);
-    int pg[4];
+    uint32_t pg[4];
     bad[x] = false;
-    id.get<4>(4 * k, a.n_pages, pg, bad[x]);
-    load_k<D, 4>(kf[x], a.kc, a.Hkv, h, pg, lane);
+    id.get<4>(4 * k, (uint32_t)a.n_pages, pg, bad[x]);
+    load_k<D, 4>(kf[x], a.kc + h * Page<D>::BYTES, a.Hkv * Page<D>::BYTES, pg, lane);
     had[x] = base[min((b0 + 4 * k) * KB + lane, ma.N - 1)];
   };
 #pragma unroll
@@ -616,13 +626,7 @@ __global__ __launch_bounds__(256, 4) void mass_few_kernel(MassArgs ma) {
         for (int i = 0; i < D / 64; ++i) s[t] = mfma8x4(qf.x[i], qf.s[i], kf[x].d[t], kf[x].s[t], s[t]);
       }
       add_weights(acc, s, ls, key0 + KB - 1 > pos || (key0 <= last - a.window && key0 + KB > a.first), key0, lim, a, lane);
-      // lane = key: that of tile c, whose sum every quarter has then
-      float mine = 0.f;
-#pragma unroll
-      for (int t = 0; t < 4; ++t) {
-        const float y = over_quarters_sum(acc[t]);
-        if (c == t) mine = y;
-      }
+      float mine = quarters_sums(acc);                     // lane = key: that of tile c
       if (bad[x]) mine = __builtin_nanf("");
       if (!seen(b)) mine = 0.f;
       if (k + x < n && key0 + lane < ma.N) out[key0 + lane] = (ma.base ? had[x] : 0.f) + mine;
@@ -686,10 +690,10 @@ __global__ __launch_bounds__(256, 3) void mass_many_kernel(MassArgs ma) {
     stage(0);
     bf16x8 k[4][D / 32];
     {
-      int pg[4];
+      uint32_t pg[4];
       u32x4 kw[4];
       uint32_t ks[4];
-      PageIds(a.tables + table * a.ts, pos, last, a.window, a.first, lane, [&](int) { return it[5] + w; }).get<4>(0, a.n_pages, pg, bad);
+      PageIds(a.tables + table * a.ts, pos, last, a.window, a.first, lane, [&](int) { return it[5] + w; }).get<4>(0, (uint32_t)a.n_pages, pg, bad);
 #pragma unroll
       for (int t = 0; t < 4; ++t) {                        // a quarter of a key, D / 4 elements, is a lane's for all steps of the products
         const uint8_t* p = a.kc + ((int64_t)pg[t] * a.Hkv + h) * Page<D>::BYTES;
