@@ -4,8 +4,13 @@ Tolerances. Stored numbers, kept keys and moved pages are compared bit for bit: 
 numbers that 32 bits hold exactly (the rotation's products are rounded one by one in both). Attention, for weights w (their sum 1), with
 A the largest sum_d |scale q_d k_d| of a row: a score is a sum of D exact products in fp32 and a product by the scale, off by at
 most (D + 4) 2^-24 A, and where Q goes in two parts of e4m3 by 2^-21 B, B the largest scale max |q| sum_d |k_d| (a part's
-step is 2^-9, its factor 2^-4, and the largest element comes to at least 128: an element is off by half of 2^-13 / 128 of that); the
-exponential and its argument add 2^-22 (1 + A): EW = 2 ((D + 4) 2^-24 A + 2^-21 B + 2^-22 (1 + A)) bounds a weight's relative error with its
+step is 2^-9, its factor 2^-4, and the largest element comes to at least 128: an element is off by half of 2^-13 / 128 of that), and by C, what
+the instruction cuts: it adds products of eight neighbouring d, each cut to whole multiples of 2^(E - 13), E the largest sum of two factors'
+exponents among them, where 1/2 has the exponent of 1, so 2^E <= 2 max |product|. A product has four bits behind its first and is whole from the
+exponent E - 9 on; one that is not is below 4 * 2^(E - 10) <= 2^-7 of the largest. With a part's own step (2^-4) the first part loses less than
+(1 + 2^-4) 2^-12 of the largest for each product below 2^-6 of it, the second, a 2^-4 of the first at most, 7 * 2^-16 a group. (Where
+elements are so small that e4m3 has no leading bit for them the cut is 2^-19 of their unit: 2^-20 B holds that too.) The
+exponential and its argument add 2^-22 (1 + A): EW = 2 ((D + 4) 2^-24 A + 2^-20 B + C + 2^-22 (1 + A)) bounds a weight's relative error with its
 sum's. P is rounded to bf16 (2^-8), the output too: |do| <= (2^-8 + EW + n 2^-24) sum w |v| + 2^-8 |o|.
 The logarithm is off by (EW + n 2^-24) / ln 2 and its own rounding; a key's weight, from R rows, by the weights' errors, that of
 the logarithm and R additions: (2 EW + (n + R + 2) 2^-24 + 2^-23 |lse|) of itself."""
@@ -51,6 +56,18 @@ def numbers(cache, value):
     return val * torch.exp2(flat[..., sc.to(cache.device)].double() - 127)
 
 
+def _cut(x, k):
+    """C of rows x [rows, D] and keys k [n, D]: [rows, n]."""
+    out = torch.empty(len(x), len(k))
+    step = max(1, 20_000_000 // k.numel())
+    for i in range(0, len(x), step):
+        p = (x[i:i + step, None].abs().float() * k.abs().float()).unflatten(-1, (-1, 8))
+        big = p.amax(-1)
+        small = ((p > 0) & (p < big[..., None] * 2.0 ** -6)).sum(-1)
+        out[i:i + step] = ((small * (1 + 2.0 ** -4) * 2.0 ** -12 + 7 * 2.0 ** -16) * big).sum(-1)
+    return out.double()
+
+
 def oracle(q, kc, vc, tables, segs, window, first, scale):
     """(out, lse base 2, mass [segments, heads, keys], bounds of out, of lse, of mass) in 64 bits."""
     T, Hq, D = q.shape
@@ -73,7 +90,8 @@ def oracle(q, kc, vc, tables, segs, window, first, scale):
             s = (x @ kh.T * scale).masked_fill(~see, -math.inf)
             A = (x.abs() @ kh.abs().T * scale).masked_fill(~see, 0).amax(-1, keepdim=True)
             B = x.abs().amax(-1, keepdim=True) * kh.abs().sum(-1).max() * scale
-            EW = 2 * ((D + 4) * 2.0 ** -24 * A + 2.0 ** -21 * B + 2.0 ** -22 * (1 + A))
+            C = (_cut(x, kh) * scale).masked_fill(~see, 0).amax(-1, keepdim=True)
+            EW = 2 * ((D + 4) * 2.0 ** -24 * A + 2.0 ** -20 * B + C + 2.0 ** -22 * (1 + A))
             ls = torch.logsumexp(s, -1, keepdim=True)
             w = torch.exp(s - ls)
             o = w @ vh
