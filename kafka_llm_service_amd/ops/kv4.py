@@ -201,7 +201,9 @@ def _mass_tables(a: np.ndarray, G: int, kv_heads: int, keys: int, window: int, f
     step = min(32, max(4, -(-nb * len(idx) * kv_heads // MASS_WGS // 4) * 4))
     b = np.arange(0, nb, step)
     s, b = np.repeat(idx, len(b)), np.tile(b, len(idx))
-    out = [np.stack([a[s, 0], a[s, 1], a[s, 2], a[s, 3], s, b, np.minimum(b + step, nb), np.zeros_like(s)], 1).astype(np.int32)]
+    single = np.concatenate([a[s], np.stack([s, b, np.minimum(b + step, nb), np.zeros_like(s)], 1)], 1).astype(np.int32)
+    if few.all():
+        return single, np.zeros((0, 12), np.int32), 0
     idx = np.nonzero(~few)[0]
     nq = (nb + 3) // 4
     s, b = np.repeat(idx, nq), np.tile(4 * np.arange(nq), len(idx))
@@ -223,7 +225,7 @@ def _mass_tables(a: np.ndarray, G: int, kv_heads: int, keys: int, window: int, f
     s, b, at = s[t], b[t], lo[t] + 16 * each[t] * i
     z = np.zeros_like(s)
     many = np.stack([a[s, 0], a[s, 1], a[s, 2], a[s, 3], s, b, at, np.minimum(at + 16 * each[t], hi[t]), slot[t], n[t] << 16 | i, z, z], 1)
-    return out[0], many[np.argsort(many[:, 6] - many[:, 7], kind="stable")].astype(np.int32), int(split.sum())
+    return single, many[np.argsort(many[:, 6] - many[:, 7], kind="stable")].astype(np.int32), int(split.sum())
 
 
 class _Take:
