@@ -13,7 +13,7 @@
 // the widening of V. 64 threads of 4100 tokens, 32/8 heads of 128: 56 us, 5.1 TB/s (a large copy's rate); one thread of 1511 7.4 us: launch,
 // four reads that wait for each other (item, page ids, pages, parts) and the join. Long portions go through kv4_tile.hip.
 #include "attn_tile.h"
-#include "kv4.h"
+#include "kv4_widen.h"
 
 #include <type_traits>
 
@@ -78,6 +78,12 @@ struct Blocks {
     count = p1 < 0 ? 0 : head + p1 / KB + 1 - tail;
   }
   __device__ __forceinline__ int operator[](int v) const { return v < head ? v : v - head + tail; }
+};
+
+struct Widen {
+  const int* tiles;
+  char* ws;
+  uint32_t from;           // first workgroup
 };
 
 template <int NP>          // of NP pages
@@ -340,8 +346,17 @@ __device__ __forceinline__ void join(float& M, float& L, f32x4& o, const float (
 // works on, the others on their way. (The loop's first form fetches without a condition, so that the waits count what is on its way.)
 // Three waves a SIMD: with whole blocks, or three halves, registers leave room for two (64 threads of 4100 tokens 65 us for 56). NQ 2, short portions: values are
 // widened once for 32 rows; 4 portions of 100 rows behind 1000 keys, 32/8 heads of 128, 23 us, of one tile of 256 widened first 31.
-template <int D, int NQ, int NW, int NB>
-__global__ __launch_bounds__(64 * NW, NQ == 1 ? 3 : 2) void attn_kernel(Args a) {
+// WIDEN: the workgroups behind the items' widen the step's long portions' keys on the way (kv4_tile.hip), which as a launch of its own would
+// wait for this one, 6 us of mostly waiting (5 tokens and 3 portions of 1100, heads of 64, window 512: 43 us apart, 39.6 together).
+template <int D, int NQ, int NW, int NB, bool WIDEN>
+__global__ __launch_bounds__(64 * NW, NQ == 1 ? 3 : 2) void attn_kernel(Args a, Widen wd) {
+  if constexpr (WIDEN) {
+    static_assert(NW == 4, "a wave a page");
+    if (blockIdx.x >= wd.from) {
+      widen_tile<D>(blockIdx.x - wd.from, a.kc, a.vc, a.n_pages, a.tables, a.ts, wd.tiles, a.Hkv, a.window, a.first, wd.ws);
+      return;
+    }
+  }
   constexpr int LD = D + 4;                                     // (16 lanes a quarter write 16 rows: other banks each)
   __shared__ float sO[NW][16][LD];
   __shared__ float sM[NW][16], sL[NW][16];
@@ -833,20 +848,22 @@ extern "C" hipError_t kafka_kv4_merge(const int* merges, int n_merges, int tile_
   return hipGetLastError();
 }
 
-// tiles of 16 nq rows, nw waves each
+// tiles of 16 nq rows, nw waves each; wtiles (four waves): what of the cache goes to ws beside them
 extern "C" hipError_t kafka_kv4_attn(const bf16* q, int64_t qs, const uint8_t* kc, const uint8_t* vc, int64_t n_pages, const int* tables,
-                                     int64_t ts, const int* items, int n_items, int nq, int nw, int T, int Hkv, int G, int D, int window, int first, float scale, bf16* out, int64_t os, float* lse,
-                                     float* part, float* plse, int* counters, hipStream_t st) {
+                                     int64_t ts, const int* items, int n_items, int nq, int nw, int T, int Hkv, int G, int D, int window,
+                                     int first, float scale, bf16* out, int64_t os, float* lse, float* part, float* plse, int* counters,
+                                     const int* wtiles, int n_wtiles, char* ws, hipStream_t st) {
   if (n_items == 0) return hipSuccess;
-  const int64_t wgs = (int64_t)Hkv * n_items;
-  if ((D != 64 && D != 128) || G < 1 || G > 16 || wgs >= 1 << 24) return hipErrorInvalidValue;
+  const int64_t wgs = (int64_t)Hkv * n_items, wws = (int64_t)Hkv * n_wtiles;
+  if ((D != 64 && D != 128) || G < 1 || G > 16 || wgs >= 1 << 24 || wws >= 1 << 24 || (n_wtiles && nw != 4)) return hipErrorInvalidValue;
   const Args a = make_args(q, qs, kc, vc, n_pages, tables, ts, items, T, Hkv, G, window, first, scale, out, os, lse, part, plse, counters);
-  auto go = [&](auto kern) { kern<<<(unsigned)wgs, 64 * nw, 0, st>>>(a); };
+  const Widen wd{wtiles, ws, (uint32_t)wgs};
+  auto go = [&](auto kern) { kern<<<(unsigned)(wgs + wws), 64 * nw, 0, st>>>(a, wd); };
   auto dim = [&](auto d) {
     constexpr int DD = decltype(d)::value;
-    if (nq == 1 && nw == 4) go(attn_kernel<DD, 1, 4, 2>);
-    else if (nq == 1 && nw == 8) go(attn_kernel<DD, 1, 8, 2>);
-    else if (nq == 2 && nw == 4) go(attn_kernel<DD, 2, 4, 2>);
+    if (nq == 1 && nw == 4) n_wtiles ? go(attn_kernel<DD, 1, 4, 2, true>) : go(attn_kernel<DD, 1, 4, 2, false>);
+    else if (nq == 1 && nw == 8) go(attn_kernel<DD, 1, 8, 2, false>);
+    else if (nq == 2 && nw == 4) n_wtiles ? go(attn_kernel<DD, 2, 4, 2, true>) : go(attn_kernel<DD, 2, 4, 2, false>);
     else return false;
     return true;
   };

@@ -18,7 +18,7 @@ hipError_t kafka_kv4_evict_copy(uint8_t* kc, uint8_t* vc, int64_t n_pages, const
                                 int N, float* new_mass, int D, hipStream_t st);
 hipError_t kafka_kv4_attn(const void* q, int64_t qs, const uint8_t* kc, const uint8_t* vc, int64_t n_pages, const int* tables, int64_t ts,
                           const int* items, int n_items, int nq, int nw, int T, int Hkv, int G, int D, int window, int first, float scale, void* out,
-                          int64_t os, float* lse, float* part, float* plse, int* counters, hipStream_t st);
+                          int64_t os, float* lse, float* part, float* plse, int* counters, const int* wtiles, int n_wtiles, char* ws, hipStream_t st);
 hipError_t kafka_kv4_tiles(const void* q, int64_t qs, const uint8_t* kc, const uint8_t* vc, int64_t n_pages, const int* tables, int64_t ts,
                            int rows, const int* items, int n_items, const int* wtiles, int n_wtiles, const int* merges, int n_merges, int T, int Hkv,
                            int G, int D, int window, int first, float scale, void* out, int64_t os, float* lse, float* part, float* plse,
@@ -195,9 +195,19 @@ Tensor attn(Tensor q, Tensor kc, Tensor vc, Tensor tables, const Plan& p, double
     out = p.covered == T ? at::empty({T, Hq, D}, q.options()) : at::zeros({T, Hq, D}, q.options());
   }
   float* lp = row_values(lse, q, kc);
+  // keys of long portions are widened beside the last launch of four waves before them, where there is one
+  const Part *wide = nullptr, *beside = nullptr;
   for (const Part& t : p.parts) {
     TORCH_CHECK_VALUE(t.items.device() == kc.device(), "kv4: the plan was made for another device");
-    Tensor part, ws, held;          // (the caching allocator orders them with the stream)
+    if (t.keys.size(0) > 0) wide = &t;
+    else if (!wide && t.waves == 4 && t.items.size(0) > 0) beside = &t;
+  }
+  Tensor ws;                        // (the caching allocator orders it with the stream)
+  if (wide) ws = at::empty({wide->keys.size(0) * H * 256 * D}, kc.options());
+  char* wp = wide ? reinterpret_cast<char*>(ws.data_ptr()) : nullptr;
+  if (!wide) beside = nullptr;
+  for (const Part& t : p.parts) {
+    Tensor part, held;
     float *pp = nullptr, *pl = nullptr;
     if (t.slots > 0) {
       const int64_t n = t.slots * H * t.rows;
@@ -210,13 +220,13 @@ Tensor attn(Tensor q, Tensor kc, Tensor vc, Tensor tables, const Plan& p, double
     if (t.keys.size(0) == 0) {
       KV4_HIP(kafka_kv4_attn(q.data_ptr(), q.stride(0), kc.data_ptr<uint8_t>(), vc.data_ptr<uint8_t>(), kc.size(0), tp, tables.stride(0), ip, ni,
                              (int)(t.rows / 16), (int)t.waves, (int)T, (int)H, (int)(Hq / H), D, (int)p.window, (int)p.first, (float)scale,
-                             out.data_ptr(), out.stride(0), lp, pp, pl, t.slots > 0 ? p.zeros(t.slots * H, held) : nullptr, stream()));
+                             out.data_ptr(), out.stride(0), lp, pp, pl, t.slots > 0 ? p.zeros(t.slots * H, held) : nullptr,
+                             &t == beside ? wide->keys.data_ptr<int>() : nullptr, &t == beside ? (int)wide->keys.size(0) : 0, wp, stream()));
     } else {
-      ws = at::empty({t.keys.size(0) * H * 256 * D}, kc.options());
       KV4_HIP(kafka_kv4_tiles(q.data_ptr(), q.stride(0), kc.data_ptr<uint8_t>(), vc.data_ptr<uint8_t>(), kc.size(0), tp, tables.stride(0),
-                              (int)t.rows, ip, ni, t.keys.data_ptr<int>(), (int)t.keys.size(0), mp, nm, (int)T, (int)H, (int)(Hq / H), D,
+                              (int)t.rows, ip, ni, t.keys.data_ptr<int>(), beside ? 0 : (int)t.keys.size(0), mp, nm, (int)T, (int)H, (int)(Hq / H), D,
                               (int)p.window, (int)p.first, (float)scale, out.data_ptr(), out.stride(0), lp, pp, pl,
-                              reinterpret_cast<char*>(ws.data_ptr()), stream()));
+                              wp, stream()));
     }
   }
   return out;

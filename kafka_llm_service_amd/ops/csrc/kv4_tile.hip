@@ -5,88 +5,16 @@
 // from there to LDS without a register or an address in between. The workspace is 4 bytes an element pair of K and V, written once and mostly
 // read from the last-level cache.
 #include "attn_tile.h"
-#include "kv4.h"
+#include "kv4_widen.h"
 
 namespace kafka {
 namespace kv4 {
 
-constexpr int TK = 64;                    // keys of a tile
-template <int D>
-struct Image {                            // of 64 keys and one head
-  static constexpr int PAGE_BYTES = PAGE * D * 2, KBYTES = TK * D * 2, BYTES = 2 * KBYTES;
-};
-
-// ---- widening -----------------------------------------------------------------------------------------------------------
-// A workgroup per tile and head, a wave per page: 16048 keys of 8 heads of 128, 83 MB, 15.5 us (5.4 TB/s, most of it into the last-level
-// cache). K: [page][d / 8][key][8], V: [page][d][16 keys: 0-3, 8-11, 4-7, 12-15], the two halves of
-// rows with d & 8 exchanged (attn_tile.h: reads of both without bank conflicts). Keys behind ``last`` become zeros, and whole pages of which
-// no row from ``pmin`` on sees a key (the table may name anything there); those of a page that is none no numbers. Tiles: table row,
-// block, last key, pmin.
 template <int D>
 __global__ __launch_bounds__(256) void widen_kernel(const uint8_t* __restrict__ kc, const uint8_t* __restrict__ vc, int64_t n_pages,
                                                     const int* __restrict__ tables, int64_t ts, const int* __restrict__ tiles, int Hkv,
                                                     int window, int first, char* __restrict__ ws) {
-  constexpr int KW = D / 32;               // words of K a lane: its quarter of a key
-  const int t = blockIdx.x / Hkv, h = blockIdx.x % Hkv;
-  const int* tl = tiles + 4 * (int64_t)t;
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, last = tl[2];
-  const int key0 = tl[1] * TK + w * PAGE;
-  char* kd = ws + ((int64_t)t * Hkv + h) * Image<D>::BYTES + w * Image<D>::PAGE_BYTES;
-  char* vd = kd + Image<D>::KBYTES;
-  const int o = lane & 15, c = lane >> 4;
-  const bool some = key0 <= last && (key0 + PAGE - 1 > tl[3] - window || key0 < first);
-  const int pid = some ? tables[tl[0] * ts + (key0 >> 4)] : 0;
-  const bool bad = pid < 0 || pid >= n_pages;
-  const int64_t at = ((int64_t)(bad ? 0 : pid) * Hkv + h) * Page<D>::BYTES;
-  {  // K: lane = (key, quarter of its elements)
-    uint32_t x[KW];
-    uint32_t e = kc[at + Page<D>::DATA + o * (D / 32) + c * (D / 32) / 4];
-#pragma unroll
-    for (int i = 0; i < KW; ++i) x[i] = *reinterpret_cast<const uint32_t*>(kc + at + o * (D / 2) + c * (D / 8) + 4 * i);
-    if (!some || key0 + o > last) {
-      e = 0;
-#pragma unroll
-      for (int i = 0; i < KW; ++i) x[i] = 0;
-    }
-    const float sc = bad ? __builtin_nanf("") : scale_of(e);
-#pragma unroll
-    for (int i = 0; i < KW; ++i) {
-      bf16x8 y = widen8(x[i], sc);
-      if (bad) {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) y[j] = (bf16)__builtin_nanf("");
-      }
-      *reinterpret_cast<bf16x8*>(kd + ((c * KW + i) * 16 + o) * 16) = y;
-    }
-  }
-  {  // V: lane = (four keys, D / 16 elements)
-    constexpr int W = D / 32;
-    const u32x4 d = *reinterpret_cast<const u32x4*>(vc + at + (c * (D / 8) + o * (D / 8) / 16) * 16);
-    const uint32_t s = *reinterpret_cast<const uint32_t*>(vc + at + Page<D>::DATA + (o * (D / 16) / 32) * 16 + c * 4);
-    uint32_t x[W][4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      uint32_t v = d[i], e = (s >> (8 * i)) & 255u;
-      if (D == 64) v >>= 16 * (o & 1);
-      if (!some || bad || key0 + 4 * c + i > last) v = 0, e = 0;
-      const float sc = scale_of(e);
-      x[0][i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(v, sc, 0));
-      x[1][i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(v, sc, 1));
-      if constexpr (D == 128) {
-        x[2][i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(v, sc, 2));
-        x[3][i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(v, sc, 3));
-      }
-    }
-#pragma unroll
-    for (int m = 0; m < W; ++m)
-#pragma unroll
-      for (int b = 0; b < 2; ++b) {
-        const uint32_t sel = b ? 0x07060302u : 0x05040100u;
-        const int row = (D / 16) * o + 2 * m + b;
-        u32x2 y = {__builtin_amdgcn_perm(x[m][1], x[m][0], sel), __builtin_amdgcn_perm(x[m][3], x[m][2], sel)};
-        *reinterpret_cast<u32x2*>(vd + row * 32 + (((c & 1) ^ ((row >> 3) & 1)) << 4) + (c >> 1) * 8) = y;
-      }
-  }
+  widen_tile<D>(blockIdx.x, kc, vc, n_pages, tables, ts, tiles, Hkv, window, first, ws);
 }
 
 // ---- attention ----------------------------------------------------------------------------------------------------------
@@ -360,7 +288,7 @@ using namespace kv4;
 extern "C" hipError_t kafka_kv4_merge(const int* merges, int n_merges, int tile_rows, int T, int Hkv, int G, int D, bf16* out, int64_t os,
                                       float* lse, float* part, float* plse, hipStream_t st);
 
-// items of 256 rows (D 128) or 128 (D 64); wtiles: what of the cache the workspace holds, tile after tile
+// items of 256 rows (D 128) or 128 (D 64); wtiles: what of the cache the workspace has to hold, tile after tile (none: it holds it already)
 extern "C" hipError_t kafka_kv4_tiles(const bf16* q, int64_t qs, const uint8_t* kc, const uint8_t* vc, int64_t n_pages, const int* tables,
                                       int64_t ts, int rows, const int* items, int n_items, const int* wtiles, int n_wtiles,
                                       const int* merges, int n_merges, int T, int Hkv, int G, int D, int window, int first, float scale, bf16* out, int64_t os,
@@ -371,10 +299,10 @@ extern "C" hipError_t kafka_kv4_tiles(const bf16* q, int64_t qs, const uint8_t* 
   const TileArgs a{q,  qs, ws, reinterpret_cast<const TileItem4*>(items), T, Hkv, G, window > 0 ? window : 1 << 30, first,
                    scale * 1.4426950408889634f, out, os, lse, part, plse};
   if (D == 128) {
-    widen_kernel<128><<<(unsigned)wws, 256, 0, st>>>(kc, vc, n_pages, tables, ts, wtiles, Hkv, a.window, first, ws);
+    if (n_wtiles) widen_kernel<128><<<(unsigned)wws, 256, 0, st>>>(kc, vc, n_pages, tables, ts, wtiles, Hkv, a.window, first, ws);
     tile_kernel<128, 8, 3><<<(unsigned)wgs, 512, 0, st>>>(a);
   } else {
-    widen_kernel<64><<<(unsigned)wws, 256, 0, st>>>(kc, vc, n_pages, tables, ts, wtiles, Hkv, a.window, first, ws);
+    if (n_wtiles) widen_kernel<64><<<(unsigned)wws, 256, 0, st>>>(kc, vc, n_pages, tables, ts, wtiles, Hkv, a.window, first, ws);
     tile_kernel<64, 4, 3><<<(unsigned)wgs, 256, 0, st>>>(a);
   }
   if (n_merges) return kafka_kv4_merge(merges, n_merges, rows, T, Hkv, G, D, out, os, lse, part, plse, st);
