@@ -38,12 +38,21 @@ struct TileArgs {
   float *lse, *part, *plse;
 };
 
+// The lane's number, where registers are few (heads of 64) counted where it is used: what is computed from one that the compiler knows stays in
+// registers through the loop, and a register too many there is a load from scratch, whose wait is one for all that is on its way to LDS
+// (8000 rows, 32/8 heads, 325 us for 288).
+template <int D>
+__device__ __forceinline__ int lane_again(int lane) {
+  if constexpr (D == 64) asm volatile("v_mbcnt_lo_u32_b32 %0, -1, 0\n\tv_mbcnt_hi_u32_b32 %0, -1, %0" : "=v"(lane));
+  return lane;
+}
+
 // NW waves of 32 rows each. A wave is a pipeline over tiles of keys: between the products of the next tile's keys stand the
 // exponentials of this one, between those of its values the rest of them and the next one's maxima, each product behind the LDS reads of the F
 // fragments after it; keys run a tile ahead of the values, and the slots that a step has read are filled again in its middle, behind one counted
 // wait and one barrier. The maximum is raised only where it has grown by more than 2^24 (sums of weights up to that are exact enough in fp32).
 // Products and exponentials bound it, in turn on the same issue slots: 8000 rows cold, 32/8 heads of 128, 1054 TFLOP/s (a large product of the
-// library 1379), of 64, which have half the products for an exponential, 759. Heads of 64: three workgroups of four waves a CU, of 128 one of
+// library 1379), of 64, which have half the products for an exponential, 879. Heads of 64: three workgroups of four waves a CU, of 128 one of
 // eight, whose ring of three slots (96 KiB) leaves no room for another. Below about 500 rows the tiles of 32 rows (kv4_attn.hip) are as fast.
 template <int D, int NW, int NSLOT>
 __global__ __launch_bounds__(64 * NW, D == 64 ? 3 : 1) void tile_kernel(TileArgs a) {
@@ -75,10 +84,10 @@ __global__ __launch_bounds__(64 * NW, D == 64 ? 3 : 1) void tile_kernel(TileArgs
   auto issue = [&](int g) {               // group g: the keys of index g, the values of g - 1
     char* kd = smem + (g % NSLOT) * KBYTES + w * (DPT / 2) * 1024;
     char* vd = smem + (NSLOT + (g + NSLOT - 1) % NSLOT) * KBYTES + w * (DPT / 2) * 1024;
-    const int at = w * (DPT / 2) * 1024;
+    const int at = w * (DPT / 2) * 1024, ln = lane_again<D>(lane);
     if (g < ntiles || g == 1)
-      dma_pieces<DPT / 2, 0>(reinterpret_cast<const bf16*>(image(min(g, ntiles - 1)) + at), 16 * lane, kd);
-    if (g > 0) dma_pieces<DPT / 2, 0>(reinterpret_cast<const bf16*>(image(g - 1) + KBYTES + at), 16 * lane, vd);
+      dma_pieces<DPT / 2, 0>(reinterpret_cast<const bf16*>(image(min(g, ntiles - 1)) + at), 16 * ln, kd);
+    if (g > 0) dma_pieces<DPT / 2, 0>(reinterpret_cast<const bf16*>(image(g - 1) + KBYTES + at), 16 * ln, vd);
   };
   f32x16 o[NT];
   float m = -INFINITY, ls[2] = {0.f, 0.f};              // (two sums: one's additions wait for each other)
@@ -98,8 +107,10 @@ __global__ __launch_bounds__(64 * NW, D == 64 ? 3 : 1) void tile_kernel(TileArgs
 #pragma unroll
     for (int g = 1; g < NSLOT; ++g)
       if (g <= ntiles) issue(g);
-    const char* const Kl = smem + (r >> 4) * PB + (h * 16 + (r & 15)) * 16;
-    const char* const Vl = smem + NSLOT * KBYTES + r * 32 + 16 * (h ^ ((r >> 3) & 1));
+    int kl = (r >> 4) * PB + (h * 16 + (r & 15)) * 16, vl = NSLOT * KBYTES + r * 32 + 16 * (h ^ ((r >> 3) & 1));
+    if (D == 64) asm volatile("" : "+v"(kl), "+v"(vl));  // (a register each, not one for every summand)
+    const char* const Kl = smem + kl;
+    const char* const Vl = smem + vl;
     bf16x8 fr[F];
     f32x16 sa[2], sb[2];
     auto kfrag = [&](const char* k, int f) { return *reinterpret_cast<const bf16x8*>(k + (f & 1) * 2 * PB + (f >> 1) * 512); };
@@ -112,9 +123,10 @@ __global__ __launch_bounds__(64 * NW, D == 64 ? 3 : 1) void tile_kernel(TileArgs
       for (int kb = 0; kb < 2; ++kb) {
         const int k0 = key0 + 32 * kb;
         if ((k0 + 31 > wmin) | ((k0 <= wmax - a.window) & (k0 + 32 > a.first))) {
+          const int k1 = k0 + 4 * (lane_again<D>(lane) >> 5);
 #pragma unroll
           for (int e = 0; e < 16; ++e) {
-            const int key = k0 + (e & 3) + 8 * (e >> 2) + 4 * h;
+            const int key = k1 + (e & 3) + 8 * (e >> 2);
             if (!(key <= limit && (key > limit - a.window || key < a.first))) s[kb][e] = -INFINITY;
           }
         }
@@ -235,22 +247,24 @@ __global__ __launch_bounds__(64 * NW, D == 64 ? 3 : 1) void tile_kernel(TileArgs
     step(std::true_type{}, j, sa, sb);
   }
   const float sum = t3_xor32_sum(ls[0] + ls[1]);
+  const int l2 = lane_again<D>(lane);
+  const int r2 = l2 & 31, h2 = l2 >> 5, R2 = 32 * w + r2, tok2 = R2 / a.G, head2 = kvh * a.G + (R2 - tok2 * a.G);
   // ---- rows, through LDS so that whole cache lines are stored
   __syncthreads();                                     // (every wave has read the last keys and values)
   const float inv = sum == 0.f ? 0.f : 1.f / sum, lse = sum == 0.f ? -INFINITY : m + log2f(sum);
-  const int64_t prow = ((int64_t)max(it.slot, 0) * a.Hkv + kvh) * (32 * NW) + R;
-  if (valid && h == 0) {
+  const int64_t prow = ((int64_t)max(it.slot, 0) * a.Hkv + kvh) * (32 * NW) + R2;
+  if (tok2 < it.tokens && h2 == 0) {
     if (it.slot >= 0) a.plse[prow] = lse;
-    else if (a.lse) a.lse[(int64_t)(it.row + tok) * Hq + head] = lse;
+    else if (a.lse) a.lse[(int64_t)(it.row + tok2) * Hq + head2] = lse;
   }
   char* slab = smem + w * 4096;                        // 32 rows of 128 bytes
-  const int cc = lane & 7, nvalid = it.tokens * a.G - 32 * w;
+  const int cc = l2 & 7, nvalid = it.tokens * a.G - 32 * w;
 #pragma unroll
   for (int rd = 0; rd < NT; ++rd) {                    // 32 columns of fp32, or every second time 64 of bf16
     if (it.slot >= 0) {
 #pragma unroll
       for (int i4 = 0; i4 < 4; ++i4)
-        *reinterpret_cast<f32x4*>(slab + r * 128 + 16 * ((2 * i4 + h) ^ (r & 7))) =
+        *reinterpret_cast<f32x4*>(slab + r2 * 128 + 16 * ((2 * i4 + h2) ^ (r2 & 7))) =
             f32x4{o[rd][4 * i4] * inv, o[rd][4 * i4 + 1] * inv, o[rd][4 * i4 + 2] * inv, o[rd][4 * i4 + 3] * inv};
     } else {
 #pragma unroll
@@ -258,7 +272,7 @@ __global__ __launch_bounds__(64 * NW, D == 64 ? 3 : 1) void tile_kernel(TileArgs
         bf16x4 v;
 #pragma unroll
         for (int j = 0; j < 4; ++j) v[j] = (bf16)(o[rd][4 * i4 + j] * inv);
-        *reinterpret_cast<bf16x4*>(slab + r * 128 + 16 * ((4 * (rd & 1) + i4) ^ (r & 7)) + 8 * h) = v;
+        *reinterpret_cast<bf16x4*>(slab + r2 * 128 + 16 * ((4 * (rd & 1) + i4) ^ (r2 & 7)) + 8 * h2) = v;
       }
       if (!(rd & 1)) continue;
     }
@@ -266,14 +280,14 @@ __global__ __launch_bounds__(64 * NW, D == 64 ? 3 : 1) void tile_kernel(TileArgs
     __builtin_amdgcn_wave_barrier();
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
-      const int row = (lane >> 3) + 8 * k;
+      const int row = (l2 >> 3) + 8 * k;
       const f32x4 v = *reinterpret_cast<const f32x4*>(slab + row * 128 + 16 * (cc ^ (row & 7)));
       if (row < nvalid) {
-        const int R2 = 32 * w + row, tok2 = R2 / a.G, head2 = kvh * a.G + R2 - tok2 * a.G;
+        const int R3 = 32 * w + row, tok3 = R3 / a.G, head3 = kvh * a.G + R3 - tok3 * a.G;
         if (it.slot >= 0)
-          *reinterpret_cast<f32x4*>(a.part + (((int64_t)it.slot * a.Hkv + kvh) * (32 * NW) + R2) * D + 32 * rd + 4 * cc) = v;
+          *reinterpret_cast<f32x4*>(a.part + (((int64_t)it.slot * a.Hkv + kvh) * (32 * NW) + R3) * D + 32 * rd + 4 * cc) = v;
         else
-          *reinterpret_cast<f32x4*>(a.out + (int64_t)(it.row + tok2) * a.os + (int64_t)head2 * D + 32 * (rd - 1) + 8 * cc) = v;
+          *reinterpret_cast<f32x4*>(a.out + (int64_t)(it.row + tok3) * a.os + (int64_t)head3 * D + 32 * (rd - 1) + 8 * cc) = v;
       }
     }
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");

@@ -129,7 +129,7 @@ def _wide(full: np.ndarray, heads: int, kv_heads: int, dim: int, window: int, fi
     """Which segments are taken in wide tiles whose keys are widened first: none or all of MANY_MIN rows or more, by the microseconds that
     both ways take. Measured (32/8 heads of 128 / 64/8 heads of 128 / 24/8 heads of 64): 512 rows cold 21 against 14 with tiles of 32 rows / 25
     against 25 / 17 against 10, 300 rows behind 1000 keys 24 against 23 / 31 against 33 / 18 against 14, 8 portions of 200 cold 20 against
-    35 / - / -, three of 1100 behind 900 in a window of 512 75 against 99 / - / 43 against 61."""
+    35 / - / -, three of 1100 behind 900 in a window of 512 75 against 99 / - / 38 against 61."""
     G = heads // kv_heads
     wide = full[:, 1] * G >= MANY_MIN
     part = full[wide]
@@ -139,10 +139,10 @@ def _wide(full: np.ndarray, heads: int, kv_heads: int, dim: int, window: int, fi
             return len(t) * kv_heads, int(_blocks(t[:, 2], t[:, 1], window, first)[1].sum()) * kv_heads
 
         wgs, blocks = work(SOME_ROWS)
-        few = 7. * max(1., wgs / 512) + blocks * dim / 128 * 0.9 / 512     # rounds of workgroups, and blocks
+        few = 7. * max(1., wgs / 512) + blocks * (0.9 if dim == 128 else 0.8) / 512     # rounds of workgroups, and blocks
         wgs, blocks = work(MANY_ROWS[dim])
         keys = int(_blocks(part[:, 2], part[:, 1], window, first)[1].sum()) * BLOCK * kv_heads
-        many = MANY_COST + blocks * dim / 128 * 2.1 / 256 + keys * dim * 5 / 4.5e6
+        many = MANY_COST + blocks * (2.1 if dim == 128 else 0.8) / 256 + keys * dim * 5 / 4.5e6
         if few <= many:
             wide[:] = False
     return wide
