@@ -586,9 +586,10 @@ __device__ __forceinline__ void of_rows(T x, T (&y)[4], int lane) {
 
 // Segments of at most 16 rows: four waves take every fourth block of an item's (at most 32), NB of them in registers. What a key had before
 // comes with it: a load that is asked for when its sum is there holds up those of the next keys. Bytes bound it, and the start and
-// end of workgroups of 28 blocks: 29 threads of 7900 tokens, 8 heads of 128, 140 MB, 35 us, 4.0 TB/s.
+// end of workgroups of 28 blocks: 29 threads of 7900 tokens, 8 heads of 128, 140 MB, 31 us, 4.5 TB/s (three blocks in registers
+// and a wave a SIMD less 35).
 template <int D, int NB>
-__global__ __launch_bounds__(256, 4) void mass_few_kernel(MassArgs ma) {
+__global__ __launch_bounds__(256, 5) void mass_few_kernel(MassArgs ma) {
   const Args& a = ma.a;
   const int* it = reinterpret_cast<const int*>(a.items) + 8 * (blockIdx.x / a.Hkv);
   const int row = it[0], rows = it[1], pos = it[2], table = it[3], seg = it[4], end = it[6];
@@ -886,9 +887,9 @@ extern "C" hipError_t kafka_kv4_mass(const bf16* q, int64_t qs, const float* lse
   if (n_few) {
     const MassArgs m = args(few);
     if (D == 128)
-      mass_few_kernel<128, 3><<<Hkv * n_few, 256, 0, st>>>(m);
+      mass_few_kernel<128, 2><<<Hkv * n_few, 256, 0, st>>>(m);
     else
-      mass_few_kernel<64, 3><<<Hkv * n_few, 256, 0, st>>>(m);
+      mass_few_kernel<64, 2><<<Hkv * n_few, 256, 0, st>>>(m);
   }
   if (n_many) {
     const MassArgs m = args(many);
