@@ -344,8 +344,8 @@ __device__ __forceinline__ void join(float& M, float& L, f32x4& o, const float (
 
 // NW waves take a tile of 16 NQ rows, every NW-th block each; their results meet in LDS. A wave has NB half blocks in registers: one that it
 // works on, the others on their way. (The loop's first form fetches without a condition, so that the waits count what is on its way.)
-// Three waves a SIMD: with whole blocks, or three halves, registers leave room for two (64 threads of 4100 tokens 65 us for 56). NQ 2, short portions: values are
-// widened once for 32 rows; 4 portions of 100 rows behind 1000 keys, 32/8 heads of 128, 23 us, of one tile of 256 widened first 31.
+// Three waves a SIMD with two half blocks each: 64 threads of 4100 tokens and 29 of 7900 56.7 and 56.7 us, three halves 57.2 and 57.6, two waves with
+// four 58.0 and 57.1, four with one 57.6 and 61.3. NQ 2, short portions: values are widened once for 32 rows; 4 portions of 100 rows behind 1000 keys, 32/8 heads of 128, 23 us, of one tile of 256 widened first 31.
 // WIDEN: the workgroups behind the items' widen the step's long portions' keys on the way (kv4_tile.hip), which as a launch of its own would
 // wait for this one, 6 us of mostly waiting (5 tokens and 3 portions of 1100, heads of 64, window 512: 43 us apart, 39.6 together).
 template <int D, int NQ, int NW, int NB, bool WIDEN>
