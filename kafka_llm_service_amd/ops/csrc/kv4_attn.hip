@@ -596,21 +596,22 @@ __global__ __launch_bounds__(256, 5) void mass_few_kernel(MassArgs ma) {
   const int row = it[0], rows = it[1], pos = it[2], table = it[3], seg = it[4], end = it[6];
   const int h = blockIdx.x % a.Hkv, lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int c = lane >> 4, last = pos + rows - 1, b0 = it[5] + w;
-  if (row < 0 || rows < 0 || row + rows > a.T || rows * a.G > 16 || end - it[5] > 32 || b0 >= end) return;
-  const Blocks list(pos, last, a.window, a.first);
-  // blocks that no row sees give nothing: behind the last key, between the first ones and the window
-  auto seen = [&](int b) { return rows > 0 && b * KB <= last && (b < list.head || b >= list.tail); };
+  if (end - it[5] > 32 || b0 >= end) return;
   const int64_t at = ((int64_t)seg * a.Hkv + h) * ma.N;
   float* out = ma.out + at;
   const float* base = ma.base ? ma.base + at : out;
   const int n = (end - b0 + 3) / 4;
-  if (rows == 0) {
+  if (rows == 0) {                                         // (of a segment without rows the first one may be any)
     for (int k = 0; k < n; ++k) {
       const int key = (b0 + 4 * k) * KB + lane;
       if (key < ma.N) out[key] = ma.base ? base[key] : 0.f;
     }
     return;
   }
+  if (row < 0 || rows < 0 || row + rows > a.T || rows * a.G > 16) return;
+  const Blocks list(pos, last, a.window, a.first);
+  // blocks that no row sees give nothing: behind the last key, between the first ones and the window
+  auto seen = [&](int b) { return b * KB <= last && (b < list.head || b >= list.tail); };
   const PageIds id(a.tables + table * a.ts, pos, last, a.window, a.first, lane, [&](int i) { return b0 + 4 * min(i, 7); });
   bool bad[NB];
   KFrag<4> kf[NB];

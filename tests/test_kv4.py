@@ -947,3 +947,32 @@ def test_split_tiles_side_by_side(cuda, monkeypatch, wide):
     torch.cuda.synchronize()
     for outs in eager + [r[1] for r in runs]:
         assert all(torch.equal(x, y) for x, y in zip(outs, want))
+
+
+# ---- segments without rows beside others ----------------------------------------------------------------------------------
+def _empty_beside(device):
+    """A segment without rows, wherever its first row would be, gives its keys nothing: they keep what they had."""
+    for segs, T in (([(0, 1, 0, 0), (5, 0, 0, 1)], 1), ([(900, 0, 77, 1), (0, 40, 100, 0), (40, 0, 3, 0), ((1 << 26) - 1, 0, 0, 2)], 40)):
+        kc, vc, tables = world(segs, 2, 128, 0, device)
+        q, lse = queries(T, 8, 128, 1, device), torch.zeros(T, 8, device=device)
+        full = [s for s in segs if s[1]]
+        plan, alone = (kv4.attn_plan(x, 8, 2, 128, device=device) for x in (segs, full))
+        out = kv4.attn(q, kc, vc, tables, plan, 0.1, lse=lse)
+        assert torch.equal(out, kv4.attn(q, kc, vc, tables, alone, 0.1))
+        want = torch.zeros(len(segs), 2, plan.keys, device=device)
+        want[[i for i, s in enumerate(segs) if s[1]]] = kv4.attn_mass(q, lse, kc, tables, alone, 0.1)
+        got = torch.full_like(want, 5.0)
+        assert kv4.attn_mass(q, lse, kc, tables, plan, 0.1, out=got) is got and torch.equal(got, want)
+        base = torch.rand(want.shape, generator=torch.Generator().manual_seed(3)).to(device)
+        got = torch.full_like(want, 5.0)
+        kv4.attn_mass(q, lse, kc, tables, plan, 0.1, base=base, out=got)
+        assert torch.equal(got, base + want)
+
+
+def test_empty_segments_beside_others_reference():
+    _empty_beside("cpu")
+
+
+@pytest.mark.gpu
+def test_empty_segments_beside_others_on_the_gpu(cuda):
+    _empty_beside(cuda)
