@@ -93,8 +93,8 @@ def read(k_cache, v_cache, slots):
 
 
 def gather(k_cache, v_cache, table, n: int, seen=None):
-    """fp32 K, V [n, heads, D] of a sequence's first n keys (no numbers where the table names a page outside of the cache); of pages
-    without a key that is ``seen``, bool [n], anything."""
+    """fp32 K, V [n, heads, D] of a sequence's first n keys (where the table names a page outside of the cache K is no numbers and V zeros,
+    so that rows in front of it, whose weights there are zero, stay numbers); of pages without a key that is ``seen``, bool [n], anything."""
     ids = table[:(n + PAGE - 1) // PAGE].long()
     if seen is not None:
         pages = torch.nn.functional.pad(seen, (0, -n % PAGE)).view(-1, PAGE).any(1)
@@ -103,7 +103,7 @@ def gather(k_cache, v_cache, table, n: int, seen=None):
     out = []
     for c, value in ((k_cache, False), (v_cache, True)):
         x = values(*unpack(c[torch.where(there, ids, torch.zeros_like(ids))], value))
-        x[~there] = math.nan
+        x[~there] = 0.0 if value else math.nan
         if seen is not None:
             x[~pages] = 0.0
         out.append(x.transpose(1, 2).flatten(0, 1)[:n])
