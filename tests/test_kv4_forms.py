@@ -1,9 +1,163 @@
-"""The 4-bit cache's kernels form by form: pages that are none in every kind of tile."""
+"""The 4-bit cache's kernels form by form: loops as deep as long sequences make them, scores without the 4-bit product's cut, pages
+that are none in every kind of tile.
+
+Tolerances of ``_sharp``: each query has one element in every eight neighbours, of at most two bits of mantissa and within a factor of
+four of each other, so that every form of the kernels takes it exactly (in e4m3 as well), a group of eight products is one exact
+number, and nothing of it is cut. A score is then a sum of D / 8 exact numbers in fp32 and a product by the scale; with an addition that cuts
+instead of rounding, 2^-23 of A = the largest sum_d |scale q_d k_d| of a row for each, S = 2 (D / 8 + 4) 2^-24 A bounds its error. The
+exponential and its argument add 2^-22 (1 + A): EW = 2 (S + 2^-22 (1 + A)) bounds a weight's relative error with its sum's. lse is off by
+(EW + n 2^-24) / ln 2 and its own rounding, a key's weight from R rows by 2 EW + (n + R + 2) 2^-24 + 2^-22 (1 + |lse|) of itself; keys that no
+row sees have received exactly nothing. The output has P in bf16 and its own rounding: (2^-8 + EW + n 2^-24) sum w |v| + 2^-8 |o|."""
+import math
+
+import numpy as np
 import pytest
 import torch
 
+from kafka_llm_service_amd import ops
 from kafka_llm_service_amd.ops import kv4
-from test_kv4 import queries, world
+from kafka_llm_service_amd.ops import kv4_reference as kref
+from kafka_llm_service_amd.ops import reference as ref
+from test_kv4 import CASES, _check_attention, _id, numbers, queries, within, world
+
+
+# ---- deep loops -----------------------------------------------------------------------------------------------------------
+def _one_piece(monkeypatch, waves=0):
+    """Plans whose tiles are taken in one piece each, those of single tokens by 4 or 8 waves."""
+    monkeypatch.setattr(kv4, "CUS", 1)
+    monkeypatch.setattr(kv4, "LEAST_SHARE", 0)
+    monkeypatch.setattr(kv4, "SHORT_TILE", 1 << 40 if waves == 4 else 0)
+    monkeypatch.setattr(kv4, "SOME_PIECE", 1 << 40)
+    monkeypatch.setattr(kv4, "MANY_BLOCKS", 1 << 40)
+    monkeypatch.setattr(kv4, "MASS_WGS", 1)
+    monkeypatch.setattr(kv4, "MASS_MANY_WGS", 1)
+
+
+def _items(case):
+    Hq, H, D, segs, window, first = case
+    p, a = kv4._plan(segs, Hq, H, D, window, first)
+    shapes, arrays = kv4._tables(a[a[:, 1] > 0], Hq, H, D, window, first)
+    return shapes, arrays, kv4._mass_tables(a, Hq // H, H, p.keys, window, first)
+
+
+#: single tokens: (waves, case); of 4 and 8 waves, more than 16 and more than 32 blocks a wave
+TOKENS = [(4, (4, 2, 128, [(0, 1, 8700, 0), (1, 1, 4500, 1), (2, 1, 100, 2)], 0, 0)),
+          (4, (8, 1, 64, [(0, 1, 8500, 0), (1, 1, 4300, 1)], 0, 0)),
+          (4, (4, 1, 128, [(0, 1, 9000, 0), (1, 2, 4444, 1)], 4300, 130)),
+          (8, (4, 1, 128, [(0, 1, 17000, 0), (1, 1, 9000, 1)], 0, 0)),
+          (8, (2, 1, 64, [(0, 1, 16999, 0), (1, 1, 700, 1)], 0, 0)),
+          (8, (3, 1, 64, [(0, 3, 12000, 0)], 9000, 20))]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("waves,case", TOKENS, ids=lambda x: _id(x) if isinstance(x, tuple) else f"{x}waves")
+def test_single_tokens_of_long_sequences(cuda, monkeypatch, waves, case):
+    _one_piece(monkeypatch, waves)
+    shapes, (items, *_), (few, many, _) = _items(case)
+    assert [s[:3] for s in shapes] == [(16, waves, 0)]
+    assert max(hi - lo for *_, lo, hi, _, _ in items.tolist()) > 16 * waves
+    if not case[4]:
+        assert max(hi - lo for *_, lo, hi, _, _ in items.tolist()) > 32 * waves
+    sizes = sorted({it[6] - it[5] for it in few.tolist()})
+    assert sizes[-1] == 32 and not len(many)                  # (eight blocks a wave, and the rest)
+    _check_attention(case, cuda)
+
+
+#: short portions: tiles of 32 rows, four waves
+SHORT = [(4, 1, 128, [(0, 9, 8300, 0), (9, 5, 4500, 1)], 0, 0), (4, 2, 64, [(0, 17, 8260, 0)], 0, 0), (5, 1, 64, [(0, 13, 9000, 0)], 4600, 130),
+         (4, 1, 128, [(0, 20, 7000, 0)], 5000, 4)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("case", SHORT, ids=_id)
+def test_short_portions_behind_long_histories(cuda, monkeypatch, case):
+    monkeypatch.setattr(kv4, "MANY_COST", 1e9)
+    _one_piece(monkeypatch)
+    shapes, (items, *_), _ = _items(case)
+    assert [s[:3] for s in shapes] == [(32, 4, 0)]
+    assert max(hi - lo for *_, lo, hi, _, _ in items.tolist()) > (16 if case[4] else 32) * 4
+    _check_attention(case, cuda)
+
+
+#: long portions: tiles of keys an item sees, odd and even numbers of them
+LONG = [(4, 1, 128, [(0, 200, 1000, 0)], 0, 0), (4, 1, 128, [(0, 150, 1100, 0)], 0, 0), (4, 1, 64, [(0, 100, 1000, 0), (100, 70, 1500, 1)], 0, 0),
+        (8, 2, 64, [(0, 70, 1230, 0)], 900, 70), (3, 1, 128, [(0, 190, 1300, 0)], 1000, 100)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("case", LONG, ids=_id)
+def test_long_portions_in_one_piece(cuda, monkeypatch, case):
+    monkeypatch.setattr(kv4, "MANY_COST", -1e9)
+    _one_piece(monkeypatch)
+    shapes, (items, *_), (_, many, slots) = _items(case)
+    assert [s[0] for s in shapes] == [kv4.MANY_ROWS[case[2]]] and shapes[0][2] == 0
+    sizes = {it[7] - it[6] for it in items.tolist()}
+    assert min(sizes) > 8 and {n % 2 for n in sizes} == {0, 1}
+    assert slots == 0 and len(many)
+    _check_attention(case, cuda)
+
+
+# ---- scores without a cut -------------------------------------------------------------------------------------------------
+def _sparse(T, Hq, D, seed=2):
+    g = torch.Generator().manual_seed(seed)
+    size = torch.tensor([1.0, 1.5, 2.0, 3.0])[torch.randint(0, 4, (T, Hq, D // 8), generator=g)]
+    size *= torch.randint(0, 2, size.shape, generator=g) * 2 - 1
+    q = torch.zeros(T, Hq, D // 8, 8)
+    return q.scatter_(-1, torch.randint(0, 8, size.shape, generator=g)[..., None], size[..., None]).flatten(-2).bfloat16()
+
+
+def _sharp(case, device):
+    Hq, H, D, segs, window, first = case
+    G = Hq // H
+    kc, vc, tables = world(segs, H, D, 5, device)
+    T = max(s[0] + s[1] for s in segs)
+    q, scale = _sparse(T, Hq, D), 0.25
+    plan = kv4.attn_plan(segs, Hq, H, D, window, first, device)
+    lse = torch.empty(T, Hq, device=device)
+    out = kv4.attn(q.to(device), kc, vc, tables, plan, scale, lse=lse).cpu()
+    mass = kv4.attn_mass(q.to(device), lse, kc, tables, plan, scale).cpu().double()
+    lse, kc, vc, tables = lse.cpu(), kc.cpu(), vc.cpu(), tables.cpu()
+    for i, (t0, rows, p0, tr) in enumerate(segs):
+        if not rows:
+            assert (mass[i] == 0).all()
+            continue
+        n = p0 + rows
+        ids = tables[tr, :(n + 15) // 16].long()
+        k, v = (numbers(c[ids], val).transpose(1, 2).flatten(0, 1)[:n] for c, val in ((kc, False), (vc, True)))
+        back = p0 + torch.arange(rows)[:, None] - torch.arange(n)[None]
+        see = (back >= 0) & ((back < window) | (torch.arange(n) < first)[None]) if window else back >= 0
+        for h in range(H):
+            want, bound = torch.zeros(n, dtype=torch.float64), torch.zeros(n, dtype=torch.float64)
+            for g in range(h * G, (h + 1) * G):
+                x = q[t0:t0 + rows, g].double()
+                s = (x @ k[:, h].T * scale).masked_fill(~see, -math.inf)
+                A = (x.abs() @ k[:, h].abs().T * scale).masked_fill(~see, 0).amax(-1, keepdim=True)
+                EW = 2 * (2 * (D // 8 + 4) * 2.0 ** -24 * A + 2.0 ** -22 * (1 + A))
+                ls = torch.logsumexp(s, -1, keepdim=True)
+                w = torch.exp(s - ls)
+                o = w @ v[:, h]
+                within(out[t0:t0 + rows, g], o, (2.0 ** -8 + EW + n * 2.0 ** -24) * (w @ v[:, h].abs()) + 2.0 ** -8 * o.abs(), "out")
+                within(lse[t0:t0 + rows, g], ls[:, 0] / math.log(2), ((EW + n * 2.0 ** -24) / math.log(2) + 2.0 ** -23 * (1 + ls.abs()))[:, 0], "lse")
+                want += w.sum(0)
+                bound += (w * (2 * EW + (n + rows * G + 2) * 2.0 ** -24 + 2.0 ** -22 * (1 + ls.abs()))).sum(0)
+            within(mass[i, h, :n], want, bound + 2.0 ** -120, "mass")
+            unseen = ~see.any(0)
+            assert (mass[i, h, :n][unseen] == 0).all() and (mass[i, h, n:] == 0).all()
+            # (no bound hides a bias: it is below a thousandth of every weight of an ordinary size)
+            assert (bound <= 1e-3 * want)[~unseen & (want > 1e-30)].all()
+
+
+@pytest.mark.parametrize("case", CASES, ids=_id)
+def test_sharp_scores_reference(case):
+    _sharp(case, "cpu")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("wide", [False, True])
+@pytest.mark.parametrize("case", CASES, ids=_id)
+def test_sharp_scores_on_the_gpu(cuda, monkeypatch, case, wide):
+    monkeypatch.setattr(kv4, "MANY_COST", -1e9 if wide else 1e9)
+    _sharp(case, cuda)
 
 
 # ---- pages that are none, in every kind of tile ---------------------------------------------------------------------------
@@ -43,3 +197,108 @@ def test_bad_pages_of_portions_reference(D, rows):
 def test_bad_pages_of_portions_on_the_gpu(cuda, monkeypatch, D, rows, cost):
     monkeypatch.setattr(kv4, "MANY_COST", cost)
     _bad_portions(cuda, D, rows)
+
+
+# ---- writer: sums of slabs that are no numbers ----------------------------------------------------------------------------
+@pytest.mark.gpu
+@pytest.mark.parametrize("T,Hq,H,D,slab", [(33, 4, 4, 64, 2), (5, 32, 8, 128, 4), (3, 3, 1, 128, 1)])
+def test_writer_of_slabs_with_infinities(cuda, T, Hq, H, D, slab):
+    """As the plain form: not a number (also the sum of two infinities) is stored as zero, an infinity as the largest."""
+    g = torch.Generator().manual_seed(4)
+    x = torch.randn(slab, T, (Hq + 2 * H) * D, generator=g)
+    flat = x.view(-1)
+    flat[::97], flat[5::301], flat[9::307], flat[3::11] = math.inf, -math.inf, math.nan, 3e38
+    pos, slots = torch.arange(T) * 7, torch.randperm(T + 20, generator=g)[:T]
+    cs = ref.rope_cos_sin(1024, D, 500000.0)
+    shape, _, dt = ops.kv_cache_shapes((T + 35) // 16, H, D, "mx4")
+    got = []
+    for dev in ("cpu", cuda):
+        q = torch.zeros(T, Hq, D, dtype=torch.bfloat16, device=dev)
+        kc, vc = torch.zeros(shape, dtype=dt, device=dev), torch.zeros(shape, dtype=dt, device=dev)
+        ops.rope_kv_write(x.to(dev), pos.to(dev), cs.to(dev), q, kc, vc, slots.to(dev), Hq, H)
+        got.append((q.cpu(), numbers(kc.cpu(), False), numbers(vc.cpu(), True)))
+    (qa, ka, va), (qb, kb, vb) = got
+    nan = qa.isnan()
+    assert nan.any() and torch.equal(nan, qb.isnan()) and torch.equal(qa[~nan], qb[~nan])
+    assert torch.equal(ka, kb) and torch.equal(va, vb) and ka.isfinite().all() and va.isfinite().all() and float(va.abs().max()) > 1e38
+
+
+# ---- engine ---------------------------------------------------------------------------------------------------------------
+def _dense4(model, tokens):
+    """Logits of the dense model in its own type whose keys and values stand for what the cache holds of them, experts one by one."""
+    from kafka_llm_service_amd.models import oracle as orc
+    from kafka_llm_service_amd.models.moe import route
+
+    cfg, D, hq, hkv = model.cfg, model.D, model.hq, model.hkv
+    t = torch.tensor(tokens, device=model.device)
+    T = t.shape[0]
+    cs = model.cos_sin[:T].float()
+    h = model.embed[t]
+    see = torch.ones(T, T, dtype=torch.bool, device=h.device).tril()
+    four = lambda x: kref.values(*kref.quant(x))
+    glu = lambda x, w13, w2: orc._lin((torch.nn.functional.silu((gu := orc._lin(x, w13).float())[:, :gu.shape[1] // 2]) * gu[:, gu.shape[1] // 2:]).to(x.dtype), w2)
+    for lw in model.layers:
+        qkv = orc._lin(orc._rms(h, lw.input_norm, cfg.rms_norm_eps), lw.qkv).view(T, hq + 2 * hkv, D)
+        q, k, v = orc._rope(qkv[:, :hq], cs).float(), four(orc._rope(qkv[:, hq:hq + hkv], cs)), four(qkv[:, hq + hkv:])
+        o = torch.empty(T, hq, D, device=h.device)
+        for x in range(hq):
+            s = (q[:, x] @ k[:, x * hkv // hq].T.contiguous() * model.scale).masked_fill(~see, -math.inf)
+            o[:, x] = torch.softmax(s, -1) @ v[:, x * hkv // hq].contiguous()
+        h = (h.float() + orc._lin(o.view(T, -1).to(h.dtype), lw.o).float()).to(h.dtype)
+        x = orc._rms(h, lw.post_norm, cfg.rms_norm_eps)
+        if lw.router is None:
+            delta = glu(x, lw.gate_up, lw.down).float()
+        else:
+            w, e = route(orc._lin(x, lw.router), cfg.num_experts_per_tok)
+            delta = torch.zeros(T, x.shape[1], device=h.device)
+            for j in range(cfg.num_experts):
+                rows = (e == j).any(-1).nonzero().flatten()
+                if rows.numel():
+                    delta[rows] += glu(x[rows], lw.w13[j], lw.w2[j]).float() * (w * (e == j))[rows].sum(-1, keepdim=True)
+        h = (h.float() + delta.to(h.dtype).float()).to(h.dtype)
+    return orc._lin(orc._rms(h, model.final_norm, cfg.rms_norm_eps), model.lm_head).float()[:, :cfg.vocab_size]
+
+
+def _served(model, device, gap, **kw):
+    """Threads that decode while long new prompts come in: every greedy token within ``gap`` of the dense form's best."""
+    from kafka_llm_service_amd.engine.engine import EngineConfig, LLMEngine
+    from kafka_llm_service_amd.engine.sequence import SamplingParams
+
+    if torch.device(device).type == "cuda":                   # (rows that nobody writes are no numbers)
+        junk = [torch.full((1 << 26,), math.nan, device=device) for _ in range(4)]
+        del junk
+    eng = LLMEngine(EngineConfig(model=model, device=device, num_kv_blocks=1024, max_model_len=4096, kv_dtype="mx4", **kw))
+    g = torch.Generator().manual_seed(13)
+    draw = lambda n: torch.randint(0, 5000, (n,), generator=g).tolist()
+    sp = SamplingParams(temperature=0.0, max_tokens=8, ignore_eos=True)
+    prompts = [draw(n) for n in (40, 9, 77, 130, 150, 181)]
+    seqs = [eng.add_request(f"a{i}", p, sp) for i, p in enumerate(prompts[:3])]
+    rows = set()
+    for i, p in enumerate(prompts[3:]):
+        for _ in range(2):
+            eng.step()
+            rows |= {(st["T"], st["B"]) for st in eng.runner.recent_stats}
+        seqs.append(eng.add_request(f"b{i}", p, sp))
+    while any(not s.finished for s in seqs):
+        eng.step()
+        rows |= {(st["T"], st["B"]) for st in eng.runner.recent_stats}
+    for p, s in zip(prompts, seqs):
+        lg = _dense4(eng.model, p + s.output_ids).cpu()
+        assert len(s.output_ids) == 8
+        for i, tok in enumerate(s.output_ids):
+            row = lg[len(p) - 1 + i]
+            assert (row.max() - row[tok]).item() < gap, f"token {i}: gap {(row.max() - row[tok]).item():.3f}"
+    return rows
+
+
+def test_engine_with_experts_cpu():
+    _served("tiny-mixtral", "cpu", 0.15)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("mode", ["auto", "blas"])
+@pytest.mark.parametrize("model", ["tiny-mixtral", "small-llama"])
+def test_engine_with_new_turns_on_the_gpu(cuda, model, mode):
+    rows = _served(model, str(cuda), 0.25, decode_gemm=mode)
+    if mode == "blas":                                        # (steps of 129 to 256 rows are padded to 16 k + 8)
+        assert any(B > 0 and T in (168, 184, 200) for T, B in rows), rows
