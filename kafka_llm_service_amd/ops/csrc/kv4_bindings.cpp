@@ -1,6 +1,7 @@
 // Python bindings of the 4-bit cache's kernels (kv4.hip, kv4_attn.hip, kv4_tile.hip). What the kernels assume of shapes, types, strides, alignment
 // and devices is checked here; index values on the device (slots, page ids, kept keys) are checked by the kernels.
 #include <torch/extension.h>
+#include <ATen/MemoryOverlap.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 #include <hip/hip_runtime.h>
@@ -45,6 +46,11 @@ bool aligned(const Tensor& t) { return reinterpret_cast<uintptr_t>(t.data_ptr())
 void on(const Tensor& t, const Tensor& home, at::ScalarType type, const char* name) {
   TORCH_CHECK_VALUE(t.is_cuda() && t.device() == home.device(), name, ": on the cache's device expected");
   TORCH_CHECK_VALUE(t.scalar_type() == type, name, ": wrong dtype");
+}
+
+// workgroups read what others may have written by then, unless both are the same memory, which each reads and writes for itself
+void apart(const Tensor& out, const Tensor& in, const char* what) {
+  TORCH_CHECK_VALUE(at::get_overlap_status(out, in) != at::MemOverlapStatus::Partial, what);
 }
 
 // head dim of a K / V page pool
@@ -191,6 +197,7 @@ Tensor attn(Tensor q, Tensor kc, Tensor vc, Tensor tables, const Plan& p, double
   if (out_.has_value()) {
     out = *out_;
     rows3(out, kc, T, Hq, D, "out");
+    apart(out, q, "attn: out and q overlap in part");
   } else {
     out = p.covered == T ? at::empty({T, Hq, D}, q.options()) : at::zeros({T, Hq, D}, q.options());
   }
@@ -254,6 +261,7 @@ Tensor attn_mass(Tensor q, Tensor lse, Tensor kc, Tensor tables, const Plan& p, 
       TORCH_CHECK_VALUE((*t)->is_contiguous() && N >= p.keys, "attn_mass: base and out contiguous, at least ", p.keys, " keys wide");
     }
   TORCH_CHECK_VALUE(!base.has_value() || !out_.has_value() || base->sizes() == out_->sizes(), "attn_mass: base and out alike");
+  if (base.has_value() && out_.has_value()) apart(*out_, *base, "attn_mass: base and out overlap in part");
   Tensor out = out_.has_value() ? *out_ : at::empty({S, H, N}, lse.options());
   const int64_t done = (p.keys + 63) / 64 * 64;
   const bool same = base.has_value() && base->data_ptr() == out.data_ptr();

@@ -50,6 +50,13 @@ def read(k_cache: torch.Tensor, v_cache: torch.Tensor, slots: torch.Tensor) -> t
     return ref.read(k_cache, v_cache, slots)
 
 
+def _check_apart(out, other, who: str) -> None:
+    """``out`` is ``other``, or they have no byte in common (as far as contiguous tensors tell)."""
+    a, b = ((t.data_ptr(), t.data_ptr() + t.numel() * t.element_size()) for t in (out, other))
+    if out.is_contiguous() and other.is_contiguous() and a != b and a[0] < b[1] and b[0] < a[1]:
+        raise ValueError(f"{who} overlap in part")
+
+
 # ---- plans --------------------------------------------------------------------------------------------------------------
 FEW_ROWS = 16              # rows (tokens x query heads of a group) of a tile for single tokens
 SOME_ROWS = 32             # of a tile for short portions
@@ -324,7 +331,7 @@ def _check_call(q, k_cache, block_tables, plan: AttnPlan, scale: float, who: str
 
 
 def attn(q, k_cache, v_cache, block_tables, plan: AttnPlan, scale: float, out=None, lse=None) -> torch.Tensor:
-    """softmax(scale q k^T) v of the plan's rows: q [T, heads, dim] bf16 -> out (a new tensor unless given), the same shape.
+    """softmax(scale q k^T) v of the plan's rows: q [T, heads, dim] bf16 -> out (a new tensor unless given; q itself may be), the same shape.
     ``lse`` fp32 [T, heads] gets the base-2 logarithm of each row's sum of 2^(scores in base 2). Rows of no segment are left as they
     were (zeros in a new ``out``). Of a page that no row of the segment sees a key of (behind the last one, or between the first ones
     and the window) the table may name anything; where it names none of the cache's for one that is seen, the rows that see it come out
@@ -339,6 +346,8 @@ def attn(q, k_cache, v_cache, block_tables, plan: AttnPlan, scale: float, out=No
         out = torch.zeros(q.shape, dtype=q.dtype)
     elif out.shape != q.shape or out.dtype != q.dtype:
         raise ValueError("kv4.attn: out like q expected")
+    else:
+        _check_apart(out, q, "kv4.attn: out and q")
     if lse is not None and (lse.shape != q.shape[:2] or lse.dtype != torch.float32):
         raise ValueError("kv4.attn: lse fp32 [T, heads] expected")
     ref.attn(q, k_cache, v_cache, block_tables, plan.segs, plan.window, plan.first, float(scale), out, lse)
@@ -363,6 +372,8 @@ def attn_mass(q, lse, k_cache, block_tables, plan: AttnPlan, scale: float, base=
     for t in (base, out):
         if t is not None and (t.shape != shape or t.dtype != torch.float32 or not t.is_contiguous() or t.shape[2] < plan.keys):
             raise ValueError(f"kv4.attn_mass: base and out contiguous fp32 [segments, kv heads, at least {plan.keys}], alike, expected")
+    if base is not None and out is not None:
+        _check_apart(out, base, "kv4.attn_mass: base and out")
     if out is None:
         out = torch.empty(shape, dtype=torch.float32)
     if base is None:

@@ -199,6 +199,45 @@ def test_bad_pages_of_portions_on_the_gpu(cuda, monkeypatch, D, rows, cost):
     _bad_portions(cuda, D, rows)
 
 
+# ---- outputs over inputs ---------------------------------------------------------------------------------------------------
+def _overlaps(device):
+    """An output may take its input's place; one that covers a part of it is refused."""
+    segs = [(0, 1, 300, 0), (1, 9, 500, 1), (10, 140, 700, 2)]
+    kc, vc, tables = world(segs, 2, 128, 0, device)
+    q = queries(151, 8, 128, 1, device)
+    plan = kv4.attn_plan(segs, 8, 2, 128, device=device)
+    lse = torch.zeros(150, 8, device=device)
+    want = kv4.attn(q[:150], kc, vc, tables, plan, 0.1, lse=lse)
+    mass = kv4.attn_mass(q[:150], lse, kc, tables, plan, 0.1)
+    for first in (0, 1):
+        both = q.clone()
+        mine, other = both[first:150 + first], both[1 - first:151 - first]
+        mine.copy_(q[:150])
+        with pytest.raises(ValueError):
+            kv4.attn(mine, kc, vc, tables, plan, 0.1, out=other)
+        assert torch.equal(mine, q[:150])
+        assert kv4.attn(mine, kc, vc, tables, plan, 0.1, out=mine) is mine and torch.equal(mine, want)
+        buf = torch.zeros(mass.numel() + 4, device=device)
+        base, out = buf[4 * first:][:mass.numel()].view(mass.shape), buf[4 * (1 - first):][:mass.numel()].view(mass.shape)
+        with pytest.raises(ValueError):
+            kv4.attn_mass(q[:150], lse, kc, tables, plan, 0.1, base=base, out=out)
+        assert (buf == 0).all()
+        kv4.attn_mass(q[:150], lse, kc, tables, plan, 0.1, base=base, out=base.view(mass.shape))
+        assert torch.equal(base, mass)
+
+
+def test_overlaps_reference():
+    _overlaps("cpu")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("wide", [False, True])
+def test_overlaps_on_the_gpu(cuda, monkeypatch, wide):
+    monkeypatch.setattr(kv4, "MANY_COST", -1e9 if wide else 1e9)
+    monkeypatch.setattr(kv4, "SOME_PIECE", 2)
+    _overlaps(cuda)
+
+
 # ---- writer: sums of slabs that are no numbers ----------------------------------------------------------------------------
 @pytest.mark.gpu
 @pytest.mark.parametrize("T,Hq,H,D,slab", [(33, 4, 4, 64, 2), (5, 32, 8, 128, 4), (3, 3, 1, 128, 1)])
