@@ -143,8 +143,12 @@ class LLMEngine:
                                           dp_attention=dpa, dtype=getattr(torch, cfg.dtype))
         self.slots = None
         if getattr(self.model, "plan", "") == "segments":
+            if cfg.kv_dtype == "mx4":
+                raise ValueError(f"kv_dtype mx4: the pages of {mc.arch} models are not kept in 4 bits (Llama and Mixtral models' are)")
             self._init_segments(cfg, mc, t0)
             return
+        if cfg.kv_dtype == "mx4":
+            ops.kv4.check_heads(self.model.hq, self.model.hkv, self.model.D)
         mode = os.environ.get("KAFKA_DECODE_GEMM", cfg.decode_gemm)
         if mode == "auto":
             mode = "stream" if self.device.type == "cuda" else "blas"

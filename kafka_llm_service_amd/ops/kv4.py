@@ -252,9 +252,15 @@ def _native(p: AttnPlan, take: _Take, shapes) -> None:
         p.native.add(rows, waves, slots, take(items, 12 if keys else 8), take(merges, 4), take(keys, 4))
 
 
-def _plan(segs, heads: int, kv_heads: int, dim: int, window: int, first: int) -> tuple[AttnPlan, np.ndarray]:
+def check_heads(heads: int, kv_heads: int, dim: int) -> None:
+    """Refuses heads that the cache's attention does not take."""
     if dim not in (64, 128) or kv_heads < 1 or heads % kv_heads or not 1 <= heads // kv_heads <= MAX_GROUP:
-        raise ValueError("kv4.attn_plan: head dim 64 or 128, 1 to 16 query heads for each key/value head")
+        raise ValueError(f"the 4-bit cache takes head dims of 64 and 128 and 1 to {MAX_GROUP} query heads for each key/value head, not {heads} / "
+                         f"{kv_heads} heads of {dim}")
+
+
+def _plan(segs, heads: int, kv_heads: int, dim: int, window: int, first: int) -> tuple[AttnPlan, np.ndarray]:
+    check_heads(heads, kv_heads, dim)
     if window < 0 or first < 0 or window >= 1 << 30 or first >= MAX_POS:
         raise ValueError("kv4.attn_plan: window and first may not be negative (window 0: every earlier position)")
     if first and not window:

@@ -341,3 +341,19 @@ def test_engine_with_new_turns_on_the_gpu(cuda, model, mode):
     rows = _served(model, str(cuda), 0.25, decode_gemm=mode)
     if mode == "blas":                                        # (steps of 129 to 256 rows are padded to 16 k + 8)
         assert any(B > 0 and T in (168, 184, 200) for T, B in rows), rows
+
+
+def test_engine_refusals():
+    """What the cache cannot hold or attend to is refused when the engine is made, not by its first step."""
+    from dataclasses import replace
+
+    from kafka_llm_service_amd.engine.engine import EngineConfig, LLMEngine
+    from kafka_llm_service_amd.models.config import get_config
+
+    make = lambda mc, kv: LLMEngine(EngineConfig(device="cpu", num_kv_blocks=64, max_model_len=256, kv_dtype=kv), model_cfg=mc)
+    tiny = replace(get_config("tiny-llama"), vocab_size=512)
+    for mc in (replace(tiny, num_heads=17, num_kv_heads=1), replace(tiny, head_dim=32), get_config("budurax-tiny")):
+        with pytest.raises(ValueError, match="4.bit|mx4"):
+            make(mc, "mx4")
+        make(mc, "bf16")
+    make(replace(tiny, num_heads=16, num_kv_heads=1), "mx4")
