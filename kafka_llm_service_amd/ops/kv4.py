@@ -65,6 +65,7 @@ MANY_WGS = {128: 256, 64: 768}    # workgroups of these that the CUs hold
 MANY_MIN = 128             # rows of a segment from which on its keys may be widened first (_wide)
 MANY_BLOCKS = 4            # least blocks of a piece of a wide tile (300 rows behind 1000 keys 25 us; of 8 blocks 30, of 16 40)
 CUS = 256
+MANY_BYTES = 8 << 30       # most that the keys widened for a call may take (2 million keys of 8 heads of 128); what is beyond goes in tiles of 32 rows
 LEAST_SHARE = 2            # blocks a CU up to which every four of them are a workgroup, one for each wave
 SHORT_TILE = 48            # blocks of a tile on average below which four waves take it, where there is more than a tile a CU (_narrow_split)
 SOME_WGS, SOME_PIECE = 256, 8     # workgroups that a launch of short portions is split towards, least blocks of a piece
@@ -133,8 +134,8 @@ def _narrow_split(count: np.ndarray, kv_heads: int, rows: int) -> tuple[int, np.
 
 
 def _wide(full: np.ndarray, heads: int, kv_heads: int, dim: int, window: int, first: int) -> np.ndarray:
-    """Which segments are taken in wide tiles whose keys are widened first: none or all of MANY_MIN rows or more, by the microseconds that
-    both ways take. Measured (32/8 heads of 128 / 64/8 heads of 128 / 24/8 heads of 64): 512 rows cold 21 against 14 with tiles of 32 rows / 25
+    """Which segments are taken in wide tiles whose keys are widened first: none or all of MANY_MIN rows or more (in their order as many as
+    MANY_BYTES hold), by the microseconds that both ways take. Measured (32/8 heads of 128 / 64/8 heads of 128 / 24/8 heads of 64): 512 rows cold 21 against 14 with tiles of 32 rows / 25
     against 25 / 17 against 10, 300 rows behind 1000 keys 24 against 23 / 31 against 33 / 18 against 14, 8 portions of 200 cold 20 against
     35 / - / -, three of 1100 behind 900 in a window of 512 75 against 99 / - / 38 against 61."""
     G = heads // kv_heads
@@ -152,7 +153,8 @@ def _wide(full: np.ndarray, heads: int, kv_heads: int, dim: int, window: int, fi
         many = MANY_COST + blocks * (2.1 if dim == 128 else 0.8) / 256 + keys * dim * 5 / 4.5e6
         if few <= many:
             wide[:] = False
-    return wide
+    size = np.where(wide, _blocks(full[:, 2], full[:, 1], window, first)[1] * kv_heads * 256 * dim, 0)
+    return wide & (np.cumsum(size) <= MANY_BYTES)
 
 
 def _wide_split(count: np.ndarray, kv_heads: int, wgs: int) -> np.ndarray:

@@ -238,6 +238,39 @@ def test_overlaps_on_the_gpu(cuda, monkeypatch, wide):
     _overlaps(cuda)
 
 
+# ---- the room that widened keys take --------------------------------------------------------------------------------------
+def _widened_bytes(case):
+    shapes, arrays, _ = _items(case)
+    return sum(s[5] for s in shapes) * case[1] * 256 * case[2], [s[0] for s in shapes]
+
+
+def test_room_of_widened_keys(monkeypatch):
+    """However many portions a step has, and however long their histories are, what is widened for them stays within its bound."""
+    segs = [(128 * i, 128, 131000, i) for i in range(64)]
+    size, shapes = _widened_bytes((32, 8, 128, segs, 0, 0))
+    assert 0 < size <= kv4.MANY_BYTES < 64 * 131128 * 8 * 512 and shapes == [32, 256]
+    g = torch.Generator().manual_seed(0)
+    r = lambda hi: int(torch.randint(0, hi, (1,), generator=g))
+    monkeypatch.setattr(kv4, "MANY_COST", -1e9)
+    for _ in range(50):
+        case = (8, 2, (64, 128)[r(2)], [(100 * i, 32 + r(68), r(9000), i) for i in range(1 + r(9))], *((0, 0) if r(2) else (1 + r(900), r(100))))
+        monkeypatch.setattr(kv4, "MANY_BYTES", 1 << (20 + r(8)))
+        assert _widened_bytes(case)[0] <= kv4.MANY_BYTES
+        monkeypatch.setattr(kv4, "MANY_BYTES", 1 << 40)
+        assert _widened_bytes(case)[1] == [kv4.MANY_ROWS[case[2]]]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("D", [64, 128])
+def test_portions_beyond_the_room_for_widened_keys(cuda, monkeypatch, D):
+    """Portions that fit and portions that do not, beside single tokens, in one call."""
+    case = (8, 2, D, [(0, 1, 300, 0), (1, 90, 400, 1), (91, 60, 1000, 2), (151, 40, 100, 3)], 0, 0)
+    monkeypatch.setattr(kv4, "MANY_COST", -1e9)
+    monkeypatch.setattr(kv4, "MANY_BYTES", 10 * 2 * 256 * D)
+    assert _widened_bytes(case) == (8 * 2 * 256 * D, [16, 32, kv4.MANY_ROWS[D]])
+    _check_attention(case, cuda)
+
+
 # ---- writer: sums of slabs that are no numbers ----------------------------------------------------------------------------
 @pytest.mark.gpu
 @pytest.mark.parametrize("T,Hq,H,D,slab", [(33, 4, 4, 64, 2), (5, 32, 8, 128, 4), (3, 3, 1, 128, 1)])
