@@ -271,6 +271,34 @@ def test_portions_beyond_the_room_for_widened_keys(cuda, monkeypatch, D):
     _check_attention(case, cuda)
 
 
+# ---- large values ---------------------------------------------------------------------------------------------------------
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,cost", [(1, 1e9), (9, 1e9), (150, -1e9)])
+@pytest.mark.parametrize("D", [64, 128])
+def test_large_values(cuda, monkeypatch, D, rows, cost):
+    """Values just below 2^104 / n, whose weights reach 2^23 times the first keys': right; other rows do not notice larger ones."""
+    monkeypatch.setattr(kv4, "MANY_COST", cost)
+    H, Hq, n = 1, 4, 2000
+    segs = [(0, rows, n - rows, 0), (rows, rows, n - rows, 1)]
+    kc, vc, tables = world(segs, H, D, 0, cuda, garbage=False)
+    order = tables[:, :n // 16].long()
+    j = torch.arange(n, device=cuda).view(-1, 16)
+    k = torch.zeros(n // 16, H, 16, D, device=cuda)
+    k[..., 0] = torch.where(j < 64, 0.0, 6.0)[:, None]
+    v = torch.full((n // 16, H, 16, D), 6 * 2.0 ** 90, device=cuda)                 # 6 * 2^90 < 2^104 / 2000
+    for s, x in ((0, v), (1, torch.full_like(v, math.inf))):
+        a, b = kref.pack_pages(k.cpu(), x.cpu())
+        kc[order[s]], vc[order[s]] = a.to(cuda), b.to(cuda)
+    q = torch.zeros(2 * rows, Hq, D, dtype=torch.bfloat16, device=cuda)
+    q[..., 0] = 1
+    scale = 23 * math.log(2) / 6                                                   # base 2: the later keys' scores are 23, the first ones' 0
+    lse = torch.zeros(2 * rows, Hq, device=cuda)
+    out = kv4.attn(q, kc, vc, tables, kv4.attn_plan(segs, Hq, H, D, device=cuda), scale, lse=lse)
+    assert torch.equal(out[:rows].float(), torch.full((rows, Hq, D), 6 * 2.0 ** 90, device=cuda))
+    want = torch.log2((n - rows + 1 + torch.arange(2 * rows, device=cuda) % rows - 64).double() * 2.0 ** 23 + 64)
+    assert ((lse.double() - want[:, None]).abs() <= 2.0 ** -12).all()              # (sums of n numbers: n 2^-24 / ln 2, a score of 23: 2^-18)
+
+
 # ---- writer: sums of slabs that are no numbers ----------------------------------------------------------------------------
 @pytest.mark.gpu
 @pytest.mark.parametrize("T,Hq,H,D,slab", [(33, 4, 4, 64, 2), (5, 32, 8, 128, 4), (3, 3, 1, 128, 1)])
