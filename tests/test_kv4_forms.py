@@ -418,3 +418,70 @@ def test_engine_refusals():
             make(mc, "mx4")
         make(mc, "bf16")
     make(replace(tiny, num_heads=16, num_kv_heads=1), "mx4")
+
+
+def test_step_of_the_cache_as_its_followers_get_it():
+    """A step's tables, planned on the host, come whole out of what a leader sends its followers."""
+    from kafka_llm_service_amd.engine import model_runner as mr
+    from kafka_llm_service_amd.engine.engine import EngineConfig, LLMEngine
+    from kafka_llm_service_amd.engine.sequence import SamplingParams
+
+    eng = LLMEngine(EngineConfig(model="tiny-llama", device="cpu", num_kv_blocks=256, max_model_len=2048, kv_dtype="mx4"))
+    g = torch.Generator().manual_seed(1)
+    draw = lambda n: torch.randint(0, 5000, (n,), generator=g).tolist()
+    eng.add_request("a", draw(100), SamplingParams(temperature=0.0, max_tokens=9, ignore_eos=True))
+    eng.step()
+    eng.step()
+    eng.add_request("b", draw(200), SamplingParams(temperature=0.0, max_tokens=9, ignore_eos=True))
+    steps, build = [], type(eng.runner).build_host
+
+    def both(batch, want=None):
+        eng.runner.mx4 = True
+        steps.append((build(eng.runner, batch, want)[0], [s.total_len for s in batch.decode], [(a, b) for _, a, b in batch.prefill]))
+        eng.runner.mx4 = False
+        return build(eng.runner, batch, want)
+
+    eng.runner.build_host = both
+    for _ in range(3):
+        eng.step()
+    assert any(d and p for _, d, p in steps)
+    z = np.zeros(0, np.float32)
+    for h, dec, pre in steps:
+        segs = [(i, 1, n - 1, i) for i, n in enumerate(dec)]
+        r = len(dec)
+        for j, (a, b) in enumerate(pre):
+            segs.append((r, b - a, a, len(dec) + j))
+            r += b - a
+        model = eng.model
+        want = kv4.step_tables(segs, model.hq, model.hkv, model.D)
+        o = h.nbt * h.bt_w + h.T
+        assert h.bt_need <= h.bt_w and h.bt_w * 16 >= want[2]
+        got, _ = mr.unpack_plan(*mr.pack_plan(h, mr.SampleParams(z, z, z.astype(np.int32), z.astype(np.int64), None, True)))
+        for x in (h, got):
+            assert np.array_equal(x.i32[o:], want) and np.array_equal(x.i32, h.i32) and np.array_equal(x.i64, h.i64)
+            assert (x.B, x.T, x.nbt, x.bt_w, x.n_rows) == (h.B, h.T, h.nbt, h.bt_w, h.n_rows)
+
+
+@pytest.mark.timeout(300)
+def test_two_ranks_on_the_cache():
+    """Tensor parallel on the 4-bit cache: both ranks' heads together give the dense form's tokens."""
+    import torch.multiprocessing as mp
+
+    import test_tp_equivalence as tp
+    from kafka_llm_service_amd.engine.engine import EngineConfig, LLMEngine
+
+    ctx = mp.get_context("spawn")
+    q, port = ctx.Queue(), tp._port()
+    procs = [ctx.Process(target=tp._group_main, args=(r, 2, port, q, {"kv_dtype": "mx4"})) for r in range(2)]
+    for p in procs:
+        p.start()
+    res = dict((m[0], m[1:]) for m in (q.get(timeout=240) for _ in range(2)))
+    for p in procs:
+        p.join(timeout=60)
+        assert p.exitcode == 0
+    model = LLMEngine(EngineConfig(**dict(tp.CFG, kv_dtype="mx4"))).model
+    for p, o in zip(tp._prompts(), res["outs"][0]):
+        lg = _dense4(model, p + o)
+        for i, tok in enumerate(o):
+            row = lg[len(p) - 1 + i]
+            assert (row.max() - row[tok]).item() < 0.15
