@@ -379,7 +379,8 @@ extern "C" hipError_t kafka_kv4_evict_keep(const float* mass, int64_t ms, int64_
   if (first < 0 || recent < 0 || (int64_t)first + recent > budget || R > 65535) return hipErrorInvalidValue;
   auto go = [&](auto kern) { kern<<<dim3(Hkv, R), KEEP_NT, 0, st>>>(mass, ms, mh, N, lens, budget, first, recent, kept, Hkv); };
   // (16 sequences of 5000 / 8300 / 12000 keys, as few a thread as hold them, 9 / 12 / 14 us, 8300 with 16 a thread 18; read again, 4 a thread at a
-  // time, 12 / 16 / 19. One of 30000 keys, which no kernel holds, 4 a thread at a time 40, 16 at a time 49)
+  // time, 12 / 16 / 19. One of 30000 keys, which no kernel holds, 4 a thread at a time 40, 16 at a time 49. With 12 and 16 a thread 18 and 51 scalar
+  // registers go through lanes: in the times above)
   if (N <= KEEP_NT * 4) go(evict_keep_kernel<4, true>);
   else if (N <= KEEP_NT * 8) go(evict_keep_kernel<8, true>);
   else if (N <= KEEP_NT * 12) go(evict_keep_kernel<12, true>);

@@ -51,9 +51,13 @@ __device__ __forceinline__ int lane_again(int lane) {
 // exponentials of this one, between those of its values the rest of them and the next one's maxima, each product behind the LDS reads of the F
 // fragments after it; keys run a tile ahead of the values, and the slots that a step has read are filled again in its middle, behind one counted
 // wait and one barrier. The maximum is raised only where it has grown by more than 2^24 (sums of weights up to that are exact enough in fp32).
-// Products and exponentials bound it, in turn on the same issue slots: 8000 rows cold, 32/8 heads of 128, 1054 TFLOP/s (a large product of the
-// library 1379), of 64, which have half the products for an exponential, 879. Heads of 64: three workgroups of four waves a CU, of 128 one of
-// eight, whose ring of three slots (96 KiB) leaves no room for another. Below about 500 rows the tiles of 32 rows (kv4_attn.hip) are as fast.
+// What bounds it, by leaving one thing out at a time: 8000 rows cold, 32/8 heads of 128, 446 us, 1175 TFLOP/s (a large product of the library
+// 1400), without the copies to LDS (32 KiB a tile and workgroup, 4.6 TB/s in all) 371, which is the products' own rate, without
+// the exponentials 421, without the reads from LDS 422; heads of 64, which have half the products for an exponential, 272 us, 965
+// TFLOP/s, without them 227, 236 and 258. So copies first, then exponentials and reads. Masks count where most blocks are at an edge: three
+// portions of 1100 rows in a window of 512, heads of 64, 28.6 us, without masks 21.6. The scalar unit runs beside: 24 million instructions for 43 million vector ones.
+// Heads of 64: three workgroups of four waves a CU, of 128 one of eight, whose ring of three slots (96 KiB) leaves no room for another. Below
+// about 500 rows the tiles of 32 rows (kv4_attn.hip) are as fast.
 template <int D, int NW, int NSLOT>
 __global__ __launch_bounds__(64 * NW, D == 64 ? 3 : 1) void tile_kernel(TileArgs a) {
   constexpr int F = D / 16, NT = D / 32, KBYTES = Image<D>::KBYTES, PB = Image<D>::PAGE_BYTES;
