@@ -45,21 +45,27 @@ __device__ __forceinline__ uint32_t narrow8(bf16x8 x, float sc) {
 }
 
 typedef int i32x8 __attribute__((ext_vector_type(8)));
+typedef uint32_t u32x6 __attribute__((ext_vector_type(6)));
 
-// a [16 rows][128] in e2m1, a lane's 32 elements of k = 32 (l >> 4) on in its first four words, times 2^(sa - 127); b [128][16 columns] in e4m3, a
-// lane's elements of k = 16 (l >> 4) on and of 64 + 16 (l >> 4) on, the block of k = 32 (l >> 4) on times 2^(sb - 127) of that lane.
+// a [16 rows][128] in e2m1, a lane's 32 elements of k = 32 (l >> 4) on in its first four words, times 2^(sa - 127); b [128][16 columns] in e2m3, a
+// lane's 32 of the same k in six words, times 2^(e - 127), e the byte BYTE of sb (255: no number).
 // The instruction adds the products of eight neighbouring k, each cut (towards zero) to multiples of 2^-13 of the largest one's power of two, and
-// such sums in fp32 (measured: beside 256 a product of 2^-5 is whole, one of 2^-6 gone, in another eight of k it is whole down to 2^-16).
+// such sums in fp32 (measured: beside 256 a product of 2^-5 is whole, one of 2^-6 gone, in another eight of k it is whole down to 2^-16). Whole numbers
+// of up to 16 steps of 1/8, which e2m3 holds all, times a key's of up to 12 halves lose nothing of that: products are multiples of 1/16 up to 12.
 // (The compiler does not know that the product needs every lane of its operands: results are pinned where control flow is uniform.)
-__device__ __forceinline__ f32x4 mfma4x8(const uint32_t* a, uint32_t sa, i32x8 b, uint32_t sb, f32x4 c) {
+template <int BYTE>
+__device__ __forceinline__ f32x4 mfma4x6(const uint32_t* a, uint32_t sa, const u32x6& b, uint32_t sb, f32x4 c) {
   const i32x8 x = {(int)a[0], (int)a[1], (int)a[2], (int)a[3], 0, 0, 0, 0};
-  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(x, b, c, 4, 0, 0, (int)sa, 0, (int)sb);
+  const i32x8 y = {(int)b[0], (int)b[1], (int)b[2], (int)b[3], (int)b[4], (int)b[5], 0, 0};
+  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(x, y, c, 4, 2, 0, (int)sa, BYTE, (int)sb);
 }
 
-// The same with the operands in each other's place: a [16 rows][128] in e4m3, b [128][16 columns] in e2m1
-__device__ __forceinline__ f32x4 mfma8x4(i32x8 a, uint32_t sa, const uint32_t* b, uint32_t sb, f32x4 c) {
-  const i32x8 x = {(int)b[0], (int)b[1], (int)b[2], (int)b[3], 0, 0, 0, 0};
-  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, x, c, 0, 4, 0, (int)sa, 0, (int)sb);
+// The same with the operands in each other's place: a [16 rows][128] in e2m3, b [128][16 columns] in e2m1
+template <int BYTE>
+__device__ __forceinline__ f32x4 mfma6x4(const u32x6& a, uint32_t sa, const uint32_t* b, uint32_t sb, f32x4 c) {
+  const i32x8 x = {(int)a[0], (int)a[1], (int)a[2], (int)a[3], (int)a[4], (int)a[5], 0, 0};
+  const i32x8 y = {(int)b[0], (int)b[1], (int)b[2], (int)b[3], 0, 0, 0, 0};
+  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(x, y, c, 2, 4, BYTE, (int)sa, 0, (int)sb);
 }
 
 __device__ __forceinline__ f32x4 mfma16(bf16x8 a, bf16x8 b, f32x4 c) {

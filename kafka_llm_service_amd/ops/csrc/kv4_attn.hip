@@ -4,7 +4,7 @@
 // those with j > p - window or j < first. A work item is a tile of a segment's tokens and a range of the blocks of 64 keys that
 // any of them sees (the first ones, then those from the window's start on: a block in the range is a place in this list).
 //
-//   S^T[key][row] = K . Q^T    A: K in four bits as it lies, B: Q in two parts of e4m3
+//   S^T[key][row] = K . Q^T    A: K in four bits as it lies, B: Q in four parts of e2m3, 20 bits of fixed point
 //   O^T[d][row]  += V^T . P    A: a lane's values of four keys, two neighbouring d's a register as they are widened (exactly), B: P as S^T's
 //                              registers hold it, beside zeros for the other d: twice the products, but no register is turned
 // The softmax runs in one pass with a running maximum per row; its sums and maxima are fp32, P is rounded to bf16 for the product.
@@ -121,7 +121,7 @@ struct PageIds {
   }
 };
 
-// (heads of 64: both halves of the lanes hold the key, for the two parts of Q)
+// (heads of 64: both halves of the lanes hold the key, for two parts of Q)
 template <int D, int NP>
 __device__ __forceinline__ void load_k(KFrag<NP>& f, const uint8_t* kh, uint32_t stride, const uint32_t (&pg)[NP], int lane) {
   const uint32_t key = lane & 15, g = (lane >> 4) & (D / 32 - 1), at = key * (D / 2) + g * 16, sc = Page<D>::DATA + key * (D / 32) + g;
@@ -146,15 +146,18 @@ __device__ __forceinline__ void load_v(VFrag<NP>& f, const uint8_t* vh, uint32_t
   }
 }
 
-// Q in e4m3, so that the matrix cores take the keys in four bits as they lie: 2^-u q = hi + lo / 16, hi the nearest e4m3, u so that the row's
-// largest element comes to 128 .. 256. A bf16 number has eight bits of mantissa, hi takes four of them and lo the rest, so the
-// sum is exact down to 2^-14 of the largest element, and off by at most 2^-21 of it below. What the instruction cuts of products below 2^-9 of
-// their eight's largest (kv4.h) comes to about 2^-16 of sum |q_d k_d|: 6e-4 in a score where that sum is 51, a sixth of P's rounding and
-// far below what four bits of K leave of it; with K widened for bf16 products 64 threads took 68 us for 56.
+// Q in fixed point, so that the matrix cores take the keys in four bits as they lie: of 32 elements the largest comes to 8 .. 16 steps, and four
+// parts hold whole numbers of up to 16 in e2m3, each counting a 32nd of the one before: 20 bits, in which an element is whole down to 2^-11 of
+// the largest (bf16 has eight bits) and off by at most 2^-19 of it below. Nothing of the products is cut (kv4.h), so scores are as
+// exact as 32 bits make them. In two parts of e4m3, in which the instruction takes twice the cycles, the cut of their products was
+// 2^-16 of sum |q_d k_d|, one-sided, and came out in lse and the masses.
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x32 __attribute__((ext_vector_type(32)));
+typedef uint32_t u32x16 __attribute__((ext_vector_type(16)));
 template <int D>
 struct QFrag {
-  i32x8 x[D / 64];          // heads of 128: hi, lo; of 64: both in one, a half of k each
-  uint32_t s[D / 64];
+  u32x6 x[D / 32];          // heads of 128: the parts; of 64: parts 0 and 2 in the lower half of the lanes (of k), 1 and 3 in the upper
+  uint32_t s;               // their scales, a byte each
 };
 
 template <int D, int NQ>
@@ -165,59 +168,74 @@ struct Rows {
   float m[NQ], l[NQ];       // maximum so far (times scale, log2), this lane's part of the sum
 };
 
-// 16 columns from column R0 of the tile on
+// 16 columns from column R0 of the tile on; a lane takes 32 elements of its column
 template <int D>
 __device__ __forceinline__ int load_q(QFrag<D>& f, const Args& a, int row, int tokens, int pos, int h, int R0, int lane) {
-  constexpr int N = D / 32;                                  // pieces of eight elements a lane
   const int R = R0 + (lane & 15), tok = R / a.G, g = R - tok * a.G, c = lane >> 4;
   const bool there = tok < tokens;
-  const bf16* p = a.q + (int64_t)(row + (there ? tok : 0)) * a.qs + (int64_t)(h * a.G + g) * D + 16 * c;
-  bf16x8 q[N];
+  const bf16* p = a.q + (int64_t)(row + (there ? tok : 0)) * a.qs + (int64_t)(h * a.G + g) * D + 32 * (c & (D / 32 - 1));
+  bf16x8 q[4];
 #pragma unroll
-  for (int i = 0; i < N; ++i) q[i] = load_bf16x8(p + 64 * (i >> 1) + 8 * (i & 1));
+  for (int i = 0; i < 4; ++i) q[i] = load_bf16x8(p + 8 * i);
   uint32_t m = 0;                                            // the largest element's bits
 #pragma unroll
-  for (int i = 0; i < N; ++i) {
+  for (int i = 0; i < 4; ++i) {
     const u32x4 b = __builtin_bit_cast(u32x4, q[i]);
 #pragma unroll
     for (int j = 0; j < 4; ++j) m = max(m, max(b[j] & 0x7fffu, (b[j] >> 16) & 0x7fffu));
   }
-  m = max(m, (uint32_t)__shfl_xor((int)m, 16, 64));
-  m = max(m, (uint32_t)__shfl_xor((int)m, 32, 64));
-  const bool finite = m < 0x7f80u;
-  const int e = max((int)(m >> 7), 30) - 7;                  // (its exponent) - 7, biased: 2^(e - 127) is 2^u
-  const float s = there ? __uint_as_float((uint32_t)(254 - e) << 23) : 0.f;
-  uint32_t hi[2 * N], lo[2 * N];
+  if (!there) m = 0;
+  const uint32_t e = max(m >> 7, 16u);                       // its exponent
+  const float s = there ? __uint_as_float((257u - e) << 23) : 0.f;
+  u32x16 x;                                                  // (eight bits from below 2^4 on: f16 holds them and what is left of them exactly)
 #pragma unroll
-  for (int i = 0; i < 2 * N; ++i) {
-    float x[4];
+  for (int i = 0; i < 16; ++i)
+    x[i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz((float)q[i >> 2][2 * (i & 3)] * s, (float)q[i >> 2][2 * (i & 3) + 1] * s));
+  // beyond the nearest whole number (of the sum with 1536, whose last bit is one; the packing rounds alike), 32 times
+  auto rest = [&]() {
+    const f16x2 big = {(_Float16)1536.f, (_Float16)1536.f};
 #pragma unroll
-    for (int j = 0; j < 4; ++j) x[j] = (float)q[i >> 1][4 * (i & 1) + j] * s;
-    int w = __builtin_amdgcn_cvt_pk_fp8_f32(x[0], x[1], 0, false);
-    w = __builtin_amdgcn_cvt_pk_fp8_f32(x[2], x[3], w, true);
-    const auto y0 = __builtin_amdgcn_cvt_pk_f32_fp8(w, false), y1 = __builtin_amdgcn_cvt_pk_f32_fp8(w, true);
-    int v = __builtin_amdgcn_cvt_pk_fp8_f32(16.f * (x[0] - y0[0]), 16.f * (x[1] - y0[1]), 0, false);
-    v = __builtin_amdgcn_cvt_pk_fp8_f32(16.f * (x[2] - y1[0]), 16.f * (x[3] - y1[1]), v, true);
-    hi[i] = finite ? (uint32_t)w : 0x7f7f7f7fu;              // (a row with an infinity or no number in it is no numbers)
-    lo[i] = finite ? (uint32_t)v : 0x7f7f7f7fu;
-  }
+    for (int i = 0; i < 16; ++i) {
+      const f16x2 y = __builtin_bit_cast(f16x2, (uint32_t)x[i]);
+      f16x2 t = y + big;
+      asm volatile("" : "+v"(t));
+      x[i] = __builtin_bit_cast(uint32_t, (y - (t - big)) * (_Float16)32.f);
+    }
+  };
+  // (packed here: or the compiler packs all parts where they are used, and has what is left of each in registers until then)
+  auto pack = [&](u32x6& part) {
+    part = __builtin_amdgcn_cvt_scalef32_pk32_fp6_f16(__builtin_bit_cast(f16x32, x), 8.f);
+    asm volatile("" : "+v"(part));
+  };
   if constexpr (D == 128) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      f.x[0][i] = (int)hi[i];
-      f.x[1][i] = (int)lo[i];
-    }
-    f.s[0] = (uint32_t)e;
-    f.s[1] = (uint32_t)e - 4u;
-  } else {
-#pragma unroll
     for (int i = 0; i < 4; ++i) {
-      f.x[0][i] = (int)hi[i];
-      f.x[0][4 + i] = (int)lo[i];
+      if (i) rest();
+      pack(f.x[i]);
     }
-    f.s[0] = c < 2 ? (uint32_t)e : (uint32_t)e - 4u;
+    f.s = e * 0x01010101u - 0x0f0a0500u;
+  } else {
+    if (c >= 2) rest();
+    pack(f.x[0]);
+    rest();
+    rest();
+    pack(f.x[1]);
+    f.s = e * 0x0101u - (c < 2 ? 0x0a00u : 0x0f05u);
   }
+  if (m >= 0x7f80u) f.s = ~0u;                               // (a row with an infinity or no number in it is no numbers)
   return there ? pos + tok : -1;
+}
+
+// the smallest part first
+template <int D, class Product>
+__device__ __forceinline__ f32x4 parts_sum(const QFrag<D>& q, Product product) {
+  f32x4 s = {0.f, 0.f, 0.f, 0.f};
+  if constexpr (D == 128) {
+    s = product(q.x[3], std::integral_constant<int, 3>{}, s);
+    s = product(q.x[2], std::integral_constant<int, 2>{}, s);
+  }
+  s = product(q.x[1], std::integral_constant<int, 1>{}, s);
+  return product(q.x[0], std::integral_constant<int, 0>{}, s);
 }
 
 // Scores of 16 NP keys
@@ -226,11 +244,8 @@ __device__ __forceinline__ void scores(const KFrag<NP>& f, const QFrag<D> (&q)[N
 #pragma unroll
   for (int t = 0; t < NP; ++t)
 #pragma unroll
-    for (int n = 0; n < NQ; ++n) {
-      s[t][n] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int i = 0; i < D / 64; ++i) s[t][n] = mfma4x8(f.d[t], f.s[t], q[n].x[i], q[n].s[i], s[t][n]);
-    }
+    for (int n = 0; n < NQ; ++n)
+      s[t][n] = parts_sum<D>(q[n], [&](const u32x6& x, auto i, f32x4 c) { return mfma4x6<decltype(i)::value>(f.d[t], f.s[t], x, q[n].s, c); });
 #pragma unroll
   for (int t = 0; t < NP; ++t)
 #pragma unroll
@@ -345,7 +360,7 @@ __device__ __forceinline__ void join(float& M, float& L, f32x4& o, const float (
 // NW waves take a tile of 16 NQ rows, every NW-th block each; their results meet in LDS. A wave has NB half blocks in registers: one that it
 // works on, the others on their way. (The loop's first form fetches without a condition, so that the waits count what is on its way.)
 // Three waves a SIMD with two half blocks each: 64 threads of 4100 tokens and 29 of 7900 56.7 and 56.7 us, three halves 57.2 and 57.6, two waves with
-// four 58.0 and 57.1, four with one 57.6 and 61.3. NQ 2, short portions: values are widened once for 32 rows; 4 portions of 100 rows behind
+// four 58.0 and 57.1, four with one 57.6 and 61.3 (with Q in two parts of e4m3; in four of e2m3 57.4 and 57.2). NQ 2, short portions: values are widened once for 32 rows; 4 portions of 100 rows behind
 // 1000 keys, 32/8 heads of 128, 23 us, as tiles of 256 rows whose keys are widened first 31. That is five times its operations' time: about a
 // hundred scalar registers of this form do not fit and go through lanes in the loop, each product with values is done twice, and values are widened for every 32 rows anew.
 // WIDEN: the workgroups behind the items' widen the step's long portions' keys on the way (kv4_tile.hip), which as a launch of its own would
@@ -588,10 +603,10 @@ __device__ __forceinline__ void of_rows(T x, T (&y)[4], int lane) {
 
 // Segments of at most 16 rows: four waves take every fourth block of an item's (at most 32), NB of them in registers. What a key had before
 // comes with it: a load that is asked for when its sum is there holds up those of the next keys. Bytes bound it, and the start and
-// end of workgroups of 28 blocks: 29 threads of 7900 tokens, 8 heads of 128, 140 MB, 31 us, 4.5 TB/s (three blocks in registers
-// and a wave a SIMD less 35).
+// end of workgroups of 28 blocks: 29 threads of 7900 tokens, 8 heads of 128, 140 MB, 36 us with the masses read from other memory each time,
+// 3.9 TB/s. Heads of 128 take four waves a SIMD: five leave too few registers for the parts of Q (103 us).
 template <int D, int NB>
-__global__ __launch_bounds__(256, 5) void mass_few_kernel(MassArgs ma) {
+__global__ __launch_bounds__(256, D == 128 ? 4 : 5) void mass_few_kernel(MassArgs ma) {
   const Args& a = ma.a;
   const int* it = reinterpret_cast<const int*>(a.items) + 8 * (blockIdx.x / a.Hkv);
   const int row = it[0], rows = it[1], pos = it[2], table = it[3], seg = it[4], end = it[6];
@@ -641,11 +656,8 @@ __global__ __launch_bounds__(256, 5) void mass_few_kernel(MassArgs ma) {
       float acc[4] = {};
       f32x4 s[4];
 #pragma unroll
-      for (int t = 0; t < 4; ++t) {
-        s[t] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int i = 0; i < D / 64; ++i) s[t] = mfma8x4(qf.x[i], qf.s[i], kf[x].d[t], kf[x].s[t], s[t]);
-      }
+      for (int t = 0; t < 4; ++t)
+        s[t] = parts_sum<D>(qf, [&](const u32x6& y, auto i, f32x4 c) { return mfma6x4<decltype(i)::value>(y, qf.s, kf[x].d[t], kf[x].s[t], c); });
       add_weights(acc, s, ls, key0 + KB - 1 > pos || (key0 <= last - a.window && key0 + KB > a.first), key0, lim, a, lane);
       float mine = quarters_sums(acc);                     // lane = key: that of tile c
       if (bad[x]) mine = __builtin_nanf("");

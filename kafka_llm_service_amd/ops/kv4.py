@@ -342,8 +342,7 @@ def attn(q, k_cache, v_cache, block_tables, plan: AttnPlan, scale: float, out=No
     """softmax(scale q k^T) v of the plan's rows: q [T, heads, dim] bf16 -> out (a new tensor unless given; q itself may be), the same shape.
     ``lse`` fp32 [T, heads] gets the base-2 logarithm of each row's sum of 2^(scores in base 2). Rows of no segment are left as they
     were (zeros in a new ``out``). Sums are formed before they are divided: with n keys values below 2^104 / n (2^78 for any n) are right, larger
-    ones, as infinities are stored, may come out as infinities or no numbers in the rows that see them. ``lse`` of tokens and short portions
-    carries what the 4-bit product cuts, about 2^-16 of sum |scale q_d k_d| (csrc/kv4.h). Of a page that no row of the segment sees a key of (behind the last one, or between the first ones
+    ones, as infinities are stored, may come out as infinities or no numbers in the rows that see them. Of a page that no row of the segment sees a key of (behind the last one, or between the first ones
     and the window) the table may name anything; where it names none of the cache's for one that is seen, the rows that see it come out
     as no numbers, and rows of the segment next to them may."""
     if _gpu(q):

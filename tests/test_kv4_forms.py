@@ -7,7 +7,10 @@ number, and nothing of it is cut. A score is then a sum of D / 8 exact numbers i
 instead of rounding, 2^-23 of A = the largest sum_d |scale q_d k_d| of a row for each, S = 2 (D / 8 + 4) 2^-24 A bounds its error. The
 exponential and its argument add 2^-22 (1 + A): EW = 2 (S + 2^-22 (1 + A)) bounds a weight's relative error with its sum's. lse is off by
 (EW + n 2^-24) / ln 2 and its own rounding, a key's weight from R rows by 2 EW + (n + R + 2) 2^-24 + 2^-22 (1 + |lse|) of itself; keys that no
-row sees have received exactly nothing. The output has P in bf16 and its own rounding: (2^-8 + EW + n 2^-24) sum w |v| + 2^-8 |o|."""
+row sees have received exactly nothing. The output has P in bf16 and its own rounding: (2^-8 + EW + n 2^-24) sum w |v| + 2^-8 |o|.
+``_fine``: queries whose elements have all eight bits of bf16, one of every eight neighbours between 1 and 2, the others between 2^-8 and 2^-5, so that
+in 20 bits of fixed point below the largest of 32 each is whole; every product is a multiple of a unit of which a row's sum of sizes has less than 2^24 (asserted), so a score is exact in fp32 in
+whatever order it is summed, and S = 2^-23 max |scale q k|."""
 import math
 
 import numpy as np
@@ -18,7 +21,7 @@ from kafka_llm_service_amd import ops
 from kafka_llm_service_amd.ops import kv4
 from kafka_llm_service_amd.ops import kv4_reference as kref
 from kafka_llm_service_amd.ops import reference as ref
-from test_kv4 import CASES, _check_attention, _id, numbers, queries, within, world
+from test_kv4 import CASES, _check_attention, _id, numbers, oracle, queries, within, world
 
 
 # ---- deep loops -----------------------------------------------------------------------------------------------------------
@@ -106,12 +109,20 @@ def _sparse(T, Hq, D, seed=2):
     return q.scatter_(-1, torch.randint(0, 8, size.shape, generator=g)[..., None], size[..., None]).flatten(-2).bfloat16()
 
 
-def _sharp(case, device):
+def _fine(T, Hq, D, seed=6):
+    g = torch.Generator().manual_seed(seed)
+    size = torch.randint(6, 9, (T, Hq, D // 8, 8), generator=g)
+    size.scatter_(-1, torch.randint(0, 8, (T, Hq, D // 8, 1), generator=g), 0)      # (of every eight one of the largest)
+    q = (1 + torch.randint(0, 128, (T, Hq, D), generator=g) / 128) * torch.exp2(-size.flatten(-2).float())
+    return (q * (torch.randint(0, 2, q.shape, generator=g) * 2 - 1)).bfloat16()
+
+
+def _sharp(case, device, fine=False):
     Hq, H, D, segs, window, first = case
     G = Hq // H
     kc, vc, tables = world(segs, H, D, 5, device)
     T = max(s[0] + s[1] for s in segs)
-    q, scale = _sparse(T, Hq, D), 0.25
+    q, scale = (_fine if fine else _sparse)(T, Hq, D), 0.25
     plan = kv4.attn_plan(segs, Hq, H, D, window, first, device)
     lse = torch.empty(T, Hq, device=device)
     out = kv4.attn(q.to(device), kc, vc, tables, plan, scale, lse=lse).cpu()
@@ -132,7 +143,14 @@ def _sharp(case, device):
                 x = q[t0:t0 + rows, g].double()
                 s = (x @ k[:, h].T * scale).masked_fill(~see, -math.inf)
                 A = (x.abs() @ k[:, h].abs().T * scale).masked_fill(~see, 0).amax(-1, keepdim=True)
-                EW = 2 * (2 * (D // 8 + 4) * 2.0 ** -24 * A + 2.0 ** -22 * (1 + A))
+                if fine:
+                    e = kref.unpack(kc[ids], False)[1].transpose(1, 2).flatten(0, 1)[:n, h].amin(-1)       # 2^-15 times 1/2 times the key's least scale
+                    assert (x.abs() @ k[:, h].abs().T / torch.exp2(e - 16.0) < 2.0 ** 24).all()
+                    A = s.masked_fill(~see, 0).abs().amax(-1, keepdim=True)
+                    S = 2.0 ** -23 * A
+                else:
+                    S = 2 * (D // 8 + 4) * 2.0 ** -24 * A
+                EW = 2 * (S + 2.0 ** -22 * (1 + A))
                 ls = torch.logsumexp(s, -1, keepdim=True)
                 w = torch.exp(s - ls)
                 o = w @ v[:, h]
@@ -158,6 +176,83 @@ def test_sharp_scores_reference(case):
 def test_sharp_scores_on_the_gpu(cuda, monkeypatch, case, wide):
     monkeypatch.setattr(kv4, "MANY_COST", -1e9 if wide else 1e9)
     _sharp(case, cuda)
+
+
+@pytest.mark.parametrize("case", CASES, ids=_id)
+def test_fine_scores_reference(case):
+    _sharp(case, "cpu", True)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("wide", [False, True])
+@pytest.mark.parametrize("case", CASES, ids=_id)
+def test_fine_scores_on_the_gpu(cuda, monkeypatch, case, wide):
+    """Nothing of a score is lost in any form: as exact as 32 bits are."""
+    monkeypatch.setattr(kv4, "MANY_COST", -1e9 if wide else 1e9)
+    _sharp(case, cuda, True)
+
+
+# ---- queries of all sizes -------------------------------------------------------------------------------------------------
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,cost", [(1, 1e9), (9, 1e9), (150, -1e9)])
+@pytest.mark.parametrize("D", [64, 128])
+def test_small_elements_beside_a_large_one(cuda, monkeypatch, D, rows, cost):
+    """An element 2^-t of its neighbour, which meets only zeros, under a scale 2^t as large: the same scores, whole down to 2^-11."""
+    monkeypatch.setattr(kv4, "MANY_COST", cost)
+    n = 400
+    segs = [(0, rows, n - rows, 0)]
+    kc, vc, tables = world(segs, 1, D, 0, cuda, garbage=False)
+    g = torch.Generator().manual_seed(2)
+    k = torch.zeros(n // 16, 1, 16, D)
+    k[..., 1] = torch.tensor([0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0])[torch.randint(0, 8, (n // 16, 1, 16), generator=g)]
+    k[..., 2] = 6.0                                           # (the scale is one; no query looks here)
+    kc[tables[0, :n // 16].long()] = kref.pack_pages(k, k)[0].to(cuda)
+    plan = kv4.attn_plan(segs, 4, 1, D, device=cuda)
+    x = k[:, 0, :, 1].flatten().double()
+    see = torch.arange(n)[None] <= n - rows + torch.arange(rows)[:, None]
+    first = None
+    for t in range(12):
+        q = torch.zeros(rows, 4, D, dtype=torch.bfloat16, device=cuda)
+        q[..., 0], q[..., 1] = 1.9921875, 1.9921875 * 2.0 ** -t
+        lse = torch.zeros(rows, 4, device=cuda)
+        out = kv4.attn(q, kc, vc, tables, plan, 0.5 * 2.0 ** t, lse=lse)
+        mass = kv4.attn_mass(q, lse, kc, tables, plan, 0.5 * 2.0 ** t)
+        if first is None:
+            first = out, lse, mass
+            want = torch.logsumexp((x * 1.9921875 * 0.5).expand(rows, n).masked_fill(~see, -math.inf), -1) / math.log(2)
+            # scores below 6, a sum of 400 numbers: (400 2^-24 + 2 * 7 * 2^-22) / ln 2
+            assert ((lse.double().cpu() - want[:, None]).abs() <= 4e-5).all()
+        assert all(torch.equal(a, b) for a, b in zip((out, lse, mass), first)), t
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,cost", [(1, 1e9), (9, 1e9), (150, -1e9)])
+@pytest.mark.parametrize("D", [64, 128])
+def test_queries_that_are_no_numbers(cuda, monkeypatch, D, rows, cost):
+    """A row with an infinity or no number in it is no numbers, those beside it and rows of zeros and of the smallest numbers are right. (Not
+    bit for bit as without it: a tile's rows raise their maxima together, and by what P is divided before it is rounded decides its last bit.)"""
+    monkeypatch.setattr(kv4, "MANY_COST", cost)
+    segs = [(0, rows, 300, 0)]
+    kc, vc, tables = world(segs, 2, D, 0, cuda)
+    q = queries(rows, 8, D, 1, cuda)
+    plan = kv4.attn_plan(segs, 8, 2, D, device=cuda)
+    lse2 = torch.zeros(rows, 8, device=cuda)
+    o, l, _, bo, bl, _ = oracle(q.cpu(), kc.cpu(), vc.cpu(), tables.cpu(), segs, 0, 0, 0.1)
+    bad = q.clone()
+    bad[-1, 3, 5], bad[-1, 6, D - 1], bad[0, 0, D // 2] = math.nan, math.inf, -math.inf
+    bad[0, 5], bad[0, 1], bad[0, 2] = 0.0, 1e-38, 0.0
+    bad[0, 1, 1::2] = -9e-41
+    out = kv4.attn(bad, kc, vc, tables, plan, 0.1, lse=lse2)
+    none = torch.zeros(rows, 8, dtype=torch.bool, device=cuda)
+    none[-1, 3] = none[-1, 6] = none[0, 0] = True
+    other = ~none
+    other[0, 5] = other[0, 1] = other[0, 2] = False
+    assert out[none].isnan().all() and lse2[none].isnan().all()
+    other = other.cpu()
+    within(out.cpu()[other], o[other], bo[other], "out")
+    within(lse2.cpu()[other], l[other], bl[other], "lse")
+    even = math.log2(301)                                     # of 301 equal weights
+    assert out[0, (1, 2, 5),].isfinite().all() and ((lse2[0, (1, 2, 5),] - even).abs() < 1e-5).all()
 
 
 # ---- pages that are none, in every kind of tile ---------------------------------------------------------------------------
