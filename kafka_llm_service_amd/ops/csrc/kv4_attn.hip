@@ -10,7 +10,7 @@
 // The softmax runs in one pass with a running maximum per row; its sums and maxima are fp32, P is rounded to bf16 for the product.
 //
 // Single tokens are bound by the pages' bytes where the work on them fits beside: the matrix cores take K as it lies, so that what is left is mostly
-// the widening of V. 64 threads of 4100 tokens, 32/8 heads of 128: 56 us, 5.1 TB/s (a large copy's rate); one thread of 1511 7.4 us: launch,
+// the widening of V. 64 threads of 4100 tokens, 32/8 heads of 128: 56 us, 5.1 TB/s (a large copy's rate); one thread of 1511 7.6 us: launch,
 // four reads that wait for each other (item, page ids, pages, parts) and the join. Long portions go through kv4_tile.hip.
 #include "attn_tile.h"
 #include "kv4_widen.h"
@@ -603,8 +603,8 @@ __device__ __forceinline__ void of_rows(T x, T (&y)[4], int lane) {
 
 // Segments of at most 16 rows: four waves take every fourth block of an item's (at most 32), NB of them in registers. What a key had before
 // comes with it: a load that is asked for when its sum is there holds up those of the next keys. Bytes bound it, and the start and
-// end of workgroups of 28 blocks: 29 threads of 7900 tokens, 8 heads of 128, 140 MB, 36 us with the masses read from other memory each time,
-// 3.9 TB/s. Heads of 128 take four waves a SIMD: five leave too few registers for the parts of Q (103 us).
+// end of workgroups of 28 blocks: 29 threads of 7900 tokens, 8 heads of 128, 140 MB, 31 us, 4.5 TB/s, behind the
+// attention over the same pages, 36 by itself over others each time. Heads of 128 take four waves a SIMD: five leave too few registers for the parts of Q (103 us).
 template <int D, int NB>
 __global__ __launch_bounds__(256, D == 128 ? 4 : 5) void mass_few_kernel(MassArgs ma) {
   const Args& a = ma.a;
