@@ -149,8 +149,9 @@ def silu_mul(x: torch.Tensor, out: torch.Tensor | None = None, act: str = "silu"
 
 
 def rope_kv_write(qkv, positions, cos_sin, q_out, k_cache, v_cache, slot_mapping, Hq: int, Hkv: int) -> None:
-    """RoPE on q/k + paged KV write; ``qkv`` is bf16 [T, W] or a split-K slab [S, T, W]. Slots below zero are left out. (The cache in 4
-    bits takes keys as the one in bf16 would hold them; not a number counts as zero there, an infinity as the largest.)"""
+    """RoPE on q/k + paged KV write; ``qkv`` is bf16 [T, W] or a split-K slab [S, T, W]. Slots below zero are left out, one
+    that is given twice holds bytes of both rows. (The cache in 4 bits takes keys as the one in bf16 would hold them; not a number counts as zero
+    there, an infinity as the largest.)"""
     if _gpu(qkv) and is_mx4_cache(k_cache):
         ext().kv4_rope_write(qkv, positions, cos_sin, q_out, k_cache, v_cache, slot_mapping, int(Hq), int(Hkv))
     elif _gpu(qkv):
