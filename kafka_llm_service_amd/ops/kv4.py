@@ -410,9 +410,9 @@ def evict_keep(mass: torch.Tensor, lens: torch.Tensor, budget: int, first: int =
 
 def evict(k_cache, v_cache, block_tables, kept, new_tables, mass=None):
     """Copies the ``kept`` keys and values (``evict_keep``) of every sequence and head from the pages of ``block_tables`` to those of
-    ``new_tables``, int32 [sequences, pages] both, in order: key i of a head becomes kept[.., i]. The new pages are none of the old ones, and
-    each is one sequence's (the old ones other sequences may share, and which their owner may free afterwards); places behind a sequence's last key are left as they
-    were, as are keys whose index, or whose page, is outside. Returns the kept keys' ``mass`` [sequences, kv heads, budget]
+    ``new_tables``, int32 [sequences, pages] both, in order: key i of a head becomes kept[.., i]. The new pages are none of the old ones
+    (which other sequences may share, and which their owner may free afterwards), and each is one sequence's alone; places behind a
+    sequence's last key are left as they were, as are keys whose index, or whose page, is outside. Returns the kept keys' ``mass`` [sequences, kv heads, budget]
     (zero behind the last) if it is given, else None."""
     if _gpu(k_cache):
         return ext().kv4_evict_copy(k_cache, v_cache, block_tables, kept, new_tables, mass)
