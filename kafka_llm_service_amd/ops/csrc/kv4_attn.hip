@@ -361,7 +361,7 @@ __device__ __forceinline__ void join(float& M, float& L, f32x4& o, const float (
 // works on, the others on their way. (The loop's first form fetches without a condition, so that the waits count what is on its way.)
 // Three waves a SIMD with two half blocks each: 64 threads of 4100 tokens and 29 of 7900 56.7 and 56.7 us, three halves 57.2 and 57.6, two waves with
 // four 58.0 and 57.1, four with one 57.6 and 61.3 (with Q in two parts of e4m3; in four of e2m3 57.4 and 57.2). NQ 2, short portions: values are widened once for 32 rows; 4 portions of 100 rows behind
-// 1000 keys, 32/8 heads of 128, 23 us, as tiles of 256 rows whose keys are widened first 31. That is five times its operations' time: about a
+// 1000 keys, 32/8 heads of 128, 23 us (26 with other inputs each time), as tiles of 256 rows whose keys are widened first 31. That is five times its operations' time: about a
 // hundred scalar registers of this form do not fit and go through lanes in the loop, each product with values is done twice, and values are widened for every 32 rows anew.
 // WIDEN: the workgroups behind the items' widen the step's long portions' keys on the way (kv4_tile.hip), which as a launch of its own would
 // wait for this one, 6 us of mostly waiting (5 tokens and 3 portions of 1100, heads of 64, window 512: 43 us apart, 39.6 together).
